@@ -1,0 +1,164 @@
+// Shared by the attention kernels (attn_prompt.hip, attn_decode.hip, attn_backward.hip):
+// element types of the 32x32 MFMAs, the paged cache's addressing, and the mapping of
+// workgroups to the row tiles of packed sequences.
+#pragma once
+#include "mfma.hpp"
+
+namespace hmx {
+namespace attn {
+
+// Operand conventions of the 32x32x16 MFMAs (lane l, h = l >> 5, l32 = l & 31):
+//   A: row l32, k = 8h..8h+7;  B: column l32, the same k
+//   C/D: column l32, rows 8i + 4h + j in register 4i + j
+template <typename T> struct El;
+template <> struct El<bf16> {
+  typedef bf16x8 v8;
+  typedef bf16x4 v4;
+  static __device__ __forceinline__ f32x16 mma32(v8 a, v8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 mma16(v8 a, v8 b, f32x4 c) { return mfma16(a, b, c); }
+};
+template <> struct El<f16> {
+  typedef f16x8 v8;
+  typedef f16x4 v4;
+  static __device__ __forceinline__ f32x16 mma32(v8 a, v8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 mma16(v8 a, v8 b, f32x4 c) { return mfma16h(a, b, c); }
+};
+
+template <typename T>
+__device__ __forceinline__ typename El<T>::v8 pack8(float a0, float a1, float a2, float a3,
+                                                    float a4, float a5, float a6, float a7) {
+  return typename El<T>::v8{(T)a0, (T)a1, (T)a2, (T)a3, (T)a4, (T)a5, (T)a6, (T)a7};
+}
+
+// the transposing LDS read of 4 keys of one column (see ld_tr in mfma.hpp): the lane's
+// own address, the 16 lanes of a group covering 4 rows x 16 columns
+template <typename T>
+__device__ __forceinline__ typename El<T>::v4 tr4(const T* p) {
+  const s16x4 r = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) s16x4*)(p));
+  return __builtin_bit_cast(typename El<T>::v4, r);
+}
+template <typename T>
+__device__ __forceinline__ typename El<T>::v8 join(typename El<T>::v4 a, typename El<T>::v4 b) {
+  return typename El<T>::v8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
+// max and sum over the two halves of a wave, in the VALU
+__device__ __forceinline__ float half_max(float a) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, a),
+                                                  __builtin_bit_cast(unsigned, a), false, false);
+  return fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
+}
+
+constexpr float NEG_INF = -__builtin_inff();
+constexpr float LOG2E = 1.4426950408889634f;
+
+// x / d and x % d for 0 <= x < 2^31 by a 64-bit reciprocal m = ceil(2^64 / d) (0: d = 1):
+// x m / 2^64 exceeds x / d by less than x / 2^64 < 1 / d, so the floor is exact
+struct FastDiv {
+  uint64_t m;
+  int32_t d;
+};
+inline FastDiv fast_div(int32_t d) {
+  return FastDiv{d <= 1 ? 0 : ~0ull / (uint64_t)d + 1, d};   // ~0 / d + 1 = ceil(2^64 / d)
+}
+__device__ __forceinline__ int fdiv(int x, const FastDiv& f) {
+  return f.m == 0 ? x : (int)__umul64hi((uint64_t)(uint32_t)x, f.m);
+}
+// the same for slots of a cache, which may pass 2^31: x d < 2^64 is all it needs
+__device__ __forceinline__ int64_t fdiv64(int64_t x, const FastDiv& f) {
+  return f.m == 0 ? x : (int64_t)__umul64hi((uint64_t)x, f.m);
+}
+
+// ------------------------------------------------------------------ paged cache
+struct Pages {
+  const char* k;
+  const char* v;
+  int64_t k_ps, k_ts, k_hs, v_ps, v_ts, v_hs;   // strides in bytes
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* lens;
+  int32_t width, num_pages;
+  FastDiv page;
+};
+
+inline Pages make_pages(const hmx_paged_kv& c) {
+  Pages p;
+  p.k = static_cast<const char*>(c.k);
+  p.v = static_cast<const char*>(c.v);
+  p.k_ps = 2 * c.k_page_stride; p.k_ts = 2 * c.k_token_stride; p.k_hs = 2 * c.k_head_stride;
+  p.v_ps = 2 * c.v_page_stride; p.v_ts = 2 * c.v_token_stride; p.v_hs = 2 * c.v_head_stride;
+  p.table = c.table; p.table_stride = c.table_stride; p.lens = c.seq_lens;
+  p.width = c.num_pages > 0 ? c.table_width : 0;   // an empty cache holds no keys
+  p.num_pages = c.num_pages; p.page = fast_div(c.page_size);
+  return p;
+}
+
+// ------------------------------------------------------------------ packed sequences
+// Rows are (token, head of the group), G to a token.  Boundaries b(0) = 0, b(1) = cu[0],
+// ..., b(N + 1) = cu[N], b(N + 2) = T cut the tokens into N sequences and the gaps before
+// and behind them.  Part e starts at tile slot f(e) = floor(b(e) G / BM) + e: between f(e)
+// and f(e + 1) lie at least ceil(rows / BM) slots, so a workgroup finds its tile from its
+// slot with a search, without a plan made of the lengths on the host.
+struct Seqs {
+  const int32_t* cu;   // NULL: N sequences of T / N tokens
+  int32_t N, T, G;
+};
+
+struct Tile {
+  int seq;             // -1: rows of no sequence
+  int bos, tokens;     // the part's first token and its tokens
+  int row0, rows;      // the tile's first row in the part, the part's rows; row0 >= rows: nothing to do
+};
+
+__device__ __forceinline__ int seq_bound(const Seqs& s, int e) {
+  if (e == 0) return 0;
+  if (e == s.N + 2) return s.T;
+  return min(max(s.cu[e - 1], 0), s.T);
+}
+
+template <int BM>
+__device__ __forceinline__ Tile find_tile(const Seqs& s, int slot) {
+  Tile t;
+  if (!s.cu) {
+    const int len = s.T / s.N, per = (int)(((int64_t)len * s.G + BM - 1) / BM);
+    t.seq = slot / max(per, 1);
+    t.bos = t.seq * len;
+    t.tokens = len;
+    t.row0 = (slot - t.seq * per) * BM;
+    t.rows = len * s.G;
+    if (t.seq >= s.N || per == 0) t.rows = 0;
+    return t;
+  }
+  const int lane = threadIdx.x & 63;
+  int lo = 0, span = s.N + 2;
+  while (span > 1) {
+    const int step = (span + 63) >> 6, e = lo + lane * step;
+    const bool in = lane * step < span &&
+                    (int64_t)seq_bound(s, min(e, s.N + 2)) * s.G / BM + e <= slot;
+    const unsigned long long m = __ballot(in) | 1ull;   // f(0) = 0 <= slot
+    const int p = 63 - __builtin_clzll(m);
+    span = min(step, span - p * step);
+    lo += p * step;
+  }
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  t.bos = seq_bound(s, lo);
+  t.tokens = max(seq_bound(s, lo + 1) - t.bos, 0);
+  t.seq = (lo == 0 || lo == s.N + 1) ? -1 : lo - 1;
+  t.row0 = (int)(slot - ((int64_t)t.bos * s.G / BM + lo)) * BM;
+  t.rows = t.tokens * s.G;
+  return t;
+}
+
+template <int BM>
+inline int64_t tile_slots(const int32_t* cu, int64_t N, int64_t T, int64_t G) {
+  if (!cu) return N * ((T / N * G + BM - 1) / BM);
+  return T * G / BM + N + 2;
+}
+
+}  // namespace attn
+}  // namespace hmx

@@ -1,0 +1,432 @@
+// Attention of one new token a sequence over a paged cache:
+//   o_n = sum_j softmax_j(scale q_n . k_j) v_j over the sequence's keys j < len_n
+// Bound by memory: every key and value is read once, by the workgroup that holds all
+// heads of its group (up to 16 columns of a matrix product).
+//
+// The lengths are known on the device only (a captured step replays with other lengths),
+// so the work is cut there: the keys of all sequences, in units of 64, form one list, and
+// worker w of W takes units [w per, (w + 1) per).  All workers get the same share whatever
+// the lengths are, and a sequence cut over several workers is joined by a second launch
+// from fp32 shares.  A worker's four waves take 32 keys in turn; nothing is shared between
+// them until a sequence's share ends.  K goes from memory to registers as the A operand
+// (S^T = K Q^T), V through the wave's own LDS tile to be read transposed
+// (O^T = V^T P^T); the next 32 keys are in flight meanwhile.
+// P is rounded to the inputs' type; scores, statistics and O stay in fp32.
+#include "attn.hpp"
+
+namespace hmx {
+namespace attn {
+
+constexpr int UNIT = 64;     // keys of a unit
+constexpr int KT = 32;       // keys of a wave's step
+constexpr int MIN_UNITS = 4; // of a worker: below that the joining costs more than it gains
+
+struct DecArgs {
+  const char* q;
+  char* o;
+  int64_t q_ts, q_hs, o_ts, o_hs;   // bytes
+  Pages pages;
+  int32_t N, HKV, G, hblocks, W;    // hblocks: blocks of 16 heads of a group
+  float c;
+  float* part;   // [W][2][HKV * hblocks][16][D], then [W][2][HKV * hblocks][16][2]
+};
+
+__device__ __forceinline__ int seq_keys(const DecArgs& a, int n) {
+  return (int)min((int64_t)max(a.pages.lens[n], 0), (int64_t)a.pages.width * a.pages.page.d);
+}
+
+// Units before sequence n, for the sequences around a worker: the total of the list and,
+// for the unit `at`, the sequence that holds it and that sequence's first unit.  All
+// threads of the workgroup call it; sh holds 8 ints.
+struct Place { int64_t total; int seq; int64_t first; };
+__device__ Place find_unit(const DecArgs& a, int64_t at, int64_t* sh) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  Place p{0, a.N, 0};
+  for (int n0 = 0; n0 < a.N; n0 += 256) {
+    const int n = n0 + tid;
+    const int u = n < a.N ? (seq_keys(a, n) + UNIT - 1) / UNIT : 0;
+    int64_t x = u;
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t y = __shfl_up(x, d, 64);
+      if (lane >= d) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) sh[wave] = x;
+    if (tid == 0) sh[4] = -1;
+    __syncthreads();
+    int64_t base = p.total;
+    for (int w = 0; w < wave; ++w) base += sh[w];
+    const int64_t begin = base + x - u;
+    if (u > 0 && at >= begin && at < begin + u) {
+      sh[4] = n;
+      sh[5] = begin;
+    }
+    __syncthreads();
+    p.total += sh[0] + sh[1] + sh[2] + sh[3];
+    if (sh[4] >= 0) {
+      p.seq = (int)sh[4];
+      p.first = sh[5];
+    }
+  }
+  return p;
+}
+
+__device__ __forceinline__ int64_t units_per(const DecArgs& a, int64_t total) {
+  const int64_t per = (total + a.W - 1) / a.W;
+  return per < MIN_UNITS ? MIN_UNITS : per;
+}
+
+// 16-byte chunk at which chunk c of key row r sits: the transposing reads take 16 rows by
+// 32 bytes, spread evenly over the banks
+template <int D> __device__ __forceinline__ int dpos(int r, int c) {
+  return D == 128 ? c ^ ((r & 7) << 1) : c ^ (((r >> 1) & 3) << 1);
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void attn_decode_kernel(DecArgs a) {
+  typedef typename El<T>::v8 v8;
+  constexpr int NS = D / 32, ND = D / 16;
+  __shared__ __align__(16) char smem[4 * KT * D * 2 > 4 * 16 * D * 4 ? 4 * KT * D * 2 : 4 * 16 * D * 4];
+  __shared__ float s_ml[4][16][2];
+  __shared__ int64_t s_scan[8];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q4 = lane >> 4, l16 = lane & 15;
+  const int hb = blockIdx.x % (a.HKV * a.hblocks), w = blockIdx.x / (a.HKV * a.hblocks);
+  const int kvh = hb % a.HKV, g0 = (hb / a.HKV) * 16;
+  const int ng = min(16, a.G - g0);
+
+  // rows without keys
+  if (w == 0) {
+    for (int n = tid; n < a.N; n += 256)
+      if (seq_keys(a, n) == 0)
+        for (int g = 0; g < ng; ++g) {
+          char* op = a.o + (int64_t)n * a.o_ts + (int64_t)(kvh * a.G + g0 + g) * a.o_hs;
+          for (int i = 0; i < D / 8; ++i) reinterpret_cast<uint4*>(op)[i] = uint4{0, 0, 0, 0};
+        }
+  }
+  Place pl = find_unit(a, 0, s_scan);
+  const int64_t per = units_per(a, pl.total);
+  const int64_t u_beg = w * per, u_end = min(pl.total, u_beg + per);
+  if (u_beg >= u_end) return;
+  pl = find_unit(a, u_beg, s_scan);
+  int seq = pl.seq;
+  int64_t first = pl.first, u = u_beg;
+
+  T* Vt = reinterpret_cast<T*>(smem) + wave * KT * D;
+  int wo[NS];                                // where the lane's chunks of a V row go
+#pragma unroll
+  for (int s = 0; s < NS; ++s) wo[s] = dpos<D>(l16, 4 * s + q4) * 8;
+  int ro[ND];                                // and where its transposing reads start
+#pragma unroll
+  for (int d = 0; d < ND; ++d) {
+    const int s = l16, r = 4 * q4 + (s >> 2);
+    ro[d] = r * D + dpos<D>(r, 2 * d + ((s & 3) >> 1)) * 8 + 4 * (s & 1);
+  }
+
+  while (u < u_end) {
+    // this worker's share of sequence seq: keys k_beg .. k_end - 1
+    int keys = seq_keys(a, seq);
+    while (keys == 0) keys = seq_keys(a, ++seq);     // u < total: a sequence with keys follows
+    const int64_t units = (keys + UNIT - 1) / UNIT;
+    const int k_beg = (int)(u - first) * UNIT;
+    const int64_t stop = min(u_end, first + units);
+    const int k_end = min(keys, (int)(stop - first) * UNIT);
+    const int32_t* table = a.pages.table + (int64_t)seq * a.pages.table_stride;
+
+    v8 qf[NS];
+    {
+      const int hq = kvh * a.G + g0 + min(l16, ng - 1);
+      const char* qp = a.q + (int64_t)seq * a.q_ts + (int64_t)hq * a.q_hs + 16 * q4;
+#pragma unroll
+      for (int s = 0; s < NS; ++s) qf[s] = *reinterpret_cast<const v8*>(qp + 64 * s);
+    }
+    f32x4 acc[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = NEG_INF, l = 0.f;
+
+    v8 kf[2][NS], vf[2][NS], kn[2][NS], vn[2][NS];
+    int pid[2];
+    bool okn[2] = {false, false}, ok[2];
+    auto fetch_pages = [&](int k0) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) pid[x] = table[fdiv(min(k0 + 16 * x + l16, k_end - 1), a.pages.page)];
+    };
+    auto load = [&](int k0) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int key = min(k0 + 16 * x + l16, k_end - 1);
+        const int64_t in = key - fdiv(key, a.pages.page) * a.pages.page.d;
+        const bool pg = (unsigned)pid[x] < (unsigned)a.pages.num_pages;
+        const int64_t p = pg ? pid[x] : 0;
+        okn[x] = pg && k0 + 16 * x + l16 < k_end;
+        const char* kp = a.pages.k + p * a.pages.k_ps + in * a.pages.k_ts + kvh * a.pages.k_hs + 16 * q4;
+        const char* vp = a.pages.v + p * a.pages.v_ps + in * a.pages.v_ts + kvh * a.pages.v_hs + 16 * q4;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          kn[x][s] = *reinterpret_cast<const v8*>(kp + 64 * s);
+          vn[x][s] = *reinterpret_cast<const v8*>(vp + 64 * s);
+        }
+      }
+    };
+    int k0 = k_beg + wave * KT;
+    if (k0 < k_end) {
+      fetch_pages(k0);
+      load(k0);
+      if (k0 + 4 * KT < k_end) fetch_pages(k0 + 4 * KT);
+    }
+    for (; k0 < k_end; k0 += 4 * KT) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        ok[x] = okn[x];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          kf[x][s] = kn[x][s];
+          vf[x][s] = vn[x][s];
+        }
+      }
+      if (k0 + 4 * KT < k_end) {
+        load(k0 + 4 * KT);
+        if (k0 + 8 * KT < k_end) fetch_pages(k0 + 8 * KT);
+      }
+      // V into the wave's tile; rows that are no keys as zeros (their probability is 0,
+      // their memory anything)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+          v8 z = vf[x][s];
+          if (!ok[x]) z = v8{0};
+          *reinterpret_cast<v8*>(Vt + (16 * x + l16) * D + wo[s]) = z;
+        }
+      f32x4 st[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        st[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < NS; ++s) st[x] = El<T>::mma16(kf[x][s], qf[s], st[x]);
+        // bit r of the ballot's low 16: row r holds a key
+        const unsigned long long live = __ballot(ok[x]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!((live >> (4 * q4 + i)) & 1)) st[x][i] = NEG_INF;
+      }
+      float mx = NEG_INF;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(st[0][i], st[1][i]));
+      mx = half_max(mx);
+      mx = fmaxf(mx, shfl_xor(mx, 16));
+      if (__any((mx - m) * a.c > 8.f)) {
+        const float mn = fmaxf(m, mx);
+        const float f = m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((m - mn) * a.c);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[d] *= f;
+      }
+      const float mc = m == NEG_INF ? 0.f : m * a.c;
+      float p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(st[i >> 2][i & 3] * a.c - mc);
+        l += p[i];
+      }
+      const v8 pf = pack8<T>(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const v8 vt = join<T>(tr4<T>(Vt + ro[d]), tr4<T>(Vt + ro[d] + 16 * D));
+        acc[d] = El<T>::mma16(vt, pf, acc[d]);
+      }
+    }
+    l += shfl_xor(l, 16);
+    l = pair_sum32(l, l);
+
+    // the four waves' shares joined through LDS: O^T rows 16 d + 4 q4 + i, column l16
+    __syncthreads();
+    float* ob = reinterpret_cast<float*>(smem);       // [wave][16][D]
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+      *reinterpret_cast<f32x4*>(ob + (wave * 16 + l16) * D + 16 * d + 4 * q4) = acc[d];
+    if (q4 == 0) {
+      s_ml[wave][l16][0] = m * a.c;
+      s_ml[wave][l16][1] = l;
+    }
+    __syncthreads();
+    const bool whole = k_beg == 0 && k_end == keys;
+    const int piece = u_beg < first ? 1 : 0;
+    const int64_t slot = ((int64_t)w * 2 + piece) * a.HKV * a.hblocks + hb;
+    float* pp = a.part + slot * 16 * D;
+    float* pm = a.part + (int64_t)a.W * 2 * a.HKV * a.hblocks * 16 * D + slot * 32;
+    for (int i = tid; i < ng * (D / 4); i += 256) {
+      const int g = i / (D / 4), d = 4 * (i % (D / 4));
+      float mm = NEG_INF, ll = 0.f;
+      for (int x = 0; x < 4; ++x) mm = fmaxf(mm, s_ml[x][g][0]);
+      const float ref = mm == NEG_INF ? 0.f : mm;
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+      for (int x = 0; x < 4; ++x) {
+        const float f = __builtin_amdgcn_exp2f(s_ml[x][g][0] - ref);
+        ll += f * s_ml[x][g][1];
+        o += f * *reinterpret_cast<const f32x4*>(ob + (x * 16 + g) * D + d);
+      }
+      if (whole) {
+        const float inv = ll == 0.f ? 0.f : 1.f / ll;
+        typename El<T>::v4 y;
+#pragma unroll
+        for (int z = 0; z < 4; ++z) y[z] = (T)(o[z] * inv);
+        *reinterpret_cast<typename El<T>::v4*>(a.o + (int64_t)seq * a.o_ts +
+                                               (int64_t)(kvh * a.G + g0 + g) * a.o_hs + 2 * d) = y;
+      } else {
+        *reinterpret_cast<f32x4*>(pp + g * D + d) = o;
+        if (d == 0) {
+          pm[2 * g] = mm;
+          pm[2 * g + 1] = ll;
+        }
+      }
+    }
+    __syncthreads();
+    u = stop;
+    first += units;
+    ++seq;
+  }
+}
+
+// Sequences cut over several workers: their shares joined.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_decode_join_kernel(DecArgs a) {
+  __shared__ int64_t s_scan[8];
+  const int hb = blockIdx.x % (a.HKV * a.hblocks), n = blockIdx.x / (a.HKV * a.hblocks);
+  const int kvh = hb % a.HKV, g0 = (hb / a.HKV) * 16, ng = min(16, a.G - g0);
+  const int keys = seq_keys(a, n);
+  if (keys <= UNIT) return;   // one unit is never cut
+  // units before sequence n, and the total
+  int64_t before = 0, total = 0;
+  for (int n0 = 0; n0 < a.N; n0 += 256) {
+    const int x = n0 + (int)threadIdx.x;
+    const int64_t u = x < a.N ? (seq_keys(a, x) + UNIT - 1) / UNIT : 0;
+    int64_t b = x < n ? u : 0, t = u;
+    for (int d = 32; d >= 1; d >>= 1) {
+      b += __shfl_xor(b, d, 64);
+      t += __shfl_xor(t, d, 64);
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+      s_scan[threadIdx.x >> 6] = b;
+      s_scan[4 + (threadIdx.x >> 6)] = t;
+    }
+    __syncthreads();
+    for (int i = 0; i < 4; ++i) {
+      before += s_scan[i];
+      total += s_scan[4 + i];
+    }
+  }
+  const int64_t per = units_per(a, total), last = before + (keys + UNIT - 1) / UNIT - 1;
+  const int64_t w0 = before / per, w1 = last / per;
+  if (w0 == w1) return;
+  const int64_t hbs = (int64_t)a.HKV * a.hblocks, stats = (int64_t)a.W * 2 * hbs * 16 * D;
+  for (int i = threadIdx.x; i < ng * (D / 4); i += 256) {
+    const int g = i / (D / 4), d = 4 * (i % (D / 4));
+    float m = NEG_INF, l = 0.f;
+    for (int64_t w = w0; w <= w1; ++w) {
+      const int64_t slot = (w * 2 + (w * per < before ? 1 : 0)) * hbs + hb;
+      m = fmaxf(m, a.part[stats + slot * 32 + 2 * g]);
+    }
+    const float ref = m == NEG_INF ? 0.f : m;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int64_t w = w0; w <= w1; ++w) {
+      const int64_t slot = (w * 2 + (w * per < before ? 1 : 0)) * hbs + hb;
+      const float f = __builtin_amdgcn_exp2f(a.part[stats + slot * 32 + 2 * g] - ref);
+      l += f * a.part[stats + slot * 32 + 2 * g + 1];
+      o += f * *reinterpret_cast<const f32x4*>(a.part + (slot * 16 + g) * D + d);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    typename El<T>::v4 y;
+#pragma unroll
+    for (int z = 0; z < 4; ++z) y[z] = (T)(o[z] * inv);
+    *reinterpret_cast<typename El<T>::v4*>(a.o + (int64_t)n * a.o_ts + (int64_t)(kvh * a.G + g0 + g) * a.o_hs +
+                                           2 * d) = y;
+  }
+}
+
+// Workers: as many as fill every compute unit twice, and no more than the keys a table
+// can hold give MIN_UNITS to.
+static int64_t workers(int64_t N, int64_t HKV, int64_t hblocks, int64_t max_keys) {
+  const int64_t most = N * ((max_keys + UNIT - 1) / UNIT);
+  int64_t w = 2ll * cu_count() / (HKV * hblocks);
+  const int64_t need = (most + MIN_UNITS - 1) / MIN_UNITS;
+  if (w > need) w = need;
+  return w < 1 ? 1 : w;
+}
+
+template <typename T, int D>
+static void launch(const DecArgs& a, bool join, hipStream_t s) {
+  const unsigned hbs = (unsigned)(a.HKV * a.hblocks);
+  hipLaunchKernelGGL((attn_decode_kernel<T, D>), dim3(hbs * (unsigned)a.W), dim3(256), 0, s, a);
+  if (join) hipLaunchKernelGGL((attn_decode_join_kernel<T, D>), dim3(hbs * (unsigned)a.N), dim3(256), 0, s, a);
+}
+
+}  // namespace attn
+}  // namespace hmx
+
+using namespace hmx;
+
+extern "C" size_t hmx_paged_attention_decode_workspace_bytes(int32_t N, int32_t H, int32_t HKV,
+                                                             int32_t D, int64_t max_keys) {
+  if (N <= 0 || HKV <= 0 || H <= 0 || H % HKV != 0 || max_keys <= 0) return 0;
+  const int64_t hb = (H / HKV + 15) / 16, w = attn::workers(N, HKV, hb, max_keys);
+  if (w == 1) return 0;
+  return (size_t)w * 2 * HKV * hb * 16 * (D + 2) * sizeof(float);
+}
+
+extern "C" int hmx_paged_attention_decode(const void* q, int64_t q_token_stride,
+                                          int64_t q_head_stride, int32_t dtype, void* o,
+                                          int64_t o_token_stride, int64_t o_head_stride,
+                                          const hmx_paged_kv* cache, int32_t N, int32_t H,
+                                          int32_t HKV, int32_t D, float scale, void* workspace,
+                                          size_t workspace_bytes, void* stream) {
+  HMX_REQUIRE(D == 64 || D == 128, HMX_EUNSUPPORTED,
+              "hmx_paged_attention_decode: head size %d not in {64, 128}", D);
+  HMX_REQUIRE(dtype == HMX_BF16 || dtype == HMX_F16, HMX_EUNSUPPORTED,
+              "hmx_paged_attention_decode: dtype code %d (bf16 or fp16)", dtype);
+  HMX_REQUIRE(N >= 0 && HKV > 0 && H > 0 && H % HKV == 0, HMX_EINVAL,
+              "hmx_paged_attention_decode: N=%d H=%d HKV=%d", N, H, HKV);
+  HMX_REQUIRE(scale > 0.f && scale < __builtin_inff(), HMX_EINVAL,
+              "hmx_paged_attention_decode: scale %g must be positive", (double)scale);
+  HMX_REQUIRE(cache && cache->num_pages >= 0 && cache->page_size > 0 && cache->table_width >= 0, HMX_EINVAL,
+              "hmx_paged_attention_decode: cache");
+  if (N == 0) return HMX_OK;
+  HMX_REQUIRE(q && o && cache->seq_lens && cache->table && cache->k && cache->v, HMX_EINVAL,
+              "hmx_paged_attention_decode: null pointer");
+  const int64_t max_keys = (int64_t)cache->table_width * cache->page_size;
+  HMX_REQUIRE(max_keys < (1ll << 31) - 256, HMX_EUNSUPPORTED,
+              "hmx_paged_attention_decode: a table row holds %lld keys", (long long)max_keys);
+  const int64_t st = q_token_stride | q_head_stride | o_token_stride | o_head_stride |
+                     cache->k_page_stride | cache->k_token_stride | cache->k_head_stride |
+                     cache->v_page_stride | cache->v_token_stride | cache->v_head_stride;
+  const uintptr_t al = (uintptr_t)q | (uintptr_t)o | (uintptr_t)cache->k | (uintptr_t)cache->v;
+  HMX_REQUIRE(st % 8 == 0 && al % 16 == 0, HMX_EINVAL,
+              "hmx_paged_attention_decode: strides must be multiples of 8 elements and pointers 16-byte aligned");
+  attn::DecArgs a{};
+  a.q = (const char*)q; a.o = (char*)o;
+  a.q_ts = 2 * q_token_stride; a.q_hs = 2 * q_head_stride;
+  a.o_ts = 2 * o_token_stride; a.o_hs = 2 * o_head_stride;
+  a.pages = attn::make_pages(*cache);
+  a.N = N; a.HKV = HKV; a.G = H / HKV; a.hblocks = (a.G + 15) / 16;
+  a.W = (int32_t)attn::workers(N, HKV, a.hblocks, max_keys);
+  a.c = scale * attn::LOG2E;
+  a.part = static_cast<float*>(workspace);
+  HMX_REQUIRE((int64_t)N * HKV * a.hblocks < (1ll << 31), HMX_EUNSUPPORTED,
+              "hmx_paged_attention_decode: %d sequences of %d heads", N, H);
+  const bool join = a.W > 1;
+  HMX_REQUIRE(!join || (workspace && (uintptr_t)workspace % 16 == 0 &&
+                        workspace_bytes >= hmx_paged_attention_decode_workspace_bytes(N, H, HKV, D, max_keys)),
+              HMX_EINVAL, "hmx_paged_attention_decode: workspace of %zu bytes is too small", workspace_bytes);
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == HMX_BF16) {
+    if (D == 64) attn::launch<bf16, 64>(a, join, s);
+    else attn::launch<bf16, 128>(a, join, s);
+  } else {
+    if (D == 64) attn::launch<f16, 64>(a, join, s);
+    else attn::launch<f16, 128>(a, join, s);
+  }
+  return check_launch("hmx_paged_attention_decode");
+}

@@ -1,0 +1,539 @@
+// Causal softmax attention of whole prompts (contiguous k, v) and of new tokens behind a
+// cached context (k, v in pages):
+//   s_ij = scale q_i . k_j  (j <= i + keys - tokens),  o_i = sum_j softmax_j(s_ij) v_j
+// in one pass over the keys with a running maximum and sum; a row without keys gives 0.
+//
+// A workgroup of four waves takes 128 rows, 32 to a wave, and walks the keys in tiles of
+// 64 staged through LDS (the next tile's loads are in flight while one is computed).
+// Rows are (token, head of the group): the heads that share keys sit in one tile, so few
+// tokens still fill the 32 columns of a matrix product and the keys are read once for all
+// of them.  Both products are formed transposed, S^T = K Q^T and O^T = V^T P^T: a lane
+// then holds one row's scores, so the softmax statistics are per-lane scalars and P^T in
+// the C layout is already the B operand of the second product (the k order it implies is
+// the one the transposing LDS reads of V are made in).
+// P is rounded to the inputs' type (half a step, 2^-9 for bf16, averaged over the keys);
+// scores, maxima, sums and O stay in fp32.
+#include "attn.hpp"
+
+namespace hmx {
+namespace attn {
+
+constexpr int BM = 128, BN = 64;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+struct FwdArgs {
+  const char *q, *k, *v;
+  char* o;
+  int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs;   // bytes
+  float* lse;          // [T, H] of the scaled scores in base 2, or NULL
+  Seqs seqs;
+  Pages pages;
+  FastDiv G;
+  int32_t H, HKV, slots, fill, nsplit;
+  float c;             // scale log2(e)
+  float* part;         // [nsplit][T * H][D], then [nsplit][T * H][2]: maximum and sum
+};
+
+// the 16-byte chunk at which chunk c of key row r sits in LDS: rows of K are read 32 at a
+// time at one chunk, rows of V four at a time over 64 bytes, each without bank conflicts
+template <int D> __device__ __forceinline__ int kpos(int r, int c) {
+  return D == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7);
+}
+template <int D> __device__ __forceinline__ int vpos(int r, int c) {
+  return D == 128 ? c ^ ((r & 3) << 2) : c ^ (((r >> 1) & 1) << 2);
+}
+
+// whether any of the eight 16-bit values is infinite or NaN
+template <typename T>
+__device__ __forceinline__ bool any_nonfinite(u32x4 x) {
+  constexpr uint32_t E = sizeof(T) == 2 && __is_same(T, bf16) ? 0x7f80u : 0x7c00u;
+  bool b = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b |= (x[i] & E) == E || ((x[i] >> 16) & E) == E;
+  return b;
+}
+
+// One key's row of k or v; NULL where its page lies outside the cache.
+template <typename T, bool PAGED>
+__device__ __forceinline__ const T* key_row(const FwdArgs& a, const Tile& t, int kvh, int j, bool value) {
+  if constexpr (PAGED) {
+    const int pi = fdiv(j, a.pages.page), pid = a.pages.table[t.seq * a.pages.table_stride + pi];
+    if ((unsigned)pid >= (unsigned)a.pages.num_pages) return nullptr;
+    const int64_t in = j - pi * a.pages.page.d;
+    return reinterpret_cast<const T*>(value ? a.pages.v + pid * a.pages.v_ps + in * a.pages.v_ts + kvh * a.pages.v_hs
+                                            : a.pages.k + pid * a.pages.k_ps + in * a.pages.k_ts + kvh * a.pages.k_hs);
+  } else {
+    return reinterpret_cast<const T*>(value ? a.v + (int64_t)(t.bos + j) * a.v_ts + kvh * a.v_hs
+                                            : a.k + (int64_t)(t.bos + j) * a.k_ts + kvh * a.k_hs);
+  }
+}
+
+// Row `row` of the part over keys k0 .. k1 - 1, unnormalised, in the layout of a split's share.
+template <int D>
+__device__ __forceinline__ float* share_row(const FwdArgs& a, int sp, int64_t r) {
+  return a.part + ((int64_t)sp * a.seqs.T * a.H + r) * D;
+}
+template <int D>
+__device__ __forceinline__ float* share_stats(const FwdArgs& a, int sp, int64_t r) {
+  const int64_t n = (int64_t)a.seqs.T * a.H;
+  return a.part + (int64_t)a.nsplit * n * D + ((int64_t)sp * n + r) * 2;
+}
+
+// The rows of one tile again, key by key in the VALU, where a value that is not finite
+// sits behind some rows' last key: 0 times it is not 0, so the matrix product has spoilt
+// those rows.  Never reached with finite values.
+template <typename T, int D, bool PAGED>
+__device__ __forceinline__ void exact_rows(const FwdArgs& a, const Tile& t, int kvh,
+                                                     int off, int k0, int k1, int sp, float* scratch) {
+  const int tid = threadIdx.x;
+  float* qs = scratch;             // D
+  float* sc = qs + D;              // 256 scores of a step
+  float* red = sc + 256;           // 4
+  const int n = min(BM, t.rows - t.row0);
+  for (int r = 0; r < n; ++r) {
+    const int row = t.row0 + r, tok = fdiv(row, a.G), h = kvh * a.G.d + row - tok * a.G.d;
+    const T* q = reinterpret_cast<const T*>(a.q + (int64_t)(t.bos + tok) * a.q_ts + (int64_t)h * a.q_hs);
+    __syncthreads();
+    if (tid < D) qs[tid] = to_f32(q[tid]);
+    __syncthreads();
+    const int kend = min(k1, off + tok + 1);
+    float m = NEG_INF, l = 0.f, o = 0.f;
+    for (int j0 = k0; j0 < kend; j0 += 256) {
+      const int j = j0 + tid;
+      float s = NEG_INF;
+      if (j < kend) {
+        const T* kp = key_row<T, PAGED>(a, t, kvh, j, false);
+        if (kp) {
+          s = 0.f;
+          for (int d = 0; d < D; ++d) s += qs[d] * to_f32(kp[d]);
+          s *= a.c;
+        }
+      }
+      float mx = s;
+      for (int x = 32; x >= 1; x >>= 1) mx = fmaxf(mx, shfl_xor(mx, x));
+      if ((tid & 63) == 0) red[tid >> 6] = mx;
+      __syncthreads();
+      const float mn = fmaxf(m, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])));
+      const float ref = mn == NEG_INF ? 0.f : mn;
+      sc[tid] = __builtin_amdgcn_exp2f(s - ref);
+      const float f = __builtin_amdgcn_exp2f(m - ref);
+      l *= f;
+      o *= f;
+      m = mn;
+      __syncthreads();
+      const int lim = min(256, kend - j0);
+      for (int i = 0; i < lim; ++i) {
+        const float p = sc[i];
+        l += p;
+        if (tid < D) {
+          const T* vp = key_row<T, PAGED>(a, t, kvh, j0 + i, true);
+          if (vp) o += p * to_f32(vp[tid]);
+        }
+      }
+      __syncthreads();
+    }
+    if (a.nsplit > 1) {
+      const int64_t at = (int64_t)(t.bos + tok) * a.H + h;
+      if (tid < D) share_row<D>(a, sp, at)[tid] = o;
+      if (tid == 0) {
+        share_stats<D>(a, sp, at)[0] = m;
+        share_stats<D>(a, sp, at)[1] = l;
+      }
+    } else if (tid < D) {
+      T* op = reinterpret_cast<T*>(a.o + (int64_t)(t.bos + tok) * a.o_ts + (int64_t)h * a.o_hs);
+      op[tid] = from_f32<T>(l == 0.f ? 0.f : o / l);
+    }
+  }
+}
+
+template <typename T, int D, bool PAGED>
+__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
+  typedef typename El<T>::v8 v8;
+  constexpr int NC = D / 8;                 // 16-byte chunks of a row
+  constexpr int NL = BN * NC / 256;         // chunks of K, and of V, a thread stages
+  constexpr int NS = D / 16, ND = D / 32;
+  __shared__ __align__(16) T Ks[2][BN * D];
+  __shared__ __align__(16) T Vs[2][BN * D];
+  __shared__ int s_bad, s_skip[2];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, l32 = lane & 31;
+  const int kvh = blockIdx.x % a.HKV;
+  // later tiles of a sequence have more keys: they go first
+  const int slot = a.slots - 1 - (int)(blockIdx.x / a.HKV);
+  const Tile t = find_tile<BM>(a.seqs, slot);
+  if (t.row0 >= t.rows || t.row0 < 0) return;
+
+  const int row = t.row0 + wave * 32 + l32;
+  const int rowc = min(row, t.rows - 1);
+  const int tok = fdiv(rowc, a.G), head = kvh * a.G.d + rowc - tok * a.G.d;
+  char* orow = a.o + (int64_t)(t.bos + tok) * a.o_ts + (int64_t)head * a.o_hs;
+  if (t.seq < 0) {                          // rows of no sequence
+    if (a.fill && row < t.rows) {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) *reinterpret_cast<u32x4*>(orow + 32 * i + 16 * h) = u32x4{0, 0, 0, 0};
+    }
+    return;
+  }
+
+  int keys = t.tokens;
+  if constexpr (PAGED)
+    keys = (int)min((int64_t)max(a.pages.lens[t.seq], 0), (int64_t)a.pages.width * a.pages.page.d);
+  const int off = keys - t.tokens;          // token i attends keys 0 .. off + i
+  const int klast = off + tok;
+  const int wrow = t.row0 + wave * 32;
+  const int w_first = off + fdiv(min(wrow, t.rows - 1), a.G);            // least last key of the wave's rows
+  const int w_last = off + fdiv(min(wrow + 31, t.rows - 1), a.G);        // and greatest
+  const int wg_first = off + fdiv(t.row0, a.G);
+  const int wg_last = off + fdiv(min(t.row0 + BM, t.rows) - 1, a.G);
+  const int nt_all = wg_last < 0 ? 0 : wg_last / BN + 1;
+  const int sp = blockIdx.y;
+  const int j_beg = (int)((int64_t)nt_all * sp / a.nsplit), j_end = (int)((int64_t)nt_all * (sp + 1) / a.nsplit);
+  if (tid == 0) s_bad = s_skip[0] = s_skip[1] = 0;
+
+  v8 qf[NS];
+  {
+    const char* qp = a.q + (int64_t)(t.bos + tok) * a.q_ts + (int64_t)head * a.q_hs + 16 * h;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) qf[s] = *reinterpret_cast<const v8*>(qp + 32 * s);
+  }
+
+  // staging: chunk index tid + 256 i -> row (tid + 256 i) / NC, chunk tid % NC
+  const int srow = tid / NC, sc = tid % NC;
+  constexpr int SR = 256 / NC;              // rows between a thread's chunks
+  u32x4 kr[NL], vr[NL];
+  int pid[NL];
+  bool skip = false;                        // the loaded tile has keys in pages outside the cache
+  auto fetch_pages = [&](int j) {
+    if constexpr (PAGED) {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int r = min(j * BN + srow + i * SR, keys - 1);
+        pid[i] = a.pages.table[t.seq * a.pages.table_stride + fdiv(r, a.pages.page)];
+      }
+    }
+  };
+  auto load_tile = [&](int j) {
+    skip = false;
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int r0 = j * BN + srow + i * SR, r = min(r0, keys - 1);
+      const char *kp, *vp;
+      bool ok = r0 < keys;
+      if constexpr (PAGED) {
+        const int64_t in = r - fdiv(r, a.pages.page) * a.pages.page.d;
+        const bool pg = (unsigned)pid[i] < (unsigned)a.pages.num_pages;
+        const int64_t p = pg ? pid[i] : 0;
+        skip |= ok && !pg;
+        ok = ok && pg;
+        kp = a.pages.k + p * a.pages.k_ps + in * a.pages.k_ts + kvh * a.pages.k_hs;
+        vp = a.pages.v + p * a.pages.v_ps + in * a.pages.v_ts + kvh * a.pages.v_hs;
+      } else {
+        kp = a.k + (int64_t)(t.bos + r) * a.k_ts + (int64_t)kvh * a.k_hs;
+        vp = a.v + (int64_t)(t.bos + r) * a.v_ts + (int64_t)kvh * a.v_hs;
+      }
+      kr[i] = *reinterpret_cast<const u32x4*>(kp + 16 * sc);
+      vr[i] = *reinterpret_cast<const u32x4*>(vp + 16 * sc);
+      if (!ok) vr[i] = u32x4{0, 0, 0, 0};   // no key: its probability is 0, its value must be finite
+    }
+  };
+
+  f32x16 acc[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) acc[i] = f32x16{0};
+  float m = NEG_INF, l = 0.f;               // running maximum of the raw scores (both halves), own half's sum
+
+  // lane offsets into the tiles
+  int ko[NS], vo[ND];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) ko[s] = l32 * D + kpos<D>(l32, 2 * s + h) * 8;
+  {
+    const int s = lane & 15, g = (lane >> 4) & 1;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      const int r = 4 * h + (s >> 2), c = 4 * d + 2 * g + ((s & 3) >> 1);
+      vo[d] = r * D + vpos<D>(r, c) * 8 + 4 * (s & 1);
+    }
+  }
+
+  if (j_beg < j_end) {
+    fetch_pages(j_beg);
+    load_tile(j_beg);
+    if (j_beg + 1 < j_end) fetch_pages(j_beg + 1);
+  }
+  for (int j = j_beg; j < j_end; ++j) {
+    T* Kb = Ks[(j - j_beg) & 1];
+    T* Vb = Vs[(j - j_beg) & 1];
+    const bool edge = (j + 1) * BN > wg_first + 1;   // some row's keys end in the tile
+    bool bad = false;
+    if constexpr (PAGED) {
+      if (skip) s_skip[(j - j_beg) & 1] = j + 1;
+    }
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+      const int r = srow + i * SR;
+      *reinterpret_cast<u32x4*>(Kb + r * D + kpos<D>(r, sc) * 8) = kr[i];
+      *reinterpret_cast<u32x4*>(Vb + r * D + vpos<D>(r, sc) * 8) = vr[i];
+      if (edge) bad |= any_nonfinite<T>(vr[i]);
+    }
+    if (bad) s_bad = 1;
+    __syncthreads();
+    if (j + 1 < j_end) {
+      load_tile(j + 1);
+      if (j + 2 < j_end) fetch_pages(j + 2);
+    }
+    const int t0 = j * BN;
+    if (t0 > w_last) continue;              // every key of the tile lies behind the wave's rows
+
+    f32x16 st[2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      st[kt] = f32x16{0};
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+        st[kt] = El<T>::mma32(*reinterpret_cast<const v8*>(Kb + ko[s] + kt * 32 * D), qf[s], st[kt]);
+    }
+    if (t0 + BN - 1 > w_first) {
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = t0 + kt * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
+          if (key > klast) st[kt][i] = NEG_INF;
+        }
+    }
+    if constexpr (PAGED) {
+      if (s_skip[(j - j_beg) & 1] == j + 1) {   // pages outside the cache hold no keys
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int key = t0 + kt * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
+            if (key <= klast && !key_row<T, true>(a, t, kvh, key, false)) st[kt][i] = NEG_INF;
+          }
+      }
+    }
+    float mx = st[0][0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, st[0][i]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[1][i]);
+    mx = half_max(mx);
+    // The reference maximum follows the running one only where it lags by more than 2^8:
+    // P then stays below 2^8, inside either type, and O is seldom rescaled.
+    if (__any((mx - m) * a.c > 8.f)) {
+      const float mn = fmaxf(m, mx);
+      const float f = m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((m - mn) * a.c);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) acc[d] *= f;
+    }
+    const float mc = m == NEG_INF ? 0.f : m * a.c;
+    v8 pf[4];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      float p[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(st[kt][i] * a.c - mc);
+        l += p[i];
+      }
+      pf[2 * kt] = pack8<T>(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
+      pf[2 * kt + 1] = pack8<T>(p[8], p[9], p[10], p[11], p[12], p[13], p[14], p[15]);
+    }
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const v8 vf = join<T>(tr4<T>(Vb + vo[d] + ks * 16 * D), tr4<T>(Vb + vo[d] + (ks * 16 + 8) * D));
+        acc[d] = El<T>::mma32(vf, pf[ks], acc[d]);
+      }
+  }
+  l = pair_sum32(l, l);
+
+  if (a.nsplit > 1) {
+    const int64_t r = (int64_t)(t.bos + tok) * a.H + head;
+    if (row < t.rows) {
+      float* pp = share_row<D>(a, sp, r) + 4 * h;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<f32x4*>(pp + 32 * d + 8 * i) =
+              f32x4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+      if (h == 0) {
+        share_stats<D>(a, sp, r)[0] = m * a.c;
+        share_stats<D>(a, sp, r)[1] = l;
+      }
+    }
+  } else if (row < t.rows) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        typename El<T>::v4 x;
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) x[jj] = (T)(acc[d][4 * i + jj] * inv);
+        *reinterpret_cast<typename El<T>::v4*>(orow + (32 * d + 8 * i + 4 * h) * 2) = x;
+      }
+    if (a.lse && h == 0)
+      a.lse[(int64_t)(t.bos + tok) * a.H + head] = m * a.c + __builtin_amdgcn_logf(l);
+  }
+  __syncthreads();
+  if (s_bad)
+    exact_rows<T, D, PAGED>(a, t, kvh, off, j_beg * BN, j_end * BN, sp, reinterpret_cast<float*>(&Ks[0][0]));
+}
+
+// The splits' shares of a row joined: sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_join_kernel(FwdArgs a) {
+  constexpr int TPR = D / 4;
+  const int kvh = blockIdx.x % a.HKV;
+  const Tile t = find_tile<BM>(a.seqs, blockIdx.x / a.HKV);
+  if (t.seq < 0 || t.row0 < 0 || t.row0 >= t.rows) return;
+  const int n = min(BM, t.rows - t.row0), d = 4 * (threadIdx.x % TPR);
+  for (int r = threadIdx.x / TPR; r < n; r += 256 / TPR) {
+    const int row = t.row0 + r, tok = fdiv(row, a.G), h = kvh * a.G.d + row - tok * a.G.d;
+    const int64_t at = (int64_t)(t.bos + tok) * a.H + h;
+    float m = NEG_INF, l = 0.f;
+    for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, share_stats<D>(a, s, at)[0]);
+    const float ref = m == NEG_INF ? 0.f : m;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.nsplit; ++s) {
+      const float* st = share_stats<D>(a, s, at);
+      const float f = __builtin_amdgcn_exp2f(st[0] - ref);
+      l += f * st[1];
+      o += f * *reinterpret_cast<const f32x4*>(share_row<D>(a, s, at) + d);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    typename El<T>::v4 x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = (T)(o[i] * inv);
+    *reinterpret_cast<typename El<T>::v4*>(a.o + (int64_t)(t.bos + tok) * a.o_ts + (int64_t)h * a.o_hs +
+                                           2 * d) = x;
+  }
+}
+
+// Splits of the keys: where the row tiles alone leave compute units idle, as many as give
+// each about two workgroups, of at least four tiles of keys (a split costs its share's
+// trip through memory and the joining launch).
+static int splits(int64_t slots, int64_t N, int HKV, int64_t max_keys, bool packed) {
+  const int64_t live = (packed ? slots - 2 : slots) * HKV, want = 2ll * cu_count();
+  int64_t s = live > 0 ? want / live : 1;
+  const int64_t most = max_keys / (4 * BN);
+  if (s > most) s = most;
+  if (s > 64) s = 64;
+  return s < 1 ? 1 : (int)s;
+}
+
+template <typename T, bool PAGED>
+static void launch_fwd(const FwdArgs& a, int D, hipStream_t s) {
+  const dim3 grid((unsigned)(a.slots * a.HKV), (unsigned)a.nsplit);
+  if (D == 64) hipLaunchKernelGGL((attn_fwd_kernel<T, 64, PAGED>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((attn_fwd_kernel<T, 128, PAGED>), grid, dim3(256), 0, s, a);
+  if (a.nsplit > 1) {
+    if (D == 64) hipLaunchKernelGGL((attn_join_kernel<T, 64>), dim3(grid.x), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attn_join_kernel<T, 128>), dim3(grid.x), dim3(256), 0, s, a);
+  }
+}
+
+}  // namespace attn
+}  // namespace hmx
+
+using namespace hmx;
+
+#define ATTN_COMMON_CHECKS(what)                                                                    HMX_REQUIRE(D == 64 || D == 128, HMX_EUNSUPPORTED, what ": head size %d not in {64, 128}", D);    HMX_REQUIRE(dtype == HMX_BF16 || dtype == HMX_F16, HMX_EUNSUPPORTED,                                          what ": dtype code %d (bf16 or fp16)", dtype);                                        HMX_REQUIRE(N >= 0 && T >= 0 && HKV > 0 && H > 0 && H % HKV == 0, HMX_EINVAL,                                 what ": N=%d T=%lld H=%d HKV=%d", N, (long long)T, H, HKV);                           HMX_REQUIRE(T * (H / HKV) < (1ll << 31) - 256, HMX_EUNSUPPORTED, what ": %lld tokens", (long long)T);   HMX_REQUIRE(scale > 0.f && scale < __builtin_inff(), HMX_EINVAL, what ": scale %g must be positive", (double)scale);
+
+extern "C" int hmx_causal_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                    const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                                    const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                                    int32_t dtype, void* o, int64_t o_token_stride,
+                                    int64_t o_head_stride, float* lse, const int32_t* cu_seqlens,
+                                    int32_t N, int64_t T, int32_t H, int32_t HKV, int32_t D,
+                                    float scale, int32_t fill_gaps, void* stream) {
+  ATTN_COMMON_CHECKS("hmx_causal_attention")
+  HMX_REQUIRE(cu_seqlens || N == 0 || T % N == 0, HMX_EINVAL, "hmx_causal_attention: T=%lld is not N=%d sequences",
+              (long long)T, N);
+  if (T == 0 || (N == 0 && !cu_seqlens)) return HMX_OK;
+  HMX_REQUIRE(q && k && v && o, HMX_EINVAL, "hmx_causal_attention: null pointer");
+  const int64_t st = q_token_stride | q_head_stride | k_token_stride | k_head_stride | v_token_stride |
+                     v_head_stride | o_token_stride | o_head_stride;
+  const uintptr_t al = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o;
+  HMX_REQUIRE(st % 8 == 0 && al % 16 == 0, HMX_EINVAL,
+              "hmx_causal_attention: strides must be multiples of 8 elements and pointers 16-byte aligned");
+  attn::FwdArgs a{};
+  a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v; a.o = (char*)o;
+  a.q_ts = 2 * q_token_stride; a.q_hs = 2 * q_head_stride;
+  a.k_ts = 2 * k_token_stride; a.k_hs = 2 * k_head_stride;
+  a.v_ts = 2 * v_token_stride; a.v_hs = 2 * v_head_stride;
+  a.o_ts = 2 * o_token_stride; a.o_hs = 2 * o_head_stride;
+  a.lse = lse;
+  a.seqs = attn::Seqs{cu_seqlens, N, (int32_t)T, H / HKV};
+  a.G = attn::fast_div(H / HKV);
+  const int64_t slots = attn::tile_slots<attn::BM>(cu_seqlens, N, T, H / HKV);
+  HMX_REQUIRE(slots * HKV < (1ll << 31), HMX_EUNSUPPORTED, "hmx_causal_attention: %lld tiles", (long long)slots);
+  a.H = H; a.HKV = HKV; a.slots = (int32_t)slots; a.fill = fill_gaps; a.nsplit = 1;
+  a.c = scale * attn::LOG2E;
+  if (dtype == HMX_BF16) attn::launch_fwd<bf16, false>(a, D, (hipStream_t)stream);
+  else attn::launch_fwd<f16, false>(a, D, (hipStream_t)stream);
+  return check_launch("hmx_causal_attention");
+}
+
+static int paged_splits(int64_t N, int64_t T, int H, int HKV, int64_t max_keys) {
+  const int32_t packed = 0;
+  return attn::splits(attn::tile_slots<attn::BM>(&packed, N, T, H / HKV), N, HKV, max_keys, true);
+}
+
+extern "C" size_t hmx_paged_causal_attention_workspace_bytes(int32_t N, int64_t T, int32_t H,
+                                                             int32_t HKV, int32_t D,
+                                                             int64_t max_keys) {
+  if (N <= 0 || T <= 0 || HKV <= 0 || H <= 0 || H % HKV != 0) return 0;
+  const int ns = paged_splits(N, T, H, HKV, max_keys);
+  return ns == 1 ? 0 : (size_t)ns * T * H * (D + 2) * sizeof(float);
+}
+
+extern "C" int hmx_paged_causal_attention(const void* q, int64_t q_token_stride,
+                                          int64_t q_head_stride, int32_t dtype, void* o,
+                                          int64_t o_token_stride, int64_t o_head_stride,
+                                          const hmx_paged_kv* cache, const int32_t* cu_seqlens,
+                                          int32_t N, int64_t T, int32_t H, int32_t HKV, int32_t D,
+                                          float scale, int32_t fill_gaps, void* workspace,
+                                          size_t workspace_bytes, void* stream) {
+  ATTN_COMMON_CHECKS("hmx_paged_causal_attention")
+  HMX_REQUIRE(cache && cache->num_pages >= 0 && cache->page_size > 0 && cache->table_width >= 0, HMX_EINVAL,
+              "hmx_paged_causal_attention: cache");
+  if (T == 0) return HMX_OK;
+  HMX_REQUIRE(q && o && cu_seqlens && (N == 0 || (cache->seq_lens && cache->table && cache->k && cache->v)),
+              HMX_EINVAL, "hmx_paged_causal_attention: null pointer");
+  const int64_t max_keys = (int64_t)cache->table_width * cache->page_size;
+  HMX_REQUIRE(max_keys < (1ll << 31) - 256, HMX_EUNSUPPORTED,
+              "hmx_paged_causal_attention: a table row holds %lld keys", (long long)max_keys);
+  const int64_t st = q_token_stride | q_head_stride | o_token_stride | o_head_stride |
+                     cache->k_page_stride | cache->k_token_stride | cache->k_head_stride |
+                     cache->v_page_stride | cache->v_token_stride | cache->v_head_stride;
+  const uintptr_t al = (uintptr_t)q | (uintptr_t)o | (uintptr_t)cache->k | (uintptr_t)cache->v;
+  HMX_REQUIRE(st % 8 == 0 && al % 16 == 0, HMX_EINVAL,
+              "hmx_paged_causal_attention: strides must be multiples of 8 elements and pointers 16-byte aligned");
+  attn::FwdArgs a{};
+  a.q = (const char*)q; a.o = (char*)o;
+  a.q_ts = 2 * q_token_stride; a.q_hs = 2 * q_head_stride;
+  a.o_ts = 2 * o_token_stride; a.o_hs = 2 * o_head_stride;
+  a.seqs = attn::Seqs{cu_seqlens, N, (int32_t)T, H / HKV};
+  a.G = attn::fast_div(H / HKV);
+  a.pages = attn::make_pages(*cache);
+  const int64_t slots = attn::tile_slots<attn::BM>(cu_seqlens, N, T, H / HKV);
+  HMX_REQUIRE(slots * HKV < (1ll << 31), HMX_EUNSUPPORTED, "hmx_paged_causal_attention: %lld tiles",
+              (long long)slots);
+  a.H = H; a.HKV = HKV; a.slots = (int32_t)slots; a.fill = fill_gaps;
+  a.nsplit = N == 0 ? 1 : paged_splits(N, T, H, HKV, max_keys);
+  a.part = static_cast<float*>(workspace);
+  HMX_REQUIRE(a.nsplit == 1 ||
+                  (workspace && (uintptr_t)workspace % 16 == 0 &&
+                   workspace_bytes >= hmx_paged_causal_attention_workspace_bytes(N, T, H, HKV, D, max_keys)),
+              HMX_EINVAL, "hmx_paged_causal_attention: workspace of %zu bytes is too small", workspace_bytes);
+  a.c = scale * attn::LOG2E;
+  if (dtype == HMX_BF16) attn::launch_fwd<bf16, true>(a, D, (hipStream_t)stream);
+  else attn::launch_fwd<f16, true>(a, D, (hipStream_t)stream);
+  return check_launch("hmx_paged_causal_attention");
+}

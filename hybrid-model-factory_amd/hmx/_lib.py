@@ -113,6 +113,17 @@ SIGNATURES: dict[str, list] = {
                              _P, _I64, _I64, _P, _I64, _I64,
                              _P, _I32, _I64, _I64, _I64, _P, _I32, _I64, _I64, _I64,
                              _P, _P, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _P],
+    "hmx_append_paged_kv": [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _I64, _I64,
+                            _P, _P, _I32, _P, _I32, _P, _I32, _I64, _I64, _I32, _I32, _I64, _I32,
+                            _I32, _I32, _P],
+    "hmx_paged_attention_decode": [_P, _I64, _I64, _I32, _P, _I64, _I64, _P, _I32, _I32, _I32,
+                                   _I32, _F32, _P, ctypes.c_size_t, _P],
+    "hmx_paged_attention_decode_workspace_bytes": [_I32, _I32, _I32, _I32, _I64],
+    "hmx_causal_attention": [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _I64, _I64,
+                             _P, _P, _I32, _I64, _I32, _I32, _I32, _F32, _I32, _P],
+    "hmx_paged_causal_attention": [_P, _I64, _I64, _I32, _P, _I64, _I64, _P, _P, _I32, _I64, _I32,
+                                   _I32, _I32, _F32, _I32, _P, ctypes.c_size_t, _P],
+    "hmx_paged_causal_attention_workspace_bytes": [_I32, _I64, _I32, _I32, _I32, _I64],
 }
 _RESTYPES = {"hmx_last_error": ctypes.c_char_p, "hmx_gdn_chunk_workspace_bytes": ctypes.c_size_t,
              "hmx_gka_chunk_workspace_bytes": ctypes.c_size_t,
@@ -120,7 +131,9 @@ _RESTYPES = {"hmx_last_error": ctypes.c_char_p, "hmx_gdn_chunk_workspace_bytes":
              "hmx_gka_train_bwd_workspace_bytes": ctypes.c_size_t,
              "hmx_gdn_train_bwd_workspace_bytes": ctypes.c_size_t,
              "hmx_ssd_chunk_workspace_bytes": ctypes.c_size_t,
-             "hmx_ssd_chunk_bwd_workspace_bytes": ctypes.c_size_t}
+             "hmx_ssd_chunk_bwd_workspace_bytes": ctypes.c_size_t,
+             "hmx_paged_attention_decode_workspace_bytes": ctypes.c_size_t,
+             "hmx_paged_causal_attention_workspace_bytes": ctypes.c_size_t}
 
 
 
@@ -175,6 +188,27 @@ def gate_proj(pg):
                  int(bool(pg.gk_from_g)))
     s._keep = (pg.A_log, pg.dt_bias, *ts)
     return ctypes.pointer(s)
+
+
+class PagedKV(ctypes.Structure):
+    """hmx_paged_kv (include/hmx.h): a paged key/value cache and its sequences."""
+    _fields_ = [("k", _P), ("k_page_stride", _I64), ("k_token_stride", _I64),
+                ("k_head_stride", _I64), ("v", _P), ("v_page_stride", _I64),
+                ("v_token_stride", _I64), ("v_head_stride", _I64), ("table", _P),
+                ("table_stride", _I64), ("seq_lens", _P), ("table_width", _I32),
+                ("num_pages", _I32), ("page_size", _I32)]
+
+
+def paged_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor | None = None,
+             seq_lens: torch.Tensor | None = None):
+    """ctypes pointer to an hmx_paged_kv of caches [pages, page size, HKV, D]; strides of
+    dimensions of one, which are never used and may be anything, go as 0."""
+    n = k_cache.shape
+    ks, vs = ([s if m > 1 else 0 for s, m in zip(t.stride()[:3], n)] for t in (k_cache, v_cache))
+    return ctypes.pointer(PagedKV(
+        k_cache.data_ptr(), *ks, v_cache.data_ptr(), *vs, ptr(table),
+        0 if table is None else table.stride(0), ptr(seq_lens),
+        0 if table is None else table.shape[1], n[0], n[1]))
 
 
 _lib = None

@@ -3,6 +3,8 @@ from .gdn import (chunk_gated_delta_rule, chunk_gated_delta_rule_gqa, fused_gdn_
                   fused_recurrent_gated_delta_rule, fused_recurrent_gated_delta_rule_gqa)
 from .gka import (chebyshev_iteration_gqa, fused_gka_gating, gka_chebyshev_gla,
                   gka_chebyshev_gla_decode, gka_chebyshev_gla_prefill, torch_decoding_one_step)
+from .attention import (append_paged_kv, causal_attention, paged_attention_decode,
+                        paged_causal_attention)
 from .conv import causal_conv1d_fn, causal_conv1d_update
 from .gates import ProjGates
 from .gdn_train import ChunkGatedDeltaRule
@@ -36,4 +38,8 @@ __all__ = [
     "rms_norm_gated",
     "causal_conv1d_fn",
     "causal_conv1d_update",
+    "causal_attention",
+    "append_paged_kv",
+    "paged_attention_decode",
+    "paged_causal_attention",
 ]

@@ -47,7 +47,9 @@ extern "C" {
                               12: hmx_causal_conv1d_fwd_blocks and
                                   hmx_causal_conv1d_update_blocks (prefix-cache block
                                   arguments);
-                              13: hmx_ssd_chunk_bwd (the SSD scan's backward) */
+                              13: hmx_ssd_chunk_bwd (the SSD scan's backward); the
+                                  attention entry points were added to 13, which
+                                  changed nothing before them */
 
 enum hmx_status {
   HMX_OK = 0,
@@ -798,6 +800,94 @@ int hmx_causal_conv1d_update_blocks(const void* x, int64_t x_token_stride, void*
                                     const int32_t* block_idx_last_scheduled_token, int32_t batch,
                                     int32_t dim, int32_t activation, int32_t pad_slot_id,
                                     void* stream);
+
+/* ---------------------------------------------------------------- attention layers */
+
+/*
+ * A paged key/value cache: k and v [num_pages, page_size, HKV, D] each with its own page,
+ * token and head strides (multiples of 8 elements, 16-byte aligned bases, D contiguous).
+ * Sequence n's key j sits in page table[n * table_stride + j / page_size] at place
+ * j % page_size; seq_lens[n] keys (values past table_width * page_size count as that).
+ * table and seq_lens are device pointers, read by the kernels only; a page outside
+ * 0 .. num_pages - 1 holds no keys.  The struct itself is a host pointer, read during the
+ * call.
+ */
+typedef struct hmx_paged_kv {
+  void* k;
+  int64_t k_page_stride, k_token_stride, k_head_stride;
+  void* v;
+  int64_t v_page_stride, v_token_stride, v_head_stride;
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* seq_lens;
+  int32_t table_width, num_pages, page_size;
+} hmx_paged_kv;
+
+/*
+ * Keys and values of new tokens into a paged cache, k (and q) rotated by their positions.
+ *  k, v [tokens, HKV, D], q [tokens, H, D] or NULL, q_out as q (may be q); bf16 or fp16,
+ *  D 64 or 128; token and head strides multiples of 8, pointers 16-byte aligned.
+ *  slots [tokens] (int64, or int32 where slots_int64 is 0): page * page_size + place;
+ *  outside the cache: padding, nothing stored.
+ *  cos_sin [max_position, rotary_dim] in any of the three types, rows cos_sin_stride apart
+ *  (a multiple of 8): rotary_dim / 2 cosines, then sines; rotary_dim a multiple of 16,
+ *  0 = no rotation.  Pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) with interleaved.
+ *  positions [tokens]; outside the table: NaN.
+ * No counterpart in the reference, whose attention layers are vLLM's own.
+ */
+int hmx_append_paged_kv(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                        const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                        const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                        int32_t dtype, void* q_out, int64_t q_out_token_stride,
+                        int64_t q_out_head_stride, const hmx_paged_kv* cache, const void* slots,
+                        int32_t slots_int64, const void* positions, int32_t positions_int64,
+                        const void* cos_sin, int32_t cos_sin_dtype, int64_t cos_sin_stride,
+                        int64_t max_position, int32_t rotary_dim, int32_t interleaved,
+                        int64_t tokens, int32_t H, int32_t HKV, int32_t D, void* stream);
+
+/*
+ * Attention of one new token a sequence: o[n] = softmax(scale q[n] . k_j) v_j over the
+ * seq_lens[n] keys of sequence n (0 keys: 0).  q, o [N, H, D]; H / HKV heads share keys;
+ * scale > 0.  workspace: hmx_paged_attention_decode_workspace_bytes bytes (16-byte
+ * aligned; 0: none needed) of scratch that no other call in flight uses; max_keys =
+ * table_width * page_size.
+ */
+size_t hmx_paged_attention_decode_workspace_bytes(int32_t N, int32_t H, int32_t HKV, int32_t D,
+                                                  int64_t max_keys);
+int hmx_paged_attention_decode(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                               int32_t dtype, void* o, int64_t o_token_stride,
+                               int64_t o_head_stride, const hmx_paged_kv* cache, int32_t N,
+                               int32_t H, int32_t HKV, int32_t D, float scale, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
+/*
+ * Causal attention over whole sequences: q, o [T, H, D], k, v [T, HKV, D]; N sequences at
+ * the device offsets cu_seqlens [N + 1] (clamped into 0 .. T), or of T / N tokens each
+ * where cu_seqlens is NULL.  lse: NULL, or fp32 [T, H], the base-2 logarithm of
+ * sum_j 2^(log2(e) scale q . k_j), as hmx_causal_attention_bwd takes it.  fill_gaps: rows
+ * of no sequence become 0 (else they are left as they were).
+ */
+int hmx_causal_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                         const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                         const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                         int32_t dtype, void* o, int64_t o_token_stride, int64_t o_head_stride,
+                         float* lse, const int32_t* cu_seqlens, int32_t N, int64_t T, int32_t H,
+                         int32_t HKV, int32_t D, float scale, int32_t fill_gaps, void* stream);
+
+/*
+ * Causal attention of new tokens over a paged cache that holds them and their context:
+ * token i of sequence n's cu_seqlens[n + 1] - cu_seqlens[n] new ones attends keys
+ * 0 .. seq_lens[n] - tokens + i (none: 0).  q, o [T, H, D]; cu_seqlens on the device, the
+ * first need not be 0.  Workspace as for the decode.
+ */
+size_t hmx_paged_causal_attention_workspace_bytes(int32_t N, int64_t T, int32_t H, int32_t HKV,
+                                                  int32_t D, int64_t max_keys);
+int hmx_paged_causal_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                               int32_t dtype, void* o, int64_t o_token_stride,
+                               int64_t o_head_stride, const hmx_paged_kv* cache,
+                               const int32_t* cu_seqlens, int32_t N, int64_t T, int32_t H,
+                               int32_t HKV, int32_t D, float scale, int32_t fill_gaps,
+                               void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
