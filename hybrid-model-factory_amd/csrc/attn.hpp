@@ -47,6 +47,25 @@ __device__ __forceinline__ typename El<T>::v8 join(typename El<T>::v4 a, typenam
   return typename El<T>::v8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
 }
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// The 16-byte chunk at which chunk c of row r of a tile sits in LDS.  Rows are read 16 at
+// a time at one chunk (row fragments) and four at a time over four chunks (the transposing
+// reads): the low two bits of the row choose among the groups of four chunks, the next
+// bits the place within, so both kinds of read are spread over all banks.
+template <int D> __device__ __forceinline__ int swz(int r, int c) {
+  return D == 128 ? c ^ (((r & 3) << 2) | ((r >> 2) & 3))
+                  : c ^ ((((r >> 1) & 1) << 2) | ((r >> 2) & 3));
+}
+
+// The element offset, in a tile at a multiple of 16 rows, at which a lane's transposing
+// reads of 32 columns (chunks 4 d .. 4 d + 3) and rows 4 h .. 4 h + 3 start; with `up` 8 rows
+// on, where the swizzle's second bit is the other one.
+template <int D> __device__ __forceinline__ int tr_offset(int lane, int d, bool up) {
+  const int s = lane & 15, g = (lane >> 4) & 1, r = 4 * (lane >> 5) + (s >> 2) + (up ? 8 : 0);
+  return r * D + swz<D>(r, 4 * d + 2 * g + ((s & 3) >> 1)) * 8 + 4 * (s & 1);
+}
+
 // max and sum over the two halves of a wave, in the VALU
 __device__ __forceinline__ float half_max(float a) {
   const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, a),

@@ -19,7 +19,6 @@ namespace hmx {
 namespace attn {
 
 constexpr int BM = 128, BN = 64;
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 struct FwdArgs {
   const char *q, *k, *v;
@@ -33,15 +32,6 @@ struct FwdArgs {
   float c;             // scale log2(e)
   float* part;         // [nsplit][T * H][D], then [nsplit][T * H][2]: maximum and sum
 };
-
-// the 16-byte chunk at which chunk c of key row r sits in LDS: rows of K are read 32 at a
-// time at one chunk, rows of V four at a time over 64 bytes, each without bank conflicts
-template <int D> __device__ __forceinline__ int kpos(int r, int c) {
-  return D == 128 ? c ^ (r & 15) : c ^ ((r >> 1) & 7);
-}
-template <int D> __device__ __forceinline__ int vpos(int r, int c) {
-  return D == 128 ? c ^ ((r & 3) << 2) : c ^ (((r >> 1) & 1) << 2);
-}
 
 // whether any of the eight 16-bit values is infinite or NaN
 template <typename T>
@@ -243,16 +233,13 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
   float m = NEG_INF, l = 0.f;               // running maximum of the raw scores (both halves), own half's sum
 
   // lane offsets into the tiles
-  int ko[NS], vo[ND];
+  int ko[NS], vo[ND], vu[ND];
 #pragma unroll
-  for (int s = 0; s < NS; ++s) ko[s] = l32 * D + kpos<D>(l32, 2 * s + h) * 8;
-  {
-    const int s = lane & 15, g = (lane >> 4) & 1;
+  for (int s = 0; s < NS; ++s) ko[s] = l32 * D + swz<D>(l32, 2 * s + h) * 8;
 #pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      const int r = 4 * h + (s >> 2), c = 4 * d + 2 * g + ((s & 3) >> 1);
-      vo[d] = r * D + vpos<D>(r, c) * 8 + 4 * (s & 1);
-    }
+  for (int d = 0; d < ND; ++d) {
+    vo[d] = tr_offset<D>(lane, d, false);
+    vu[d] = tr_offset<D>(lane, d, true);
   }
 
   if (j_beg < j_end) {
@@ -271,8 +258,8 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
       const int r = srow + i * SR;
-      *reinterpret_cast<u32x4*>(Kb + r * D + kpos<D>(r, sc) * 8) = kr[i];
-      *reinterpret_cast<u32x4*>(Vb + r * D + vpos<D>(r, sc) * 8) = vr[i];
+      *reinterpret_cast<u32x4*>(Kb + r * D + swz<D>(r, sc) * 8) = kr[i];
+      *reinterpret_cast<u32x4*>(Vb + r * D + swz<D>(r, sc) * 8) = vr[i];
       if (edge) bad |= any_nonfinite<T>(vr[i]);
     }
     if (bad) s_bad = 1;
@@ -345,7 +332,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
     for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        const v8 vf = join<T>(tr4<T>(Vb + vo[d] + ks * 16 * D), tr4<T>(Vb + vo[d] + (ks * 16 + 8) * D));
+        const v8 vf = join<T>(tr4<T>(Vb + vo[d] + ks * 16 * D), tr4<T>(Vb + vu[d] + ks * 16 * D));
         acc[d] = El<T>::mma32(vf, pf[ks], acc[d]);
       }
   }

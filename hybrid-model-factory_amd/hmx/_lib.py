@@ -121,6 +121,9 @@ SIGNATURES: dict[str, list] = {
     "hmx_paged_attention_decode_workspace_bytes": [_I32, _I32, _I32, _I32, _I64],
     "hmx_causal_attention": [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _I64, _I64,
                              _P, _P, _I32, _I64, _I32, _I32, _I32, _F32, _I32, _P],
+    "hmx_causal_attention_bwd": [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _I64,
+                                 _I64, _P, _I64, _I64, _P, _P, _I32, _I64, _I32, _I32, _I32, _F32,
+                                 _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P],
     "hmx_paged_causal_attention": [_P, _I64, _I64, _I32, _P, _I64, _I64, _P, _P, _I32, _I64, _I32,
                                    _I32, _I32, _F32, _I32, _P, ctypes.c_size_t, _P],
     "hmx_paged_causal_attention_workspace_bytes": [_I32, _I64, _I32, _I32, _I32, _I64],

@@ -5,6 +5,7 @@ from .gka import (chebyshev_iteration_gqa, fused_gka_gating, gka_chebyshev_gla,
                   gka_chebyshev_gla_decode, gka_chebyshev_gla_prefill, torch_decoding_one_step)
 from .attention import (append_paged_kv, causal_attention, paged_attention_decode,
                         paged_causal_attention)
+from .attention_train import CausalAttention
 from .conv import causal_conv1d_fn, causal_conv1d_update
 from .gates import ProjGates
 from .gdn_train import ChunkGatedDeltaRule
@@ -39,6 +40,7 @@ __all__ = [
     "causal_conv1d_fn",
     "causal_conv1d_update",
     "causal_attention",
+    "CausalAttention",
     "append_paged_kv",
     "paged_attention_decode",
     "paged_causal_attention",

@@ -875,6 +875,24 @@ int hmx_causal_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
                          int32_t HKV, int32_t D, float scale, int32_t fill_gaps, void* stream);
 
 /*
+ * The backward of hmx_causal_attention (bf16): dq [T, H, D], dk, dv [T, HKV, D] from the
+ * inputs, the output o, its gradient dout and the forward's lse; k's and v's summed over
+ * the heads that share them, all sums in a fixed order.  Rows of no sequence become 0.
+ * delta: fp32 scratch [T, H].
+ */
+int hmx_causal_attention_bwd(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                             const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                             const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                             int32_t dtype, const void* o, int64_t o_token_stride,
+                             int64_t o_head_stride, const void* dout, int64_t do_token_stride,
+                             int64_t do_head_stride, const float* lse, const int32_t* cu_seqlens,
+                             int32_t N, int64_t T, int32_t H, int32_t HKV, int32_t D, float scale,
+                             void* dq, int64_t dq_token_stride, int64_t dq_head_stride, void* dk,
+                             int64_t dk_token_stride, int64_t dk_head_stride, void* dv,
+                             int64_t dv_token_stride, int64_t dv_head_stride, float* delta,
+                             void* stream);
+
+/*
  * Causal attention of new tokens over a paged cache that holds them and their context:
  * token i of sequence n's cu_seqlens[n + 1] - cu_seqlens[n] new ones attends keys
  * 0 .. seq_lens[n] - tokens + i (none: 0).  q, o [T, H, D]; cu_seqlens on the device, the

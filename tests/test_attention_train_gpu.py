@@ -1,0 +1,114 @@
+"""The backward of causal attention on the GPU against the float64 formulas and differences.
+
+Elementwise tolerances: dS is rounded to bf16 (half a step of itself), the row term dO . O
+sees O rounded and formed from rounded probabilities (two half steps of sum |dO| p |v|),
+and fp32 scores leave 2^-11 of each term's magnitude (2^-12 in P, and in the sum that
+normalises it); the sums of magnitudes come from the oracle.  The gradient is rounded once
+more.  The norm-wise bound is the one of the other ops' outputs."""
+import pytest
+import torch
+
+import hmx
+from attn_util import bounds_of, half_step, randn, ref
+from util import OUT_REL, rel_err
+
+pytestmark = pytest.mark.gpu
+BF = torch.bfloat16
+
+
+def _check(grads, want, mags, what):
+    e = half_step(BF)
+    for name, g, w, m, n in zip("qkv", grads, want, mags, (3, 3, 1)):
+        assert torch.isfinite(g).all(), f"{what} d{name}: non-finite"
+        t = (n * e + 2.0 ** -11) * m
+        tol = t + e * (w.abs() + t) + 1e-30
+        worst = ((g.double().cpu() - w).abs() - tol).max().item()
+        assert worst <= 0, f"{what} d{name}: {worst:.3e} past its tolerance"
+        assert rel_err(g, w) <= OUT_REL, f"{what} d{name}: {rel_err(g, w):.3e}"
+
+
+def _inputs(seed, B, T, H, HKV, D):
+    gen = torch.Generator().manual_seed(seed)
+    return [randn(gen, B, T, n, D) for n in (H, HKV, HKV, H)]
+
+
+@pytest.mark.parametrize("T,H,HKV,D", [
+    (1, 2, 1, 128), (2, 4, 4, 64), (31, 6, 2, 64), (33, 8, 1, 128), (64, 2, 2, 128), (65, 3, 3, 64),
+    (129, 7, 1, 128), (257, 4, 2, 128), (300, 8, 2, 64), (640, 2, 1, 128),
+])
+def test_grads_one_sequence(dev, T, H, HKV, D):
+    q, k, v, do = _inputs(T, 1, T, H, HKV, D)
+    ins = [x.to(dev).requires_grad_() for x in (q, k, v)]
+    o = hmx.causal_attention(*ins)
+    grads = torch.autograd.grad(o, ins, do.to(dev))
+    (_, *want), mags = ref.causal_grads(q[0], k[0], v[0], D ** -0.5, [(0, T)], do[0])
+    _check([g[0] for g in grads], want, mags, f"T={T}")
+    assert torch.equal(o.detach(), hmx.causal_attention(*[x.detach() for x in ins]))
+
+
+@pytest.mark.parametrize("cu", [[0, 5, 5, 70, 200], [3, 4, 5, 130], [0, 128, 200], [0, 0, 190],
+                                [0, *range(1, 71), 200]])
+def test_grads_packed(dev, cu):
+    T, H, HKV, D = 200, 6, 2, 64
+    q, k, v, do = _inputs(len(cu), 1, T, H, HKV, D)
+    ins = [x.to(dev).requires_grad_() for x in (q, k, v)]
+    o = hmx.causal_attention(*ins, cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=dev))
+    grads = torch.autograd.grad(o, ins, do.to(dev))
+    (_, *want), mags = ref.causal_grads(q[0], k[0], v[0], D ** -0.5, bounds_of(cu), do[0])
+    _check([g[0] for g in grads], want, mags, str(cu))
+    for g in grads:
+        assert (g[0, :cu[0]] == 0).all() and (g[0, cu[-1]:] == 0).all()
+
+
+def test_grads_batch_scale_strides_and_repeat(dev):
+    """A batch of slices of one projection, an expanded output gradient, and the same bits
+    on a second run."""
+    B, T, H, HKV, D = 3, 90, 4, 2, 128
+    gen = torch.Generator().manual_seed(0)
+    qkv = randn(gen, B, T, (H + 2 * HKV) * D)
+    x = qkv.to(dev).requires_grad_()
+    runs = []
+    for _ in range(2):
+        q, k, v = (y.view(B, T, -1, D) for y in x.split([H * D, HKV * D, HKV * D], -1))
+        o = hmx.causal_attention(q, k, v, 0.1)
+        runs.append(torch.autograd.grad(o.sum(), x)[0])
+    assert torch.equal(*runs)
+    got = runs[0].view(B, T, -1, D).split([H, HKV, HKV], 2)
+    for b in range(B):
+        q, k, v = (y.view(T, -1, D) for y in qkv[b].split([H * D, HKV * D, HKV * D], -1))
+        (_, *want), mags = ref.causal_grads(q, k, v, 0.1, [(0, T)], torch.ones(T, H, D))
+        _check([g[b] for g in got], want, mags, f"b={b}")
+
+
+def test_gradient_against_differences(dev):
+    """<gradient, direction> against the central difference of the float64 forward: the
+    gradient's rounding (half a step of each product's magnitude, and 3 more as above) is
+    what separates them."""
+    T, H, HKV, D = 70, 4, 2, 64
+    q, k, v, do = _inputs(11, 1, T, H, HKV, D)
+    ins = [x.to(dev).requires_grad_() for x in (q, k, v)]
+    grads = torch.autograd.grad(hmx.causal_attention(*ins), ins, do.to(dev))
+    _, mags = ref.causal_grads(q[0], k[0], v[0], D ** -0.5, [(0, T)], do[0])
+    gen = torch.Generator().manual_seed(12)
+    base = [x[0].double() for x in (q, k, v)]
+    loss = lambda xs: (ref.causal(*xs, D ** -0.5, [(0, T)])[0] * do[0].double()).sum().item()
+    for i in range(3):
+        u = torch.randn(base[i].shape, generator=gen, dtype=torch.float64)
+        h = 1e-4
+        hi, lo = ([x + s * h * u if j == i else x for j, x in enumerate(base)] for s in (1, -1))
+        diff = (loss(hi) - loss(lo)) / (2 * h)
+        got = (grads[i][0].double().cpu() * u).sum().item()
+        # rounding errors of the elements are independent: their root sum of squares, fivefold
+        tol = 5 * 4 * half_step(BF) * (mags[i] * u.abs()).square().sum().sqrt().item()
+        assert abs(got - diff) <= tol + 1e-6 * abs(diff), (i, got, diff, tol)
+
+
+def test_refusals(dev):
+    q, k, v, _ = (x.to(dev).requires_grad_() for x in _inputs(1, 1, 8, 2, 2, 64))
+    with pytest.raises(ValueError, match="out"):
+        hmx.causal_attention(q, k, v, out=torch.empty_like(q))
+    h = [x.detach().half().requires_grad_() for x in (q, k, v)]
+    with pytest.raises(NotImplementedError, match="bf16"):
+        hmx.causal_attention(*h)
+    with torch.no_grad():
+        hmx.causal_attention(*h)
