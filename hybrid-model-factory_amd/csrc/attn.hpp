@@ -73,6 +73,35 @@ __device__ __forceinline__ float half_max(float a) {
   return fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
 }
 
+// 16 bytes a lane from memory into LDS without a trip through registers: lane l's go to
+// lds + 16 l (uniform, in M0), from base (uniform) + off or from its own address.  The
+// compiler does not see the write: a tile is read after dma_wait() and a barrier.  (M0 is
+// reserved and cannot be named as clobbered; nothing the compiler emits in these kernels
+// keeps a value in it.)
+__device__ __forceinline__ uint32_t lds_addr(const void* p) {
+  return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)(p);
+}
+__device__ __forceinline__ void dma16(uint32_t lds, const char* base, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :: "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void dma16(uint32_t lds, const char* at) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :: "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(at) : "memory");
+}
+template <int N> __device__ __forceinline__ void dma_wait() {   // all but the last N
+  asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
+}
+// an int32 at a uniform index of memory that no kernel in flight writes
+__device__ __forceinline__ int uniform_load(const int32_t* p, int64_t i) {
+  return *((__attribute__((address_space(4))) const int32_t*)(uintptr_t)(p + i));
+}
+template <typename P> __device__ __forceinline__ P* uniform_ptr(P* p) {
+  const uint64_t x = (uint64_t)p;
+  return (P*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)x) |
+              (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32);
+}
+
 constexpr float NEG_INF = -__builtin_inff();
 constexpr float LOG2E = 1.4426950408889634f;
 

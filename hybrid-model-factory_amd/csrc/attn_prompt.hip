@@ -136,17 +136,23 @@ __device__ __forceinline__ void exact_rows(const FwdArgs& a, const Tile& t, int 
   }
 }
 
+// The loop is software-pipelined by halves of 32 keys: while a half's probabilities are
+// formed in the VALU, the matrix cores form the next half's scores, then its product with V
+// while the second sixteen probabilities and the next half's maximum are formed.  A step of
+// the loop multiplies K's keys 64 j .. 64 j + 63 and V's 64 j - 32 .. 64 j + 31, so both
+// tiles have two buffers, and arrive in LDS directly, a step ahead of their use.
 template <typename T, int D, bool PAGED>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
   typedef typename El<T>::v8 v8;
   constexpr int NC = D / 8;                 // 16-byte chunks of a row
-  constexpr int NL = BN * NC / 256;         // chunks of K, and of V, a thread stages
+  constexpr int RI = 64 / NC, NL = 16 / RI; // rows of a wave's load, loads of its 16 rows of a tile
   constexpr int NS = D / 16, ND = D / 32;
-  __shared__ __align__(16) T Ks[2][BN * D];
-  __shared__ __align__(16) T Vs[2][BN * D];
-  __shared__ int s_bad, s_skip[2];
+  constexpr int TILE = BN * D * 2;          // bytes
+  __shared__ __align__(1024) char smem[4 * TILE];   // K, K, V, V
+  __shared__ int s_bad, s_skip[4];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, l32 = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // uniform, and known to be
   const int kvh = blockIdx.x % a.HKV;
   // later tiles of a sequence have more keys: they go first
   const int slot = a.slots - 1 - (int)(blockIdx.x / a.HKV);
@@ -167,7 +173,9 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
 
   int keys = t.tokens;
   if constexpr (PAGED)
-    keys = (int)min((int64_t)max(a.pages.lens[t.seq], 0), (int64_t)a.pages.width * a.pages.page.d);
+    keys = (int)min((int64_t)max(uniform_load(a.pages.lens, t.seq), 0),
+                    (int64_t)a.pages.width * a.pages.page.d);
+  keys = __builtin_amdgcn_readfirstlane(keys);
   const int off = keys - t.tokens;          // token i attends keys 0 .. off + i
   const int klast = off + tok;
   const int wrow = t.row0 + wave * 32;
@@ -178,7 +186,9 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
   const int nt_all = wg_last < 0 ? 0 : wg_last / BN + 1;
   const int sp = blockIdx.y;
   const int j_beg = (int)((int64_t)nt_all * sp / a.nsplit), j_end = (int)((int64_t)nt_all * (sp + 1) / a.nsplit);
-  if (tid == 0) s_bad = s_skip[0] = s_skip[1] = 0;
+  const int u_beg = 2 * j_beg, u_last = min(2 * j_end - 1, w_last < 0 ? -1 : w_last / 32);   // the wave's halves
+  if (tid < 4) s_skip[tid] = 0;
+  if (tid == 0) s_bad = 0;
 
   v8 qf[NS];
   {
@@ -187,154 +197,222 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
     for (int s = 0; s < NS; ++s) qf[s] = *reinterpret_cast<const v8*>(qp + 32 * s);
   }
 
-  // staging: chunk index tid + 256 i -> row (tid + 256 i) / NC, chunk tid % NC
-  const int srow = tid / NC, sc = tid % NC;
-  constexpr int SR = 256 / NC;              // rows between a thread's chunks
-  u32x4 kr[NL], vr[NL];
-  int pid[NL];
-  bool skip = false;                        // the loaded tile has keys in pages outside the cache
-  auto fetch_pages = [&](int j) {
-    if constexpr (PAGED) {
+  // Staging: the wave brings rows 16 wave .. 16 wave + 15 of a tile, RI to a load; the lane's
+  // chunk is the one that the swizzle puts at its place.
+  uint32_t koff[NL], voff[NL];
+  const int64_t kts = PAGED ? a.pages.k_ts : a.k_ts, vts = PAGED ? a.pages.v_ts : a.v_ts;
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const int r = i * RI + lane / NC, c = swz<D>(wave * 16 + r, lane % NC);
+    koff[i] = (uint32_t)(r * (int)kts + 16 * c);
+    voff[i] = (uint32_t)(r * (int)vts + 16 * c);
+  }
+  const char* kbase = (PAGED ? a.pages.k : a.k + (int64_t)t.bos * a.k_ts) + (int64_t)kvh * (PAGED ? a.pages.k_hs : a.k_hs);
+  const char* vbase = (PAGED ? a.pages.v : a.v + (int64_t)t.bos * a.v_ts) + (int64_t)kvh * (PAGED ? a.pages.v_hs : a.v_hs);
+  const bool whole = !PAGED || a.pages.page.d % 16 == 0;   // the wave's 16 rows lie in one page
+  auto stage_rows = [&](int j, int r0, bool value) __attribute__((always_inline)) {
+    const uint32_t lds = lds_addr(smem) + (value ? 2 * TILE : 0) + (j & 1) * TILE + wave * 16 * D * 2;
+    const char* base = value ? vbase : kbase;
+    const int64_t ts = value ? vts : kts;
+    if (!PAGED && r0 >= 0 && r0 + 16 <= keys) {
+      const char* b = uniform_ptr(base + r0 * ts);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) dma16(lds + i * RI * D * 2, b, value ? voff[i] : koff[i]);
+    } else if (PAGED && whole) {
+      // rows behind the last key are the page's own: what they hold is masked
+      const int r = max(min(r0, (keys - 1) & ~15), 0), p = fdiv(r, a.pages.page);
+      int id = uniform_load(a.pages.table, t.seq * a.pages.table_stride + __builtin_amdgcn_readfirstlane(p));
+      if ((unsigned)id >= (unsigned)a.pages.num_pages) {
+        if (r0 >= 0 && r0 < keys) s_skip[(r0 / BN) & 3] = r0 / BN + 1;
+        id = 0;
+      }
+      const char* b = uniform_ptr(base + id * (value ? a.pages.v_ps : a.pages.k_ps) + (r - p * a.pages.page.d) * ts);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) dma16(lds + i * RI * D * 2, b, value ? voff[i] : koff[i]);
+    } else {
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const int r = min(j * BN + srow + i * SR, keys - 1);
-        pid[i] = a.pages.table[t.seq * a.pages.table_stride + fdiv(r, a.pages.page)];
+        const int q = r0 + i * RI + lane / NC, r = max(min(q, keys - 1), 0);
+        const char* b = base;
+        if constexpr (PAGED) {
+          const int p = fdiv(r, a.pages.page);
+          int id = a.pages.table[t.seq * a.pages.table_stride + p];
+          if ((unsigned)id >= (unsigned)a.pages.num_pages) {
+            if (q >= 0 && q < keys) s_skip[(q / BN) & 3] = q / BN + 1;
+            id = 0;
+          }
+          b += id * (value ? a.pages.v_ps : a.pages.k_ps) + (r - p * a.pages.page.d) * ts;
+        } else {
+          b += r * ts;
+        }
+        dma16(lds + i * RI * D * 2, b + 16 * swz<D>(wave * 16 + i * RI + lane / NC, lane % NC));
       }
     }
   };
-  auto load_tile = [&](int j) {
-    skip = false;
+  auto stage = [&](int j) __attribute__((always_inline)) {                 // the keys and values of step j
+    if (j < j_end) stage_rows(j, j * BN + wave * 16, false);
+    stage_rows(j, j * BN - 32 + wave * 16, true);
+  };
+  // Rows of step j's V that are no keys to 0 (their probability is 0, their memory anything),
+  // and a look for values that are not finite where some row's keys end among them.
+  auto mend = [&](int j) __attribute__((always_inline)) {
+    const int r0 = j * BN - 32;
+    const bool edge = r0 + BN > wg_first + 1, out = r0 < j_beg * BN || r0 + BN > keys;
+    const bool hole = PAGED && (s_skip[j & 3] == j + 1 || s_skip[(j - 1) & 3] == j);
+    if (!(edge || out || hole)) return;
+    T* Vb = reinterpret_cast<T*>(smem + (2 + (j & 1)) * TILE);
+    bool bad = false;
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int r0 = j * BN + srow + i * SR, r = min(r0, keys - 1);
-      const char *kp, *vp;
-      bool ok = r0 < keys;
+    for (int i = 0; i < BN * NC / 256; ++i) {
+      const int q = r0 + (tid + 256 * i) / NC;
+      u32x4* p = reinterpret_cast<u32x4*>(Vb + (tid + 256 * i) * 8);
+      bool key = q >= 0 && q < keys;
       if constexpr (PAGED) {
-        const int64_t in = r - fdiv(r, a.pages.page) * a.pages.page.d;
-        const bool pg = (unsigned)pid[i] < (unsigned)a.pages.num_pages;
-        const int64_t p = pg ? pid[i] : 0;
-        skip |= ok && !pg;
-        ok = ok && pg;
-        kp = a.pages.k + p * a.pages.k_ps + in * a.pages.k_ts + kvh * a.pages.k_hs;
-        vp = a.pages.v + p * a.pages.v_ps + in * a.pages.v_ts + kvh * a.pages.v_hs;
-      } else {
-        kp = a.k + (int64_t)(t.bos + r) * a.k_ts + (int64_t)kvh * a.k_hs;
-        vp = a.v + (int64_t)(t.bos + r) * a.v_ts + (int64_t)kvh * a.v_hs;
+        if (hole && key) key = key_row<T, true>(a, t, kvh, q, true) != nullptr;
       }
-      kr[i] = *reinterpret_cast<const u32x4*>(kp + 16 * sc);
-      vr[i] = *reinterpret_cast<const u32x4*>(vp + 16 * sc);
-      if (!ok) vr[i] = u32x4{0, 0, 0, 0};   // no key: its probability is 0, its value must be finite
+      if (key) bad |= any_nonfinite<T>(*p);
+      else *p = u32x4{0, 0, 0, 0};
     }
+    if (bad) s_bad = 1;
+    __syncthreads();
   };
 
   f32x16 acc[ND];
 #pragma unroll
   for (int i = 0; i < ND; ++i) acc[i] = f32x16{0};
-  float m = NEG_INF, l = 0.f;               // running maximum of the raw scores (both halves), own half's sum
+  float m = NEG_INF, l = 0.f, mc = 0.f;     // reference maximum of the raw scores, own half's sum, m c
 
-  // lane offsets into the tiles
+  // the lane's byte offsets into the tiles; flip() takes them to the other buffers
   int ko[NS], vo[ND], vu[ND];
 #pragma unroll
-  for (int s = 0; s < NS; ++s) ko[s] = l32 * D + swz<D>(l32, 2 * s + h) * 8;
+  for (int s = 0; s < NS; ++s) ko[s] = (j_beg & 1) * TILE + (l32 * D + swz<D>(l32, 2 * s + h) * 8) * 2;
 #pragma unroll
   for (int d = 0; d < ND; ++d) {
-    vo[d] = tr_offset<D>(lane, d, false);
-    vu[d] = tr_offset<D>(lane, d, true);
+    vo[d] = (j_beg & 1) * TILE + tr_offset<D>(lane, d, false) * 2;
+    vu[d] = (j_beg & 1) * TILE + tr_offset<D>(lane, d, true) * 2;
   }
-
-  if (j_beg < j_end) {
-    fetch_pages(j_beg);
-    load_tile(j_beg);
-    if (j_beg + 1 < j_end) fetch_pages(j_beg + 1);
-  }
-  for (int j = j_beg; j < j_end; ++j) {
-    T* Kb = Ks[(j - j_beg) & 1];
-    T* Vb = Vs[(j - j_beg) & 1];
-    const bool edge = (j + 1) * BN > wg_first + 1;   // some row's keys end in the tile
-    bool bad = false;
+  auto flip = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < NS; ++s) ko[s] ^= TILE;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      vo[d] ^= TILE;
+      vu[d] ^= TILE;
+    }
+  };
+  auto scores = [&](int kt, f32x16& st) __attribute__((always_inline)) {
+    st = f32x16{0};
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+      st = El<T>::mma32(*reinterpret_cast<const v8*>(smem + ko[s] + kt * 32 * D * 2), qf[s], st);
+  };
+  auto mask = [&](int u, f32x16& st) __attribute__((always_inline)) {
+    const int k0 = u * 32 + 4 * h;
+    if (u * 32 + 31 > w_first) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (k0 + 8 * (i >> 2) + (i & 3) > klast) st[i] = NEG_INF;
+    }
     if constexpr (PAGED) {
-      if (skip) s_skip[(j - j_beg) & 1] = j + 1;
-    }
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int r = srow + i * SR;
-      *reinterpret_cast<u32x4*>(Kb + r * D + swz<D>(r, sc) * 8) = kr[i];
-      *reinterpret_cast<u32x4*>(Vb + r * D + swz<D>(r, sc) * 8) = vr[i];
-      if (edge) bad |= any_nonfinite<T>(vr[i]);
-    }
-    if (bad) s_bad = 1;
-    __syncthreads();
-    if (j + 1 < j_end) {
-      load_tile(j + 1);
-      if (j + 2 < j_end) fetch_pages(j + 2);
-    }
-    const int t0 = j * BN;
-    if (t0 > w_last) continue;              // every key of the tile lies behind the wave's rows
-
-    f32x16 st[2];
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      st[kt] = f32x16{0};
-#pragma unroll
-      for (int s = 0; s < NS; ++s)
-        st[kt] = El<T>::mma32(*reinterpret_cast<const v8*>(Kb + ko[s] + kt * 32 * D), qf[s], st[kt]);
-    }
-    if (t0 + BN - 1 > w_first) {
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      if (s_skip[(u >> 1) & 3] == (u >> 1) + 1) {   // pages outside the cache hold no keys
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int key = t0 + kt * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
-          if (key > klast) st[kt][i] = NEG_INF;
+          const int key = k0 + 8 * (i >> 2) + (i & 3);
+          if (key <= klast && !key_row<T, true>(a, t, kvh, key, false)) st[i] = NEG_INF;
         }
-    }
-    if constexpr (PAGED) {
-      if (s_skip[(j - j_beg) & 1] == j + 1) {   // pages outside the cache hold no keys
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int key = t0 + kt * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
-            if (key <= klast && !key_row<T, true>(a, t, kvh, key, false)) st[kt][i] = NEG_INF;
-          }
       }
     }
-    float mx = st[0][0];
+  };
+  auto maximum = [&](const f32x16& st) __attribute__((always_inline)) {
+    float x = fmaxf(st[0], st[1]);
 #pragma unroll
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, st[0][i]);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[1][i]);
-    mx = half_max(mx);
-    // The reference maximum follows the running one only where it lags by more than 2^8:
-    // P then stays below 2^8, inside either type, and O is seldom rescaled.
+    for (int i = 2; i < 16; ++i) x = fmaxf(x, st[i]);
+    return half_max(x);
+  };
+  // The reference maximum follows the running one only where it lags by more than 2^8:
+  // P then stays below 2^8, inside either type, and O is seldom rescaled.
+  auto follow = [&](float mx) __attribute__((always_inline)) {
     if (__any((mx - m) * a.c > 8.f)) {
       const float mn = fmaxf(m, mx);
       const float f = m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((m - mn) * a.c);
       m = mn;
+      mc = m == NEG_INF ? 0.f : m * a.c;
       l *= f;
 #pragma unroll
       for (int d = 0; d < ND; ++d) acc[d] *= f;
     }
-    const float mc = m == NEG_INF ? 0.f : m * a.c;
-    v8 pf[4];
+  };
+  auto probs = [&](const f32x16& st, int b) __attribute__((always_inline)) {
+    float p[8];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      float p[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(st[kt][i] * a.c - mc);
-        l += p[i];
-      }
-      pf[2 * kt] = pack8<T>(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
-      pf[2 * kt + 1] = pack8<T>(p[8], p[9], p[10], p[11], p[12], p[13], p[14], p[15]);
+    for (int i = 0; i < 8; ++i) {
+      p[i] = __builtin_amdgcn_exp2f(st[b + i] * a.c - mc);
+      l += p[i];
     }
+    return pack8<T>(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
+  };
+  auto values = [&](int r, v8 pf) __attribute__((always_inline)) {   // 16 rows of V from row r of the tile
+    const char* Vb = smem + 2 * TILE + r * D * 2;
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        const v8 vf = join<T>(tr4<T>(Vb + vo[d] + ks * 16 * D), tr4<T>(Vb + vu[d] + ks * 16 * D));
-        acc[d] = El<T>::mma32(vf, pf[ks], acc[d]);
+    for (int d = 0; d < ND; ++d)
+      acc[d] = El<T>::mma32(join<T>(tr4<T>(reinterpret_cast<const T*>(Vb + vo[d])),
+                                    tr4<T>(reinterpret_cast<const T*>(Vb + vu[d]))), pf, acc[d]);
+  };
+  // half u, whose scores are cur, against V's rows r of its tile; nxt receives the next
+  // half's scores from K's half kt
+  auto half = [&](int u, const f32x16& cur, f32x16& nxt, int kt, int r) __attribute__((always_inline)) {
+    scores(kt, nxt);
+    v8 p0 = probs(cur, 0);
+    asm volatile("" : "+v"(p0));            // formed here, beside the products, not behind the mask
+    mask(u + 1, nxt);
+    values(r, p0);
+    const v8 p1 = probs(cur, 8);
+    values(r + 16, p1);
+    follow(maximum(nxt));
+  };
+  auto last_half = [&](const f32x16& cur, int r) __attribute__((always_inline)) {
+    values(r, probs(cur, 0));
+    values(r + 16, probs(cur, 8));
+  };
+  auto arrive = [&](int j) __attribute__((always_inline)) {                // step j's tiles are there, step j + 1's on their way
+    dma_wait<0>();
+    __syncthreads();
+    if (j < j_end) stage(j + 1);
+    mend(j);
+  };
+
+  if (j_beg < j_end) {
+    __syncthreads();                        // the flags are clear
+    stage(j_beg);
+    int j = j_beg;
+    arrive(j);
+    if (u_last >= u_beg) {
+      f32x16 s0, s1;
+      scores(0, s0);
+      mask(u_beg, s0);
+      follow(maximum(s0));
+      if (u_last == u_beg) {
+        last_half(s0, 32);
+      } else {
+        half(u_beg, s0, s1, 1, 32);
+        const int jf = (u_last + 1) >> 1;
+        for (++j; j < jf; ++j) {
+          arrive(j);
+          flip();
+          half(2 * j - 1, s1, s0, 0, 0);
+          half(2 * j, s0, s1, 1, 32);
+        }
+        arrive(j);
+        flip();
+        if (u_last & 1) {
+          last_half(s1, 0);
+        } else {
+          half(2 * j - 1, s1, s0, 0, 0);
+          last_half(s0, 32);
+        }
       }
+    }
+    for (++j; j <= j_end; ++j) arrive(j);   // other waves' rows see further
   }
   l = pair_sum32(l, l);
 
@@ -369,7 +447,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
   }
   __syncthreads();
   if (s_bad)
-    exact_rows<T, D, PAGED>(a, t, kvh, off, j_beg * BN, j_end * BN, sp, reinterpret_cast<float*>(&Ks[0][0]));
+    exact_rows<T, D, PAGED>(a, t, kvh, off, j_beg * BN, j_end * BN, sp, reinterpret_cast<float*>(smem));
 }
 
 // The splits' shares of a row joined: sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.
