@@ -33,12 +33,13 @@ template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void attn_bwd_dq_kernel(BwdArgs a) {
   typedef typename El<T>::v8 v8;
   typedef typename El<T>::v4 v4;
-  constexpr int QN = D == 128 ? 32 : 64;    // keys of a tile
-  constexpr int NC = D / 8, NL = QN * NC / 256, NS = D / 16, ND = D / 32;
+  constexpr int QN = 64;                    // keys of a tile
+  constexpr int NC = D / 8, RI = 64 / NC, NL = 16 / RI, NS = D / 16, ND = D / 32;
   __shared__ __align__(16) T Ks[2][QN * D];
   __shared__ __align__(16) T Vs[2][QN * D];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, l32 = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // uniform, and known to be
   const int kvh = blockIdx.x % a.HKV;
   const Tile t = find_tile<QM>(a.seqs, a.slots - 1 - (int)(blockIdx.x / a.HKV));
   if (t.row0 >= t.rows || t.row0 < 0) return;
@@ -71,15 +72,32 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_dq_kernel(BwdArgs a) {
   const float lse = a.lse[gt * a.H + head];
   if (h == 0 && row < t.rows) a.delta[gt * a.H + head] = delta;
 
-  const int srow = tid / NC, sc = tid % NC;
-  constexpr int SR = 256 / NC;
-  u32x4 kr[NL], vr[NL];
-  auto load_tile = [&](int j) {
+  // staging as in the forward: the wave brings rows 16 wave .. 16 wave + 15 of a tile
+  uint32_t koff[NL], voff[NL];
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int64_t r = t.bos + min(j * QN + srow + i * SR, keys - 1);
-      kr[i] = *reinterpret_cast<const u32x4*>(a.k + r * a.k_ts + (int64_t)kvh * a.k_hs + 16 * sc);
-      vr[i] = *reinterpret_cast<const u32x4*>(a.v + r * a.v_ts + (int64_t)kvh * a.v_hs + 16 * sc);
+  for (int i = 0; i < NL; ++i) {
+    const int r = i * RI + lane / NC, c = swz<D>(wave * 16 + r, lane % NC);
+    koff[i] = (uint32_t)(r * (int)a.k_ts + 16 * c);
+    voff[i] = (uint32_t)(r * (int)a.v_ts + 16 * c);
+  }
+  const char* kbase = a.k + (int64_t)t.bos * a.k_ts + (int64_t)kvh * a.k_hs;
+  const char* vbase = a.v + (int64_t)t.bos * a.v_ts + (int64_t)kvh * a.v_hs;
+  auto stage = [&](int j) __attribute__((always_inline)) {
+    const uint32_t kl = lds_addr(Ks[j & 1]) + wave * 16 * D * 2, vl = lds_addr(Vs[j & 1]) + wave * 16 * D * 2;
+    const int r0 = j * QN + wave * 16;
+    if (r0 + 16 <= keys) {
+      const char *kb = uniform_ptr(kbase + r0 * a.k_ts), *vb = uniform_ptr(vbase + r0 * a.v_ts);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) dma16(kl + i * RI * D * 2, kb, koff[i]);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) dma16(vl + i * RI * D * 2, vb, voff[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int x = i * RI + lane / NC, r = min(r0 + x, keys - 1), c = 16 * swz<D>(wave * 16 + x, lane % NC);
+        dma16(kl + i * RI * D * 2, kbase + r * a.k_ts + c);
+        dma16(vl + i * RI * D * 2, vbase + r * a.v_ts + c);
+      }
     }
   };
   int ko[NS], to[ND], tu[ND];
@@ -94,17 +112,12 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_dq_kernel(BwdArgs a) {
 #pragma unroll
   for (int i = 0; i < ND; ++i) acc[i] = f32x16{0};
 
-  load_tile(0);
+  stage(0);
   for (int j = 0; j < nt; ++j) {
-    T *Kb = Ks[j & 1], *Vb = Vs[j & 1];
-#pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int r = srow + i * SR;
-      *reinterpret_cast<u32x4*>(Kb + r * D + swz<D>(r, sc) * 8) = kr[i];
-      *reinterpret_cast<u32x4*>(Vb + r * D + swz<D>(r, sc) * 8) = vr[i];
-    }
+    const T *Kb = Ks[j & 1], *Vb = Vs[j & 1];
+    dma_wait<0>();
     __syncthreads();
-    if (j + 1 < nt) load_tile(j + 1);
+    if (j + 1 < nt) stage(j + 1);
     const int t0 = j * QN;
     if (t0 > w_last) continue;
 #pragma unroll
@@ -116,13 +129,15 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_dq_kernel(BwdArgs a) {
 #pragma unroll
       for (int s = 0; s < NS; ++s)
         dp = El<T>::mma32(*reinterpret_cast<const v8*>(Vb + ko[s] + kt * 32 * D), df[s], dp);
-      const bool masked = t0 + kt * 32 + 31 > w_first;
+      if (t0 + kt * 32 + 31 > w_first) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (t0 + kt * 32 + 8 * (i >> 2) + 4 * h + (i & 3) > tok) st[i] = NEG_INF;
+      }
       float ds[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        float p = __builtin_amdgcn_exp2f(st[i] * a.c - lse);
-        if (masked && t0 + kt * 32 + 8 * (i >> 2) + 4 * h + (i & 3) > tok) p = 0.f;
-        ds[i] = p * (dp[i] - delta);
+        ds[i] = __builtin_amdgcn_exp2f(st[i] * a.c - lse) * (dp[i] - delta);
       }
       const v8 d0 = pack8<T>(ds[0], ds[1], ds[2], ds[3], ds[4], ds[5], ds[6], ds[7]);
       const v8 d1 = pack8<T>(ds[8], ds[9], ds[10], ds[11], ds[12], ds[13], ds[14], ds[15]);
@@ -148,22 +163,28 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_dq_kernel(BwdArgs a) {
   }
 }
 
-constexpr int KM = 128, KR = 32;     // dK, dV: keys of a workgroup, rows of a step
+constexpr int KM = 128, KR = 64;     // dK, dV: keys of a workgroup, rows of a tile
 
+// A wave holds 32 keys: their K and V rows as B operands and dK^T, dV^T as accumulators in
+// registers (one wave a SIMD), and walks the rows from its first key on.  Pipelined by units
+// of 32 rows: S and dP of the next unit are formed by the matrix cores while P and dS of
+// this one are formed in the VALU.  Tiles of 64 rows of Q and dO arrive in LDS directly, in
+// a ring of three: a step still multiplies with the last unit of the tile before.
 template <typename T, int D>
 __global__ __launch_bounds__(256, 1) void attn_bwd_dkv_kernel(BwdArgs a) {
   typedef typename El<T>::v8 v8;
   typedef typename El<T>::v4 v4;
-  constexpr int NC = D / 8, NL = KR * NC / 256, NS = D / 16, ND = D / 32;
-  __shared__ __align__(16) T Qs[2][KR * D];
-  __shared__ __align__(16) T Os[2][KR * D];
-  __shared__ __align__(16) float Ls[2][2][KR];
+  constexpr int NC = D / 8, RI = 64 / NC, NL = 16 / RI, NS = D / 16, ND = D / 32;
+  constexpr int TILE = KR * D * 2;          // bytes
+  __shared__ __align__(1024) char smem[6 * TILE];        // [3][Q, dO]
+  __shared__ __align__(16) float Ls[3][2][KR];           // lse and delta of the rows
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, l32 = lane & 31;
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kvh = blockIdx.x % a.HKV;
-  Seqs ks = a.seqs;
-  ks.G = 1;
-  const Tile t = find_tile<KM>(ks, (int)(blockIdx.x / a.HKV));
+  Seqs sk = a.seqs;
+  sk.G = 1;
+  const Tile t = find_tile<KM>(sk, (int)(blockIdx.x / a.HKV));
   if (t.row0 >= t.rows || t.row0 < 0) return;
   const int key = t.row0 + wave * 32 + l32, keyc = min(key, t.tokens - 1);
   const int64_t gk = t.bos + keyc;
@@ -184,89 +205,144 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_dkv_kernel(BwdArgs a) {
     kf[s] = *reinterpret_cast<const v8*>(a.k + gk * a.k_ts + (int64_t)kvh * a.k_hs + 32 * s + 16 * h);
     vf[s] = *reinterpret_cast<const v8*>(a.v + gk * a.v_ts + (int64_t)kvh * a.v_hs + 32 * s + 16 * h);
   }
-  const int rows = t.tokens * a.G.d;
-  const int j0 = (int)((int64_t)t.row0 * a.G.d / KR), nt = (rows + KR - 1) / KR;
-  const int wk0 = t.row0 + wave * 32;       // the wave's first key
+  const int G = a.G.d, rows = t.tokens * G, nt = (rows + KR - 1) / KR;
+  const int wk0 = min(t.row0 + wave * 32, t.tokens - 1);           // the wave's first key
+  const int j_wg = t.row0 * G / KR, j_own = wk0 * G / KR;          // first tiles with rows that see them
+  const int first = key * G;                                        // the key's first row
 
-  const int srow = tid / NC, sc = tid % NC;
-  constexpr int SR = 256 / NC;
-  u32x4 qr[NL], dr[NL];
-  float lr = 0.f;
-  auto load_tile = [&](int j) {
+  // Staging: rows 16 wave .. + 15 of a tile, RI to a load.  Where G divides a tile's rows, a
+  // lane's rows of all tiles are one head's, at offsets that do not change.
+  const bool even = KR % G == 0;
+  uint32_t qoff[NL], ooff[NL];
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int r = min(j * KR + srow + i * SR, rows - 1), tk = fdiv(r, a.G);
-      const int64_t hd = kvh * a.G.d + r - tk * a.G.d, g = t.bos + tk;
-      qr[i] = *reinterpret_cast<const u32x4*>(a.q + g * a.q_ts + hd * a.q_hs + 16 * sc);
-      dr[i] = *reinterpret_cast<const u32x4*>(a.dout + g * a.do_ts + hd * a.do_hs + 16 * sc);
+  for (int i = 0; i < NL; ++i) {
+    const int x = wave * 16 + i * RI + lane / NC, tk = fdiv(x, a.G), hd = kvh * G + x - tk * G;
+    const int c = swz<D>(x, lane % NC);
+    qoff[i] = (uint32_t)(tk * (int)a.q_ts + hd * (int)a.q_hs + 16 * c);
+    ooff[i] = (uint32_t)(tk * (int)a.do_ts + hd * (int)a.do_hs + 16 * c);
+  }
+  const char *qbase = a.q + (int64_t)t.bos * a.q_ts, *obase = a.dout + (int64_t)t.bos * a.do_ts;
+  const int tpt = KR / G;                   // tokens of a tile where G divides it
+  float lr = 0.f;
+  auto stage = [&](int j, int buf) __attribute__((always_inline)) {
+    const uint32_t ql = lds_addr(smem) + buf * 2 * TILE + wave * 16 * D * 2, ol = ql + TILE;
+    if (even && (j + 1) * KR <= rows) {
+      const char *qb = uniform_ptr(qbase + (int64_t)j * tpt * a.q_ts), *ob = uniform_ptr(obase + (int64_t)j * tpt * a.do_ts);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) dma16(ql + i * RI * D * 2, qb, qoff[i]);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) dma16(ol + i * RI * D * 2, ob, ooff[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NL; ++i) {
+        const int x = wave * 16 + i * RI + lane / NC, r = min(j * KR + x, rows - 1), tk = fdiv(r, a.G);
+        const int64_t hd = kvh * G + r - tk * G;
+        const int c = 16 * swz<D>(x, lane % NC);
+        dma16(ql + i * RI * D * 2, qbase + tk * a.q_ts + hd * a.q_hs + c);
+        dma16(ol + i * RI * D * 2, obase + tk * a.do_ts + hd * a.do_hs + c);
+      }
     }
     if (tid < 2 * KR) {
       const int r0 = j * KR + (tid & (KR - 1)), r = min(r0, rows - 1), tk = fdiv(r, a.G);
-      const int64_t at = (int64_t)(t.bos + tk) * a.H + kvh * a.G.d + r - tk * a.G.d;
-      lr = (tid < KR ? a.lse : a.delta)[at];
+      lr = (tid < KR ? a.lse : a.delta)[(int64_t)(t.bos + tk) * a.H + kvh * G + r - tk * G];
       if (tid < KR && r0 >= rows) lr = __builtin_inff();   // no row: its P is 0
     }
   };
-  int qo[NS], to[ND], tu[ND];
+  int qo[NS], to[ND], tu[ND];               // byte offsets into a tile
 #pragma unroll
-  for (int s = 0; s < NS; ++s) qo[s] = l32 * D + swz<D>(l32, 2 * s + h) * 8;
+  for (int s = 0; s < NS; ++s) qo[s] = (l32 * D + swz<D>(l32, 2 * s + h) * 8) * 2;
 #pragma unroll
   for (int d = 0; d < ND; ++d) {
-    to[d] = tr_offset<D>(lane, d, false);
-    tu[d] = tr_offset<D>(lane, d, true);
+    to[d] = tr_offset<D>(lane, d, false) * 2;
+    tu[d] = tr_offset<D>(lane, d, true) * 2;
   }
   f32x16 ak[ND], av[ND];
 #pragma unroll
   for (int i = 0; i < ND; ++i) ak[i] = av[i] = f32x16{0};
 
-  load_tile(j0);
-  for (int j = j0; j < nt; ++j) {
-    T *Qb = Qs[j & 1], *Ob = Os[j & 1];
-    float* Lb = &Ls[j & 1][0][0];
+  // S and dP of unit x (0, 1) of the tile in buf
+  auto scores = [&](int buf, int x, f32x16& st, f32x16& dp) __attribute__((always_inline)) {
+    const char *q = smem + buf * 2 * TILE + x * 32 * D * 2, *o = q + TILE;
+    st = dp = f32x16{0};
 #pragma unroll
-    for (int i = 0; i < NL; ++i) {
-      const int r = srow + i * SR;
-      *reinterpret_cast<u32x4*>(Qb + r * D + swz<D>(r, sc) * 8) = qr[i];
-      *reinterpret_cast<u32x4*>(Ob + r * D + swz<D>(r, sc) * 8) = dr[i];
+    for (int s = 0; s < NS; ++s) {
+      st = El<T>::mma32(*reinterpret_cast<const v8*>(q + qo[s]), kf[s], st);
+      dp = El<T>::mma32(*reinterpret_cast<const v8*>(o + qo[s]), vf[s], dp);
     }
-    if (tid < 2 * KR) Lb[tid] = lr;
-    __syncthreads();
-    if (j + 1 < nt) load_tile(j + 1);
-    const int r_last = min(j * KR + KR, rows) - 1;
-    if (fdiv(r_last, a.G) < wk0) continue;  // every row of the step lies before the wave's keys
-    const bool masked = fdiv(j * KR, a.G) < wk0 + 31;
-
-    f32x16 st = {0}, dp = {0};
+  };
+  auto mask = [&](int u, f32x16& st) __attribute__((always_inline)) {   // rows before the key do not see it
+    if (u * 32 < (wk0 + 31) * G) {
 #pragma unroll
-    for (int s = 0; s < NS; ++s) st = El<T>::mma32(*reinterpret_cast<const v8*>(Qb + qo[s]), kf[s], st);
+      for (int i = 0; i < 16; ++i)
+        if (u * 32 + 8 * (i >> 2) + 4 * h + (i & 3) < first) st[i] = NEG_INF;
+    }
+  };
+  // P and dS of a unit, in place as B operands
+  auto grads = [&](int buf, int x, const f32x16& st, const f32x16& dp, v8 (&pf)[2], v8 (&sf)[2])
+      __attribute__((always_inline)) {
+    const float* ls = &Ls[buf][0][x * 32 + 4 * h];
 #pragma unroll
-    for (int s = 0; s < NS; ++s) dp = El<T>::mma32(*reinterpret_cast<const v8*>(Ob + qo[s]), vf[s], dp);
-    float p[16], ds[16];
+    for (int b = 0; b < 2; ++b) {
+      float p[8], ds[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f32x4 ls = *reinterpret_cast<const f32x4*>(Lb + 8 * i + 4 * h);
-      const f32x4 dl = *reinterpret_cast<const f32x4*>(Lb + KR + 8 * i + 4 * h);
+      for (int i = 0; i < 2; ++i) {
+        const f32x4 le = *reinterpret_cast<const f32x4*>(ls + 16 * b + 8 * i);
+        const f32x4 dl = *reinterpret_cast<const f32x4*>(ls + KR + 16 * b + 8 * i);
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int e = 4 * i + x;
-        p[e] = __builtin_amdgcn_exp2f(st[e] * a.c - ls[x]);
-        if (masked && fdiv(min(j * KR + 8 * i + 4 * h + x, rows - 1), a.G) < key) p[e] = 0.f;
-        ds[e] = p[e] * (dp[e] - dl[x]);
+        for (int y = 0; y < 4; ++y) {
+          const int e = 8 * b + 4 * i + y, z = 4 * i + y;
+          p[z] = __builtin_amdgcn_exp2f(st[e] * a.c - le[y]);
+          ds[z] = p[z] * (dp[e] - dl[y]);
+        }
       }
+      pf[b] = pack8<T>(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
+      sf[b] = pack8<T>(ds[0], ds[1], ds[2], ds[3], ds[4], ds[5], ds[6], ds[7]);
     }
+  };
+  auto gather = [&](int buf, int x, const v8 (&pf)[2], const v8 (&sf)[2]) __attribute__((always_inline)) {
+    const char *q = smem + buf * 2 * TILE + x * 32 * D * 2, *o = q + TILE;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int b = 8 * s;
-      const v8 pf = pack8<T>(p[b], p[b + 1], p[b + 2], p[b + 3], p[b + 4], p[b + 5], p[b + 6], p[b + 7]);
-      const v8 sf = pack8<T>(ds[b], ds[b + 1], ds[b + 2], ds[b + 3], ds[b + 4], ds[b + 5], ds[b + 6], ds[b + 7]);
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int d = 0; d < ND; ++d) {
-        const T *op = Ob + s * 16 * D, *qp = Qb + s * 16 * D;
-        av[d] = El<T>::mma32(join<T>(tr4<T>(op + to[d]), tr4<T>(op + tu[d])), pf, av[d]);
-        ak[d] = El<T>::mma32(join<T>(tr4<T>(qp + to[d]), tr4<T>(qp + tu[d])), sf, ak[d]);
+        const int at = b * 16 * D * 2;
+        av[d] = El<T>::mma32(join<T>(tr4<T>(reinterpret_cast<const T*>(o + to[d] + at)),
+                                     tr4<T>(reinterpret_cast<const T*>(o + tu[d] + at))), pf[b], av[d]);
+        ak[d] = El<T>::mma32(join<T>(tr4<T>(reinterpret_cast<const T*>(q + to[d] + at)),
+                                     tr4<T>(reinterpret_cast<const T*>(q + tu[d] + at))), sf[b], ak[d]);
       }
+  };
+
+  f32x16 s0, d0, s1, d1;
+  v8 pf[2], sf[2];
+  stage(j_wg, 0);
+  int buf = 0, prev = 2;
+  for (int j = j_wg; j < nt; ++j) {
+    dma_wait<0>();
+    if (tid < 2 * KR) (&Ls[buf][0][0])[tid] = lr;
+    __syncthreads();
+    const int next = buf == 2 ? 0 : buf + 1;
+    if (j + 1 < nt) stage(j + 1, next);
+    if (j > j_own) {
+      mask(2 * j - 1, s1);
+      scores(buf, 0, s0, d0);
+      grads(prev, 1, s1, d1, pf, sf);
+      gather(prev, 1, pf, sf);
+    } else if (j == j_own) {
+      scores(buf, 0, s0, d0);
     }
+    if (j >= j_own) {
+      mask(2 * j, s0);
+      scores(buf, 1, s1, d1);
+      grads(buf, 0, s0, d0, pf, sf);
+      gather(buf, 0, pf, sf);
+    }
+    prev = buf;
+    buf = next;
   }
+  mask(2 * nt - 1, s1);
+  grads(prev, 1, s1, d1, pf, sf);
+  gather(prev, 1, pf, sf);
   if (key < t.tokens) {
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -310,7 +386,7 @@ extern "C" int hmx_causal_attention_bwd(
   HMX_REQUIRE(dtype == HMX_BF16, HMX_EUNSUPPORTED, "hmx_causal_attention_bwd: dtype code %d (bf16 only)", dtype);
   HMX_REQUIRE(N >= 0 && T >= 0 && HKV > 0 && H > 0 && H % HKV == 0, HMX_EINVAL,
               "hmx_causal_attention_bwd: N=%d T=%lld H=%d HKV=%d", N, (long long)T, H, HKV);
-  HMX_REQUIRE(T * (H / HKV) < (1ll << 31) - 256, HMX_EUNSUPPORTED, "hmx_causal_attention_bwd: %lld tokens",
+  HMX_REQUIRE(T * (H / HKV) < (1ll << 30), HMX_EUNSUPPORTED, "hmx_causal_attention_bwd: %lld tokens",
               (long long)T);
   HMX_REQUIRE(scale > 0.f && scale < __builtin_inff(), HMX_EINVAL,
               "hmx_causal_attention_bwd: scale %g must be positive", (double)scale);
