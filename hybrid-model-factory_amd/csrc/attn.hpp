@@ -66,6 +66,11 @@ template <int D> __device__ __forceinline__ int tr_offset(int lane, int d, bool 
   return r * D + swz<D>(r, 4 * d + 2 * g + ((s & 3) >> 1)) * 8 + 4 * (s & 1);
 }
 
+// Nothing moves across it: the kernels' inner blocks are written in the order in which they
+// are to issue, a few instructions between two fences (loads ahead of their use, vector
+// instructions between matrix products); left to itself the scheduler gathers them by kind.
+__device__ __forceinline__ void fence() { __builtin_amdgcn_sched_barrier(0); }
+
 // max and sum over the two halves of a wave, in the VALU
 __device__ __forceinline__ float half_max(float a) {
   const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, a),
@@ -87,6 +92,10 @@ __device__ __forceinline__ void dma16(uint32_t lds, const char* base, uint32_t o
 }
 __device__ __forceinline__ void dma16(uint32_t lds, const char* at) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :: "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(at) : "memory");
+}
+__device__ __forceinline__ void dma4(uint32_t lds, const char* at) {   // 4 bytes a lane, to lds + 4 l
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
                :: "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(at) : "memory");
 }
 template <int N> __device__ __forceinline__ void dma_wait() {   // all but the last N

@@ -11,6 +11,8 @@
 // else stays in fp32.
 #include "attn.hpp"
 
+#include <type_traits>
+
 namespace hmx {
 namespace attn {
 
@@ -166,18 +168,20 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_dq_kernel(BwdArgs a) {
 constexpr int KM = 128, KR = 64;     // dK, dV: keys of a workgroup, rows of a tile
 
 // A wave holds 32 keys: their K and V rows as B operands and dK^T, dV^T as accumulators in
-// registers (one wave a SIMD), and walks the rows from its first key on.  Pipelined by units
+// registers (one wave a SIMD), and walks the rows that see them.  Pipelined by units
 // of 32 rows: S and dP of the next unit are formed by the matrix cores while P and dS of
 // this one are formed in the VALU.  Tiles of 64 rows of Q and dO arrive in LDS directly, in
-// a ring of three: a step still multiplies with the last unit of the tile before.
+// a ring of four, two tiles ahead: a step still multiplies with the last unit of the tile
+// before (with one tile ahead, 2.91 ms where two take 2.77 at 8 x 4096 tokens, 32 / 8 heads).
 template <typename T, int D>
 __global__ __launch_bounds__(256, 1) void attn_bwd_dkv_kernel(BwdArgs a) {
   typedef typename El<T>::v8 v8;
   typedef typename El<T>::v4 v4;
   constexpr int NC = D / 8, RI = 64 / NC, NL = 16 / RI, NS = D / 16, ND = D / 32;
   constexpr int TILE = KR * D * 2;          // bytes
-  __shared__ __align__(1024) char smem[6 * TILE];        // [3][Q, dO]
-  __shared__ __align__(16) float Ls[3][2][KR];           // lse and delta of the rows
+  constexpr int RING = 4;
+  __shared__ __align__(1024) char smem[RING * 2 * TILE];  // [RING][Q, dO]
+  __shared__ __align__(16) float Ls[RING][2][KR];         // lse and delta of the rows
 
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -223,7 +227,6 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_dkv_kernel(BwdArgs a) {
   }
   const char *qbase = a.q + (int64_t)t.bos * a.q_ts, *obase = a.dout + (int64_t)t.bos * a.do_ts;
   const int tpt = KR / G;                   // tokens of a tile where G divides it
-  float lr = 0.f;
   auto stage = [&](int j, int buf) __attribute__((always_inline)) {
     const uint32_t ql = lds_addr(smem) + buf * 2 * TILE + wave * 16 * D * 2, ol = ql + TILE;
     if (even && (j + 1) * KR <= rows) {
@@ -242,11 +245,9 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_dkv_kernel(BwdArgs a) {
         dma16(ol + i * RI * D * 2, obase + tk * a.do_ts + hd * a.do_hs + c);
       }
     }
-    if (tid < 2 * KR) {
-      const int r0 = j * KR + (tid & (KR - 1)), r = min(r0, rows - 1), tk = fdiv(r, a.G);
-      lr = (tid < KR ? a.lse : a.delta)[(int64_t)(t.bos + tk) * a.H + kvh * G + r - tk * G];
-      if (tid < KR && r0 >= rows) lr = __builtin_inff();   // no row: its P is 0
-    }
+    const int r = min(j * KR + lane, rows - 1), tk = fdiv(r, a.G);   // wave 0 (and 2) lse, 1 (and 3) delta
+    dma4(lds_addr(&Ls[buf][wave & 1][0]), reinterpret_cast<const char*>(
+        ((wave & 1) ? a.delta : a.lse) + ((int64_t)(t.bos + tk) * a.H + kvh * G + r - tk * G)));
   };
   int qo[NS], to[ND], tu[ND];               // byte offsets into a tile
 #pragma unroll
@@ -260,89 +261,130 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_dkv_kernel(BwdArgs a) {
 #pragma unroll
   for (int i = 0; i < ND; ++i) ak[i] = av[i] = f32x16{0};
 
-  // S and dP of unit x (0, 1) of the tile in buf
-  auto scores = [&](int buf, int x, f32x16& st, f32x16& dp) __attribute__((always_inline)) {
-    const char *q = smem + buf * 2 * TILE + x * 32 * D * 2, *o = q + TILE;
-    st = dp = f32x16{0};
+  auto mask = [&](int u, f32x16& st) __attribute__((always_inline)) {
+    // rows before the key do not see it, and rows behind the last are none
+    if (u * 32 < (wk0 + 31) * G || u * 32 + 32 > rows) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = u * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
+        if (r < first || r >= rows) st[i] = NEG_INF;
+      }
+    }
+  };
+  // The two parts of a unit's work that the pipeline keeps apart: S and dP of unit xn of the
+  // tile in bn (NEXT), and P, dS and their products for unit xc of the tile in bc, whose S
+  // and dP are st and dp (THIS); together, the first part's products hide the second's
+  // exponentials.  LDS reads run AHEAD steps before their use, also into the unit that is
+  // NEXT in the following call (FOLLOW: unit xf of the tile in bf).
+  constexpr int AHEAD = NS / 2;
+  constexpr int E = 16 / NS;                // elements of P formed beside a step of the first part
+  v8 qa[NS], oa[NS];
+  f32x4 le[4], dl[4];
+  auto rows_of = [&](int buf, int x, int s) __attribute__((always_inline)) {
+    const char* q = smem + buf * 2 * TILE + x * 32 * D * 2;
+    qa[s] = *reinterpret_cast<const v8*>(q + qo[s]);
+    oa[s] = *reinterpret_cast<const v8*>(q + TILE + qo[s]);
+  };
+  auto work = [&](auto NEXT, auto THIS, auto FOLLOW, int bn, int xn, f32x16& sn, f32x16& dn, int bc, int xc,
+                  const f32x16& st, const f32x16& dp, int bf, int xf) __attribute__((always_inline)) {
+    constexpr bool next = decltype(NEXT)::value, cur = decltype(THIS)::value, follow = decltype(FOLLOW)::value;
+    const char *qc = smem + bc * 2 * TILE + xc * 32 * D * 2, *oc = qc + TILE;
+    v8 qt[2 * ND], ot[2 * ND], pf[2], sf[2];
+    float p[16], ds[16];
+    auto cols_of = [&](int g) __attribute__((always_inline)) {
+      const int d = g % ND, at = (g / ND) * 16 * D * 2;
+      ot[g] = join<T>(tr4<T>(reinterpret_cast<const T*>(oc + to[d] + at)), tr4<T>(reinterpret_cast<const T*>(oc + tu[d] + at)));
+      qt[g] = join<T>(tr4<T>(reinterpret_cast<const T*>(qc + to[d] + at)), tr4<T>(reinterpret_cast<const T*>(qc + tu[d] + at)));
+    };
+    auto pack = [&](int b) __attribute__((always_inline)) {
+      const int z = 8 * b;
+      pf[b] = pack8<T>(p[z], p[z + 1], p[z + 2], p[z + 3], p[z + 4], p[z + 5], p[z + 6], p[z + 7]);
+      sf[b] = pack8<T>(ds[z], ds[z + 1], ds[z + 2], ds[z + 3], ds[z + 4], ds[z + 5], ds[z + 6], ds[z + 7]);
+    };
+    fence();
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      st = El<T>::mma32(*reinterpret_cast<const v8*>(q + qo[s]), kf[s], st);
-      dp = El<T>::mma32(*reinterpret_cast<const v8*>(o + qo[s]), vf[s], dp);
+      if constexpr (next) {
+        if (s + AHEAD < NS) rows_of(bn, xn, s + AHEAD);
+      }
+      if constexpr (cur) {
+        if (s + AHEAD >= NS) cols_of(s + AHEAD - NS);
+      }
+      if constexpr (next) {
+        sn = El<T>::mma32(qa[s], kf[s], s == 0 ? f32x16{0} : sn);
+        dn = El<T>::mma32(oa[s], vf[s], s == 0 ? f32x16{0} : dn);
+      }
+      if constexpr (cur) {
+#pragma unroll
+        for (int e = s * E; e < s * E + E; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(st[e] * a.c - le[e >> 2][e & 3]);
+          ds[e] = p[e] * (dp[e] - dl[e >> 2][e & 3]);
+        }
+        if (s == NS / 2 - 1) pack(0);
+        if (s == NS - 1) pack(1);
+      }
+      fence();
     }
-  };
-  auto mask = [&](int u, f32x16& st) __attribute__((always_inline)) {   // rows before the key do not see it
-    if (u * 32 < (wk0 + 31) * G) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (u * 32 + 8 * (i >> 2) + 4 * h + (i & 3) < first) st[i] = NEG_INF;
-    }
-  };
-  // P and dS of a unit, in place as B operands
-  auto grads = [&](int buf, int x, const f32x16& st, const f32x16& dp, v8 (&pf)[2], v8 (&sf)[2])
-      __attribute__((always_inline)) {
-    const float* ls = &Ls[buf][0][x * 32 + 4 * h];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      float p[8], ds[8];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const f32x4 le = *reinterpret_cast<const f32x4*>(ls + 16 * b + 8 * i);
-        const f32x4 dl = *reinterpret_cast<const f32x4*>(ls + KR + 16 * b + 8 * i);
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const int e = 8 * b + 4 * i + y, z = 4 * i + y;
-          p[z] = __builtin_amdgcn_exp2f(st[e] * a.c - le[y]);
-          ds[z] = p[z] * (dp[e] - dl[y]);
+    for (int g = 0; g < 2 * ND; ++g) {
+      if constexpr (cur) {
+        if (g + AHEAD < 2 * ND) cols_of(g + AHEAD);
+      }
+      if constexpr (follow) {
+        if (g >= 2 * ND - AHEAD) rows_of(bf, xf, g - 2 * ND + AHEAD);
+      }
+      if constexpr (next) {                 // the row terms of the unit that is THIS in the following call
+        if (g < 4) {
+          const float* ls = &Ls[bn][0][xn * 32 + 4 * h];
+          le[g] = *reinterpret_cast<const f32x4*>(ls + 8 * g);
+          dl[g] = *reinterpret_cast<const f32x4*>(ls + KR + 8 * g);
         }
       }
-      pf[b] = pack8<T>(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
-      sf[b] = pack8<T>(ds[0], ds[1], ds[2], ds[3], ds[4], ds[5], ds[6], ds[7]);
+      if constexpr (cur) {
+        av[g % ND] = El<T>::mma32(ot[g], pf[g / ND], av[g % ND]);
+        ak[g % ND] = El<T>::mma32(qt[g], sf[g / ND], ak[g % ND]);
+      }
+      fence();
     }
   };
-  auto gather = [&](int buf, int x, const v8 (&pf)[2], const v8 (&sf)[2]) __attribute__((always_inline)) {
-    const char *q = smem + buf * 2 * TILE + x * 32 * D * 2, *o = q + TILE;
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        const int at = b * 16 * D * 2;
-        av[d] = El<T>::mma32(join<T>(tr4<T>(reinterpret_cast<const T*>(o + to[d] + at)),
-                                     tr4<T>(reinterpret_cast<const T*>(o + tu[d] + at))), pf[b], av[d]);
-        ak[d] = El<T>::mma32(join<T>(tr4<T>(reinterpret_cast<const T*>(q + to[d] + at)),
-                                     tr4<T>(reinterpret_cast<const T*>(q + tu[d] + at))), sf[b], ak[d]);
-      }
-  };
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
 
   f32x16 s0, d0, s1, d1;
-  v8 pf[2], sf[2];
-  stage(j_wg, 0);
-  int buf = 0, prev = 2;
-  for (int j = j_wg; j < nt; ++j) {
-    dma_wait<0>();
-    if (tid < 2 * KR) (&Ls[buf][0][0])[tid] = lr;
+  int buf = RING - 1, next = 0;             // of the tile at work, and of the one after it
+  auto arrive = [&](int j) __attribute__((always_inline)) {   // tile j is there, the RING - 2 after it on their way
+    if (j + RING - 3 < nt) dma_wait<(RING - 3) * (2 * NL + 1)>();
+    else dma_wait<0>();
     __syncthreads();
-    const int next = buf == 2 ? 0 : buf + 1;
-    if (j + 1 < nt) stage(j + 1, next);
-    if (j > j_own) {
-      mask(2 * j - 1, s1);
-      scores(buf, 0, s0, d0);
-      grads(prev, 1, s1, d1, pf, sf);
-      gather(prev, 1, pf, sf);
-    } else if (j == j_own) {
-      scores(buf, 0, s0, d0);
-    }
-    if (j >= j_own) {
-      mask(2 * j, s0);
-      scores(buf, 1, s1, d1);
-      grads(buf, 0, s0, d0, pf, sf);
-      gather(buf, 0, pf, sf);
-    }
-    prev = buf;
+    if (j + RING - 2 < nt) stage(j + RING - 2, (next + RING - 2) % RING);
+  };
+  auto advance = [&]() __attribute__((always_inline)) {
     buf = next;
+    next = (next + 1) % RING;
+  };
+  int j = j_wg;
+#pragma unroll
+  for (int i = 0; i < RING - 2; ++i)
+    if (j + i < nt) stage(j + i, i);
+  for (; j <= j_own; ++j) {                 // rows before the wave's keys
+    arrive(j);
+    advance();
   }
+#pragma unroll
+  for (int s = 0; s < AHEAD; ++s) rows_of(buf, 0, s);
+  work(yes, no, yes, buf, 0, s0, d0, buf, 0, s0, d0, buf, 1);
+  for (; j < nt; ++j) {                     // tile j - 1, with the beginning of tile j
+    mask(2 * j - 2, s0);
+    arrive(j);
+    work(yes, yes, yes, buf, 1, s1, d1, buf, 0, s0, d0, next, 0);
+    mask(2 * j - 1, s1);
+    work(yes, yes, yes, next, 0, s0, d0, buf, 1, s1, d1, next, 1);
+    advance();
+  }
+  mask(2 * nt - 2, s0);
+  work(yes, yes, no, buf, 1, s1, d1, buf, 0, s0, d0, buf, 0);
   mask(2 * nt - 1, s1);
-  grads(prev, 1, s1, d1, pf, sf);
-  gather(prev, 1, pf, sf);
+  work(no, yes, no, buf, 0, s0, d0, buf, 1, s1, d1, buf, 0);
   if (key < t.tokens) {
 #pragma unroll
     for (int d = 0; d < ND; ++d)
