@@ -35,39 +35,38 @@ __device__ __forceinline__ int seq_keys(const DecArgs& a, int n) {
   return (int)min((int64_t)max(a.pages.lens[n], 0), (int64_t)a.pages.width * a.pages.page.d);
 }
 
-// Units before sequence n, for the sequences around a worker: the total of the list and,
-// for the unit `at`, the sequence that holds it and that sequence's first unit.  All
-// threads of the workgroup call it; sh holds 8 ints.
-struct Place { int64_t total; int seq; int64_t first; };
-__device__ Place find_unit(const DecArgs& a, int64_t at, int64_t* sh) {
+// The list of units, seen by one workgroup: `total` units, and where unit w * per lies, per
+// being the workers' share: its sequence and that sequence's first unit.  Every thread adds
+// up the sequences of its own run of N / 256.  All threads call it; sh holds 8 int64.
+struct Place { int64_t total, per; int seq; int64_t first; };
+__device__ __forceinline__ int64_t units_per(const DecArgs& a, int64_t total);
+__device__ __forceinline__ Place find_share(const DecArgs& a, int w, int64_t* sh) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  Place p{0, a.N, 0};
-  for (int n0 = 0; n0 < a.N; n0 += 256) {
-    const int n = n0 + tid;
-    const int u = n < a.N ? (seq_keys(a, n) + UNIT - 1) / UNIT : 0;
-    int64_t x = u;
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t y = __shfl_up(x, d, 64);
-      if (lane >= d) x += y;
-    }
-    __syncthreads();
-    if (lane == 63) sh[wave] = x;
-    if (tid == 0) sh[4] = -1;
-    __syncthreads();
-    int64_t base = p.total;
-    for (int w = 0; w < wave; ++w) base += sh[w];
-    const int64_t begin = base + x - u;
-    if (u > 0 && at >= begin && at < begin + u) {
-      sh[4] = n;
-      sh[5] = begin;
-    }
-    __syncthreads();
-    p.total += sh[0] + sh[1] + sh[2] + sh[3];
-    if (sh[4] >= 0) {
-      p.seq = (int)sh[4];
-      p.first = sh[5];
-    }
+  const int run = (a.N + 255) >> 8, n0 = min(tid * run, a.N), n1 = min(n0 + run, a.N);
+  int64_t mine = 0;
+  for (int n = n0; n < n1; ++n) mine += (seq_keys(a, n) + UNIT - 1) / UNIT;
+  int64_t x = mine;
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t y = __shfl_up(x, d, 64);
+    if (lane >= d) x += y;
   }
+  if (lane == 63) sh[wave] = x;
+  __syncthreads();
+  int64_t before = x - mine;
+  for (int i = 0; i < wave; ++i) before += sh[i];
+  Place p;
+  p.total = sh[0] + sh[1] + sh[2] + sh[3];
+  p.per = units_per(a, p.total);
+  const int64_t at = w * p.per;
+  if (at >= before && at < before + mine) {   // one thread, where there is such a unit
+    int n = n0;
+    for (int64_t u; (u = (seq_keys(a, n) + UNIT - 1) / UNIT) <= at - before; ++n) before += u;
+    sh[4] = n;
+    sh[5] = before;
+  }
+  __syncthreads();
+  p.seq = (int)sh[4];
+  p.first = sh[5];
   return p;
 }
 
@@ -104,11 +103,9 @@ __global__ __launch_bounds__(256, 2) void attn_decode_kernel(DecArgs a) {
           for (int i = 0; i < D / 8; ++i) reinterpret_cast<uint4*>(op)[i] = uint4{0, 0, 0, 0};
         }
   }
-  Place pl = find_unit(a, 0, s_scan);
-  const int64_t per = units_per(a, pl.total);
-  const int64_t u_beg = w * per, u_end = min(pl.total, u_beg + per);
+  const Place pl = find_share(a, w, s_scan);
+  const int64_t per = pl.per, u_beg = w * per, u_end = min(pl.total, u_beg + per);
   if (u_beg >= u_end) return;
-  pl = find_unit(a, u_beg, s_scan);
   int seq = pl.seq;
   int64_t first = pl.first, u = u_beg;
 
@@ -290,60 +287,73 @@ __global__ __launch_bounds__(256, 2) void attn_decode_kernel(DecArgs a) {
   }
 }
 
-// Sequences cut over several workers: their shares joined.
+// Sequences cut over several workers: their shares joined.  A workgroup takes one head of
+// one sequence; its threads take the shares in turn, D / 4 to a share, and meet in LDS.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_decode_join_kernel(DecArgs a) {
+  constexpr int TPS = D / 4, SH = 256 / TPS;
   __shared__ int64_t s_scan[8];
-  const int hb = blockIdx.x % (a.HKV * a.hblocks), n = blockIdx.x / (a.HKV * a.hblocks);
-  const int kvh = hb % a.HKV, g0 = (hb / a.HKV) * 16, ng = min(16, a.G - g0);
+  __shared__ __align__(16) f32x4 s_o[SH][TPS];
+  __shared__ float s_ml[SH][2];
+  const int H = a.HKV * a.G, head = blockIdx.x % H, n = blockIdx.x / H;
+  const int kvh = head / a.G, g = head - kvh * a.G, hb = (g >> 4) * a.HKV + kvh;
+  const int tid = threadIdx.x, lane = tid & 63;
   const int keys = seq_keys(a, n);
-  if (keys <= UNIT) return;   // one unit is never cut
-  // units before sequence n, and the total
-  int64_t before = 0, total = 0;
-  for (int n0 = 0; n0 < a.N; n0 += 256) {
-    const int x = n0 + (int)threadIdx.x;
-    const int64_t u = x < a.N ? (seq_keys(a, x) + UNIT - 1) / UNIT : 0;
-    int64_t b = x < n ? u : 0, t = u;
-    for (int d = 32; d >= 1; d >>= 1) {
-      b += __shfl_xor(b, d, 64);
-      t += __shfl_xor(t, d, 64);
-    }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) {
-      s_scan[threadIdx.x >> 6] = b;
-      s_scan[4 + (threadIdx.x >> 6)] = t;
-    }
-    __syncthreads();
-    for (int i = 0; i < 4; ++i) {
-      before += s_scan[i];
-      total += s_scan[4 + i];
-    }
+  if (keys <= UNIT) return;                 // one unit is never cut
+  int64_t before = 0, total = 0;            // units before sequence n, and of all
+  for (int x = tid; x < a.N; x += 256) {
+    const int64_t u = (seq_keys(a, x) + UNIT - 1) / UNIT;
+    total += u;
+    if (x < n) before += u;
   }
+  for (int d = 32; d >= 1; d >>= 1) {
+    before += __shfl_xor(before, d, 64);
+    total += __shfl_xor(total, d, 64);
+  }
+  if (lane == 0) {
+    s_scan[tid >> 6] = before;
+    s_scan[4 + (tid >> 6)] = total;
+  }
+  __syncthreads();
+  before = s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
+  total = s_scan[4] + s_scan[5] + s_scan[6] + s_scan[7];
   const int64_t per = units_per(a, total), last = before + (keys + UNIT - 1) / UNIT - 1;
-  const int64_t w0 = before / per, w1 = last / per;
+  const int w0 = (int)(before / per), w1 = (int)(last / per);
   if (w0 == w1) return;
   const int64_t hbs = (int64_t)a.HKV * a.hblocks, stats = (int64_t)a.W * 2 * hbs * 16 * D;
-  for (int i = threadIdx.x; i < ng * (D / 4); i += 256) {
-    const int g = i / (D / 4), d = 4 * (i % (D / 4));
-    float m = NEG_INF, l = 0.f;
-    for (int64_t w = w0; w <= w1; ++w) {
-      const int64_t slot = (w * 2 + (w * per < before ? 1 : 0)) * hbs + hb;
-      m = fmaxf(m, a.part[stats + slot * 32 + 2 * g]);
-    }
-    const float ref = m == NEG_INF ? 0.f : m;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int64_t w = w0; w <= w1; ++w) {
-      const int64_t slot = (w * 2 + (w * per < before ? 1 : 0)) * hbs + hb;
-      const float f = __builtin_amdgcn_exp2f(a.part[stats + slot * 32 + 2 * g] - ref);
-      l += f * a.part[stats + slot * 32 + 2 * g + 1];
-      o += f * *reinterpret_cast<const f32x4*>(a.part + (slot * 16 + g) * D + d);
+  const int d = tid % TPS, sh = tid / TPS;
+  float m = NEG_INF, l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int w = w0 + sh; w <= w1; w += SH) {
+    const int64_t slot = ((int64_t)w * 2 + (w * per < before ? 1 : 0)) * hbs + hb;
+    const float* ml = a.part + stats + slot * 32 + 2 * (g & 15);
+    const f32x4 x = *reinterpret_cast<const f32x4*>(a.part + (slot * 16 + (g & 15)) * D + 4 * d);
+    const float mn = fmaxf(m, ml[0]), ref = mn == NEG_INF ? 0.f : mn;
+    const float f = __builtin_amdgcn_exp2f(m - ref), e = __builtin_amdgcn_exp2f(ml[0] - ref);
+    l = l * f + ml[1] * e;
+    o = o * f + x * e;
+    m = mn;
+  }
+  s_o[sh][d] = o;
+  if (d == 0) {
+    s_ml[sh][0] = m;
+    s_ml[sh][1] = l;
+  }
+  __syncthreads();
+  if (sh == 0) {
+    for (int i = 1; i < SH; ++i) {
+      const float mi = s_ml[i][0], mn = fmaxf(m, mi), ref = mn == NEG_INF ? 0.f : mn;
+      const float f = __builtin_amdgcn_exp2f(m - ref), e = __builtin_amdgcn_exp2f(mi - ref);
+      l = l * f + s_ml[i][1] * e;
+      o = o * f + s_o[i][d] * e;
+      m = mn;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     typename El<T>::v4 y;
 #pragma unroll
     for (int z = 0; z < 4; ++z) y[z] = (T)(o[z] * inv);
-    *reinterpret_cast<typename El<T>::v4*>(a.o + (int64_t)n * a.o_ts + (int64_t)(kvh * a.G + g0 + g) * a.o_hs +
-                                           2 * d) = y;
+    *reinterpret_cast<typename El<T>::v4*>(a.o + (int64_t)n * a.o_ts + (int64_t)head * a.o_hs + 8 * d) = y;
   }
 }
 
@@ -361,7 +371,8 @@ template <typename T, int D>
 static void launch(const DecArgs& a, bool join, hipStream_t s) {
   const unsigned hbs = (unsigned)(a.HKV * a.hblocks);
   hipLaunchKernelGGL((attn_decode_kernel<T, D>), dim3(hbs * (unsigned)a.W), dim3(256), 0, s, a);
-  if (join) hipLaunchKernelGGL((attn_decode_join_kernel<T, D>), dim3(hbs * (unsigned)a.N), dim3(256), 0, s, a);
+  if (join)
+    hipLaunchKernelGGL((attn_decode_join_kernel<T, D>), dim3((unsigned)(a.HKV * a.G * a.N)), dim3(256), 0, s, a);
 }
 
 }  // namespace attn
@@ -414,7 +425,7 @@ extern "C" int hmx_paged_attention_decode(const void* q, int64_t q_token_stride,
   a.W = (int32_t)attn::workers(N, HKV, a.hblocks, max_keys);
   a.c = scale * attn::LOG2E;
   a.part = static_cast<float*>(workspace);
-  HMX_REQUIRE((int64_t)N * HKV * a.hblocks < (1ll << 31), HMX_EUNSUPPORTED,
+  HMX_REQUIRE((int64_t)N * H < (1ll << 31), HMX_EUNSUPPORTED,
               "hmx_paged_attention_decode: %d sequences of %d heads", N, H);
   const bool join = a.W > 1;
   HMX_REQUIRE(!join || (workspace && (uintptr_t)workspace % 16 == 0 &&
