@@ -207,7 +207,12 @@ def paged_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor |
     """ctypes pointer to an hmx_paged_kv of caches [pages, page size, HKV, D]; strides of
     dimensions of one, which are never used and may be anything, go as 0."""
     n = k_cache.shape
-    ks, vs = ([s if m > 1 else 0 for s, m in zip(t.stride()[:3], n)] for t in (k_cache, v_cache))
+    if k_cache.is_contiguous() and v_cache.is_contiguous():
+        hs = n[3]
+        ts = n[2] * hs
+        ks = vs = (n[1] * ts, ts, hs)
+    else:
+        ks, vs = ([x if m > 1 else 0 for x, m in zip(t.stride()[:3], n)] for t in (k_cache, v_cache))
     return ctypes.pointer(PagedKV(
         k_cache.data_ptr(), *ks, v_cache.data_ptr(), *vs, ptr(table),
         0 if table is None else table.stride(0), ptr(seq_lens),

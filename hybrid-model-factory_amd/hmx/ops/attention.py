@@ -15,7 +15,7 @@ so a captured graph replays with other lengths.
 """
 from __future__ import annotations
 
-import contextlib
+import functools
 
 import torch
 
@@ -26,17 +26,18 @@ _HEAD_SIZES = (64, 128)
 
 
 def _same_device(ref: torch.Tensor, *tensors: torch.Tensor | None) -> None:
-    _lib.require_gpu(ref, *tensors)
+    dev = ref.get_device()
     for t in tensors:
-        if t is not None and t.device != ref.device:
+        if t is not None and t.get_device() != dev:
+            _lib.require_gpu(ref, t)
             raise ValueError(f"tensors on {ref.device} and {t.device}")
+    if dev < 0:
+        _lib.require_gpu(ref)
 
 
-def _on_device(t: torch.Tensor):
-    """Launches go to the current device: make it the tensor's."""
-    if t.get_device() == torch._C._cuda_getDevice():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def _elsewhere(t: torch.Tensor) -> bool:
+    """Whether t's device is not the current one, to which launches go."""
+    return t.get_device() != torch._C._cuda_getDevice()
 
 
 def _check_types(what: str, q: torch.Tensor, *others: torch.Tensor | None) -> None:
@@ -51,6 +52,8 @@ def _check_types(what: str, q: torch.Tensor, *others: torch.Tensor | None) -> No
 
 def _aligned(t: torch.Tensor) -> bool:
     """Whether 16-byte loads reach every row of [..., heads, D] in place."""
+    if t.is_contiguous():
+        return t.data_ptr() % 16 == 0
     st, n = t.stride(), t.shape
     return (st[-1] == 1 and t.data_ptr() % 16 == 0
             and all(s % 8 == 0 or m == 1 for s, m in zip(st[:-1], n[:-1])))
@@ -59,6 +62,9 @@ def _aligned(t: torch.Tensor) -> bool:
 def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
     """(t, token stride, head stride) of [tokens, heads, D], or of [B, T, heads, D] whose
     tokens lie at one stride; a contiguous copy where there is no such view."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        H, D = t.shape[-2:]
+        return t, H * D, D
     B = t.shape[0] if t.dim() == 4 else 1
     T = t.shape[-3]
     if not _aligned(t) or (B > 1 and T > 1 and t.stride(0) != T * t.stride(1)):
@@ -79,6 +85,17 @@ def _out(out: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
     return out
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(name: str, device: int, *sizes: int) -> int:
+    """A workspace's size, which depends on the sizes and the device's compute units alone."""
+    return int(getattr(_lib.load(), name)(*sizes))
+
+
+def _workspace(name: str, like: torch.Tensor, *sizes: int) -> tuple[torch.Tensor | None, int]:
+    n = _workspace_bytes(name, like.get_device(), *sizes)
+    return (torch.empty(n, dtype=torch.uint8, device=like.device), n) if n else (None, 0)
+
+
 def _scale(scale: float | None, D: int) -> float:
     scale = D ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
@@ -96,7 +113,8 @@ def _offsets(cu_seqlens: torch.Tensor, T: int, device: torch.device) -> torch.Te
     if cu_seqlens.is_cuda:
         if cu_seqlens.device != device:
             raise ValueError(f"tensors on {device} and {cu_seqlens.device}")
-        return cu_seqlens.to(torch.int32).contiguous()
+        return cu_seqlens if cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous() \
+            else cu_seqlens.to(torch.int32).contiguous()
     seq_bounds(cu_seqlens, 1, T)
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("cu_seqlens must be on the device where a graph is captured")
@@ -139,22 +157,25 @@ def check_qkv(what: str, q, k, v, cu_seqlens) -> None:
 def attention_forward(q, k, v, scale, cu_seqlens, out, want_lse):
     """(o, base-2 log-sum-exp of the scaled scores [B * T, H] fp32 or None, device offsets or None)."""
     check_qkv("causal_attention", q, k, v, cu_seqlens)
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return attention_forward(q, k, v, scale, cu_seqlens, out, want_lse)
     B, T, H, D = q.shape
     scale = _scale(scale, D)
     o = _out(out, q)
-    _same_device(q, o)
-    with _on_device(q):
-        cu = None if cu_seqlens is None else _offsets(cu_seqlens, T, q.device)
-        N = B if cu is None else cu.shape[0] - 1
-        lse = torch.empty(B * T, H, dtype=torch.float32, device=q.device) if want_lse else None
-        q, qts, qhs = _rows(q)
-        k, kts, khs = _rows(k)
-        v, vts, vhs = _rows(v)
-        _, ots, ohs = _rows(o)
-        _lib.call("hmx_causal_attention", q.data_ptr(), qts, qhs, k.data_ptr(), kts, khs,
-                  v.data_ptr(), vts, vhs, _lib.dtype_code(q), o.data_ptr(), ots, ohs,
-                  _lib.ptr(lse), _lib.ptr(cu), N, B * T, H, k.shape[2], D, scale,
-                  int(out is None), _lib.stream_of(q))
+    if out is not None:
+        _same_device(q, o)
+    cu = None if cu_seqlens is None else _offsets(cu_seqlens, T, q.device)
+    N = B if cu is None else cu.shape[0] - 1
+    lse = torch.empty(B * T, H, dtype=torch.float32, device=q.device) if want_lse else None
+    q, qts, qhs = _rows(q)
+    k, kts, khs = _rows(k)
+    v, vts, vhs = _rows(v)
+    _, ots, ohs = _rows(o)
+    _lib.call("hmx_causal_attention", q.data_ptr(), qts, qhs, k.data_ptr(), kts, khs,
+              v.data_ptr(), vts, vhs, _lib.dtype_code(q), o.data_ptr(), ots, ohs,
+              _lib.ptr(lse), _lib.ptr(cu), N, B * T, H, k.shape[2], D, scale,
+              int(out is None), _lib.stream_of(q))
     return o, lse, cu
 
 
@@ -220,31 +241,35 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
             cos_sin = cos_sin.contiguous()
     H = 0 if q is None else q.shape[1]
     _same_device(k, v, k_cache, v_cache, slot_mapping, q, positions, cos_sin, q_out)
-    with _on_device(k):
-        ret = None
-        if q is not None:
-            if cos_sin is None and q_out is None:
-                ret, q = q, None                    # nothing to do for q
-            else:
-                ret = _out(q_out, q)
-        if T:
-            k, kts, khs = _rows(k)
-            v, vts, vhs = _rows(v)
-            qts = qhs = ots = ohs = 0
-            if q is not None:
-                q, qts, qhs = _rows(q)
-                _, ots, ohs = _rows(ret)
-            slot_mapping = slot_mapping.contiguous()
-            positions = None if positions is None else positions.contiguous()
-            cache = _lib.paged_kv(k_cache, v_cache)
-            _lib.call("hmx_append_paged_kv", _lib.ptr(q), qts, qhs, k.data_ptr(), kts, khs,
-                      v.data_ptr(), vts, vhs, _lib.dtype_code(k), None if q is None else ret.data_ptr(),
-                      ots, ohs, cache, slot_mapping.data_ptr(), int(slot_mapping.dtype == torch.int64),
-                      _lib.ptr(positions), int(positions is not None and positions.dtype == torch.int64),
-                      _lib.ptr(cos_sin), 0 if cos_sin is None else _lib.dtype_code(cos_sin),
-                      0 if cos_sin is None else cos_sin.stride(0),
-                      0 if cos_sin is None else cos_sin.shape[0], R, int(bool(interleaved)), T, H, HKV,
-                      D, _lib.stream_of(k))
+    if _elsewhere(k):
+        with torch.cuda.device(k.device):
+            return append_paged_kv(k, v, k_cache, v_cache, slot_mapping, q=q, positions=positions,
+                                   cos_sin=cos_sin, interleaved=interleaved, q_out=q_out)
+    ret = None
+    if q is not None:
+        if cos_sin is None and q_out is None:
+            ret, q = q, None                    # nothing to do for q
+        else:
+            ret = _out(q_out, q)
+    if T == 0:
+        return ret
+    k, kts, khs = _rows(k)
+    v, vts, vhs = _rows(v)
+    qts = qhs = ots = ohs = 0
+    if q is not None:
+        q, qts, qhs = _rows(q)
+        _, ots, ohs = _rows(ret)
+    slot_mapping = slot_mapping.contiguous()
+    cs = (None, 0, None, 0, 0, 0)
+    if cos_sin is not None:
+        positions = positions.contiguous()
+        cs = (positions.data_ptr(), int(positions.dtype == torch.int64), cos_sin.data_ptr(),
+              _lib.dtype_code(cos_sin), cos_sin.stride(0), cos_sin.shape[0])
+    _lib.call("hmx_append_paged_kv", _lib.ptr(q), qts, qhs, k.data_ptr(), kts, khs,
+              v.data_ptr(), vts, vhs, _lib.dtype_code(k), None if q is None else ret.data_ptr(),
+              ots, ohs, _lib.paged_kv(k_cache, v_cache), slot_mapping.data_ptr(),
+              int(slot_mapping.dtype == torch.int64), *cs, R, int(bool(interleaved)), T, H, HKV,
+              D, _lib.stream_of(k))
     return ret
 
 
@@ -271,15 +296,16 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     _same_device(q, k_cache, v_cache, block_table, seq_lens, o)
     if N == 0:
         return o
-    with _on_device(q):
-        q, qts, qhs = _rows(q)
-        _, ots, ohs = _rows(o)
-        most = block_table.shape[1] * k_cache.shape[1]
-        ws_bytes = int(_lib.load().hmx_paged_attention_decode_workspace_bytes(N, H, HKV, D, most))
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-        _lib.call("hmx_paged_attention_decode", q.data_ptr(), qts, qhs, _lib.dtype_code(q),
-                  o.data_ptr(), ots, ohs, _lib.paged_kv(k_cache, v_cache, block_table, seq_lens),
-                  N, H, HKV, D, scale, _lib.ptr(ws), ws_bytes, _lib.stream_of(q))
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, scale, out=o)
+    q, qts, qhs = _rows(q)
+    _, ots, ohs = _rows(o)
+    ws, ws_bytes = _workspace("hmx_paged_attention_decode_workspace_bytes", q, N, H, HKV, D,
+                              block_table.shape[1] * k_cache.shape[1])
+    _lib.call("hmx_paged_attention_decode", q.data_ptr(), qts, qhs, _lib.dtype_code(q),
+              o.data_ptr(), ots, ohs, _lib.paged_kv(k_cache, v_cache, block_table, seq_lens),
+              N, H, HKV, D, scale, _lib.ptr(ws), ws_bytes, _lib.stream_of(q))
     return o
 
 
@@ -309,17 +335,19 @@ def paged_causal_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     scale = _scale(scale, D)
     o = _out(out, q)
     _same_device(q, k_cache, v_cache, block_table, seq_lens, o)
-    with _on_device(q):
-        cu = _offsets(cu_seqlens, T, q.device)
-        if T == 0:
-            return o
-        q, qts, qhs = _rows(q)
-        _, ots, ohs = _rows(o)
-        most = block_table.shape[1] * k_cache.shape[1]
-        ws_bytes = int(_lib.load().hmx_paged_causal_attention_workspace_bytes(N, T, H, HKV, D, most))
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device) if ws_bytes else None
-        _lib.call("hmx_paged_causal_attention", q.data_ptr(), qts, qhs, _lib.dtype_code(q),
-                  o.data_ptr(), ots, ohs, _lib.paged_kv(k_cache, v_cache, block_table, seq_lens),
-                  _lib.ptr(cu), N, T, H, HKV, D, scale, int(out is None), _lib.ptr(ws), ws_bytes,
-                  _lib.stream_of(q))
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return paged_causal_attention(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens,
+                                          scale, out=out)
+    cu = _offsets(cu_seqlens, T, q.device)
+    if T == 0:
+        return o
+    q, qts, qhs = _rows(q)
+    _, ots, ohs = _rows(o)
+    ws, ws_bytes = _workspace("hmx_paged_causal_attention_workspace_bytes", q, N, T, H, HKV, D,
+                              block_table.shape[1] * k_cache.shape[1])
+    _lib.call("hmx_paged_causal_attention", q.data_ptr(), qts, qhs, _lib.dtype_code(q),
+              o.data_ptr(), ots, ohs, _lib.paged_kv(k_cache, v_cache, block_table, seq_lens),
+              _lib.ptr(cu), N, T, H, HKV, D, scale, int(out is None), _lib.ptr(ws), ws_bytes,
+              _lib.stream_of(q))
     return o

@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from .attention import _on_device, _rows, _scale, attention_forward, check_qkv
+from .attention import _elsewhere, _rows, _scale, attention_forward, check_qkv
 
 
 class CausalAttention(torch.autograd.Function):
@@ -32,19 +32,20 @@ class CausalAttention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
         q, k, v, o, lse, cu = ctx.saved_tensors
-        B, T, H, D = q.shape
-        HKV = k.shape[2]
-        with _on_device(q):
-            N = B if cu is None else cu.shape[0] - 1
-            dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
-            delta = torch.empty_like(lse)
-            args = []
-            for x in (q, k, v, o, do.to(torch.bfloat16)):
-                x, ts, hs = _rows(x)
-                args.append((x, ts, hs))
-            flat = [y for x, ts, hs in args for y in (x.data_ptr(), ts, hs)]
-            grads = [y for x in (dq, dk, dv) for y in (x.data_ptr(), *_rows(x)[1:])]
-            _lib.call("hmx_causal_attention_bwd", *flat[:9], _lib.HMX_BF16, *flat[9:], lse.data_ptr(),
-                      _lib.ptr(cu), N, B * T, H, HKV, D, ctx.scale, *grads, delta.data_ptr(),
-                      _lib.stream_of(q))
-        return dq, dk, dv, None, None
+        if _elsewhere(q):
+            with torch.cuda.device(q.device):
+                return (*_backward(q, k, v, o, lse, cu, do, ctx.scale), None, None)
+        return (*_backward(q, k, v, o, lse, cu, do, ctx.scale), None, None)
+
+
+def _backward(q, k, v, o, lse, cu, do, scale):
+    B, T, H, D = q.shape
+    dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
+    delta = torch.empty_like(lse)
+    rows = [_rows(x) for x in (q, k, v, o, do.to(torch.bfloat16))]     # held until the launch
+    ins = [y for x, ts, hs in rows for y in (x.data_ptr(), ts, hs)]
+    grads = [y for x in (dq, dk, dv) for y in (x.data_ptr(), *_rows(x)[1:])]
+    _lib.call("hmx_causal_attention_bwd", *ins[:9], _lib.HMX_BF16, *ins[9:], lse.data_ptr(),
+              _lib.ptr(cu), B if cu is None else cu.shape[0] - 1, B * T, H, k.shape[2], D, scale,
+              *grads, delta.data_ptr(), _lib.stream_of(q))
+    return dq, dk, dv

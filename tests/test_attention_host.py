@@ -1,0 +1,158 @@
+"""Host-side checks of the attention ops (CPU): refusals before any launch, the C entry
+points' own checks, and the oracle's gradients against differences."""
+import ctypes
+
+import pytest
+import torch
+
+import hmx
+from hmx import _lib
+from oracle import attention as ref
+
+BF = torch.bfloat16
+
+
+def _qkv(B=1, T=4, H=4, HKV=2, D=64, dtype=BF):
+    return (torch.zeros(B, T, H, D, dtype=dtype), torch.zeros(B, T, HKV, D, dtype=dtype),
+            torch.zeros(B, T, HKV, D, dtype=dtype))
+
+
+def _cache(pages=3, page=16, HKV=2, D=64, dtype=BF):
+    return torch.zeros(pages, page, HKV, D, dtype=dtype), torch.zeros(pages, page, HKV, D, dtype=dtype)
+
+
+def test_causal_attention_refusals():
+    q, k, v = _qkv()
+    cu = torch.tensor([0, 4], dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="GPU"):
+        hmx.causal_attention(q, k, v)
+    with pytest.raises(ValueError, match="Batch size expected to be 1"):
+        hmx.causal_attention(*_qkv(B=2), cu_seqlens=cu)
+    with pytest.raises(NotImplementedError, match="bf16 or fp16"):
+        hmx.causal_attention(*_qkv(dtype=torch.float32))
+    with pytest.raises(NotImplementedError, match="head size"):
+        hmx.causal_attention(*_qkv(D=96))
+    with pytest.raises(ValueError, match="differ"):
+        hmx.causal_attention(q, k.half(), v)
+    with pytest.raises(ValueError, match="cannot share"):
+        hmx.causal_attention(*_qkv(H=3))
+    for bad in ((q[0], k, v), (q, k[:, :3], v), (q, k, v[:, :, :1]), (q, k[..., :32], v[..., :32])):
+        with pytest.raises(ValueError):
+            hmx.causal_attention(*bad)
+
+
+@pytest.mark.parametrize("cu", [[1, 4], [0, 5], [0, 3, 2], []])
+def test_bad_host_offsets(cu):
+    from hmx.ops.attention import _offsets
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        _offsets(torch.tensor(cu, dtype=torch.int32), 4, torch.device("cuda", 0))
+    with pytest.raises(ValueError, match="int32 or int64"):
+        _offsets(torch.tensor([0.0, 4.0]), 4, torch.device("cuda", 0))
+
+
+@pytest.mark.parametrize("scale", [0.0, -1.0, float("nan"), float("inf")])
+def test_bad_scale(scale):
+    from hmx.ops.attention import _scale
+    with pytest.raises(ValueError, match="positive"):
+        _scale(scale, 64)
+
+
+def test_append_refusals():
+    k = torch.zeros(5, 2, 64, dtype=BF)
+    kc, vc = _cache()
+    slots = torch.arange(5)
+    cs, pos = torch.zeros(9, 64), torch.arange(5)
+    call = lambda **kw: hmx.append_paged_kv(**{**dict(k=k, v=k, k_cache=kc, v_cache=vc, slot_mapping=slots), **kw})
+    with pytest.raises(RuntimeError, match="GPU"):
+        call()
+    for kw in (dict(v=k[:4]), dict(slot_mapping=slots[:4]), dict(slot_mapping=slots.float()),
+               dict(cos_sin=cs), dict(positions=pos), dict(cos_sin=cs[:, :24], positions=pos),
+               dict(cos_sin=torch.zeros(9, 128), positions=pos), dict(cos_sin=cs, positions=pos[:2]),
+               dict(k_cache=kc[:, :, :1]), dict(v_cache=vc[:2]), dict(q=torch.zeros(4, 4, 64, dtype=BF)),
+               dict(q_out=k), dict(k_cache=kc.half(), v_cache=vc.half()),
+               dict(k_cache=kc[..., ::1].transpose(2, 3).contiguous().transpose(2, 3))):
+        with pytest.raises(ValueError):
+            call(**kw)
+    with pytest.raises(NotImplementedError):
+        call(k=k.float(), v=k.float())
+
+
+def test_paged_refusals():
+    kc, vc = _cache()
+    table, lens = torch.zeros(2, 3, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    q = torch.zeros(2, 4, 64, dtype=BF)
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="GPU"):
+        hmx.paged_attention_decode(q, kc, vc, table, lens)
+    with pytest.raises(RuntimeError, match="GPU"):
+        hmx.paged_causal_attention(q, kc, vc, table, lens, cu)
+    for kw in (dict(block_table=table.long()), dict(seq_lens=lens.long()), dict(seq_lens=lens[:1]),
+               dict(block_table=table[:1]), dict(q=q[:, :3]), dict(scale=0.0), dict(q=q[0]),
+               dict(out=q[:, :2]), dict(out=q.half()), dict(k_cache=kc[:, :8]),
+               dict(block_table=table.t().contiguous().t())):
+        args = {**dict(q=q, k_cache=kc, v_cache=vc, block_table=table, seq_lens=lens), **kw}
+        with pytest.raises(ValueError):
+            hmx.paged_attention_decode(**args)
+        with pytest.raises(ValueError):
+            hmx.paged_causal_attention(cu_seqlens=cu, **args)
+
+
+def test_c_entry_points_check_before_launching():
+    """Sizes, types, strides and workspaces are refused by the library itself."""
+    kv = _lib.PagedKV(0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 4, 3, 16)
+    p = ctypes.pointer(kv)
+    dec = lambda N=1, H=4, HKV=2, D=64, dt=1, scale=1.0: _lib.call(
+        "hmx_paged_attention_decode", None, 0, 0, dt, None, 0, 0, p, N, H, HKV, D, scale, None, 0, None)
+    with pytest.raises(NotImplementedError, match="head size 96"):
+        dec(D=96)
+    with pytest.raises(NotImplementedError, match="dtype"):
+        dec(dt=0)
+    with pytest.raises(ValueError, match="H=3"):
+        dec(H=3)
+    with pytest.raises(ValueError, match="positive"):
+        dec(scale=0.0)
+    with pytest.raises(ValueError, match="null pointer"):
+        dec()
+    dec(N=0)
+    with pytest.raises(ValueError, match="is not N"):
+        _lib.call("hmx_causal_attention", None, 0, 0, None, 0, 0, None, 0, 0, 1, None, 0, 0, None, None,
+                  2, 7, 4, 2, 64, 1.0, 1, None)
+    with pytest.raises(ValueError, match="null pointer"):
+        _lib.call("hmx_causal_attention", None, 0, 0, None, 0, 0, None, 0, 0, 1, None, 0, 0, None, None,
+                  1, 7, 4, 2, 64, 1.0, 1, None)
+    with pytest.raises(NotImplementedError, match="bf16 only"):
+        _lib.call("hmx_causal_attention_bwd", *([None, 0, 0] * 3), 2, *([None, 0, 0] * 2), None, None, 1, 7,
+                  4, 2, 64, 1.0, *([None, 0, 0] * 3), None, None)
+    with pytest.raises(NotImplementedError, match="rotary_dim"):
+        _lib.call("hmx_append_paged_kv", None, 0, 0, None, 0, 0, None, 0, 0, 1, None, 0, 0, p, None, 1,
+                  None, 0, None, 0, 0, 0, 24, 0, 5, 4, 2, 64, None)
+
+
+def test_oracle_gradients_against_differences():
+    """causal_grads (formulas) against central differences of causal (definition)."""
+    gen = torch.Generator().manual_seed(0)
+    T, H, HKV, D = 9, 4, 2, 5
+    bounds = [(0, 4), (4, 4), (5, 9)]
+    xs = [torch.randn(T, n, D, generator=gen, dtype=torch.float64) for n in (H, HKV, HKV)]
+    do = torch.randn(T, H, D, generator=gen, dtype=torch.float64)
+    (o, *grads), _ = ref.causal_grads(*xs, 0.4, bounds, do)
+    assert (o - ref.causal(*xs, 0.4, bounds)[0]).abs().max() < 1e-13
+    loss = lambda ys: (ref.causal(*ys, 0.4, bounds)[0] * do).sum()
+    for i in range(3):
+        u = torch.randn(xs[i].shape, generator=gen, dtype=torch.float64)
+        hi, lo = ([x + s * 1e-5 * u if j == i else x for j, x in enumerate(xs)] for s in (1, -1))
+        diff = (loss(hi) - loss(lo)) / 2e-5
+        assert abs(diff - (grads[i] * u).sum()) < 1e-8 * (1 + abs(diff))
+
+
+def test_oracle_rotation_and_rows_by_hand():
+    x = torch.tensor([[[1.0, 2.0, 3.0, 4.0, 5.0]]])
+    cs = torch.tensor([[0.0, 1.0, 1.0, 0.0]])                    # turns pair 0 by a quarter, pair 1 not
+    assert ref.rotate(x, cs, torch.tensor([0]), False)[0, 0].tolist() == [-3.0, 2.0, 1.0, 4.0, 5.0]
+    assert ref.rotate(x, cs, torch.tensor([0]), True)[0, 0].tolist() == [-2.0, 1.0, 3.0, 4.0, 5.0]
+    q = torch.zeros(3, 1, 2)
+    k = torch.zeros(2, 1, 2)
+    v = torch.tensor([[[1.0, 3.0]], [[3.0, float("inf")]]])
+    o, a = ref.rows(q, k, v, 1.0, -1)                            # row 0 has no key, row 2 both
+    assert o[0].tolist() == [[0.0, 0.0]] and o[1].tolist() == [[1.0, 3.0]]
+    assert o[2, 0, 0] == 2.0 and o[2, 0, 1] == float("inf")
