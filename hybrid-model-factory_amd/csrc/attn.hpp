@@ -18,6 +18,11 @@ template <> struct El<bf16> {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
   static __device__ __forceinline__ f32x4 mma16(v8 a, v8 b, f32x4 c) { return mfma16(a, b, c); }
+  // 16x16x16: row (column) l & 15, k = 4 (l >> 4) .. + 3, the C layout of a tile
+  static __device__ __forceinline__ f32x4 mma16k16(v4 a, v4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c,
+                                                     0, 0, 0);
+  }
 };
 template <> struct El<f16> {
   typedef f16x8 v8;
@@ -26,6 +31,7 @@ template <> struct El<f16> {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
   static __device__ __forceinline__ f32x4 mma16(v8 a, v8 b, f32x4 c) { return mfma16h(a, b, c); }
+  static __device__ __forceinline__ f32x4 mma16k16(v4 a, v4 b, f32x4 c) { return mfma16h_k16(a, b, c); }
 };
 
 template <typename T>
@@ -76,6 +82,13 @@ __device__ __forceinline__ float half_max(float a) {
   const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, a),
                                                   __builtin_bit_cast(unsigned, a), false, false);
   return fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
+}
+
+// over the lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float q4_max(float a) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, a),
+                                                  __builtin_bit_cast(unsigned, a), false, false);
+  return half_max(fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1])));
 }
 
 // 16 bytes a lane from memory into LDS without a trip through registers: lane l's go to

@@ -7,10 +7,10 @@
 // so the work is cut there: the keys of all sequences, in units of 64, form one list, and
 // worker w of W takes units [w per, (w + 1) per).  All workers get the same share whatever
 // the lengths are, and a sequence cut over several workers is joined by a second launch
-// from fp32 shares.  A worker's four waves take 32 keys in turn; nothing is shared between
-// them until a sequence's share ends.  K goes from memory to registers as the A operand
-// (S^T = K Q^T), V through the wave's own LDS tile to be read transposed
-// (O^T = V^T P^T); the next 32 keys are in flight meanwhile.
+// from fp32 shares.  A worker's four waves take 16 keys in turn; nothing is shared between
+// them until a sequence's share ends.  K and V rows go straight into the wave's own ring in
+// LDS, whole rows to a load, RING - 1 turns ahead, and are read there as the A operands of
+// S^T = K Q^T and (transposed) of O^T = V^T P^T.
 // P is rounded to the inputs' type; scores, statistics and O stay in fp32.
 #include "attn.hpp"
 
@@ -18,15 +18,19 @@ namespace hmx {
 namespace attn {
 
 constexpr int UNIT = 64;     // keys of a unit
-constexpr int KT = 32;       // keys of a wave's step
+constexpr int KT = 16;       // keys of a wave's turn
+constexpr int NW = 4;        // waves
 constexpr int MIN_UNITS = 4; // of a worker: below that the joining costs more than it gains
+// Where a table holds no more keys than this, a worker takes whole sequences: one launch and
+// no scan of the lengths (one sequence of 700 keys: SHORT_FIGURES).
+constexpr int SHORT_KEYS = 1024;
 
 struct DecArgs {
   const char* q;
   char* o;
   int64_t q_ts, q_hs, o_ts, o_hs;   // bytes
   Pages pages;
-  int32_t N, HKV, G, hblocks, W;    // hblocks: blocks of 16 heads of a group
+  int32_t N, HKV, G, hblocks, W;    // hblocks: blocks of 16 heads of a group; W = 0: worker w takes sequence w
   float c;
   float* part;   // [W][2][HKV * hblocks][16][D], then [W][2][HKV * hblocks][16][2]
 };
@@ -75,59 +79,75 @@ __device__ __forceinline__ int64_t units_per(const DecArgs& a, int64_t total) {
   return per < MIN_UNITS ? MIN_UNITS : per;
 }
 
-// 16-byte chunk at which chunk c of key row r sits: the transposing reads take 16 rows by
-// 32 bytes, spread evenly over the banks
-template <int D> __device__ __forceinline__ int dpos(int r, int c) {
-  return D == 128 ? c ^ ((r & 7) << 1) : c ^ (((r >> 1) & 3) << 1);
-}
-
 template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void attn_decode_kernel(DecArgs a) {
+__global__ __launch_bounds__(64 * NW) void attn_decode_kernel(DecArgs a) {
   typedef typename El<T>::v8 v8;
-  constexpr int NS = D / 32, ND = D / 16;
-  __shared__ __align__(16) char smem[4 * KT * D * 2 > 4 * 16 * D * 4 ? 4 * KT * D * 2 : 4 * 16 * D * 4];
-  __shared__ float s_ml[4][16][2];
+  typedef typename El<T>::v4 v4;
+  constexpr int NS = D / 32, ND = D / 16, NC = D / 8;
+  constexpr int RI = 64 / NC, NL = KT / RI;  // rows of a load, loads of K (and V) of a turn
+  constexpr int RING = D == 128 ? 4 : 8;     // turns: 128 KB of LDS for the four waves
+  constexpr int KV = KT * D * 2;             // bytes of a turn's K, and of its V behind it
+  __shared__ __align__(1024) char smem[NW * RING * 2 * KV];   // the rings, then the shares [16][D] in fp32
+  __shared__ float s_ml[NW][16][2];
   __shared__ int64_t s_scan[8];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, q4 = lane >> 4, l16 = lane & 15;
+  const int tid = threadIdx.x, lane = tid & 63, q4 = lane >> 4, l16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hb = blockIdx.x % (a.HKV * a.hblocks), w = blockIdx.x / (a.HKV * a.hblocks);
   const int kvh = hb % a.HKV, g0 = (hb / a.HKV) * 16;
   const int ng = min(16, a.G - g0);
 
-  // rows without keys
-  if (w == 0) {
-    for (int n = tid; n < a.N; n += 256)
-      if (seq_keys(a, n) == 0)
-        for (int g = 0; g < ng; ++g) {
-          char* op = a.o + (int64_t)n * a.o_ts + (int64_t)(kvh * a.G + g0 + g) * a.o_hs;
-          for (int i = 0; i < D / 8; ++i) reinterpret_cast<uint4*>(op)[i] = uint4{0, 0, 0, 0};
-        }
+  auto zero_row = [&](int n) {
+    for (int i = tid; i < ng * (D / 8); i += 64 * NW)
+      *reinterpret_cast<u32x4*>(a.o + (int64_t)n * a.o_ts + (int64_t)(kvh * a.G + g0 + i / (D / 8)) * a.o_hs +
+                                16 * (i % (D / 8))) = u32x4{0, 0, 0, 0};
+  };
+  int seq = __builtin_amdgcn_readfirstlane(w);
+  int64_t first = 0, u_beg = 0, u_end;
+  if (a.W == 0) {
+    u_end = (seq_keys(a, w) + UNIT - 1) / UNIT;
+    if (u_end == 0) zero_row(w);
+  } else {
+    // rows without keys, a worker every W-th sequence
+    for (int n = w; n < a.N; n += a.W)
+      if (seq_keys(a, n) == 0) zero_row(n);
+    const Place pl = find_share(a, w, s_scan);
+    u_beg = w * pl.per;
+    u_end = min(pl.total, u_beg + pl.per);
+    seq = __builtin_amdgcn_readfirstlane(pl.seq);
+    first = pl.first;
   }
-  const Place pl = find_share(a, w, s_scan);
-  const int64_t per = pl.per, u_beg = w * per, u_end = min(pl.total, u_beg + per);
   if (u_beg >= u_end) return;
-  int seq = pl.seq;
-  int64_t first = pl.first, u = u_beg;
+  int64_t u = u_beg;
 
-  T* Vt = reinterpret_cast<T*>(smem) + wave * KT * D;
-  int wo[NS];                                // where the lane's chunks of a V row go
+  char* ring = smem + wave * RING * 2 * KV;
+  const uint32_t ring_at = lds_addr(ring);
+  int ko[NS], vo[ND];                       // the lane's byte offsets into a turn's K and V
 #pragma unroll
-  for (int s = 0; s < NS; ++s) wo[s] = dpos<D>(l16, 4 * s + q4) * 8;
-  int ro[ND];                                // and where its transposing reads start
+  for (int s = 0; s < NS; ++s) ko[s] = (l16 * D + swz<D>(l16, 4 * s + q4) * 8) * 2;
 #pragma unroll
   for (int d = 0; d < ND; ++d) {
-    const int s = l16, r = 4 * q4 + (s >> 2);
-    ro[d] = r * D + dpos<D>(r, 2 * d + ((s & 3) >> 1)) * 8 + 4 * (s & 1);
+    const int r = 4 * q4 + (l16 >> 2);
+    vo[d] = KV + (r * D + swz<D>(r, 2 * d + ((l16 & 3) >> 1)) * 8 + 4 * (l16 & 1)) * 2;
   }
+  uint32_t koff[NL], voff[NL];              // and its chunks' offsets from the turn's first row in a page
+#pragma unroll
+  for (int i = 0; i < NL; ++i) {
+    const int r = i * RI + lane / NC, c = swz<D>(r, lane % NC);
+    koff[i] = (uint32_t)(r * (int)a.pages.k_ts + 16 * c);
+    voff[i] = (uint32_t)(r * (int)a.pages.v_ts + 16 * c);
+  }
+  const char *kbase = a.pages.k + (int64_t)kvh * a.pages.k_hs, *vbase = a.pages.v + (int64_t)kvh * a.pages.v_hs;
+  const bool one_page = a.pages.page.d % KT == 0;   // a turn's rows lie in one page
 
   while (u < u_end) {
     // this worker's share of sequence seq: keys k_beg .. k_end - 1
-    int keys = seq_keys(a, seq);
-    while (keys == 0) keys = seq_keys(a, ++seq);     // u < total: a sequence with keys follows
+    int keys = __builtin_amdgcn_readfirstlane(seq_keys(a, seq));
+    while (keys == 0) keys = __builtin_amdgcn_readfirstlane(seq_keys(a, ++seq));     // u < total: a sequence with keys follows
     const int64_t units = (keys + UNIT - 1) / UNIT;
-    const int k_beg = (int)(u - first) * UNIT;
+    const int k_beg = __builtin_amdgcn_readfirstlane((int)(u - first) * UNIT);
     const int64_t stop = min(u_end, first + units);
-    const int k_end = min(keys, (int)(stop - first) * UNIT);
+    const int k_end = __builtin_amdgcn_readfirstlane(min(keys, (int)(stop - first) * UNIT));
     const int32_t* table = a.pages.table + (int64_t)seq * a.pages.table_stride;
 
     v8 qf[NS];
@@ -142,77 +162,67 @@ __global__ __launch_bounds__(256, 2) void attn_decode_kernel(DecArgs a) {
     for (int d = 0; d < ND; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = NEG_INF, l = 0.f;
 
-    v8 kf[2][NS], vf[2][NS], kn[2][NS], vn[2][NS];
-    int pid[2];
-    bool okn[2] = {false, false}, ok[2];
-    auto fetch_pages = [&](int k0) {
+    // turn x of the wave's: keys k_beg + (x NW + wave) KT ..; live: which of its rows are keys
+    const int turns = k_end - k_beg > wave * KT ? (k_end - k_beg - wave * KT + NW * KT - 1) / (NW * KT) : 0;
+    uint32_t live[RING];
+    auto fetch = [&](int x) __attribute__((always_inline)) {
+      const int k0 = k_beg + (x * NW + wave) * KT;
+      const uint32_t lds = ring_at + (x % RING) * 2 * KV;
+      const int n = k_end - k0;
+      uint32_t mask = n >= KT ? (1u << KT) - 1 : (1u << n) - 1;
+      if (one_page) {
+        // rows behind the last key are the page's own: what they hold is masked
+        const int p = __builtin_amdgcn_readfirstlane(fdiv(k0, a.pages.page));
+        int id = uniform_load(table, p);
+        if ((unsigned)id >= (unsigned)a.pages.num_pages) id = 0, mask = 0;
+        const int64_t in = k0 - p * a.pages.page.d;
+        const char *kb = uniform_ptr(kbase + id * a.pages.k_ps + in * a.pages.k_ts);
+        const char *vb = uniform_ptr(vbase + id * a.pages.v_ps + in * a.pages.v_ts);
 #pragma unroll
-      for (int x = 0; x < 2; ++x) pid[x] = table[fdiv(min(k0 + 16 * x + l16, k_end - 1), a.pages.page)];
+        for (int i = 0; i < NL; ++i) dma16(lds + i * RI * D * 2, kb, koff[i]);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) dma16(lds + KV + i * RI * D * 2, vb, voff[i]);
+      } else {
+        const int mine = min(k0 + l16, k_end - 1);
+        mask &= (uint32_t)__ballot((unsigned)table[fdiv(mine, a.pages.page)] < (unsigned)a.pages.num_pages);
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+          const int x16 = i * RI + lane / NC, key = min(k0 + x16, k_end - 1), p = fdiv(key, a.pages.page);
+          int id = table[p];
+          if ((unsigned)id >= (unsigned)a.pages.num_pages) id = 0;
+          const int64_t in = key - p * a.pages.page.d;
+          const int c = 16 * swz<D>(x16, lane % NC);
+          dma16(lds + i * RI * D * 2, kbase + id * a.pages.k_ps + in * a.pages.k_ts + c);
+          dma16(lds + KV + i * RI * D * 2, vbase + id * a.pages.v_ps + in * a.pages.v_ts + c);
+        }
+      }
+      return mask;
     };
-    auto load = [&](int k0) {
+    // x is a multiple of RING plus the constant i: live[] stays in registers
+    auto turn = [&](int x, int i) __attribute__((always_inline)) {
+      if (x + RING - 2 < turns) dma_wait<(RING - 2) * 2 * NL>();
+      else dma_wait<0>();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the turn before has been read
+      char* tile = ring + i * 2 * KV;
+      const uint32_t mask = live[i];
+      if (x + RING - 1 < turns) live[(i + RING - 1) % RING] = fetch(x + RING - 1);
+      if (mask != (1u << KT) - 1) {
+        // V rows that are no keys to 0: their probability is 0, their memory anything
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int key = min(k0 + 16 * x + l16, k_end - 1);
-        const int64_t in = key - fdiv(key, a.pages.page) * a.pages.page.d;
-        const bool pg = (unsigned)pid[x] < (unsigned)a.pages.num_pages;
-        const int64_t p = pg ? pid[x] : 0;
-        okn[x] = pg && k0 + 16 * x + l16 < k_end;
-        const char* kp = a.pages.k + p * a.pages.k_ps + in * a.pages.k_ts + kvh * a.pages.k_hs + 16 * q4;
-        const char* vp = a.pages.v + p * a.pages.v_ps + in * a.pages.v_ts + kvh * a.pages.v_hs + 16 * q4;
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-          kn[x][s] = *reinterpret_cast<const v8*>(kp + 64 * s);
-          vn[x][s] = *reinterpret_cast<const v8*>(vp + 64 * s);
-        }
+        for (int z = 0; z < NL; ++z)
+          if (!((mask >> (z * RI + lane / NC)) & 1))
+            *reinterpret_cast<u32x4*>(tile + KV + (z * 64 + lane) * 16) = u32x4{0, 0, 0, 0};
       }
-    };
-    int k0 = k_beg + wave * KT;
-    if (k0 < k_end) {
-      fetch_pages(k0);
-      load(k0);
-      if (k0 + 4 * KT < k_end) fetch_pages(k0 + 4 * KT);
-    }
-    for (; k0 < k_end; k0 += 4 * KT) {
+      f32x4 st = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        ok[x] = okn[x];
+      for (int s = 0; s < NS; ++s) st = El<T>::mma16(*reinterpret_cast<const v8*>(tile + ko[s]), qf[s], st);
+      if (mask != (1u << KT) - 1) {
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-          kf[x][s] = kn[x][s];
-          vf[x][s] = vn[x][s];
-        }
+        for (int z = 0; z < 4; ++z)
+          if (!((mask >> (4 * q4 + z)) & 1)) st[z] = NEG_INF;
       }
-      if (k0 + 4 * KT < k_end) {
-        load(k0 + 4 * KT);
-        if (k0 + 8 * KT < k_end) fetch_pages(k0 + 8 * KT);
-      }
-      // V into the wave's tile; rows that are no keys as zeros (their probability is 0,
-      // their memory anything)
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-          v8 z = vf[x][s];
-          if (!ok[x]) z = v8{0};
-          *reinterpret_cast<v8*>(Vt + (16 * x + l16) * D + wo[s]) = z;
-        }
-      f32x4 st[2];
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        st[x] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < NS; ++s) st[x] = El<T>::mma16(kf[x][s], qf[s], st[x]);
-        // bit r of the ballot's low 16: row r holds a key
-        const unsigned long long live = __ballot(ok[x]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (!((live >> (4 * q4 + i)) & 1)) st[x][i] = NEG_INF;
-      }
-      float mx = NEG_INF;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(st[0][i], st[1][i]));
-      mx = half_max(mx);
-      mx = fmaxf(mx, shfl_xor(mx, 16));
+      float mx = fmaxf(fmaxf(st[0], st[1]), fmaxf(st[2], st[3]));
+      mx = q4_max(mx);
       if (__any((mx - m) * a.c > 8.f)) {
         const float mn = fmaxf(m, mx);
         const float f = m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((m - mn) * a.c);
@@ -222,23 +232,28 @@ __global__ __launch_bounds__(256, 2) void attn_decode_kernel(DecArgs a) {
         for (int d = 0; d < ND; ++d) acc[d] *= f;
       }
       const float mc = m == NEG_INF ? 0.f : m * a.c;
-      float p[8];
+      v4 pf;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(st[i >> 2][i & 3] * a.c - mc);
-        l += p[i];
+      for (int z = 0; z < 4; ++z) {
+        const float p = __builtin_amdgcn_exp2f(st[z] * a.c - mc);
+        l += p;
+        pf[z] = (T)p;
       }
-      const v8 pf = pack8<T>(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
 #pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        const v8 vt = join<T>(tr4<T>(Vt + ro[d]), tr4<T>(Vt + ro[d] + 16 * D));
-        acc[d] = El<T>::mma16(vt, pf, acc[d]);
-      }
+      for (int d = 0; d < ND; ++d)
+        acc[d] = El<T>::mma16k16(tr4<T>(reinterpret_cast<const T*>(tile + vo[d])), pf, acc[d]);
+    };
+#pragma unroll
+    for (int i = 0; i < RING - 1; ++i)
+      if (i < turns) live[i] = fetch(i);
+    for (int x = 0; x < turns; x += RING) {
+#pragma unroll
+      for (int i = 0; i < RING; ++i)
+        if (x + i < turns) turn(x + i, i);
     }
-    l += shfl_xor(l, 16);
-    l = pair_sum32(l, l);
+    l = q4_sum(l);
 
-    // the four waves' shares joined through LDS: O^T rows 16 d + 4 q4 + i, column l16
+    // the waves' shares joined through LDS: O^T rows 16 d + 4 q4 + i, column l16
     __syncthreads();
     float* ob = reinterpret_cast<float*>(smem);       // [wave][16][D]
 #pragma unroll
@@ -254,13 +269,13 @@ __global__ __launch_bounds__(256, 2) void attn_decode_kernel(DecArgs a) {
     const int64_t slot = ((int64_t)w * 2 + piece) * a.HKV * a.hblocks + hb;
     float* pp = a.part + slot * 16 * D;
     float* pm = a.part + (int64_t)a.W * 2 * a.HKV * a.hblocks * 16 * D + slot * 32;
-    for (int i = tid; i < ng * (D / 4); i += 256) {
+    for (int i = tid; i < ng * (D / 4); i += 64 * NW) {
       const int g = i / (D / 4), d = 4 * (i % (D / 4));
       float mm = NEG_INF, ll = 0.f;
-      for (int x = 0; x < 4; ++x) mm = fmaxf(mm, s_ml[x][g][0]);
+      for (int x = 0; x < NW; ++x) mm = fmaxf(mm, s_ml[x][g][0]);
       const float ref = mm == NEG_INF ? 0.f : mm;
       f32x4 o = {0.f, 0.f, 0.f, 0.f};
-      for (int x = 0; x < 4; ++x) {
+      for (int x = 0; x < NW; ++x) {
         const float f = __builtin_amdgcn_exp2f(s_ml[x][g][0] - ref);
         ll += f * s_ml[x][g][1];
         o += f * *reinterpret_cast<const f32x4*>(ob + (x * 16 + g) * D + d);
@@ -357,11 +372,12 @@ __global__ __launch_bounds__(256) void attn_decode_join_kernel(DecArgs a) {
   }
 }
 
-// Workers: as many as fill every compute unit twice, and no more than the keys a table
-// can hold give MIN_UNITS to.
+// Workers: as many as there are compute units (a workgroup fills one's LDS), and no more than
+// the keys a table can hold give MIN_UNITS to.
 static int64_t workers(int64_t N, int64_t HKV, int64_t hblocks, int64_t max_keys) {
+  if (max_keys <= SHORT_KEYS) return 0;
   const int64_t most = N * ((max_keys + UNIT - 1) / UNIT);
-  int64_t w = 2ll * cu_count() / (HKV * hblocks);
+  int64_t w = cu_count() / (HKV * hblocks);
   const int64_t need = (most + MIN_UNITS - 1) / MIN_UNITS;
   if (w > need) w = need;
   return w < 1 ? 1 : w;
@@ -370,7 +386,7 @@ static int64_t workers(int64_t N, int64_t HKV, int64_t hblocks, int64_t max_keys
 template <typename T, int D>
 static void launch(const DecArgs& a, bool join, hipStream_t s) {
   const unsigned hbs = (unsigned)(a.HKV * a.hblocks);
-  hipLaunchKernelGGL((attn_decode_kernel<T, D>), dim3(hbs * (unsigned)a.W), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((attn_decode_kernel<T, D>), dim3(hbs * (unsigned)(a.W ? a.W : a.N)), dim3(64 * NW), 0, s, a);
   if (join)
     hipLaunchKernelGGL((attn_decode_join_kernel<T, D>), dim3((unsigned)(a.HKV * a.G * a.N)), dim3(256), 0, s, a);
 }
@@ -384,7 +400,7 @@ extern "C" size_t hmx_paged_attention_decode_workspace_bytes(int32_t N, int32_t 
                                                              int32_t D, int64_t max_keys) {
   if (N <= 0 || HKV <= 0 || H <= 0 || H % HKV != 0 || max_keys <= 0) return 0;
   const int64_t hb = (H / HKV + 15) / 16, w = attn::workers(N, HKV, hb, max_keys);
-  if (w == 1) return 0;
+  if (w <= 1) return 0;
   return (size_t)w * 2 * HKV * hb * 16 * (D + 2) * sizeof(float);
 }
 
