@@ -11,8 +11,8 @@
 // then holds one row's scores, so the softmax statistics are per-lane scalars and P^T in
 // the C layout is already the B operand of the second product (the k order it implies is
 // the one the transposing LDS reads of V are made in).
-// P is rounded to the inputs' type (half a step, 2^-9 for bf16, averaged over the keys);
-// scores, maxima, sums and O stay in fp32.
+// P is rounded to the inputs' type (half a step of each, averaged over the keys); scores,
+// maxima, sums and O stay in fp32.
 #include "attn.hpp"
 
 namespace hmx {
@@ -142,7 +142,7 @@ __device__ __forceinline__ void exact_rows(const FwdArgs& a, const Tile& t, int 
 // the loop multiplies K's keys 64 j .. 64 j + 63 and V's 64 j - 32 .. 64 j + 31, so both
 // tiles have two buffers, and arrive in LDS directly, a step ahead of their use.
 template <typename T, int D, bool PAGED>
-__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs a) {
   typedef typename El<T>::v8 v8;
   constexpr int NC = D / 8;                 // 16-byte chunks of a row
   constexpr int RI = 64 / NC, NL = 16 / RI; // rows of a wave's load, loads of its 16 rows of a tile
@@ -361,14 +361,50 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
   // half u, whose scores are cur, against V's rows r of its tile; nxt receives the next
   // half's scores from K's half kt
   auto half = [&](int u, const f32x16& cur, f32x16& nxt, int kt, int r) __attribute__((always_inline)) {
-    scores(kt, nxt);
-    v8 p0 = probs(cur, 0);
-    asm volatile("" : "+v"(p0));            // formed here, beside the products, not behind the mask
+    const char *Kb = smem + kt * 32 * D * 2, *Vb = smem + 2 * TILE + r * D * 2;
+    constexpr int AHEAD = 2;                // LDS reads run so many products ahead
+    v8 kf[NS], vf[2 * ND], pf[2];
+    float p[16], mx = NEG_INF;
+    auto key_of = [&](int s) __attribute__((always_inline)) { kf[s] = *reinterpret_cast<const v8*>(Kb + ko[s]); };
+    auto value_of = [&](int g) __attribute__((always_inline)) {
+      const char* v = Vb + (g / ND) * 16 * D * 2;
+      vf[g] = join<T>(tr4<T>(reinterpret_cast<const T*>(v + vo[g % ND])), tr4<T>(reinterpret_cast<const T*>(v + vu[g % ND])));
+    };
+    auto element = [&](int i) __attribute__((always_inline)) {
+      p[i] = __builtin_amdgcn_exp2f(cur[i] * a.c - mc);
+      l += p[i];
+    };
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s) key_of(s);
+    fence();
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      if (s + AHEAD < NS) key_of(s + AHEAD);
+      else value_of(s + AHEAD - NS);
+      nxt = El<T>::mma32(kf[s], qf[s], s == 0 ? f32x16{0} : nxt);
+#pragma unroll
+      for (int i = s * 8 / NS; i < (s + 1) * 8 / NS; ++i) element(i);
+      fence();
+    }
+    pf[0] = pack8<T>(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
+    asm volatile("" : "+v"(pf[0]));         // formed here, not behind the mask
     mask(u + 1, nxt);
-    values(r, p0);
-    const v8 p1 = probs(cur, 8);
-    values(r + 16, p1);
-    follow(maximum(nxt));
+#pragma unroll
+    for (int g = 0; g < 2 * ND; ++g) {
+      if (g + AHEAD < 2 * ND) value_of(g + AHEAD);
+      acc[g % ND] = El<T>::mma32(vf[g], pf[g / ND], acc[g % ND]);
+      if (g < ND) {
+#pragma unroll
+        for (int i = g * 8 / ND; i < (g + 1) * 8 / ND; ++i) element(8 + i);
+        if (g == ND - 1) pf[1] = pack8<T>(p[8], p[9], p[10], p[11], p[12], p[13], p[14], p[15]);
+      } else {
+
+#pragma unroll
+        for (int i = (g - ND) * 16 / ND; i < (g - ND + 1) * 16 / ND; ++i) mx = fmaxf(mx, nxt[i]);
+      }
+      fence();
+    }
+    follow(half_max(mx));
   };
   auto last_half = [&](const f32x16& cur, int r) __attribute__((always_inline)) {
     values(r, probs(cur, 0));
@@ -450,39 +486,36 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(FwdArgs a) {
     exact_rows<T, D, PAGED>(a, t, kvh, off, j_beg * BN, j_end * BN, sp, reinterpret_cast<float*>(smem));
 }
 
-// The splits' shares of a row joined: sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.
+// The splits' shares of a row joined: sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.  The
+// tokens of all sequences lie between the first and the last offset.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_join_kernel(FwdArgs a) {
   constexpr int TPR = D / 4;
-  const int kvh = blockIdx.x % a.HKV;
-  const Tile t = find_tile<BM>(a.seqs, blockIdx.x / a.HKV);
-  if (t.seq < 0 || t.row0 < 0 || t.row0 >= t.rows) return;
-  const int n = min(BM, t.rows - t.row0), d = 4 * (threadIdx.x % TPR);
-  for (int r = threadIdx.x / TPR; r < n; r += 256 / TPR) {
-    const int row = t.row0 + r, tok = fdiv(row, a.G), h = kvh * a.G.d + row - tok * a.G.d;
-    const int64_t at = (int64_t)(t.bos + tok) * a.H + h;
-    float m = NEG_INF, l = 0.f;
-    for (int s = 0; s < a.nsplit; ++s) m = fmaxf(m, share_stats<D>(a, s, at)[0]);
-    const float ref = m == NEG_INF ? 0.f : m;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.nsplit; ++s) {
-      const float* st = share_stats<D>(a, s, at);
-      const float f = __builtin_amdgcn_exp2f(st[0] - ref);
-      l += f * st[1];
-      o += f * *reinterpret_cast<const f32x4*>(share_row<D>(a, s, at) + d);
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    typename El<T>::v4 x;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = (T)(o[i] * inv);
-    *reinterpret_cast<typename El<T>::v4*>(a.o + (int64_t)(t.bos + tok) * a.o_ts + (int64_t)h * a.o_hs +
-                                           2 * d) = x;
+  const int64_t r = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  const int tok = (int)(r / a.H), h = (int)(r - (int64_t)tok * a.H), d = 4 * (threadIdx.x % TPR);
+  if (tok >= a.seqs.T || tok < a.seqs.cu[0] || tok >= a.seqs.cu[a.seqs.N]) return;
+  float m = NEG_INF, l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < a.nsplit; ++s) {
+    const float* st = share_stats<D>(a, s, r);
+    const f32x4 x = *reinterpret_cast<const f32x4*>(share_row<D>(a, s, r) + d);
+    const float mn = fmaxf(m, st[0]), ref = mn == NEG_INF ? 0.f : mn;
+    const float f = __builtin_amdgcn_exp2f(m - ref), e = __builtin_amdgcn_exp2f(st[0] - ref);
+    l = l * f + e * st[1];
+    o = o * f + x * e;
+    m = mn;
   }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  typename El<T>::v4 x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = (T)(o[i] * inv);
+  *reinterpret_cast<typename El<T>::v4*>(a.o + (int64_t)tok * a.o_ts + (int64_t)h * a.o_hs + 2 * d) = x;
 }
 
 // Splits of the keys: where the row tiles alone leave compute units idle, as many as give
-// each about two workgroups, of at least four tiles of keys (a split costs its share's
-// trip through memory and the joining launch).
+// each about two workgroups (what runs at once), of at least four tiles of keys (a split
+// costs its share's trip through memory and the joining launch).
 static int splits(int64_t slots, int64_t N, int HKV, int64_t max_keys, bool packed) {
   const int64_t live = (packed ? slots - 2 : slots) * HKV, want = 2ll * cu_count();
   int64_t s = live > 0 ? want / live : 1;
@@ -498,8 +531,10 @@ static void launch_fwd(const FwdArgs& a, int D, hipStream_t s) {
   if (D == 64) hipLaunchKernelGGL((attn_fwd_kernel<T, 64, PAGED>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((attn_fwd_kernel<T, 128, PAGED>), grid, dim3(256), 0, s, a);
   if (a.nsplit > 1) {
-    if (D == 64) hipLaunchKernelGGL((attn_join_kernel<T, 64>), dim3(grid.x), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((attn_join_kernel<T, 128>), dim3(grid.x), dim3(256), 0, s, a);
+    const int64_t rows = (int64_t)a.seqs.T * a.H, rpb = 1024 / D;
+    const dim3 jg((unsigned)((rows + rpb - 1) / rpb));
+    if (D == 64) hipLaunchKernelGGL((attn_join_kernel<T, 64>), jg, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attn_join_kernel<T, 128>), jg, dim3(256), 0, s, a);
   }
 }
 
