@@ -10,7 +10,8 @@ kernels are forward-only, so a backward through them raises NotImplementedError
 instead of silently returning no gradient.  The in-place decode ops declare their
 mutations; torch refuses autograd through them by itself.  The training GKA op
 with its backward is the autograd function behind ``hmx.gka_chebyshev_gla`` and
-``hmx.ChebyshevIteration`` (hmx.ops.gka_train).
+``hmx.ChebyshevIteration`` (hmx.ops.gka_train).  ``causal_attention`` is differentiable
+here too: its backward is a registered op of its own.
 
 ``torch.ops.hmx.<name>`` is the registered op; the functions of the same name
 in this module wrap it with the reference's Python signature (optional
@@ -298,6 +299,91 @@ def _(x, z, weight, eps, norm_before_gate):
 _forward_only(_norm, "rms_norm_gated")
 
 
+# --------------------------------------------------------------------- attention layers
+@torch.library.custom_op("hmx::causal_attention", mutates_args=())
+def _attention(q: Tensor, k: Tensor, v: Tensor, scale: Optional[float],
+               cu_seqlens: Optional[Tensor]) -> tuple[Tensor, Tensor]:
+    o, lse, _ = ops.attention.attention_forward(q, k, v, scale, cu_seqlens, None, True)
+    return o, lse
+
+
+@_attention.register_fake
+def _(q, k, v, scale, cu_seqlens):
+    return (q.new_empty(q.shape),
+            q.new_empty(q.shape[0] * q.shape[1], q.shape[2], dtype=torch.float32))
+
+
+@torch.library.custom_op("hmx::causal_attention_bwd", mutates_args=())
+def _attention_bwd(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, do: Tensor,
+                   scale: Optional[float], cu_seqlens: Optional[Tensor]
+                   ) -> tuple[Tensor, Tensor, Tensor]:
+    return ops.attention_train.attention_backward(q, k, v, o, lse, cu_seqlens, do, scale)
+
+
+@_attention_bwd.register_fake
+def _(q, k, v, o, lse, do, scale, cu_seqlens):
+    return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+
+
+def _attention_setup(ctx, inputs, output):
+    q, k, v, ctx.scale, cu_seqlens = inputs
+    o, lse = output
+    ctx.save_for_backward(q, k, v, o, lse, cu_seqlens)
+    ctx.mark_non_differentiable(lse)
+
+
+def _attention_grad(ctx, do, dlse):
+    q, k, v, o, lse, cu_seqlens = ctx.saved_tensors
+    return (*torch.ops.hmx.causal_attention_bwd(q, k, v, o, lse, do, ctx.scale, cu_seqlens), None,
+            None)
+
+
+_attention.register_autograd(_attention_grad, setup_context=_attention_setup)
+
+
+@torch.library.custom_op("hmx::append_paged_kv", mutates_args=("k_cache", "v_cache"))
+def _append(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, slot_mapping: Tensor,
+            q: Optional[Tensor], positions: Optional[Tensor], cos_sin: Optional[Tensor],
+            interleaved: bool) -> Tensor:
+    out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ops.append_paged_kv(k, v, k_cache, v_cache, slot_mapping, q=q, positions=positions,
+                        cos_sin=cos_sin, interleaved=interleaved, q_out=out)
+    return k.new_empty(0) if q is None else out
+
+
+@_append.register_fake
+def _(k, v, k_cache, v_cache, slot_mapping, q, positions, cos_sin, interleaved):
+    return k.new_empty(0) if q is None else q.new_empty(q.shape)
+
+
+@torch.library.custom_op("hmx::paged_attention_decode", mutates_args=())
+def _paged_decode(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor,
+                  seq_lens: Tensor, scale: Optional[float]) -> Tensor:
+    return ops.paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, scale)
+
+
+@_paged_decode.register_fake
+def _(q, k_cache, v_cache, block_table, seq_lens, scale):
+    return q.new_empty(q.shape)
+
+
+_forward_only(_paged_decode, "paged_attention_decode")
+
+
+@torch.library.custom_op("hmx::paged_causal_attention", mutates_args=())
+def _paged_prompt(q: Tensor, k_cache: Tensor, v_cache: Tensor, block_table: Tensor,
+                  seq_lens: Tensor, cu_seqlens: Tensor, scale: Optional[float]) -> Tensor:
+    return ops.paged_causal_attention(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale)
+
+
+@_paged_prompt.register_fake
+def _(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale):
+    return q.new_empty(q.shape)
+
+
+_forward_only(_paged_prompt, "paged_causal_attention")
+
+
 # ------------------------------------------------------- reference-signature wrappers
 def chunk_gated_delta_rule_gqa(q, k, v, g, beta, scale=None, initial_state=None,
                                output_final_state=False, cu_seqlens=None,
@@ -423,7 +509,34 @@ def rms_norm_gated(x, z, weight, eps=1e-5, norm_before_gate=True):
     return torch.ops.hmx.rms_norm_gated(x, z, weight, float(eps), bool(norm_before_gate))
 
 
+def causal_attention(q, k, v, scale=None, cu_seqlens=None):
+    """``torch.ops.hmx.causal_attention`` with hmx.causal_attention's arguments; the output
+    alone, differentiable."""
+    return torch.ops.hmx.causal_attention(q, k, v, scale, cu_seqlens)[0]
+
+
+def append_paged_kv(k, v, k_cache, v_cache, slot_mapping, *, q=None, positions=None, cos_sin=None,
+                    interleaved=False):
+    """``torch.ops.hmx.append_paged_kv``; the caches are written in place, q (None without
+    one) is returned rotated."""
+    out = torch.ops.hmx.append_paged_kv(k, v, k_cache, v_cache, slot_mapping, q, positions, cos_sin,
+                                        bool(interleaved))
+    return None if q is None else out
+
+
+def paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, scale=None):
+    """``torch.ops.hmx.paged_attention_decode``."""
+    return torch.ops.hmx.paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, scale)
+
+
+def paged_causal_attention(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale=None):
+    """``torch.ops.hmx.paged_causal_attention``."""
+    return torch.ops.hmx.paged_causal_attention(q, k_cache, v_cache, block_table, seq_lens,
+                                                cu_seqlens, scale)
+
+
 __all__ = ["chunk_gated_delta_rule_gqa", "fused_recurrent_gated_delta_rule_gqa",
            "gka_chebyshev_gla_prefill", "gka_chebyshev_gla_decode",
            "mamba_chunk_scan_combined_varlen", "selective_state_update", "causal_conv1d_fn",
-           "causal_conv1d_update", "rms_norm_gated"]
+           "causal_conv1d_update", "rms_norm_gated", "causal_attention", "append_paged_kv",
+           "paged_attention_decode", "paged_causal_attention"]

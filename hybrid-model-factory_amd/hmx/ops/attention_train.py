@@ -9,7 +9,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from .attention import _elsewhere, _rows, _scale, attention_forward, check_qkv
+from .attention import _elsewhere, _offsets, _rows, _scale, attention_forward, check_qkv
 
 
 class CausalAttention(torch.autograd.Function):
@@ -32,13 +32,19 @@ class CausalAttention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, do):
         q, k, v, o, lse, cu = ctx.saved_tensors
-        if _elsewhere(q):
-            with torch.cuda.device(q.device):
-                return (*_backward(q, k, v, o, lse, cu, do, ctx.scale), None, None)
-        return (*_backward(q, k, v, o, lse, cu, do, ctx.scale), None, None)
+        return (*attention_backward(q, k, v, o, lse, cu, do, ctx.scale), None, None)
 
 
-def _backward(q, k, v, o, lse, cu, do, scale):
+def attention_backward(q, k, v, o, lse, cu_seqlens, do, scale):
+    """(dq, dk, dv) of causal_attention from its inputs, output, row statistics and the
+    output's gradient."""
+    if q.dtype != torch.bfloat16:
+        raise NotImplementedError(f"causal_attention: a gradient needs bf16, got {q.dtype}")
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return attention_backward(q, k, v, o, lse, cu_seqlens, do, scale)
+    scale = _scale(scale, q.shape[-1])
+    cu = None if cu_seqlens is None else _offsets(cu_seqlens, q.shape[1], q.device)
     B, T, H, D = q.shape
     dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
     delta = torch.empty_like(lse)

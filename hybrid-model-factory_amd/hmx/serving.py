@@ -1,5 +1,6 @@
 """The vLLM layers' mixer cores over hmx ops: ``gdn_forward_core``,
-``gka_forward_core`` and ``mamba2_conv_ssm_forward``.
+``gka_forward_core`` and ``mamba2_conv_ssm_forward``, and beside them
+``attention_forward_core`` for the softmax attention layers between the mixers.
 
 These restate ``PrimedGatedDeltaNetAttention._forward_core``
 (vllm-inference/src/primed_vllm/primed_gdn_layer.py:635-936) and
@@ -452,6 +453,53 @@ def mamba2_conv_ssm_forward(layer, projected_states: torch.Tensor, output: torch
             xd[:, 2 * xb:].view(nd, H, N), layer.D[:, None].expand(H, P), z=None,
             dt_bias=layer.dt_bias[:, None].expand(H, P), dt_softplus=True,
             state_batch_indices=src, dst_state_batch_indices=dst, out=out[:nd])
+
+
+def attention_forward_core(layer, qkv: torch.Tensor, positions: torch.Tensor | None,
+                           core_attn_out: torch.Tensor, attn_metadata, k_cache: torch.Tensor,
+                           v_cache: torch.Tensor) -> None:
+    """The attention layer of a hybrid model over a paged cache, as the mixer cores above
+    run theirs: the position rotation and the append in one launch, then the batch's decodes
+    (first, one token each) and its prefills, each written into ``core_attn_out`` in place.
+
+    ``layer``: num_heads, num_kv_heads, head_dim, tp_size, ``scaling`` (None: head_dim **
+    -0.5) and ``rotary_emb`` (None, or an object with cos_sin_cache [max position, rotary
+    dim] and is_neox_style).  ``qkv`` [tokens, (H + 2 HKV) * head_dim] is the fused
+    projection's output, with the layer's norms on q and k applied; ``positions`` [tokens];
+    ``core_attn_out`` [tokens, H, head_dim]; caches [pages, page size, HKV, head_dim].
+    ``attn_metadata`` (None in the profile run, which writes nothing): num_actual_tokens,
+    num_decodes, num_decode_tokens, num_prefills, query_start_loc [N + 1], seq_lens [N] (the
+    step's tokens among them), block_table [N, width], slot_mapping [tokens]; int32 on the
+    device (slot_mapping int64 too), and nothing is read back.  Where decodes carry draft
+    tokens (num_decode_tokens > num_decodes) all requests go through the prefill form.  Rows
+    past num_actual_tokens are left as they were."""
+    md = attn_metadata
+    if md is None:
+        return
+    n, tp, D = md.num_actual_tokens, layer.tp_size, layer.head_dim
+    H, HKV = layer.num_heads // tp, layer.num_kv_heads // tp
+    qkv = _cut(qkv, 0, n)
+    q, k, v = (x.view(n, -1, D) for x in qkv.split([H * D, HKV * D, HKV * D], dim=-1))
+    rope = getattr(layer, "rotary_emb", None)
+    if rope is not None:
+        if positions is None:
+            raise ValueError("rotary_emb needs the tokens' positions")
+        q = ops.append_paged_kv(k, v, k_cache, v_cache, md.slot_mapping[:n], q=q,
+                                positions=positions[:n], cos_sin=rope.cos_sin_cache,
+                                interleaved=not rope.is_neox_style)
+    else:
+        ops.append_paged_kv(k, v, k_cache, v_cache, md.slot_mapping[:n])
+    scale = getattr(layer, "scaling", None)
+    nd, npf = md.num_decodes, md.num_prefills
+    if md.num_decode_tokens != nd:
+        nd, npf = 0, nd + npf
+    if nd > 0:
+        ops.paged_attention_decode(q[:nd], k_cache, v_cache, md.block_table[:nd], md.seq_lens[:nd],
+                                   scale, out=core_attn_out[:nd])
+    if npf > 0:
+        ops.paged_causal_attention(q, k_cache, v_cache, md.block_table[nd:nd + npf],
+                                   md.seq_lens[nd:nd + npf], md.query_start_loc[nd:nd + npf + 1],
+                                   scale, out=core_attn_out[:n])
 
 
 def _mamba2_prefill_blocks(layer, md, hbc, dt, x, out, idx_p, lc_p, ls_p, conv_state, ssm_state,

@@ -156,3 +156,21 @@ def test_oracle_rotation_and_rows_by_hand():
     o, a = ref.rows(q, k, v, 1.0, -1)                            # row 0 has no key, row 2 both
     assert o[0].tolist() == [[0.0, 0.0]] and o[1].tolist() == [[1.0, 3.0]]
     assert o[2, 0, 0] == 2.0 and o[2, 0, 1] == float("inf")
+
+
+def test_registered_with_fakes_and_mutations():
+    import hmx.library  # noqa: F401
+    m = torch.device("meta")
+    q, k = torch.empty(1, 9, 4, 64, dtype=BF, device=m), torch.empty(1, 9, 2, 64, dtype=BF, device=m)
+    o, lse = torch.ops.hmx.causal_attention(q, k, k, None, None)
+    assert o.shape == q.shape and o.dtype == BF and lse.shape == (9, 4) and lse.dtype == torch.float32
+    g = torch.ops.hmx.causal_attention_bwd(q, k, k, o, lse, o, None, None)
+    assert [x.shape for x in g] == [q.shape, k.shape, k.shape]
+    kc = torch.empty(3, 16, 2, 64, dtype=BF, device=m)
+    tab, n = torch.empty(9, 2, dtype=torch.int32, device=m), torch.empty(9, dtype=torch.int32, device=m)
+    assert torch.ops.hmx.paged_attention_decode(q[0], kc, kc, tab, n, None).shape == (9, 4, 64)
+    assert torch.ops.hmx.paged_causal_attention(q[0], kc, kc, tab, n, n, None).shape == (9, 4, 64)
+    assert torch.ops.hmx.append_paged_kv(k[0], k[0], kc, kc.clone(), n, q[0], None, None, False).shape == (9, 4, 64)
+    w = {a.name for a in torch.ops.hmx.append_paged_kv.default._schema.arguments
+         if a.alias_info is not None and a.alias_info.is_write}
+    assert w == {"k_cache", "v_cache"}
