@@ -156,6 +156,14 @@ struct Pages {
   FastDiv page;
 };
 
+// the kernels reach the 16 rows of a load group by 32-bit offsets
+inline bool near_rows(int64_t token_stride) { return token_stride >= 0 && token_stride < (1ll << 25); }
+
+// a cache or a table of no pages may be NULL: it holds no keys
+inline bool has_pages(const hmx_paged_kv& c) {
+  return c.num_pages == 0 || c.table_width == 0 || (c.k && c.v && c.table);
+}
+
 inline Pages make_pages(const hmx_paged_kv& c) {
   Pages p;
   p.k = static_cast<const char*>(c.k);

@@ -26,6 +26,7 @@ struct BwdArgs {
   Seqs seqs;           // rows of tokens x G
   FastDiv G;
   int32_t H, HKV, slots;
+  int32_t fixed;       // a tile's rows lie at fixed 32-bit offsets from its first token
   float c, scale;
 };
 
@@ -216,20 +217,20 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_dkv_kernel(BwdArgs a) {
 
   // Staging: rows 16 wave .. + 15 of a tile, RI to a load.  Where G divides a tile's rows, a
   // lane's rows of all tiles are one head's, at offsets that do not change.
-  const bool even = KR % G == 0;
   uint32_t qoff[NL], ooff[NL];
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
-    const int x = wave * 16 + i * RI + lane / NC, tk = fdiv(x, a.G), hd = kvh * G + x - tk * G;
+    const int x = wave * 16 + i * RI + lane / NC, tk = fdiv(x, a.G), g = x - tk * G;
     const int c = swz<D>(x, lane % NC);
-    qoff[i] = (uint32_t)(tk * (int)a.q_ts + hd * (int)a.q_hs + 16 * c);
-    ooff[i] = (uint32_t)(tk * (int)a.do_ts + hd * (int)a.do_hs + 16 * c);
+    qoff[i] = (uint32_t)(tk * a.q_ts + g * a.q_hs + 16 * c);
+    ooff[i] = (uint32_t)(tk * a.do_ts + g * a.do_hs + 16 * c);
   }
-  const char *qbase = a.q + (int64_t)t.bos * a.q_ts, *obase = a.dout + (int64_t)t.bos * a.do_ts;
+  const char* qbase = a.q + (int64_t)t.bos * a.q_ts + (int64_t)kvh * G * a.q_hs;
+  const char* obase = a.dout + (int64_t)t.bos * a.do_ts + (int64_t)kvh * G * a.do_hs;
   const int tpt = KR / G;                   // tokens of a tile where G divides it
   auto stage = [&](int j, int buf) __attribute__((always_inline)) {
     const uint32_t ql = lds_addr(smem) + buf * 2 * TILE + wave * 16 * D * 2, ol = ql + TILE;
-    if (even && (j + 1) * KR <= rows) {
+    if (a.fixed && (j + 1) * KR <= rows) {
       const char *qb = uniform_ptr(qbase + (int64_t)j * tpt * a.q_ts), *ob = uniform_ptr(obase + (int64_t)j * tpt * a.do_ts);
 #pragma unroll
       for (int i = 0; i < NL; ++i) dma16(ql + i * RI * D * 2, qb, qoff[i]);
@@ -239,10 +240,9 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_dkv_kernel(BwdArgs a) {
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
         const int x = wave * 16 + i * RI + lane / NC, r = min(j * KR + x, rows - 1), tk = fdiv(r, a.G);
-        const int64_t hd = kvh * G + r - tk * G;
-        const int c = 16 * swz<D>(x, lane % NC);
-        dma16(ql + i * RI * D * 2, qbase + tk * a.q_ts + hd * a.q_hs + c);
-        dma16(ol + i * RI * D * 2, obase + tk * a.do_ts + hd * a.do_hs + c);
+        const int g = r - tk * G, c = 16 * swz<D>(x, lane % NC);
+        dma16(ql + i * RI * D * 2, qbase + tk * a.q_ts + g * a.q_hs + c);
+        dma16(ol + i * RI * D * 2, obase + tk * a.do_ts + g * a.do_hs + c);
       }
     }
     const int r = min(j * KR + lane, rows - 1), tk = fdiv(r, a.G);   // wave 0 (and 2) lse, 1 (and 3) delta
@@ -445,6 +445,8 @@ extern "C" int hmx_causal_attention_bwd(
                        (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv;
   HMX_REQUIRE(st % 8 == 0 && al % 16 == 0, HMX_EINVAL,
               "hmx_causal_attention_bwd: strides must be multiples of 8 elements and pointers 16-byte aligned");
+  HMX_REQUIRE(attn::near_rows(k_token_stride) && attn::near_rows(v_token_stride), HMX_EUNSUPPORTED,
+              "hmx_causal_attention_bwd: token strides of k and v past 2^25 elements");
   attn::BwdArgs a{};
   a.q = (const char*)q; a.k = (const char*)k; a.v = (const char*)v; a.o = (const char*)o;
   a.dout = (const char*)dout; a.dq = (char*)dq; a.dk = (char*)dk; a.dv = (char*)dv;
@@ -462,6 +464,9 @@ extern "C" int hmx_causal_attention_bwd(
   a.H = H; a.HKV = HKV;
   a.c = scale * attn::LOG2E;
   a.scale = scale;
+  const int64_t G = H / HKV, span = attn::KR / G;
+  a.fixed = attn::KR % G == 0 && span * a.q_ts + G * a.q_hs < (1ll << 31) &&
+            span * a.do_ts + G * a.do_hs < (1ll << 31);
   const int64_t qs = attn::tile_slots<attn::QM>(cu_seqlens, N, T, H / HKV);
   const int64_t ks = attn::tile_slots<attn::KM>(cu_seqlens, N, T, 1);
   HMX_REQUIRE(qs * HKV < (1ll << 31), HMX_EUNSUPPORTED, "hmx_causal_attention_bwd: %lld tiles", (long long)qs);

@@ -421,7 +421,7 @@ extern "C" int hmx_paged_attention_decode(const void* q, int64_t q_token_stride,
   HMX_REQUIRE(cache && cache->num_pages >= 0 && cache->page_size > 0 && cache->table_width >= 0, HMX_EINVAL,
               "hmx_paged_attention_decode: cache");
   if (N == 0) return HMX_OK;
-  HMX_REQUIRE(q && o && cache->seq_lens && cache->table && cache->k && cache->v, HMX_EINVAL,
+  HMX_REQUIRE(q && o && cache->seq_lens && attn::has_pages(*cache), HMX_EINVAL,
               "hmx_paged_attention_decode: null pointer");
   const int64_t max_keys = (int64_t)cache->table_width * cache->page_size;
   HMX_REQUIRE(max_keys < (1ll << 31) - 256, HMX_EUNSUPPORTED,
@@ -432,6 +432,8 @@ extern "C" int hmx_paged_attention_decode(const void* q, int64_t q_token_stride,
   const uintptr_t al = (uintptr_t)q | (uintptr_t)o | (uintptr_t)cache->k | (uintptr_t)cache->v;
   HMX_REQUIRE(st % 8 == 0 && al % 16 == 0, HMX_EINVAL,
               "hmx_paged_attention_decode: strides must be multiples of 8 elements and pointers 16-byte aligned");
+  HMX_REQUIRE(attn::near_rows(cache->k_token_stride) && attn::near_rows(cache->v_token_stride), HMX_EUNSUPPORTED,
+              "hmx_paged_attention_decode: token strides of the cache past 2^25 elements");
   attn::DecArgs a{};
   a.q = (const char*)q; a.o = (char*)o;
   a.q_ts = 2 * q_token_stride; a.q_hs = 2 * q_head_stride;

@@ -67,7 +67,8 @@ def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
         return t, H * D, D
     B = t.shape[0] if t.dim() == 4 else 1
     T = t.shape[-3]
-    if not _aligned(t) or (B > 1 and T > 1 and t.stride(0) != T * t.stride(1)):
+    if not _aligned(t) or (B > 1 and T > 1 and t.stride(0) != T * t.stride(1)) \
+            or (T > 1 and t.stride(-3) >= 1 << 25):
         t = t.contiguous()
     ts = t.stride(-3) if T > 1 or B == 1 else t.stride(0)
     # strides of dimensions of one are never used, and may be anything
@@ -129,7 +130,7 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     q [B, T, H, D], k and v [B, T, HKV, D]; with ``cu_seqlens`` (N + 1 offsets into the
     tokens, B = 1) each of the N packed sequences by itself.  ``scale`` (default
     D ** -0.5) must be positive.  Returns [B, T, H, D] in q's type; rows of no sequence
-    are 0, or left as they were in ``out``.  A value that is not finite reaches the rows
+    are 0, or left as they were in ``out`` (which may not overlap an input).  A value that is not finite reaches the rows
     that attend it and no others.
 
     Differentiable in q, k and v for bf16 (hmx.CausalAttention)."""
@@ -209,7 +210,7 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
 
     ``slot_mapping`` [T] (int32 or int64): page * page size + place in the page; a token
     whose slot is negative or past the cache is padding and stores nothing.  Two tokens
-    with one slot leave either of the two there.  With ``cos_sin`` [max position, R] (fp32,
+    with one slot leave a mix of the two there.  With ``cos_sin`` [max position, R] (fp32,
     bf16 or fp16; R a multiple of 16 up to D: R / 2 cosines, then R / 2 sines) and
     ``positions`` [T] the first R elements of every q and k head turn by their position's
     angles, in pairs (i, i + R / 2), or (2i, 2i + 1) with ``interleaved``; a position
@@ -281,7 +282,8 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     q [N, H, D]; ``seq_lens`` [N] int32: keys of each sequence, the new token's among them
     (append_paged_kv stores it first); 0 gives a row of 0, and a length past the table
     row's pages counts as all of them.  ``block_table`` [N, width] int32; a page outside
-    the cache holds no keys.  Returns [N, H, D] in q's type."""
+    the cache holds no keys.  Returns [N, H, D] in q's type (``out``, which may not overlap
+    an input)."""
     what = "paged_attention_decode"
     if q.dim() != 3:
         raise ValueError(f"{what}: q [N, H, D], got {tuple(q.shape)}")
@@ -321,7 +323,8 @@ def paged_causal_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     sequences pass with its own offsets); ``seq_lens`` [N] int32 counts each sequence's
     keys, the new tokens' among them: token i of n attends keys 0 .. seq_len - n + i, and
     gives 0 where that is none.  Cache and table as in paged_attention_decode.  Returns
-    [T, H, D] in q's type; rows of no sequence are 0, or left as they were in ``out``."""
+    [T, H, D] in q's type; rows of no sequence are 0, or left as they were in ``out`` (which
+    may not overlap an input)."""
     what = "paged_causal_attention"
     if q.dim() != 3:
         raise ValueError(f"{what}: q [T, H, D], got {tuple(q.shape)}")

@@ -272,3 +272,37 @@ def test_append_without_rotation_and_in_place(dev):
     far = hmx.append_paged_kv(k, v, both[:, 0], both[:, 1], slots, q=q,
                               positions=torch.tensor([0, 9, -1, 3, 1], device=dev), cos_sin=cs)
     assert torch.isnan(far[1:3]).all() and torch.isfinite(far[[0, 3, 4]]).all()
+
+
+def test_no_pages_no_keys(dev):
+    """An empty cache, and a table without columns, hold no keys: rows of 0."""
+    q = torch.ones(2, 4, 64, dtype=BF, device=dev)
+    lens = torch.tensor([5, 0], dtype=torch.int32, device=dev)
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device=dev)
+    for pages, width in ((0, 3), (4, 0)):
+        kc = torch.ones(pages, 16, 2, 64, dtype=BF, device=dev)
+        table = torch.zeros(2, width, dtype=torch.int32, device=dev)
+        assert (hmx.paged_attention_decode(q, kc, kc, table, lens) == 0).all()
+        assert (hmx.paged_causal_attention(q, kc, kc, table, lens, cu) == 0).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_long_caches_past_32_bit_offsets(dev, D):
+    """Pages more than 4 GiB into the cache, in both paged forms and the append."""
+    H, HKV, page = 4, 2, 256
+    pages = (5 << 30) // (page * HKV * D * 2)
+    kc = torch.zeros(pages, page, HKV, D, dtype=BF, device=dev)
+    vc = torch.zeros(pages, page, HKV, D, dtype=BF, device=dev)
+    gen = torch.Generator().manual_seed(D)
+    L = 700
+    table = torch.tensor([[pages - 1, 3, pages - 2]], dtype=torch.int32)
+    k, v = randn(gen, L, HKV, D), randn(gen, L, HKV, D)
+    j = torch.arange(L)
+    slots = table[0].long()[j // page] * page + j % page
+    hmx.append_paged_kv(k.to(dev), v.to(dev), kc, vc, slots.to(dev))
+    assert torch.equal(kc[pages - 1].cpu(), k[:page]) and torch.equal(vc[pages - 2, :L - 512].cpu(), v[512:])
+    q = randn(gen, 3, H, D)
+    dv = (kc, vc, table.to(dev), torch.tensor([L], dtype=torch.int32, device=dev))
+    o, a = ref.rows(q, k, v, D ** -0.5, L - 3)
+    check_o(hmx.paged_causal_attention(q.to(dev), *dv, torch.tensor([0, 3])), o, a, v, "new tokens")
+    check_o(hmx.paged_attention_decode(q[2:].to(dev), *dv), o[2:], a[2:], v, "one token")

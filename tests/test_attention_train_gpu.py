@@ -112,3 +112,15 @@ def test_refusals(dev):
         hmx.causal_attention(*h)
     with torch.no_grad():
         hmx.causal_attention(*h)
+
+
+def test_grads_of_head_major_inputs_and_an_odd_group(dev):
+    """Heads outermost in memory (large head strides), and groups that do not divide a tile."""
+    for H, HKV, D in ((8, 2, 64), (10, 2, 128), (48, 1, 64)):
+        T = 150
+        q, k, v, do = _inputs(H, 1, T, H, HKV, D)
+        ins = [x.to(dev).transpose(1, 2).contiguous().transpose(1, 2).requires_grad_() for x in (q, k, v)]
+        g = do.to(dev).transpose(1, 2).contiguous().transpose(1, 2)
+        grads = torch.autograd.grad(hmx.causal_attention(*ins), ins, g)
+        (_, *want), mags = ref.causal_grads(q[0], k[0], v[0], D ** -0.5, [(0, T)], do[0])
+        _check([x[0] for x in grads], want, mags, f"H={H}")
