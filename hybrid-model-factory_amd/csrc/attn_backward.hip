@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_dq_kernel(BwdArgs a) {
   }
   delta = pair_sum32(delta, delta);
   const float lse = a.lse[gt * a.H + head];
-  if (h == 0 && row < t.rows) a.delta[gt * a.H + head] = delta;
+  float over = 0.f;                         // the sum of dS, own half's keys
 
   // staging as in the forward: the wave brings rows 16 wave .. 16 wave + 15 of a tile
   uint32_t koff[NL], voff[NL];
@@ -141,6 +141,7 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_dq_kernel(BwdArgs a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         ds[i] = __builtin_amdgcn_exp2f(st[i] * a.c - lse) * (dp[i] - delta);
+        over += ds[i];
       }
       const v8 d0 = pack8<T>(ds[0], ds[1], ds[2], ds[3], ds[4], ds[5], ds[6], ds[7]);
       const v8 d1 = pack8<T>(ds[8], ds[9], ds[10], ds[11], ds[12], ds[13], ds[14], ds[15]);
@@ -153,6 +154,10 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_dq_kernel(BwdArgs a) {
         }
     }
   }
+  // P sums to 1, so dS would sum to 0 had delta been formed from an exact O: what it does
+  // sum to is delta's error, and dK gets a delta without it.
+  over = pair_sum32(over, over);
+  if (h == 0 && row < t.rows) a.delta[gt * a.H + head] = delta + over;
   if (row < t.rows) {
 #pragma unroll
     for (int d = 0; d < ND; ++d)

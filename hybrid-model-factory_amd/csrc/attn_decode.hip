@@ -11,7 +11,8 @@
 // them until a sequence's share ends.  K and V rows go straight into the wave's own ring in
 // LDS, whole rows to a load, RING - 1 turns ahead, and are read there as the A operands of
 // S^T = K Q^T and (transposed) of O^T = V^T P^T.
-// P is rounded to the inputs' type; scores, statistics and O stay in fp32.
+// P enters its product as the inputs' type and, beside it, what that rounding leaves: the
+// matrix cores wait for memory anyway.  Scores, statistics and O stay in fp32.
 #include "attn.hpp"
 
 namespace hmx {
@@ -232,16 +233,19 @@ __global__ __launch_bounds__(64 * NW) void attn_decode_kernel(DecArgs a) {
         for (int d = 0; d < ND; ++d) acc[d] *= f;
       }
       const float mc = m == NEG_INF ? 0.f : m * a.c;
-      v4 pf;
+      v4 pf, pr;                            // P and what its rounding leaves
 #pragma unroll
       for (int z = 0; z < 4; ++z) {
         const float p = __builtin_amdgcn_exp2f(st[z] * a.c - mc);
         l += p;
         pf[z] = (T)p;
+        pr[z] = (T)(p - (float)pf[z]);
       }
 #pragma unroll
-      for (int d = 0; d < ND; ++d)
-        acc[d] = El<T>::mma16k16(tr4<T>(reinterpret_cast<const T*>(tile + vo[d])), pf, acc[d]);
+      for (int d = 0; d < ND; ++d) {
+        const v4 v = tr4<T>(reinterpret_cast<const T*>(tile + vo[d]));
+        acc[d] = El<T>::mma16k16(v, pr, El<T>::mma16k16(v, pf, acc[d]));
+      }
     };
 #pragma unroll
     for (int i = 0; i < RING - 1; ++i)
