@@ -232,6 +232,38 @@ __device__ __forceinline__ Tile find_tile(const Seqs& s, int slot) {
   return t;
 }
 
+// The tile of the block in place `at`, heaviest first: a row tile's work grows with the keys
+// before it, so a sequence's tiles go from the last (LAST) to the first, or from the first
+// where the first have most; and of up to 62 packed sequences those with most keys come
+// first (their lengths are in the lanes of a wave; more go as they lie).  Whatever comes
+// last then is short.  lens: the sequences' keys, NULL where they are their tokens.
+template <int BM, bool LAST>
+__device__ __forceinline__ Tile next_tile(const Seqs& s, const int32_t* lens, int at, int slots) {
+  if (!s.cu || s.N < 1 || s.N > 62) return find_tile<BM>(s, LAST ? slots - 1 - at : at);
+  const int lane = threadIdx.x & 63, parts = s.N + 2;
+  const bool in = lane < parts, gap = lane == 0 || lane == s.N + 1;
+  const int bos = in ? seq_bound(s, lane) : 0;
+  const int tokens = in ? max(seq_bound(s, lane + 1) - bos, 0) : 0;
+  const int tiles = (int)(((int64_t)tokens * s.G + BM - 1) / BM);
+  const int keys = gap ? -1 : lens ? lens[min(max(lane - 1, 0), s.N - 1)] : tokens;
+  int start = 0;                              // tiles of the parts before this lane's
+  for (int f = 0; f < parts; ++f) {
+    const int k = __builtin_amdgcn_readlane(keys, f), n = __builtin_amdgcn_readlane(tiles, f);
+    start += k > keys || (k == keys && f < lane) ? n : 0;
+  }
+  const unsigned long long m = __ballot(in && at >= start && at < start + tiles);
+  Tile t{-1, 0, 0, 0, 0};
+  if (m == 0) return t;
+  const int e = __builtin_ctzll(m);
+  t.seq = e == 0 || e == s.N + 1 ? -1 : e - 1;
+  t.bos = __builtin_amdgcn_readlane(bos, e);
+  t.tokens = __builtin_amdgcn_readlane(tokens, e);
+  const int i = at - __builtin_amdgcn_readlane(start, e);
+  t.row0 = (LAST ? __builtin_amdgcn_readlane(tiles, e) - 1 - i : i) * BM;
+  t.rows = t.tokens * s.G;
+  return t;
+}
+
 template <int BM>
 inline int64_t tile_slots(const int32_t* cu, int64_t N, int64_t T, int64_t G) {
   if (!cu) return N * ((T / N * G + BM - 1) / BM);

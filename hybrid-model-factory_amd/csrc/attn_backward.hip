@@ -44,7 +44,7 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_dq_kernel(BwdArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // uniform, and known to be
   const int kvh = blockIdx.x % a.HKV;
-  const Tile t = find_tile<QM>(a.seqs, a.slots - 1 - (int)(blockIdx.x / a.HKV));
+  const Tile t = next_tile<QM, true>(a.seqs, nullptr, blockIdx.x / a.HKV, a.slots);
   if (t.row0 >= t.rows || t.row0 < 0) return;
   const int row = t.row0 + wave * 32 + l32, rowc = min(row, t.rows - 1);
   const int tok = fdiv(rowc, a.G), head = kvh * a.G.d + rowc - tok * a.G.d;
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(256, 1) void attn_bwd_dkv_kernel(BwdArgs a) {
   const int kvh = blockIdx.x % a.HKV;
   Seqs sk = a.seqs;
   sk.G = 1;
-  const Tile t = find_tile<KM>(sk, (int)(blockIdx.x / a.HKV));
+  const Tile t = next_tile<KM, false>(sk, nullptr, blockIdx.x / a.HKV, a.slots);
   if (t.row0 >= t.rows || t.row0 < 0) return;
   const int key = t.row0 + wave * 32 + l32, keyc = min(key, t.tokens - 1);
   const int64_t gk = t.bos + keyc;

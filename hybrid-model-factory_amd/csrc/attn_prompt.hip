@@ -154,9 +154,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // uniform, and known to be
   const int kvh = blockIdx.x % a.HKV;
-  // later tiles of a sequence have more keys: they go first
-  const int slot = a.slots - 1 - (int)(blockIdx.x / a.HKV);
-  const Tile t = find_tile<BM>(a.seqs, slot);
+  const Tile t = next_tile<BM, true>(a.seqs, PAGED ? a.pages.lens : nullptr, blockIdx.x / a.HKV, a.slots);
   if (t.row0 >= t.rows || t.row0 < 0) return;
 
   const int row = t.row0 + wave * 32 + l32;

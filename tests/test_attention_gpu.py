@@ -284,6 +284,11 @@ def test_no_pages_no_keys(dev):
         table = torch.zeros(2, width, dtype=torch.int32, device=dev)
         assert (hmx.paged_attention_decode(q, kc, kc, table, lens) == 0).all()
         assert (hmx.paged_causal_attention(q, kc, kc, table, lens, cu) == 0).all()
+    none = torch.tensor([1], dtype=torch.int32, device=dev)       # no sequence at all
+    assert (hmx.paged_causal_attention(q, kc, kc, table[:0], lens[:0], none) == 0).all()
+    assert hmx.paged_attention_decode(q[:0], kc, kc, table[:0], lens[:0]).shape == (0, 4, 64)
+    assert (hmx.causal_attention(q[None], q[None], q[None], cu_seqlens=none) == 0).all()
+    assert hmx.causal_attention(q[None, :0], q[None, :0], q[None, :0]).shape == (1, 0, 4, 64)
 
 
 @pytest.mark.parametrize("D", [64, 128])
@@ -306,3 +311,16 @@ def test_long_caches_past_32_bit_offsets(dev, D):
     o, a = ref.rows(q, k, v, D ** -0.5, L - 3)
     check_o(hmx.paged_causal_attention(q.to(dev), *dv, torch.tensor([0, 3])), o, a, v, "new tokens")
     check_o(hmx.paged_attention_decode(q[2:].to(dev), *dv), o[2:], a[2:], v, "one token")
+
+
+def test_many_packed_sequences(dev):
+    """More sequences than a wave has lanes, and just as many, empty ones among them."""
+    for N in (61, 62, 63, 64, 130):
+        cu = [0]
+        for i in range(N):
+            cu.append(cu[-1] + (i * 29) % 37 * (i % 4 > 0))
+        T, H, HKV, D = cu[-1] + 3, 4, 2, 64
+        q, k, v = _case(N, T, H, HKV, D, BF)
+        out = hmx.causal_attention(q.to(dev), k.to(dev), v.to(dev), cu_seqlens=torch.tensor(cu, device=dev))
+        o, a = ref.causal(q[0], k[0], v[0], D ** -0.5, bounds_of(cu))
+        check_o(out[0], o, a, v[0], f"{N} sequences")
