@@ -19,6 +19,7 @@ namespace hmx {
 namespace attn {
 
 constexpr int BM = 128, BN = 64;
+constexpr float NO_MC = -1e30f;
 
 struct FwdArgs {
   const char *q, *k, *v;
@@ -209,7 +210,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
   const char* vbase = (PAGED ? a.pages.v : a.v + (int64_t)t.bos * a.v_ts) + (int64_t)kvh * (PAGED ? a.pages.v_hs : a.v_hs);
   const bool whole = !PAGED || a.pages.page.d % 16 == 0;   // the wave's 16 rows lie in one page
   auto stage_rows = [&](int j, int r0, bool value) __attribute__((always_inline)) {
-    const uint32_t lds = lds_addr(smem) + (value ? 2 * TILE : 0) + (j & 1) * TILE + wave * 16 * D * 2;
+    const uint32_t lds = lds_addr(smem) + (value ? 2 * TILE : 0) + ((j - j_beg) & 1) * TILE + wave * 16 * D * 2;
     const char* base = value ? vbase : kbase;
     const int64_t ts = value ? vts : kts;
     if (!PAGED && r0 >= 0 && r0 + 16 <= keys) {
@@ -258,7 +259,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
     const bool edge = r0 + BN > wg_first + 1, out = r0 < j_beg * BN || r0 + BN > keys;
     const bool hole = PAGED && (s_skip[j & 3] == j + 1 || s_skip[(j - 1) & 3] == j);
     if (!(edge || out || hole)) return;
-    T* Vb = reinterpret_cast<T*>(smem + (2 + (j & 1)) * TILE);
+    T* Vb = reinterpret_cast<T*>(smem + (2 + ((j - j_beg) & 1)) * TILE);
     bool bad = false;
 #pragma unroll
     for (int i = 0; i < BN * NC / 256; ++i) {
@@ -278,16 +279,18 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
   f32x16 acc[ND];
 #pragma unroll
   for (int i = 0; i < ND; ++i) acc[i] = f32x16{0};
-  float m = NEG_INF, l = 0.f, mc = 0.f;     // reference maximum of the raw scores, own half's sum, m c
+  // reference maximum of the raw scores, m c (where there is none, so low that any score makes
+  // P infinite), and own half's sum of P
+  float m = NEG_INF, mc = NO_MC, l = 0.f;
 
   // the lane's byte offsets into the tiles; flip() takes them to the other buffers
   int ko[NS], vo[ND], vu[ND];
 #pragma unroll
-  for (int s = 0; s < NS; ++s) ko[s] = (j_beg & 1) * TILE + (l32 * D + swz<D>(l32, 2 * s + h) * 8) * 2;
+  for (int s = 0; s < NS; ++s) ko[s] = (l32 * D + swz<D>(l32, 2 * s + h) * 8) * 2;
 #pragma unroll
   for (int d = 0; d < ND; ++d) {
-    vo[d] = (j_beg & 1) * TILE + tr_offset<D>(lane, d, false) * 2;
-    vu[d] = (j_beg & 1) * TILE + tr_offset<D>(lane, d, true) * 2;
+    vo[d] = tr_offset<D>(lane, d, false) * 2;
+    vu[d] = tr_offset<D>(lane, d, true) * 2;
   }
   auto flip = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -327,50 +330,50 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
     for (int i = 2; i < 16; ++i) x = fmaxf(x, st[i]);
     return half_max(x);
   };
-  // The reference maximum follows the running one only where it lags by more than 2^8:
-  // P then stays below 2^8, inside either type, and O is seldom rescaled.
-  auto follow = [&](float mx) __attribute__((always_inline)) {
-    if (__any((mx - m) * a.c > 8.f)) {
-      const float mn = fmaxf(m, mx);
-      const float f = m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((m - mn) * a.c);
-      m = mn;
-      mc = m == NEG_INF ? 0.f : m * a.c;
-      l *= f;
+  auto follow = [&](float mx) __attribute__((always_inline)) {   // the reference becomes the running maximum
+    const float mn = fmaxf(m, mx), f = m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((m - mn) * a.c);
+    m = mn;
+    mc = m == NEG_INF ? NO_MC : m * a.c;
+    l *= f;
 #pragma unroll
-      for (int d = 0; d < ND; ++d) acc[d] *= f;
-    }
+    for (int d = 0; d < ND; ++d) acc[d] *= f;
   };
-  auto probs = [&](const f32x16& st, int b) __attribute__((always_inline)) {
-    float p[8];
+  // The reference need not be the maximum, only near it.  EAGER: it follows the maximum of the
+  // next half where that is more than 2^8 ahead.  Otherwise the maxima are not formed at all:
+  // P and its sum are formed with the reference at hand, and a half whose sum passes 2^12 in
+  // some row (so also one with a row's first keys) is formed again after the reference has
+  // followed.  P stays below 2^12 either way, inside either type, and O is seldom rescaled.
+  // The second way takes 10 vector instructions less of 86 a half (prompt of 32768, 16 / 4
+  // heads: 4.03 -> 3.87 ms) and 16 registers more, which the paged kernel does not have.
+  constexpr bool EAGER = PAGED;
+  auto element = [&](const f32x16& st, int i, float* p, float& sum) __attribute__((always_inline)) {
+    p[i] = __builtin_amdgcn_exp2f(st[i] * a.c - mc);
+    sum += p[i];
+  };
+  auto settle = [&](const f32x16& st, float* p, float& sum) __attribute__((always_inline)) {
+    if (__any(sum > 4096.f)) {
+      follow(maximum(st));
+      sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      p[i] = __builtin_amdgcn_exp2f(st[b + i] * a.c - mc);
-      l += p[i];
+      for (int i = 0; i < 16; ++i) element(st, i, p, sum);
     }
+    l += sum;
+  };
+  auto pack = [&](const float* p) __attribute__((always_inline)) {
     return pack8<T>(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
   };
-  auto values = [&](int r, v8 pf) __attribute__((always_inline)) {   // 16 rows of V from row r of the tile
-    const char* Vb = smem + 2 * TILE + r * D * 2;
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-      acc[d] = El<T>::mma32(join<T>(tr4<T>(reinterpret_cast<const T*>(Vb + vo[d])),
-                                    tr4<T>(reinterpret_cast<const T*>(Vb + vu[d]))), pf, acc[d]);
-  };
   // half u, whose scores are cur, against V's rows r of its tile; nxt receives the next
-  // half's scores from K's half kt
-  auto half = [&](int u, const f32x16& cur, f32x16& nxt, int kt, int r) __attribute__((always_inline)) {
-    const char *Kb = smem + kt * 32 * D * 2, *Vb = smem + 2 * TILE + r * D * 2;
-    constexpr int AHEAD = 2;                // LDS reads run so many products ahead
+  // half's scores from K's half kt; the tiles are the buffers at `at`
+  constexpr int AHEAD = 2;                  // LDS reads run so many products ahead
+  auto half = [&](int u, const f32x16& cur, f32x16& nxt, int at, int kt, int r) __attribute__((always_inline)) {
+    const char *Kb = smem + at + kt * 32 * D * 2, *Vb = smem + at + 2 * TILE + r * D * 2;
+    constexpr int E = EAGER ? 8 : 16;       // elements of P formed beside the scores
     v8 kf[NS], vf[2 * ND], pf[2];
-    float p[16], mx = NEG_INF;
+    float p[16], sum = 0.f, mx = NEG_INF;
     auto key_of = [&](int s) __attribute__((always_inline)) { kf[s] = *reinterpret_cast<const v8*>(Kb + ko[s]); };
     auto value_of = [&](int g) __attribute__((always_inline)) {
       const char* v = Vb + (g / ND) * 16 * D * 2;
       vf[g] = join<T>(tr4<T>(reinterpret_cast<const T*>(v + vo[g % ND])), tr4<T>(reinterpret_cast<const T*>(v + vu[g % ND])));
-    };
-    auto element = [&](int i) __attribute__((always_inline)) {
-      p[i] = __builtin_amdgcn_exp2f(cur[i] * a.c - mc);
-      l += p[i];
     };
 #pragma unroll
     for (int s = 0; s < AHEAD; ++s) key_of(s);
@@ -381,34 +384,62 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
       else value_of(s + AHEAD - NS);
       nxt = El<T>::mma32(kf[s], qf[s], s == 0 ? f32x16{0} : nxt);
 #pragma unroll
-      for (int i = s * 8 / NS; i < (s + 1) * 8 / NS; ++i) element(i);
+      for (int i = s * E / NS; i < (s + 1) * E / NS; ++i) element(cur, i, p, EAGER ? l : sum);
       fence();
     }
-    pf[0] = pack8<T>(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
-    asm volatile("" : "+v"(pf[0]));         // formed here, not behind the mask
+    if constexpr (EAGER) {
+      pf[0] = pack(p);
+      asm volatile("" : "+v"(pf[0]));       // formed here, not behind the mask
+    } else {
+      settle(cur, p, sum);
+    }
     mask(u + 1, nxt);
+    if constexpr (!EAGER) pf[0] = pack(p);
 #pragma unroll
     for (int g = 0; g < 2 * ND; ++g) {
       if (g + AHEAD < 2 * ND) value_of(g + AHEAD);
       acc[g % ND] = El<T>::mma32(vf[g], pf[g / ND], acc[g % ND]);
-      if (g < ND) {
+      if constexpr (EAGER) {
+        if (g < ND) {
 #pragma unroll
-        for (int i = g * 8 / ND; i < (g + 1) * 8 / ND; ++i) element(8 + i);
-        if (g == ND - 1) pf[1] = pack8<T>(p[8], p[9], p[10], p[11], p[12], p[13], p[14], p[15]);
+          for (int i = g * 8 / ND; i < (g + 1) * 8 / ND; ++i) element(cur, 8 + i, p, l);
+          if (g == ND - 1) pf[1] = pack(p + 8);
+        } else {
+#pragma unroll
+          for (int i = (g - ND) * 16 / ND; i < (g - ND + 1) * 16 / ND; ++i) mx = fmaxf(mx, nxt[i]);
+        }
       } else {
-
-#pragma unroll
-        for (int i = (g - ND) * 16 / ND; i < (g - ND + 1) * 16 / ND; ++i) mx = fmaxf(mx, nxt[i]);
+        if (g == 0) pf[1] = pack(p + 8);
       }
       fence();
     }
-    follow(half_max(mx));
+    if constexpr (EAGER) {
+      mx = half_max(mx);
+      if (__any((mx - m) * a.c > 8.f)) follow(mx);
+    }
   };
   auto last_half = [&](const f32x16& cur, int r) __attribute__((always_inline)) {
-    values(r, probs(cur, 0));
-    values(r + 16, probs(cur, 8));
+    float p[16], sum = 0.f;
+    if constexpr (!EAGER) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) element(cur, i, p, sum);
+      settle(cur, p, sum);
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      if constexpr (EAGER) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) element(cur, 8 * b + i, p, l);
+      }
+      const v8 pf = pack(p + 8 * b);
+      const char* Vb = smem + 2 * TILE + (r + 16 * b) * D * 2;
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+        acc[d] = El<T>::mma32(join<T>(tr4<T>(reinterpret_cast<const T*>(Vb + vo[d])),
+                                      tr4<T>(reinterpret_cast<const T*>(Vb + vu[d]))), pf, acc[d]);
+    }
   };
-  auto arrive = [&](int j) __attribute__((always_inline)) {                // step j's tiles are there, step j + 1's on their way
+  auto arrive = [&](int j) __attribute__((always_inline)) {   // step j's tiles are there, step j + 1's on their way
     dma_wait<0>();
     __syncthreads();
     if (j < j_end) stage(j + 1);
@@ -428,20 +459,31 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
       if (u_last == u_beg) {
         last_half(s0, 32);
       } else {
-        half(u_beg, s0, s1, 1, 32);
+        half(u_beg, s0, s1, 0, 1, 32);
         const int jf = (u_last + 1) >> 1;
-        for (++j; j < jf; ++j) {
+        ++j;
+        if constexpr (!PAGED) {             // two steps, so that the buffers are constants
+          for (; j + 1 < jf; j += 2) {      // (over pages the code of two would not fit the cache)
+            arrive(j);
+            half(2 * j - 1, s1, s0, TILE, 0, 0);
+            half(2 * j, s0, s1, TILE, 1, 32);
+            arrive(j + 1);
+            half(2 * j + 1, s1, s0, 0, 0, 0);
+            half(2 * j + 2, s0, s1, 0, 1, 32);
+          }
+        }
+        for (; j < jf; ++j) {
           arrive(j);
           flip();
-          half(2 * j - 1, s1, s0, 0, 0);
-          half(2 * j, s0, s1, 1, 32);
+          half(2 * j - 1, s1, s0, 0, 0, 0);
+          half(2 * j, s0, s1, 0, 1, 32);
         }
         arrive(j);
         flip();
         if (u_last & 1) {
           last_half(s1, 0);
         } else {
-          half(2 * j - 1, s1, s0, 0, 0);
+          half(2 * j - 1, s1, s0, 0, 0, 0);
           last_half(s0, 32);
         }
       }
