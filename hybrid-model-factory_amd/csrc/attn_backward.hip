@@ -22,7 +22,7 @@ struct BwdArgs {
   int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, o_ts, o_hs, do_ts, do_hs;   // bytes
   int64_t dq_ts, dq_hs, dk_ts, dk_hs, dv_ts, dv_hs;
   const float* lse;    // [T, H]
-  float* delta;        // [2, T, H]: delta, and lse - P_UP
+  float* delta;        // [T, H]
   Seqs seqs;           // rows of tokens x G
   FastDiv G;
   int32_t H, HKV, slots;
@@ -31,7 +31,6 @@ struct BwdArgs {
 };
 
 constexpr int QM = 128;              // dQ: rows of a workgroup
-constexpr float P_UP = 14.f;         // P is held times 2^14 for dK and dV: fp16 then keeps its precision down to 2^-28
 
 template <typename T, int D>
 __global__ __launch_bounds__(256, 2) void attn_bwd_dq_kernel(BwdArgs a) {
@@ -158,10 +157,7 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_dq_kernel(BwdArgs a) {
   // P sums to 1, so dS would sum to 0 had delta been formed from an exact O: what it does
   // sum to is delta's error, and dK gets a delta without it.
   over = pair_sum32(over, over);
-  if (h == 0 && row < t.rows) {
-    a.delta[gt * a.H + head] = delta + over;
-    a.delta[((int64_t)a.seqs.T + gt) * a.H + head] = lse - P_UP;
-  }
+  if (h == 0 && row < t.rows) a.delta[gt * a.H + head] = delta + over;
   if (row < t.rows) {
 #pragma unroll
     for (int d = 0; d < ND; ++d)
@@ -175,223 +171,238 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_dq_kernel(BwdArgs a) {
   }
 }
 
-constexpr int KM = 128, KR = 32;     // dK, dV: keys of a workgroup, rows of a unit
+constexpr int KM = 128, KR = 64;     // dK, dV: keys of a workgroup, rows of a tile
 
-// Two waves share 32 keys and a SIMD: one forms S = Q K^T, P and dV^T += dO^T P, the other
-// dP = dO V^T, dS and dK^T += Q^T dS, a unit of 32 rows behind; P goes from the first to the
-// second through LDS in fp16 (2^-12 of it, against the 2^-9 of dS's own rounding).  The two
-// are the same program over Q and dO in each other's places, and each holds one operand and
-// one accumulator, so both fit a SIMD at 256 registers: where one wave did all of it, alone
-// on its SIMD, its waits and its issue were the bound (2.69 ms at 8 x 4096 tokens, 32 / 8
-// heads, against DKV_FIGURE).  In each, the next unit's first product is formed while this
-// unit's exponentials (or differences) are.  Units arrive in LDS directly, in a ring of eight.
+// A wave holds 32 keys: their K and V rows as B operands and dK^T, dV^T as accumulators in
+// registers (one wave a SIMD), and walks the rows that see them.  Pipelined by units
+// of 32 rows: S and dP of the next unit are formed by the matrix cores while P and dS of
+// this one are formed in the VALU.  Tiles of 64 rows of Q and dO arrive in LDS directly, in
+// a ring of four, two tiles ahead: a step still multiplies with the last unit of the tile
+// before (with one tile ahead, 2.91 ms where two take 2.77 at 8 x 4096 tokens, 32 / 8 heads).
 template <typename T, int D>
-__global__ __launch_bounds__(512, 2) void attn_bwd_dkv_kernel(BwdArgs a) {
+__global__ __launch_bounds__(256, 1) void attn_bwd_dkv_kernel(BwdArgs a) {
   typedef typename El<T>::v8 v8;
   typedef typename El<T>::v4 v4;
-  constexpr int NC = D / 8, RI = 64 / NC, NL = 8 / RI, NS = D / 16, ND = D / 32;
-  constexpr int RING = 8, UNIT = KR * D * 2;                 // bytes of a unit's Q, and of its dO
-  __shared__ __align__(1024) char smem[RING * 2 * UNIT];     // [RING][Q, dO]
-  __shared__ __align__(1024) f16 Ps[2][4][2][64][8];         // P of a unit: [unit][keys][half][lane]
-  __shared__ __align__(16) float Ls[RING][2][KR];            // lse - 14 and delta of the rows
+  constexpr int NC = D / 8, RI = 64 / NC, NL = 16 / RI, NS = D / 16, ND = D / 32;
+  constexpr int TILE = KR * D * 2;          // bytes
+  constexpr int RING = 4;
+  __shared__ __align__(1024) char smem[RING * 2 * TILE];  // [RING][Q, dO]
+  __shared__ __align__(16) float Ls[RING][2][KR];         // lse and delta of the rows
 
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), grp = wave & 3, role = wave >> 2;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kvh = blockIdx.x % a.HKV;
   Seqs sk = a.seqs;
   sk.G = 1;
   const Tile t = next_tile<KM, false>(sk, nullptr, blockIdx.x / a.HKV, a.slots);
   if (t.row0 >= t.rows || t.row0 < 0) return;
-  const int key = t.row0 + grp * 32 + l32, keyc = min(key, t.tokens - 1);
+  const int key = t.row0 + wave * 32 + l32, keyc = min(key, t.tokens - 1);
   const int64_t gk = t.bos + keyc;
-  char* out = role ? a.dk + gk * a.dk_ts + (int64_t)kvh * a.dk_hs : a.dv + gk * a.dv_ts + (int64_t)kvh * a.dv_hs;
+  char* dkr = a.dk + gk * a.dk_ts + (int64_t)kvh * a.dk_hs;
+  char* dvr = a.dv + gk * a.dv_ts + (int64_t)kvh * a.dv_hs;
   if (t.seq < 0) {
     if (key < t.tokens)
 #pragma unroll
-      for (int i = 0; i < NS; ++i) *reinterpret_cast<u32x4*>(out + 32 * i + 16 * h) = u32x4{0, 0, 0, 0};
+      for (int i = 0; i < NS; ++i) {
+        *reinterpret_cast<u32x4*>(dkr + 32 * i + 16 * h) = u32x4{0, 0, 0, 0};
+        *reinterpret_cast<u32x4*>(dvr + 32 * i + 16 * h) = u32x4{0, 0, 0, 0};
+      }
     return;
   }
-  v8 of[NS];                                // the wave's operand: its keys' K, or their V
-  {
-    const char* kv = role ? a.v + gk * a.v_ts + (int64_t)kvh * a.v_hs : a.k + gk * a.k_ts + (int64_t)kvh * a.k_hs;
+  v8 kf[NS], vf[NS];
 #pragma unroll
-    for (int s = 0; s < NS; ++s) of[s] = *reinterpret_cast<const v8*>(kv + 32 * s + 16 * h);
+  for (int s = 0; s < NS; ++s) {
+    kf[s] = *reinterpret_cast<const v8*>(a.k + gk * a.k_ts + (int64_t)kvh * a.k_hs + 32 * s + 16 * h);
+    vf[s] = *reinterpret_cast<const v8*>(a.v + gk * a.v_ts + (int64_t)kvh * a.v_hs + 32 * s + 16 * h);
   }
-  const int G = a.G.d, rows = t.tokens * G, nu = (rows + KR - 1) / KR;
-  const int wk0 = min(t.row0 + grp * 32, t.tokens - 1);            // the wave's first key
-  const int u_wg = t.row0 * G / KR, u_own = wk0 * G / KR;          // first units with rows that see them
+  const int G = a.G.d, rows = t.tokens * G, nt = (rows + KR - 1) / KR;
+  const int wk0 = min(t.row0 + wave * 32, t.tokens - 1);           // the wave's first key
+  const int j_wg = t.row0 * G / KR, j_own = wk0 * G / KR;          // first tiles with rows that see them
   const int first = key * G;                                        // the key's first row
 
-  // Staging: waves 0-3 bring Q's rows of a unit, 4-7 dO's, 8 each.  Where G divides a unit's
-  // rows, a lane's rows of all units are one head's, at offsets that do not change.
-  const int64_t r_ts = role ? a.do_ts : a.q_ts, r_hs = role ? a.do_hs : a.q_hs;
-  const char* rbase = uniform_ptr((role ? a.dout : a.q) + (int64_t)t.bos * r_ts + (int64_t)kvh * G * r_hs);
-  uint32_t roff[NL];
+  // Staging: rows 16 wave .. + 15 of a tile, RI to a load.  Where G divides a tile's rows, a
+  // lane's rows of all tiles are one head's, at offsets that do not change.
+  uint32_t qoff[NL], ooff[NL];
 #pragma unroll
   for (int i = 0; i < NL; ++i) {
-    const int x = grp * 8 + i * RI + lane / NC, tk = fdiv(x, a.G), g = x - tk * G;
-    roff[i] = (uint32_t)(tk * r_ts + g * r_hs + 16 * swz<D>(x, lane % NC));
+    const int x = wave * 16 + i * RI + lane / NC, tk = fdiv(x, a.G), g = x - tk * G;
+    const int c = swz<D>(x, lane % NC);
+    qoff[i] = (uint32_t)(tk * a.q_ts + g * a.q_hs + 16 * c);
+    ooff[i] = (uint32_t)(tk * a.do_ts + g * a.do_hs + 16 * c);
   }
-  const int tpu = KR / G;                   // tokens of a unit where G divides it
-  auto stage = [&](int u) __attribute__((always_inline)) {
-    const int slot = u % RING;
-    const uint32_t lds = lds_addr(smem) + (slot * 2 + role) * UNIT + grp * 8 * D * 2;
-    if (a.fixed && (u + 1) * KR <= rows) {
-      const char* b = uniform_ptr(rbase + (int64_t)u * tpu * r_ts);
+  const char* qbase = a.q + (int64_t)t.bos * a.q_ts + (int64_t)kvh * G * a.q_hs;
+  const char* obase = a.dout + (int64_t)t.bos * a.do_ts + (int64_t)kvh * G * a.do_hs;
+  const int tpt = KR / G;                   // tokens of a tile where G divides it
+  auto stage = [&](int j, int buf) __attribute__((always_inline)) {
+    const uint32_t ql = lds_addr(smem) + buf * 2 * TILE + wave * 16 * D * 2, ol = ql + TILE;
+    if (a.fixed && (j + 1) * KR <= rows) {
+      const char *qb = uniform_ptr(qbase + (int64_t)j * tpt * a.q_ts), *ob = uniform_ptr(obase + (int64_t)j * tpt * a.do_ts);
 #pragma unroll
-      for (int i = 0; i < NL; ++i) dma16(lds + i * RI * D * 2, b, roff[i]);
+      for (int i = 0; i < NL; ++i) dma16(ql + i * RI * D * 2, qb, qoff[i]);
+#pragma unroll
+      for (int i = 0; i < NL; ++i) dma16(ol + i * RI * D * 2, ob, ooff[i]);
     } else {
 #pragma unroll
       for (int i = 0; i < NL; ++i) {
-        const int x = grp * 8 + i * RI + lane / NC, r = min(u * KR + x, rows - 1), tk = fdiv(r, a.G);
-        dma16(lds + i * RI * D * 2, rbase + tk * r_ts + (r - tk * G) * r_hs + 16 * swz<D>(x, lane % NC));
+        const int x = wave * 16 + i * RI + lane / NC, r = min(j * KR + x, rows - 1), tk = fdiv(r, a.G);
+        const int g = r - tk * G, c = 16 * swz<D>(x, lane % NC);
+        dma16(ql + i * RI * D * 2, qbase + tk * a.q_ts + g * a.q_hs + c);
+        dma16(ol + i * RI * D * 2, obase + tk * a.do_ts + g * a.do_hs + c);
       }
     }
-    // the rows' terms, 32 lanes each (every wave brings them: its loads are counted)
-    const int r = min(u * KR + l32, rows - 1), tk = fdiv(r, a.G);
-    const float* terms = a.delta + (h ? 0 : (int64_t)a.seqs.T * a.H);
-    dma4(lds_addr(&Ls[slot][0][0]),
-         reinterpret_cast<const char*>(terms + ((int64_t)(t.bos + tk) * a.H + kvh * G + r - tk * G)));
+    const int r = min(j * KR + lane, rows - 1), tk = fdiv(r, a.G);   // wave 0 (and 2) lse, 1 (and 3) delta
+    dma4(lds_addr(&Ls[buf][wave & 1][0]), reinterpret_cast<const char*>(
+        ((wave & 1) ? a.delta : a.lse) + ((int64_t)(t.bos + tk) * a.H + kvh * G + r - tk * G)));
   };
-  int ro[NS], to[ND], tu[ND];               // byte offsets into a unit: rows, and columns of the other operand
+  int qo[NS], to[ND], tu[ND];               // byte offsets into a tile
 #pragma unroll
-  for (int s = 0; s < NS; ++s) ro[s] = role * UNIT + (l32 * D + swz<D>(l32, 2 * s + h) * 8) * 2;
+  for (int s = 0; s < NS; ++s) qo[s] = (l32 * D + swz<D>(l32, 2 * s + h) * 8) * 2;
 #pragma unroll
   for (int d = 0; d < ND; ++d) {
-    to[d] = (1 - role) * UNIT + tr_offset<D>(lane, d, false) * 2;
-    tu[d] = (1 - role) * UNIT + tr_offset<D>(lane, d, true) * 2;
+    to[d] = tr_offset<D>(lane, d, false) * 2;
+    tu[d] = tr_offset<D>(lane, d, true) * 2;
   }
-  f32x16 acc[ND];
+  f32x16 ak[ND], av[ND];
 #pragma unroll
-  for (int i = 0; i < ND; ++i) acc[i] = f32x16{0};
+  for (int i = 0; i < ND; ++i) ak[i] = av[i] = f32x16{0};
 
   auto mask = [&](int u, f32x16& st) __attribute__((always_inline)) {
     // rows before the key do not see it, and rows behind the last are none
-    if (u * KR < (wk0 + 31) * G || (u + 1) * KR > rows) {
+    if (u * 32 < (wk0 + 31) * G || u * 32 + 32 > rows) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int r = u * KR + 8 * (i >> 2) + 4 * h + (i & 3);
+        const int r = u * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
         if (r < first || r >= rows) st[i] = NEG_INF;
       }
     }
   };
-  // The first product of unit u + 1 into sn (NEXT), and what follows from unit u's, st (THIS).
-  // LDS reads run AHEAD steps before their use.
-  constexpr int AHEAD = 2, E = 16 / NS;
-  auto work = [&](auto ROLE, auto NEXT, auto THIS, int u, f32x16& sn, const f32x16& st) __attribute__((always_inline)) {
-    constexpr bool scores = decltype(ROLE)::value, next = decltype(NEXT)::value, cur = decltype(THIS)::value;
-    const char *rn = smem + (u + 1) % RING * 2 * UNIT, *cc = smem + (u + RING) % RING * 2 * UNIT;
-    v8 ra[NS], ct[2 * ND], pf[2];
-    f32x4 term[4];
-    f16x8 ph[2];
-    float x[16];
-    auto rows_of = [&](int s) __attribute__((always_inline)) { ra[s] = *reinterpret_cast<const v8*>(rn + ro[s]); };
+  // The two parts of a unit's work that the pipeline keeps apart: S and dP of unit xn of the
+  // tile in bn (NEXT), and P, dS and their products for unit xc of the tile in bc, whose S
+  // and dP are st and dp (THIS); together, the first part's products hide the second's
+  // exponentials.  LDS reads run AHEAD steps before their use, also into the unit that is
+  // NEXT in the following call (FOLLOW: unit xf of the tile in bf).
+  constexpr int AHEAD = NS / 2;
+  constexpr int E = 16 / NS;                // elements of P formed beside a step of the first part
+  v8 qa[NS], oa[NS];
+  f32x4 le[4], dl[4];
+  auto rows_of = [&](int buf, int x, int s) __attribute__((always_inline)) {
+    const char* q = smem + buf * 2 * TILE + x * 32 * D * 2;
+    qa[s] = *reinterpret_cast<const v8*>(q + qo[s]);
+    oa[s] = *reinterpret_cast<const v8*>(q + TILE + qo[s]);
+  };
+  auto work = [&](auto NEXT, auto THIS, auto FOLLOW, int bn, int xn, f32x16& sn, f32x16& dn, int bc, int xc,
+                  const f32x16& st, const f32x16& dp, int bf, int xf) __attribute__((always_inline)) {
+    constexpr bool next = decltype(NEXT)::value, cur = decltype(THIS)::value, follow = decltype(FOLLOW)::value;
+    const char *qc = smem + bc * 2 * TILE + xc * 32 * D * 2, *oc = qc + TILE;
+    v8 qt[2 * ND], ot[2 * ND], pf[2], sf[2];
+    float p[16], ds[16];
     auto cols_of = [&](int g) __attribute__((always_inline)) {
-      const char* c = cc + (g / ND) * 16 * D * 2;
-      ct[g] = join<T>(tr4<T>(reinterpret_cast<const T*>(c + to[g % ND])), tr4<T>(reinterpret_cast<const T*>(c + tu[g % ND])));
+      const int d = g % ND, at = (g / ND) * 16 * D * 2;
+      ot[g] = join<T>(tr4<T>(reinterpret_cast<const T*>(oc + to[d] + at)), tr4<T>(reinterpret_cast<const T*>(oc + tu[d] + at)));
+      qt[g] = join<T>(tr4<T>(reinterpret_cast<const T*>(qc + to[d] + at)), tr4<T>(reinterpret_cast<const T*>(qc + tu[d] + at)));
     };
-    if constexpr (next) {
-#pragma unroll
-      for (int s = 0; s < AHEAD; ++s) rows_of(s);
-    }
-    if constexpr (cur) {
-      const float* ls = &Ls[(u + RING) % RING][scores ? 0 : 1][4 * h];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) term[i] = *reinterpret_cast<const f32x4*>(ls + 8 * i);
-      if constexpr (!scores) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b) ph[b] = *reinterpret_cast<const f16x8*>(&Ps[u & 1][grp][b][lane][0]);
-      }
-    }
+    auto pack = [&](int b) __attribute__((always_inline)) {
+      const int z = 8 * b;
+      pf[b] = pack8<T>(p[z], p[z + 1], p[z + 2], p[z + 3], p[z + 4], p[z + 5], p[z + 6], p[z + 7]);
+      sf[b] = pack8<T>(ds[z], ds[z + 1], ds[z + 2], ds[z + 3], ds[z + 4], ds[z + 5], ds[z + 6], ds[z + 7]);
+    };
     fence();
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
       if constexpr (next) {
-        if (s + AHEAD < NS) rows_of(s + AHEAD);
+        if (s + AHEAD < NS) rows_of(bn, xn, s + AHEAD);
       }
       if constexpr (cur) {
         if (s + AHEAD >= NS) cols_of(s + AHEAD - NS);
       }
-      if constexpr (next) sn = El<T>::mma32(ra[s], of[s], s == 0 ? f32x16{0} : sn);
+      if constexpr (next) {
+        sn = El<T>::mma32(qa[s], kf[s], s == 0 ? f32x16{0} : sn);
+        dn = El<T>::mma32(oa[s], vf[s], s == 0 ? f32x16{0} : dn);
+      }
       if constexpr (cur) {
 #pragma unroll
-        for (int e = s * E; e < s * E + E; ++e)
-          x[e] = scores ? __builtin_amdgcn_exp2f(st[e] * a.c - term[e >> 2][e & 3])
-                        : (float)ph[e >> 3][e & 7] * (st[e] - term[e >> 2][e & 3]);
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-          if (s == (b + 1) * NS / 2 - 1) {
-            const float* y = x + 8 * b;
-            pf[b] = pack8<T>(y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]);
-            if constexpr (scores)
-              *reinterpret_cast<f16x8*>(&Ps[u & 1][grp][b][lane][0]) =
-                  pack8<f16>(y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]);
-          }
+        for (int e = s * E; e < s * E + E; ++e) {
+          p[e] = __builtin_amdgcn_exp2f(st[e] * a.c - le[e >> 2][e & 3]);
+          ds[e] = p[e] * (dp[e] - dl[e >> 2][e & 3]);
+        }
+        if (s == NS / 2 - 1) pack(0);
+        if (s == NS - 1) pack(1);
       }
       fence();
     }
-    if constexpr (cur) {
 #pragma unroll
-      for (int g = 0; g < 2 * ND; ++g) {
+    for (int g = 0; g < 2 * ND; ++g) {
+      if constexpr (cur) {
         if (g + AHEAD < 2 * ND) cols_of(g + AHEAD);
-        acc[g % ND] = El<T>::mma32(ct[g], pf[g / ND], acc[g % ND]);
-        fence();
       }
+      if constexpr (follow) {
+        if (g >= 2 * ND - AHEAD) rows_of(bf, xf, g - 2 * ND + AHEAD);
+      }
+      if constexpr (next) {                 // the row terms of the unit that is THIS in the following call
+        if (g < 4) {
+          const float* ls = &Ls[bn][0][xn * 32 + 4 * h];
+          le[g] = *reinterpret_cast<const f32x4*>(ls + 8 * g);
+          dl[g] = *reinterpret_cast<const f32x4*>(ls + KR + 8 * g);
+        }
+      }
+      if constexpr (cur) {
+        av[g % ND] = El<T>::mma32(ot[g], pf[g / ND], av[g % ND]);
+        ak[g % ND] = El<T>::mma32(qt[g], sf[g / ND], ak[g % ND]);
+      }
+      fence();
     }
   };
-  // step k: unit k + 1 is there, the RING - 3 after it on their way
-  auto arrive = [&](int k) __attribute__((always_inline)) {
-    if (k + RING - 3 < nu) dma_wait<(RING - 4) * (NL + 1)>();
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
+
+  f32x16 s0, d0, s1, d1;
+  int buf = RING - 1, next = 0;             // of the tile at work, and of the one after it
+  auto arrive = [&](int j) __attribute__((always_inline)) {   // tile j is there, the RING - 2 after it on their way
+    if (j + RING - 3 < nt) dma_wait<(RING - 3) * (2 * NL + 1)>();
     else dma_wait<0>();
     __syncthreads();
-    if (k + RING - 2 < nu) stage(k + RING - 2);
+    if (j + RING - 2 < nt) stage(j + RING - 2, (next + RING - 2) % RING);
   };
-  // the first waves take unit k at step k, the others unit k - 1
-  auto run = [&](auto ROLE) __attribute__((always_inline)) {
-    constexpr std::true_type yes{};
-    constexpr std::false_type no{};
-    constexpr int lag = decltype(ROLE)::value ? 0 : 1;
-    f32x16 s0, s1;
-    int k = u_wg - 1;
-    for (; k - lag < u_own - 1; ++k) arrive(k);        // rows before the wave's keys
-    arrive(k);
-    work(ROLE, yes, no, k - lag, s0, s0);
-    int u = ++k - lag;                                 // scored: in s0
-    for (; u + 2 < nu; u += 2) {
-      arrive(k++);
-      if constexpr (!lag) mask(u, s0);
-      work(ROLE, yes, yes, u, s1, s0);
-      arrive(k++);
-      if constexpr (!lag) mask(u + 1, s1);
-      work(ROLE, yes, yes, u + 1, s0, s1);
-    }
-    arrive(k++);
-    if constexpr (!lag) mask(u, s0);
-    if (u + 1 < nu) {
-      work(ROLE, yes, yes, u, s1, s0);
-      arrive(k++);
-      if constexpr (!lag) mask(u + 1, s1);
-      work(ROLE, no, yes, u + 1, s0, s1);
-    } else {
-      work(ROLE, no, yes, u, s1, s0);
-    }
-    for (; k <= nu; ++k) arrive(k);
+  auto advance = [&]() __attribute__((always_inline)) {
+    buf = next;
+    next = (next + 1) % RING;
   };
+  int j = j_wg;
 #pragma unroll
-  for (int i = 0; i < RING - 3; ++i)
-    if (u_wg + i < nu) stage(u_wg + i);
-  if (role == 0) run(std::true_type{});
-  else run(std::false_type{});
+  for (int i = 0; i < RING - 2; ++i)
+    if (j + i < nt) stage(j + i, i);
+  for (; j <= j_own; ++j) {                 // rows before the wave's keys
+    arrive(j);
+    advance();
+  }
+#pragma unroll
+  for (int s = 0; s < AHEAD; ++s) rows_of(buf, 0, s);
+  work(yes, no, yes, buf, 0, s0, d0, buf, 0, s0, d0, buf, 1);
+  for (; j < nt; ++j) {                     // tile j - 1, with the beginning of tile j
+    mask(2 * j - 2, s0);
+    arrive(j);
+    work(yes, yes, yes, buf, 1, s1, d1, buf, 0, s0, d0, next, 0);
+    mask(2 * j - 1, s1);
+    work(yes, yes, yes, next, 0, s0, d0, buf, 1, s1, d1, next, 1);
+    advance();
+  }
+  mask(2 * nt - 2, s0);
+  work(yes, yes, no, buf, 1, s1, d1, buf, 0, s0, d0, buf, 0);
+  mask(2 * nt - 1, s1);
+  work(no, yes, no, buf, 0, s0, d0, buf, 1, s1, d1, buf, 0);
   if (key < t.tokens) {
-    const float f = __builtin_amdgcn_exp2f(-P_UP) * (role ? a.scale : 1.f);
 #pragma unroll
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        v4 y;
+        v4 x, y;
 #pragma unroll
-        for (int jj = 0; jj < 4; ++jj) y[jj] = (T)(acc[d][4 * i + jj] * f);
-        *reinterpret_cast<v4*>(out + (32 * d + 8 * i + 4 * h) * 2) = y;
+        for (int jj = 0; jj < 4; ++jj) {
+          x[jj] = (T)(ak[d][4 * i + jj] * a.scale);
+          y[jj] = (T)av[d][4 * i + jj];
+        }
+        *reinterpret_cast<v4*>(dkr + (32 * d + 8 * i + 4 * h) * 2) = x;
+        *reinterpret_cast<v4*>(dvr + (32 * d + 8 * i + 4 * h) * 2) = y;
       }
   }
 }
@@ -401,7 +412,7 @@ static void launch_bwd(BwdArgs a, int64_t q_slots, int64_t k_slots, hipStream_t 
   a.slots = (int32_t)q_slots;
   hipLaunchKernelGGL((attn_bwd_dq_kernel<T, D>), dim3((unsigned)(q_slots * a.HKV)), dim3(256), 0, s, a);
   a.slots = (int32_t)k_slots;
-  hipLaunchKernelGGL((attn_bwd_dkv_kernel<T, D>), dim3((unsigned)(k_slots * a.HKV)), dim3(512), 0, s, a);
+  hipLaunchKernelGGL((attn_bwd_dkv_kernel<T, D>), dim3((unsigned)(k_slots * a.HKV)), dim3(256), 0, s, a);
 }
 
 }  // namespace attn

@@ -47,7 +47,7 @@ def attention_backward(q, k, v, o, lse, cu_seqlens, do, scale):
     cu = None if cu_seqlens is None else _offsets(cu_seqlens, q.shape[1], q.device)
     B, T, H, D = q.shape
     dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
-    delta = torch.empty(2, *lse.shape, dtype=torch.float32, device=q.device)
+    delta = torch.empty_like(lse)
     rows = [_rows(x) for x in (q, k, v, o, do.to(torch.bfloat16))]     # held until the launch
     ins = [y for x, ts, hs in rows for y in (x.data_ptr(), ts, hs)]
     grads = [y for x in (dq, dk, dv) for y in (x.data_ptr(), *_rows(x)[1:])]

@@ -878,7 +878,7 @@ int hmx_causal_attention(const void* q, int64_t q_token_stride, int64_t q_head_s
  * The backward of hmx_causal_attention (bf16): dq [T, H, D], dk, dv [T, HKV, D] from the
  * inputs, the output o, its gradient dout and the forward's lse; k's and v's summed over
  * the heads that share them, all sums in a fixed order.  Rows of no sequence become 0.
- * delta: fp32 scratch [2, T, H].
+ * delta: fp32 scratch [T, H].
  */
 int hmx_causal_attention_bwd(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                              const void* k, int64_t k_token_stride, int64_t k_head_stride,
