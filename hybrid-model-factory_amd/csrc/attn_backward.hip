@@ -115,14 +115,13 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_dq_kernel(BwdArgs a) {
 #pragma unroll
   for (int i = 0; i < ND; ++i) acc[i] = f32x16{0};
 
-  stage(0);
-  for (int j = 0; j < nt; ++j) {
-    const T *Kb = Ks[j & 1], *Vb = Vs[j & 1];
+  auto step = [&](int j, int buf) __attribute__((always_inline)) {
+    const T *Kb = Ks[buf], *Vb = Vs[buf];
     dma_wait<0>();
     __syncthreads();
     if (j + 1 < nt) stage(j + 1);
     const int t0 = j * QN;
-    if (t0 > w_last) continue;
+    if (t0 > w_last) return;
 #pragma unroll
     for (int kt = 0; kt < QN / 32; ++kt) {
       f32x16 st = {0}, dp = {0};
@@ -153,6 +152,11 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_dq_kernel(BwdArgs a) {
           acc[d] = El<T>::mma32(join<T>(tr4<T>(kp + to[d]), tr4<T>(kp + tu[d])), ks ? d1 : d0, acc[d]);
         }
     }
+  };
+  stage(0);
+  for (int j = 0; j < nt; j += 2) {         // two steps, so that the buffers are constants
+    step(j, 0);
+    if (j + 1 < nt) step(j + 1, 1);
   }
   // P sums to 1, so dS would sum to 0 had delta been formed from an exact O: what it does
   // sum to is delta's error, and dK gets a delta without it.
