@@ -133,7 +133,7 @@ extern "C" int hmx_append_paged_kv(const void* q, int64_t q_token_stride, int64_
   HMX_REQUIRE(cache->num_pages >= 0 && cache->page_size > 0, HMX_EINVAL,
               "hmx_append_paged_kv: %d pages of %d", cache->num_pages, cache->page_size);
   if (tokens == 0) return HMX_OK;
-  HMX_REQUIRE(k && v && slots && cache->k && cache->v && (!q_out || q), HMX_EINVAL,
+  HMX_REQUIRE(k && v && slots && (cache->num_pages == 0 || (cache->k && cache->v)) && (!q_out || q), HMX_EINVAL,
               "hmx_append_paged_kv: null pointer");
   HMX_REQUIRE(rotary_dim == 0 || (positions && cos_sin && max_position > 0 &&
                                   cos_sin_dtype >= 0 && cos_sin_dtype <= 2),

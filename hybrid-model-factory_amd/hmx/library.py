@@ -317,6 +317,15 @@ def _(q, k, v, scale, cu_seqlens):
 def _attention_bwd(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, do: Tensor,
                    scale: Optional[float], cu_seqlens: Optional[Tensor]
                    ) -> tuple[Tensor, Tensor, Tensor]:
+    for name, t in (("o", o), ("do", do)):
+        if t.shape != q.shape or t.dtype != q.dtype:
+            raise ValueError(f"causal_attention_bwd: {name} {tuple(t.shape)} {t.dtype} must be q's")
+    if q.dim() != 4 or tuple(lse.shape) != (q.shape[0] * q.shape[1], q.shape[2]) \
+            or lse.dtype != torch.float32 or not lse.is_contiguous():
+        raise ValueError(f"causal_attention_bwd: lse [B * T, H] fp32 of q {tuple(q.shape)}, got "
+                         f"{tuple(lse.shape)} {lse.dtype}")
+    ops.attention.check_qkv("causal_attention_bwd", q, k, v, cu_seqlens)
+    ops.attention._same_device(q, o, lse, do)
     return ops.attention_train.attention_backward(q, k, v, o, lse, cu_seqlens, do, scale)
 
 

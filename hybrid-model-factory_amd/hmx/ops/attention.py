@@ -83,6 +83,8 @@ def _out(out: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
     if not _aligned(out) or (out.dim() == 4 and out.shape[0] > 1 and out.shape[1] > 1
                              and out.stride(0) != out.shape[1] * out.stride(1)):
         raise ValueError("out must have D contiguous, 16-byte aligned rows and tokens at one stride")
+    if not out.is_contiguous() and any(s == 0 and m > 1 for s, m in zip(out.stride(), out.shape)):
+        raise ValueError("out must have a place of its own for every row")
     return out
 
 
@@ -130,8 +132,8 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     q [B, T, H, D], k and v [B, T, HKV, D]; with ``cu_seqlens`` (N + 1 offsets into the
     tokens, B = 1) each of the N packed sequences by itself.  ``scale`` (default
     D ** -0.5) must be positive.  Returns [B, T, H, D] in q's type; rows of no sequence
-    are 0, or left as they were in ``out`` (which may not overlap an input).  A value that is not finite reaches the rows
-    that attend it and no others.
+    are 0, or left as they were in ``out`` (which may not overlap an input).  A value that
+    is not finite reaches the rows that attend it and no others.
 
     Differentiable in q, k and v for bf16 (hmx.CausalAttention)."""
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):

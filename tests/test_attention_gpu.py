@@ -324,3 +324,14 @@ def test_many_packed_sequences(dev):
         out = hmx.causal_attention(q.to(dev), k.to(dev), v.to(dev), cu_seqlens=torch.tensor(cu, device=dev))
         o, a = ref.causal(q[0], k[0], v[0], D ** -0.5, bounds_of(cu))
         check_o(out[0], o, a, v[0], f"{N} sequences")
+
+
+def test_append_to_an_empty_cache(dev):
+    """A cache of no pages stores nothing; q is rotated all the same."""
+    gen = torch.Generator().manual_seed(21)
+    k, q = randn(gen, 3, 2, 64).to(dev), randn(gen, 3, 4, 64).to(dev)
+    cs = torch.cat([torch.zeros(4, 8), torch.ones(4, 8)], 1).to(dev)      # a quarter turn
+    kc = torch.empty(0, 16, 2, 64, dtype=BF, device=dev)
+    idx = torch.zeros(3, dtype=torch.int32, device=dev)
+    got = hmx.append_paged_kv(k, k, kc, kc, idx, q=q, positions=idx, cos_sin=cs)
+    assert torch.equal(got, torch.cat([-q[..., 8:16], q[..., :8], q[..., 16:]], -1))

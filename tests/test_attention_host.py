@@ -174,3 +174,29 @@ def test_registered_with_fakes_and_mutations():
     w = {a.name for a in torch.ops.hmx.append_paged_kv.default._schema.arguments
          if a.alias_info is not None and a.alias_info.is_write}
     assert w == {"k_cache", "v_cache"}
+
+
+def test_out_with_rows_on_one_place_is_refused():
+    from hmx.ops.attention import _out
+    q = torch.zeros(1, 4, 2, 64, dtype=BF)
+    assert _out(torch.zeros(1, 4, 4, 64, dtype=BF)[:, :, 1:3], q) is not None
+    for bad in (torch.zeros(1, 1, 2, 64, dtype=BF).expand(1, 4, 2, 64),
+                torch.zeros(1, 4, 1, 64, dtype=BF).expand(1, 4, 2, 64)):
+        with pytest.raises(ValueError, match="place of its own"):
+            _out(bad, q)
+
+
+def test_registered_backward_refuses_other_shapes():
+    import hmx.library  # noqa: F401
+    q, k, v = _qkv()
+    lse = torch.zeros(4, 4)
+    bwd = lambda o=q, lse=lse, do=q: torch.ops.hmx.causal_attention_bwd(q, k, v, o, lse, do, None, None)
+    with pytest.raises(ValueError, match="o .* must be q's"):
+        bwd(o=q[:, :3])
+    with pytest.raises(ValueError, match="do .* must be q's"):
+        bwd(do=q.float())
+    for bad in (lse[:3], lse.double(), torch.zeros(4, 8)[:, ::2]):
+        with pytest.raises(ValueError, match="lse"):
+            bwd(lse=bad)
+    with pytest.raises(RuntimeError, match="GPU"):
+        bwd()
