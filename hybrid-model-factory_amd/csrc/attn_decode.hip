@@ -13,6 +13,10 @@
 // S^T = K Q^T and (transposed) of O^T = V^T P^T.
 // P enters its product as the inputs' type and, beside it, what that rounding leaves: the
 // matrix cores wait for memory anyway.  Scores, statistics and O stay in fp32.
+//
+// Measured: 256 sequences to 8192 keys, 32 / 8 heads of 128 (4.7 GB), 829 us, 5.7 TB/s, where
+// a large copy reaches 4.7 - 5.1 (875 us where the rows came through registers); two
+// sequences to 131072 keys, 14 / 2 heads of 64, 31 - 35 us with the joining.
 #include "attn.hpp"
 
 namespace hmx {
@@ -23,7 +27,8 @@ constexpr int KT = 16;       // keys of a wave's turn
 constexpr int NW = 4;        // waves
 constexpr int MIN_UNITS = 4; // of a worker: below that the joining costs more than it gains
 // Where a table holds no more keys than this, a worker takes whole sequences: one launch and
-// no scan of the lengths (one sequence of 700 keys: SHORT_FIGURES).
+// no scan of the lengths (one sequence of 700 keys, 32 / 8 heads: 16.7 us a call where a cut
+// and its joining take 19.6).
 constexpr int SHORT_KEYS = 1024;
 
 struct DecArgs {
