@@ -9,10 +9,10 @@
 // Products are transposed where that leaves P and dS as B operands in the C layout.
 // P and dS are rounded to bf16 (half a step, as the inputs themselves are); everything
 // else stays in fp32.  What that costs against float64, where rounding the results alone makes
-// an error of 1.7e-3: dV 2.3e-3; dK 2.3e-3; dQ 2.8e-3, for delta is formed from the rounded O.
-// Keeping eight more bits of O beside it took dQ's to 2.6e-3 for 1.2 % of the step and half as
-// much memory again as O's (the other part of delta's error is O's own, from P's rounding);
-// dS in two parts would take it to 2.3e-3, for a tenth of the step.
+// an error of 1.7e-3: dK 2.3e-3; dQ 2.8e-3, for delta is formed from the rounded O.  Keeping
+// eight more bits of O beside it took dQ's to 2.6e-3, for 1.2 % of the step and half as much
+// memory again as O's (the rest of delta's error is O's own, from P's rounding), and a product
+// more with what dS's rounding leaves would take about a tenth of the step: neither is done.
 //
 // Measured at 8 x 4096 tokens, 32 / 8 heads of 128 (forward 1.10 ms): dQ 1.53 ms, 1.08 PFLOP/s;
 // dK and dV 2.45 ms, 0.9; a large matrix product reaches 1.22 - 1.26.
