@@ -191,6 +191,14 @@ struct Tile {
   int seq;             // -1: rows of no sequence
   int bos, tokens;     // the part's first token and its tokens
   int row0, rows;      // the tile's first row in the part, the part's rows; row0 >= rows: nothing to do
+  int sp, ns;          // the split of its keys, of ns
+};
+
+// How the keys of row tiles are split, for kernels whose shares are joined: `even` splits of
+// every tile, or, where the sequences' keys are at hand (next_tile), splits of one length, at
+// most `most` a tile and `blocks` in all.
+struct Splits {
+  int32_t even, most, blocks;
 };
 
 __device__ __forceinline__ int seq_bound(const Seqs& s, int e) {
@@ -202,6 +210,8 @@ __device__ __forceinline__ int seq_bound(const Seqs& s, int e) {
 template <int BM>
 __device__ __forceinline__ Tile find_tile(const Seqs& s, int slot) {
   Tile t;
+  t.sp = 0;
+  t.ns = 1;
   if (!s.cu) {
     const int len = s.T / s.N, per = (int)(((int64_t)len * s.G + BM - 1) / BM);
     t.seq = slot / max(per, 1);
@@ -234,31 +244,61 @@ __device__ __forceinline__ Tile find_tile(const Seqs& s, int slot) {
 
 // The tile of the block in place `at`, heaviest first: a row tile's work grows with the keys
 // before it, so a sequence's tiles go from the last (LAST) to the first, or from the first
-// where the first have most; and of up to 62 packed sequences those with most keys come
+// where the first have most; and of up to LANE_SEQS packed sequences those with most keys come
 // first (their lengths are in the lanes of a wave; more go as they lie).  Whatever comes
-// last then is short.  lens: the sequences' keys, NULL where they are their tokens.
+// last then is short.  Splits of unequal sequences get one length, the work over (blocks -
+// tiles): rounded up for every tile they are no more than `blocks`, so all run at once and end
+// together.  lens: the sequences' keys, NULL where they are their tokens.
+constexpr int LANE_SEQS = 62;
 template <int BM, bool LAST>
-__device__ __forceinline__ Tile next_tile(const Seqs& s, const int32_t* lens, int at, int slots) {
-  if (!s.cu || s.N < 1 || s.N > 62) return find_tile<BM>(s, LAST ? slots - 1 - at : at);
+__device__ __forceinline__ Tile next_tile(const Seqs& s, const int32_t* lens, int at, int slots,
+                                          Splits split = Splits{1, 1, 0}) {
+  if (!s.cu || s.N < 1 || s.N > LANE_SEQS) {
+    const int sp = split.even > 1 ? at / slots : 0;
+    at -= sp * slots;
+    Tile t = find_tile<BM>(s, LAST ? slots - 1 - at : at);
+    t.sp = sp;
+    t.ns = split.even;
+    return t;
+  }
   const int lane = threadIdx.x & 63, parts = s.N + 2;
   const bool in = lane < parts, gap = lane == 0 || lane == s.N + 1;
   const int bos = in ? seq_bound(s, lane) : 0;
   const int tokens = in ? max(seq_bound(s, lane + 1) - bos, 0) : 0;
   const int tiles = (int)(((int64_t)tokens * s.G + BM - 1) / BM);
   const int keys = gap ? -1 : lens ? lens[min(max(lane - 1, 0), s.N - 1)] : tokens;
-  int start = 0;                              // tiles of the parts before this lane's
+  int ns = 1;
+  if (split.even > 1) {
+    const int kt = gap ? 0 : max(keys, 0) / 64 + 1;
+    int64_t work = (int64_t)tiles * kt;
+    int all = tiles;
+    for (int d = 32; d >= 1; d >>= 1) {
+      work += __shfl_xor(work, d, 64);
+      all += __shfl_xor(all, d, 64);
+    }
+    const int over = max(split.blocks - all, 1);
+    const int share = (int)max((work + over - 1) / over, (int64_t)4);
+    ns = min(max((kt + share - 1) / share, 1), split.most);
+  }
+  const int blocks = tiles * ns;
+  int start = 0;                              // blocks of the parts before this lane's
   for (int f = 0; f < parts; ++f) {
-    const int k = __builtin_amdgcn_readlane(keys, f), n = __builtin_amdgcn_readlane(tiles, f);
+    const int k = __builtin_amdgcn_readlane(keys, f), n = __builtin_amdgcn_readlane(blocks, f);
     start += k > keys || (k == keys && f < lane) ? n : 0;
   }
-  const unsigned long long m = __ballot(in && at >= start && at < start + tiles);
-  Tile t{-1, 0, 0, 0, 0};
+  const unsigned long long m = __ballot(in && at >= start && at < start + blocks);
+  Tile t{-1, 0, 0, 0, 0, 0, 1};
   if (m == 0) return t;
   const int e = __builtin_ctzll(m);
   t.seq = e == 0 || e == s.N + 1 ? -1 : e - 1;
   t.bos = __builtin_amdgcn_readlane(bos, e);
   t.tokens = __builtin_amdgcn_readlane(tokens, e);
-  const int i = at - __builtin_amdgcn_readlane(start, e);
+  int i = at - __builtin_amdgcn_readlane(start, e);
+  t.ns = __builtin_amdgcn_readlane(ns, e);
+  if (split.even > 1) {
+    t.sp = i % t.ns;
+    i /= t.ns;
+  }
   t.row0 = (LAST ? __builtin_amdgcn_readlane(tiles, e) - 1 - i : i) * BM;
   t.rows = t.tokens * s.G;
   return t;

@@ -19,8 +19,9 @@
 // both, so what pays is fewer instructions.  Measured: one prompt of 32768, 16 / 4 heads of
 // 128, 3.75 - 4.0 ms, 1.1 PFLOP/s (a large matrix product reaches 1.22 - 1.26); packed prompts
 // of 64-wide heads, whose exponentials weigh twice as much against their products, 392 us at
-// 0.84; pieces of prompts over pages 850 us at 0.97; 32 draft tokens behind 16384 keys 75 us and
-// the joining 5, 4.3 TB/s.
+// 0.84; pieces of prompts over pages 850 us at 0.97; draft tokens of eight
+// sequences to 16384 keys 64 us and the joining 5, 5.1 TB/s (76 us where every sequence's keys
+// were cut into as many splits).
 #include "attn.hpp"
 
 namespace hmx {
@@ -28,6 +29,7 @@ namespace attn {
 
 constexpr int BM = 128, BN = 64;
 constexpr float NO_MC = -1e30f;
+constexpr uint32_t NO_SHARE = 0x7fc00000u;   // a NaN, in the place of a share's maximum: there is none
 
 struct FwdArgs {
   const char *q, *k, *v;
@@ -37,7 +39,8 @@ struct FwdArgs {
   Seqs seqs;
   Pages pages;
   FastDiv G;
-  int32_t H, HKV, slots, fill, nsplit;
+  int32_t H, HKV, slots, fill, nsplit;   // nsplit: split.most
+  Splits split;
   float c;             // scale log2(e)
   float* part;         // [nsplit][T * H][D], then [nsplit][T * H][2]: maximum and sum
 };
@@ -165,7 +168,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // uniform, and known to be
   const int kvh = blockIdx.x % a.HKV;
-  const Tile t = next_tile<BM, true>(a.seqs, PAGED ? a.pages.lens : nullptr, blockIdx.x / a.HKV, a.slots);
+  const Tile t = next_tile<BM, true>(a.seqs, PAGED ? a.pages.lens : nullptr, blockIdx.x / a.HKV, a.slots,
+                                       PAGED ? a.split : Splits{1, 1, 0});
   if (t.row0 >= t.rows || t.row0 < 0) return;
 
   const int row = t.row0 + wave * 32 + l32;
@@ -193,8 +197,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
   const int wg_first = off + fdiv(t.row0, a.G);
   const int wg_last = off + fdiv(min(t.row0 + BM, t.rows) - 1, a.G);
   const int nt_all = wg_last < 0 ? 0 : wg_last / BN + 1;
-  const int sp = blockIdx.y;
-  const int j_beg = (int)((int64_t)nt_all * sp / a.nsplit), j_end = (int)((int64_t)nt_all * (sp + 1) / a.nsplit);
+  const int sp = t.sp, ns = t.ns;
+  const int j_beg = (int)((int64_t)nt_all * sp / ns), j_end = (int)((int64_t)nt_all * (sp + 1) / ns);
   const int u_beg = 2 * j_beg, u_last = min(2 * j_end - 1, w_last < 0 ? -1 : w_last / 32);   // the wave's halves
   if (tid < 4) s_skip[tid] = 0;
   if (tid == 0) s_bad = 0;
@@ -515,6 +519,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
       if (h == 0) {
         share_stats<D>(a, sp, r)[0] = m * a.c;
         share_stats<D>(a, sp, r)[1] = l;
+        if (sp == ns - 1)
+          for (int s = ns; s < a.nsplit; ++s) share_stats<D>(a, s, r)[0] = __builtin_bit_cast(float, NO_SHARE);
       }
     }
   } else if (row < t.rows) {
@@ -544,10 +550,13 @@ __global__ __launch_bounds__(256) void attn_join_kernel(FwdArgs a) {
   const int64_t r = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
   const int tok = (int)(r / a.H), h = (int)(r - (int64_t)tok * a.H), d = 4 * (threadIdx.x % TPR);
   if (tok >= a.seqs.T || tok < a.seqs.cu[0] || tok >= a.seqs.cu[a.seqs.N]) return;
+  int ns = 0;
+#pragma unroll 8
+  for (int s = 0; s < a.nsplit; ++s) ns += __builtin_bit_cast(uint32_t, share_stats<D>(a, s, r)[0]) != NO_SHARE;
   float m = NEG_INF, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = 0; s < a.nsplit; ++s) {
+  for (int s = 0; s < ns; ++s) {
     const float* st = share_stats<D>(a, s, r);
     const f32x4 x = *reinterpret_cast<const f32x4*>(share_row<D>(a, s, r) + d);
     const float mn = fmaxf(m, st[0]), ref = mn == NEG_INF ? 0.f : mn;
@@ -563,21 +572,24 @@ __global__ __launch_bounds__(256) void attn_join_kernel(FwdArgs a) {
   *reinterpret_cast<typename El<T>::v4*>(a.o + (int64_t)tok * a.o_ts + (int64_t)h * a.o_hs + 2 * d) = x;
 }
 
-// Splits of the keys: where the row tiles alone leave compute units idle, as many as give
-// each about two workgroups (what runs at once), of at least four tiles of keys (a split
-// costs its share's trip through memory and the joining launch).
-static int splits(int64_t slots, int64_t N, int HKV, int64_t max_keys, bool packed) {
-  const int64_t live = (packed ? slots - 2 : slots) * HKV, want = 2ll * cu_count();
-  int64_t s = live > 0 ? want / live : 1;
-  const int64_t most = max_keys / (4 * BN);
-  if (s > most) s = most;
-  if (s > 64) s = 64;
-  return s < 1 ? 1 : (int)s;
+// Splits of the keys, where the row tiles alone leave compute units idle: as many as give each
+// about two workgroups (what runs at once), of at least four tiles of keys (a split costs its
+// share's trip through memory and the joining launch).  A tile of a longer sequence may take
+// twice as many.
+static Splits splits(int64_t slots, int HKV, int64_t max_keys) {
+  const int64_t live = (slots - 2) * HKV, want = 2ll * cu_count(), most = max_keys / (4 * BN);
+  int64_t even = live > 0 ? want / live : 1;
+  if (even > most) even = most;
+  if (even > 64) even = 64;
+  if (even <= 1) return Splits{1, 1, 0};
+  return Splits{(int32_t)even, (int32_t)(2 * even < most ? 2 * even : most), (int32_t)(want / HKV)};
 }
 
 template <typename T, bool PAGED>
 static void launch_fwd(const FwdArgs& a, int D, hipStream_t s) {
-  const dim3 grid((unsigned)(a.slots * a.HKV), (unsigned)a.nsplit);
+  int64_t blocks = a.slots;                 // of a kv head
+  if (a.nsplit > 1) blocks = a.seqs.N > LANE_SEQS ? blocks * a.split.even : blocks + a.split.blocks;
+  const dim3 grid((unsigned)(blocks * a.HKV));
   if (D == 64) hipLaunchKernelGGL((attn_fwd_kernel<T, 64, PAGED>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((attn_fwd_kernel<T, 128, PAGED>), grid, dim3(256), 0, s, a);
   if (a.nsplit > 1) {
@@ -632,16 +644,16 @@ extern "C" int hmx_causal_attention(const void* q, int64_t q_token_stride, int64
   return check_launch("hmx_causal_attention");
 }
 
-static int paged_splits(int64_t N, int64_t T, int H, int HKV, int64_t max_keys) {
+static attn::Splits paged_splits(int64_t N, int64_t T, int H, int HKV, int64_t max_keys) {
   const int32_t packed = 0;
-  return attn::splits(attn::tile_slots<attn::BM>(&packed, N, T, H / HKV), N, HKV, max_keys, true);
+  return attn::splits(attn::tile_slots<attn::BM>(&packed, N, T, H / HKV), HKV, max_keys);
 }
 
 extern "C" size_t hmx_paged_causal_attention_workspace_bytes(int32_t N, int64_t T, int32_t H,
                                                              int32_t HKV, int32_t D,
                                                              int64_t max_keys) {
   if (N <= 0 || T <= 0 || HKV <= 0 || H <= 0 || H % HKV != 0) return 0;
-  const int ns = paged_splits(N, T, H, HKV, max_keys);
+  const int ns = paged_splits(N, T, H, HKV, max_keys).most;
   return ns == 1 ? 0 : (size_t)ns * T * H * (D + 2) * sizeof(float);
 }
 
@@ -680,7 +692,8 @@ extern "C" int hmx_paged_causal_attention(const void* q, int64_t q_token_stride,
   HMX_REQUIRE(slots * HKV < (1ll << 31), HMX_EUNSUPPORTED, "hmx_paged_causal_attention: %lld tiles",
               (long long)slots);
   a.H = H; a.HKV = HKV; a.slots = (int32_t)slots; a.fill = fill_gaps;
-  a.nsplit = N == 0 ? 1 : paged_splits(N, T, H, HKV, max_keys);
+  a.split = N == 0 ? attn::Splits{1, 1, 0} : paged_splits(N, T, H, HKV, max_keys);
+  a.nsplit = a.split.most;
   a.part = static_cast<float*>(workspace);
   HMX_REQUIRE(a.nsplit == 1 ||
                   (workspace && (uintptr_t)workspace % 16 == 0 &&

@@ -335,3 +335,30 @@ def test_append_to_an_empty_cache(dev):
     idx = torch.zeros(3, dtype=torch.int32, device=dev)
     got = hmx.append_paged_kv(k, k, kc, kc, idx, q=q, positions=idx, cos_sin=cs)
     assert torch.equal(got, torch.cat([-q[..., 8:16], q[..., :8], q[..., 16:]], -1))
+
+
+@pytest.mark.parametrize("news,lens,H,HKV,D", [
+    ([3, 1, 2, 40], [9000, 3, 700, 4096], 4, 1, 128), ([1, 1], [20000, 1], 14, 2, 64),
+    ([2, 0, 5] * 22, [1500, 0, 40] * 22, 2, 1, 64), ([8] * 3, [8192, 8, 8191], 128, 128, 64),
+])
+def test_paged_causal_attention_few_rows_long_contexts(dev, news, lens, H, HKV, D):
+    """Keys split over workgroups, as many to a sequence as its length asks for."""
+    gen = torch.Generator().manual_seed(sum(lens))
+    kc, vc, table, ks, vs = paged(gen, lens, 16, HKV, D, BF)
+    cu = [1]
+    for n in news:
+        cu.append(cu[-1] + n)
+    q = randn(gen, cu[-1] + 1, H, D)
+    args = [x.to(dev) for x in (kc, vc, table)]
+    args += [torch.tensor(x, dtype=torch.int32, device=dev) for x in (lens, cu)]
+    out = hmx.paged_causal_attention(q.to(dev), *args)
+    for n, (b, e) in enumerate(bounds_of(cu)):
+        o, a = ref.rows(q[b:e], ks[n], vs[n], D ** -0.5, lens[n] - (e - b))
+        check_o(out[b:e], o, a, vs[n], f"sequence {n} of {lens[n]}")
+    assert (out[:1] == 0).all() and (out[cu[-1]:] == 0).all()
+    # an infinite score reaches the row's output whichever share holds it
+    q = q.abs()
+    page, at = divmod(lens[0] // 3, 16)
+    args[0][table[0, page], at] = float("inf")
+    out = hmx.paged_causal_attention(q.to(dev), *args)
+    assert out[cu[0]:cu[1]].isnan().all() and out[cu[1]:].isfinite().all()
