@@ -20,7 +20,7 @@
 // 128, 3.75 - 4.0 ms, 1.1 PFLOP/s (a large matrix product reaches 1.22 - 1.26); packed prompts
 // of 64-wide heads, whose exponentials weigh twice as much against their products, 392 us at
 // 0.84; pieces of prompts over pages 850 us at 0.97; draft tokens of eight
-// sequences to 16384 keys 64 us and the joining 5, 5.1 TB/s (76 us where every sequence's keys
+// sequences to 16384 keys 64 - 72 us and the joining 5 (76 us where every sequence's keys
 // were cut into as many splits).
 #include "attn.hpp"
 
