@@ -39,7 +39,7 @@ struct FwdArgs {
   Seqs seqs;
   Pages pages;
   FastDiv G;
-  int32_t H, HKV, slots, fill, nsplit;   // nsplit: split.most
+  int32_t H, HKV, slots, fill, nsplit, places;   // nsplit: split.most
   Splits split;
   float c;             // scale log2(e)
   float* part;         // [nsplit][T * H][D], then [nsplit][T * H][2]: maximum and sum
@@ -168,8 +168,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);   // uniform, and known to be
   const int kvh = blockIdx.x % a.HKV;
-  const Tile t = next_tile<BM, true>(a.seqs, PAGED ? a.pages.lens : nullptr, blockIdx.x / a.HKV, a.slots,
-                                       PAGED ? a.split : Splits{1, 1, 0});
+  const Tile t = next_tile<BM, true>(a.seqs, PAGED ? a.pages.lens : nullptr, place(blockIdx.x / a.HKV, gridDim.x / a.HKV, a.places), a.slots,
+                                       a.split);
   if (t.row0 >= t.rows || t.row0 < 0) return;
 
   const int row = t.row0 + wave * 32 + l32;
@@ -549,7 +549,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(FwdArgs a) {
   constexpr int TPR = D / 4;
   const int64_t r = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
   const int tok = (int)(r / a.H), h = (int)(r - (int64_t)tok * a.H), d = 4 * (threadIdx.x % TPR);
-  if (tok >= a.seqs.T || tok < a.seqs.cu[0] || tok >= a.seqs.cu[a.seqs.N]) return;
+  if (tok >= a.seqs.T || (a.seqs.cu && (tok < a.seqs.cu[0] || tok >= a.seqs.cu[a.seqs.N]))) return;
   int ns = 0;
 #pragma unroll 8
   for (int s = 0; s < a.nsplit; ++s) ns += __builtin_bit_cast(uint32_t, share_stats<D>(a, s, r)[0]) != NO_SHARE;
@@ -570,25 +570,29 @@ __global__ __launch_bounds__(256) void attn_join_kernel(FwdArgs a) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] = (T)(o[i] * inv);
   *reinterpret_cast<typename El<T>::v4*>(a.o + (int64_t)tok * a.o_ts + (int64_t)h * a.o_hs + 2 * d) = x;
+  if (a.lse && d == 0) a.lse[r] = m + __builtin_amdgcn_logf(l);
 }
 
 // Splits of the keys, where the row tiles alone leave compute units idle: as many as give each
-// about two workgroups (what runs at once), of at least four tiles of keys (a split costs its
-// share's trip through memory and the joining launch).  A tile of a longer sequence may take
-// twice as many.
-static Splits splits(int64_t slots, int HKV, int64_t max_keys) {
-  const int64_t live = (slots - 2) * HKV, want = 2ll * cu_count(), most = max_keys / (4 * BN);
+// about two workgroups (what runs at once).  A split costs its share's trip through memory and
+// the joining launch, so it has at least `least` tiles of keys: four over pages, where there
+// are few rows, eight over contiguous keys.  A tile of a longer sequence may take twice as many.
+// Prompts, without splits and with: 2048 tokens, 8 / 2 heads of 128, 42.5 -> 31.6 us; 4096,
+// 4 / 4 of 64, 58 -> 28; 16384, 2 / 1 of 128, 276 -> 175.
+static Splits splits(int64_t tiles, int HKV, int64_t max_keys, int least) {
+  const int64_t live = tiles * HKV, want = 2ll * cu_count(), most = max_keys / (least * BN);
   int64_t even = live > 0 ? want / live : 1;
   if (even > most) even = most;
   if (even > 64) even = 64;
-  if (even <= 1) return Splits{1, 1, 0};
-  return Splits{(int32_t)even, (int32_t)(2 * even < most ? 2 * even : most), (int32_t)(want / HKV)};
+  if (even <= 1) return NO_SPLITS;
+  return Splits{(int32_t)even, (int32_t)(2 * even < most ? 2 * even : most), (int32_t)(want / HKV), least};
 }
 
 template <typename T, bool PAGED>
-static void launch_fwd(const FwdArgs& a, int D, hipStream_t s) {
+static void launch_fwd(FwdArgs a, int D, hipStream_t s) {
+  a.places = (int32_t)(cu_count() / a.HKV);
   int64_t blocks = a.slots;                 // of a kv head
-  if (a.nsplit > 1) blocks = a.seqs.N > LANE_SEQS ? blocks * a.split.even : blocks + a.split.blocks;
+  if (a.nsplit > 1) blocks = !a.seqs.cu || a.seqs.N > LANE_SEQS ? blocks * a.split.even : blocks + a.split.blocks;
   const dim3 grid((unsigned)(blocks * a.HKV));
   if (D == 64) hipLaunchKernelGGL((attn_fwd_kernel<T, 64, PAGED>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((attn_fwd_kernel<T, 128, PAGED>), grid, dim3(256), 0, s, a);
@@ -607,13 +611,28 @@ using namespace hmx;
 
 #define ATTN_COMMON_CHECKS(what)                                                                    HMX_REQUIRE(D == 64 || D == 128, HMX_EUNSUPPORTED, what ": head size %d not in {64, 128}", D);    HMX_REQUIRE(dtype == HMX_BF16 || dtype == HMX_F16, HMX_EUNSUPPORTED,                                          what ": dtype code %d (bf16 or fp16)", dtype);                                        HMX_REQUIRE(N >= 0 && T >= 0 && HKV > 0 && H > 0 && H % HKV == 0, HMX_EINVAL,                                 what ": N=%d T=%lld H=%d HKV=%d", N, (long long)T, H, HKV);                           HMX_REQUIRE(T * (H / HKV) < (1ll << 30), HMX_EUNSUPPORTED, what ": %lld tokens", (long long)T);   HMX_REQUIRE(scale > 0.f && scale < __builtin_inff(), HMX_EINVAL, what ": scale %g must be positive", (double)scale);
 
+static attn::Splits prompt_splits(int64_t N, int64_t T, int H, int HKV, bool packed) {
+  if (N <= 0 || T <= 0) return attn::NO_SPLITS;
+  const int32_t some = 0;
+  const int64_t slots = attn::tile_slots<attn::BM>(packed ? &some : nullptr, N, T, H / HKV);
+  return attn::splits(packed ? slots - 2 : slots, HKV, packed ? T : T / N, 8);
+}
+
+extern "C" size_t hmx_causal_attention_workspace_bytes(int32_t N, int64_t T, int32_t H, int32_t HKV,
+                                                       int32_t D, int32_t packed) {
+  if (N <= 0 || T <= 0 || HKV <= 0 || H <= 0 || H % HKV != 0) return 0;
+  const int ns = prompt_splits(N, T, H, HKV, packed != 0).most;
+  return ns == 1 ? 0 : (size_t)ns * T * H * (D + 2) * sizeof(float);
+}
+
 extern "C" int hmx_causal_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                                     const void* k, int64_t k_token_stride, int64_t k_head_stride,
                                     const void* v, int64_t v_token_stride, int64_t v_head_stride,
                                     int32_t dtype, void* o, int64_t o_token_stride,
                                     int64_t o_head_stride, float* lse, const int32_t* cu_seqlens,
                                     int32_t N, int64_t T, int32_t H, int32_t HKV, int32_t D,
-                                    float scale, int32_t fill_gaps, void* stream) {
+                                    float scale, int32_t fill_gaps, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
   ATTN_COMMON_CHECKS("hmx_causal_attention")
   HMX_REQUIRE(cu_seqlens || N == 0 || T % N == 0, HMX_EINVAL, "hmx_causal_attention: T=%lld is not N=%d sequences",
               (long long)T, N);
@@ -637,7 +656,14 @@ extern "C" int hmx_causal_attention(const void* q, int64_t q_token_stride, int64
   a.G = attn::fast_div(H / HKV);
   const int64_t slots = attn::tile_slots<attn::BM>(cu_seqlens, N, T, H / HKV);
   HMX_REQUIRE(slots * HKV < (1ll << 31), HMX_EUNSUPPORTED, "hmx_causal_attention: %lld tiles", (long long)slots);
-  a.H = H; a.HKV = HKV; a.slots = (int32_t)slots; a.fill = fill_gaps; a.nsplit = 1;
+  a.H = H; a.HKV = HKV; a.slots = (int32_t)slots; a.fill = fill_gaps;
+  a.split = prompt_splits(N, T, H, HKV, cu_seqlens != nullptr);
+  a.nsplit = a.split.most;
+  a.part = static_cast<float*>(workspace);
+  HMX_REQUIRE(a.nsplit == 1 ||
+                  (workspace && (uintptr_t)workspace % 16 == 0 &&
+                   workspace_bytes >= hmx_causal_attention_workspace_bytes(N, T, H, HKV, D, cu_seqlens != nullptr)),
+              HMX_EINVAL, "hmx_causal_attention: workspace of %zu bytes is too small", workspace_bytes);
   a.c = scale * attn::LOG2E;
   if (dtype == HMX_BF16) attn::launch_fwd<bf16, false>(a, D, (hipStream_t)stream);
   else attn::launch_fwd<f16, false>(a, D, (hipStream_t)stream);
@@ -646,7 +672,7 @@ extern "C" int hmx_causal_attention(const void* q, int64_t q_token_stride, int64
 
 static attn::Splits paged_splits(int64_t N, int64_t T, int H, int HKV, int64_t max_keys) {
   const int32_t packed = 0;
-  return attn::splits(attn::tile_slots<attn::BM>(&packed, N, T, H / HKV), HKV, max_keys);
+  return attn::splits(attn::tile_slots<attn::BM>(&packed, N, T, H / HKV) - 2, HKV, max_keys, 4);
 }
 
 extern "C" size_t hmx_paged_causal_attention_workspace_bytes(int32_t N, int64_t T, int32_t H,
@@ -692,7 +718,7 @@ extern "C" int hmx_paged_causal_attention(const void* q, int64_t q_token_stride,
   HMX_REQUIRE(slots * HKV < (1ll << 31), HMX_EUNSUPPORTED, "hmx_paged_causal_attention: %lld tiles",
               (long long)slots);
   a.H = H; a.HKV = HKV; a.slots = (int32_t)slots; a.fill = fill_gaps;
-  a.split = N == 0 ? attn::Splits{1, 1, 0} : paged_splits(N, T, H, HKV, max_keys);
+  a.split = N == 0 ? attn::NO_SPLITS : paged_splits(N, T, H, HKV, max_keys);
   a.nsplit = a.split.most;
   a.part = static_cast<float*>(workspace);
   HMX_REQUIRE(a.nsplit == 1 ||

@@ -120,7 +120,8 @@ SIGNATURES: dict[str, list] = {
                                    _I32, _F32, _P, ctypes.c_size_t, _P],
     "hmx_paged_attention_decode_workspace_bytes": [_I32, _I32, _I32, _I32, _I64],
     "hmx_causal_attention": [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _I64, _I64,
-                             _P, _P, _I32, _I64, _I32, _I32, _I32, _F32, _I32, _P],
+                             _P, _P, _I32, _I64, _I32, _I32, _I32, _F32, _I32, _P, ctypes.c_size_t, _P],
+    "hmx_causal_attention_workspace_bytes": [_I32, _I64, _I32, _I32, _I32, _I32],
     "hmx_causal_attention_bwd": [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _I64,
                                  _I64, _P, _I64, _I64, _P, _P, _I32, _I64, _I32, _I32, _I32, _F32,
                                  _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P],
@@ -136,6 +137,7 @@ _RESTYPES = {"hmx_last_error": ctypes.c_char_p, "hmx_gdn_chunk_workspace_bytes":
              "hmx_ssd_chunk_workspace_bytes": ctypes.c_size_t,
              "hmx_ssd_chunk_bwd_workspace_bytes": ctypes.c_size_t,
              "hmx_paged_attention_decode_workspace_bytes": ctypes.c_size_t,
+             "hmx_causal_attention_workspace_bytes": ctypes.c_size_t,
              "hmx_paged_causal_attention_workspace_bytes": ctypes.c_size_t}
 
 

@@ -175,10 +175,12 @@ def attention_forward(q, k, v, scale, cu_seqlens, out, want_lse):
     k, kts, khs = _rows(k)
     v, vts, vhs = _rows(v)
     _, ots, ohs = _rows(o)
+    ws, ws_bytes = _workspace("hmx_causal_attention_workspace_bytes", q, N, B * T, H, k.shape[2], D,
+                              int(cu is not None))
     _lib.call("hmx_causal_attention", q.data_ptr(), qts, qhs, k.data_ptr(), kts, khs,
               v.data_ptr(), vts, vhs, _lib.dtype_code(q), o.data_ptr(), ots, ohs,
               _lib.ptr(lse), _lib.ptr(cu), N, B * T, H, k.shape[2], D, scale,
-              int(out is None), _lib.stream_of(q))
+              int(out is None), _lib.ptr(ws), ws_bytes, _lib.stream_of(q))
     return o, lse, cu
 
 

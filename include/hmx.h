@@ -865,14 +865,19 @@ int hmx_paged_attention_decode(const void* q, int64_t q_token_stride, int64_t q_
  * the device offsets cu_seqlens [N + 1] (clamped into 0 .. T), or of T / N tokens each
  * where cu_seqlens is NULL.  lse: NULL, or fp32 [T, H], the base-2 logarithm of
  * sum_j 2^(log2(e) scale q . k_j), as hmx_causal_attention_bwd takes it.  fill_gaps: rows
- * of no sequence become 0 (else they are left as they were).
+ * of no sequence become 0 (else they are left as they were).  workspace: 16-byte aligned,
+ * needed where *_workspace_bytes is not 0 (few rows: their keys are split, packed with
+ * cu_seqlens); its contents before and after do not matter.
  */
+size_t hmx_causal_attention_workspace_bytes(int32_t N, int64_t T, int32_t H, int32_t HKV, int32_t D,
+                                            int32_t packed);
 int hmx_causal_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                          const void* k, int64_t k_token_stride, int64_t k_head_stride,
                          const void* v, int64_t v_token_stride, int64_t v_head_stride,
                          int32_t dtype, void* o, int64_t o_token_stride, int64_t o_head_stride,
                          float* lse, const int32_t* cu_seqlens, int32_t N, int64_t T, int32_t H,
-                         int32_t HKV, int32_t D, float scale, int32_t fill_gaps, void* stream);
+                         int32_t HKV, int32_t D, float scale, int32_t fill_gaps, void* workspace,
+                         size_t workspace_bytes, void* stream);
 
 /*
  * The backward of hmx_causal_attention (bf16): dq [T, H, D], dk, dv [T, HKV, D] from the

@@ -362,3 +362,24 @@ def test_paged_causal_attention_few_rows_long_contexts(dev, news, lens, H, HKV, 
     args[0][table[0, page], at] = float("inf")
     out = hmx.paged_causal_attention(q.to(dev), *args)
     assert out[cu[0]:cu[1]].isnan().all() and out[cu[1]:].isfinite().all()
+
+
+@pytest.mark.parametrize("B,T,cu,H,HKV,D,dtype", [
+    (1, 2048, None, 8, 2, 128, BF), (2, 1500, None, 4, 4, 64, FP), (1, 3001, None, 7, 1, 64, BF),
+    (1, 3000, [4, 1800, 1800, 1803, 2900], 4, 1, 128, FP),
+    (1, 1600, [0] + [1000 + 9 * i for i in range(66)], 2, 2, 64, BF),
+])
+def test_causal_attention_few_rows_many_keys(dev, B, T, cu, H, HKV, D, dtype):
+    """Rows too few for the chip: their keys are split over workgroups and joined."""
+    gen = torch.Generator().manual_seed(T + H)
+    q, k, v = (randn(gen, B, T, n, D, dtype=dtype) for n in (H, HKV, HKV))
+    # values that no row before them may see
+    k[:, -1], v[:, -1] = float("nan"), float("inf")
+    out = hmx.causal_attention(q.to(dev), k.to(dev), v.to(dev),
+                               cu_seqlens=None if cu is None else torch.tensor(cu, device=dev))
+    for b in range(B):
+        bounds = [(0, T)] if cu is None else bounds_of(cu)
+        n = bounds[-1][1] - (bounds[-1][1] == T)          # the last row sees the NaN
+        o, a = ref.causal(q[b], k[b], v[b], D ** -0.5, [(x, min(y, n)) for x, y in bounds])
+        check_o(out[b, :n], o[:n], a[:n], v[b, :n], f"{B} x {T}")
+        assert n == T or cu is not None and cu[-1] < T or out[b, -1].isnan().all()

@@ -116,10 +116,10 @@ def test_c_entry_points_check_before_launching():
     dec(N=0)
     with pytest.raises(ValueError, match="is not N"):
         _lib.call("hmx_causal_attention", None, 0, 0, None, 0, 0, None, 0, 0, 1, None, 0, 0, None, None,
-                  2, 7, 4, 2, 64, 1.0, 1, None)
+                  2, 7, 4, 2, 64, 1.0, 1, None, 0, None)
     with pytest.raises(ValueError, match="null pointer"):
         _lib.call("hmx_causal_attention", None, 0, 0, None, 0, 0, None, 0, 0, 1, None, 0, 0, None, None,
-                  1, 7, 4, 2, 64, 1.0, 1, None)
+                  1, 7, 4, 2, 64, 1.0, 1, None, 0, None)
     with pytest.raises(NotImplementedError, match="bf16 only"):
         _lib.call("hmx_causal_attention_bwd", *([None, 0, 0] * 3), 2, *([None, 0, 0] * 2), None, None, 1, 7,
                   4, 2, 64, 1.0, *([None, 0, 0] * 3), None, None)
@@ -200,3 +200,13 @@ def test_registered_backward_refuses_other_shapes():
             bwd(lse=bad)
     with pytest.raises(RuntimeError, match="GPU"):
         bwd()
+
+
+def test_short_workspaces_are_refused():
+    """Few rows with many keys need a workspace; too small a one launches nothing."""
+    n = _lib.load().hmx_causal_attention_workspace_bytes(1, 2048, 8, 2, 128, 0)
+    assert n > 0 and _lib.load().hmx_causal_attention_workspace_bytes(1, 197, 8, 2, 128, 0) == 0
+    for ws, size in ((None, n), (256, n - 1)):
+        with pytest.raises(ValueError, match="too small"):
+            _lib.call("hmx_causal_attention", 256, 1024, 128, 256, 256, 128, 256, 256, 128, 1, 256, 1024, 128,
+                      None, None, 1, 2048, 8, 2, 128, 1.0, 1, ws, size, None)

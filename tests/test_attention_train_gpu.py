@@ -124,3 +124,15 @@ def test_grads_of_head_major_inputs_and_an_odd_group(dev):
         grads = torch.autograd.grad(hmx.causal_attention(*ins), ins, g)
         (_, *want), mags = ref.causal_grads(q[0], k[0], v[0], D ** -0.5, [(0, T)], do[0])
         _check([x[0] for x in grads], want, mags, f"H={H}")
+
+
+@pytest.mark.parametrize("cu", [None, [0, 700, 700, 2000]])
+def test_grads_where_the_forward_splits_its_keys(dev, cu):
+    T, H, HKV, D = 2000, 2, 1, 64
+    q, k, v, do = _inputs(3, 1, T, H, HKV, D)
+    ins = [x.to(dev).requires_grad_() for x in (q, k, v)]
+    o = hmx.causal_attention(*ins, cu_seqlens=None if cu is None else torch.tensor(cu, device=dev))
+    grads = torch.autograd.grad(o, ins, do.to(dev))
+    bounds = [(0, T)] if cu is None else bounds_of(cu)
+    (_, *want), mags = ref.causal_grads(q[0], k[0], v[0], D ** -0.5, bounds, do[0])
+    _check([g[0] for g in grads], want, mags, str(cu))
