@@ -611,11 +611,14 @@ using namespace hmx;
 
 #define ATTN_COMMON_CHECKS(what)                                                                    HMX_REQUIRE(D == 64 || D == 128, HMX_EUNSUPPORTED, what ": head size %d not in {64, 128}", D);    HMX_REQUIRE(dtype == HMX_BF16 || dtype == HMX_F16, HMX_EUNSUPPORTED,                                          what ": dtype code %d (bf16 or fp16)", dtype);                                        HMX_REQUIRE(N >= 0 && T >= 0 && HKV > 0 && H > 0 && H % HKV == 0, HMX_EINVAL,                                 what ": N=%d T=%lld H=%d HKV=%d", N, (long long)T, H, HKV);                           HMX_REQUIRE(T * (H / HKV) < (1ll << 30), HMX_EUNSUPPORTED, what ": %lld tokens", (long long)T);   HMX_REQUIRE(scale > 0.f && scale < __builtin_inff(), HMX_EINVAL, what ": scale %g must be positive", (double)scale);
 
+// Packed lengths are on the device: the longest sequence is taken to be at most four times
+// their mean (many short prompts are not split, nor sent through a workspace for it), and
+// more sequences than next_tile can weigh are not split.
 static attn::Splits prompt_splits(int64_t N, int64_t T, int H, int HKV, bool packed) {
-  if (N <= 0 || T <= 0) return attn::NO_SPLITS;
+  if (N <= 0 || T <= 0 || (packed && N > attn::LANE_SEQS)) return attn::NO_SPLITS;
   const int32_t some = 0;
   const int64_t slots = attn::tile_slots<attn::BM>(packed ? &some : nullptr, N, T, H / HKV);
-  return attn::splits(packed ? slots - 2 : slots, HKV, packed ? T : T / N, 8);
+  return attn::splits(packed ? slots - 2 : slots, HKV, packed && N <= 4 ? T : packed ? 4 * T / N : T / N, 8);
 }
 
 extern "C" size_t hmx_causal_attention_workspace_bytes(int32_t N, int64_t T, int32_t H, int32_t HKV,

@@ -866,8 +866,8 @@ int hmx_paged_attention_decode(const void* q, int64_t q_token_stride, int64_t q_
  * where cu_seqlens is NULL.  lse: NULL, or fp32 [T, H], the base-2 logarithm of
  * sum_j 2^(log2(e) scale q . k_j), as hmx_causal_attention_bwd takes it.  fill_gaps: rows
  * of no sequence become 0 (else they are left as they were).  workspace: 16-byte aligned,
- * needed where *_workspace_bytes is not 0 (few rows: their keys are split, packed with
- * cu_seqlens); its contents before and after do not matter.
+ * needed where *_workspace_bytes is not 0 (few rows with many keys); its contents before and
+ * after do not matter.  packed: whether cu_seqlens is given.
  */
 size_t hmx_causal_attention_workspace_bytes(int32_t N, int64_t T, int32_t H, int32_t HKV, int32_t D,
                                             int32_t packed);
