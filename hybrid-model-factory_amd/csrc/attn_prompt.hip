@@ -223,6 +223,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
   const char* kbase = (PAGED ? a.pages.k : a.k + (int64_t)t.bos * a.k_ts) + (int64_t)kvh * (PAGED ? a.pages.k_hs : a.k_hs);
   const char* vbase = (PAGED ? a.pages.v : a.v + (int64_t)t.bos * a.v_ts) + (int64_t)kvh * (PAGED ? a.pages.v_hs : a.v_hs);
   const bool whole = !PAGED || a.pages.page.d % 16 == 0;   // the wave's 16 rows lie in one page
+  // s_skip[j & 3] = j + 1: some page of key tile j lies outside the cache.  Only the staging of
+  // the tile's keys says so, in the step before the tile's own; while a step's waves read the
+  // flags of tiles j and j - 1 (mend has a barrier behind them), stage(j + 1) writes tile
+  // j + 1's alone.  Values need none: those that a product takes are of tiles whose keys were
+  // staged.
   auto stage_rows = [&](int j, int r0, bool value) __attribute__((always_inline)) {
     const uint32_t lds = lds_addr(smem) + (value ? 2 * TILE : 0) + ((j - j_beg) & 1) * TILE + wave * 16 * D * 2;
     const char* base = value ? vbase : kbase;
@@ -236,7 +241,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
       const int r = max(min(r0, (keys - 1) & ~15), 0), p = fdiv(r, a.pages.page);
       int id = uniform_load(a.pages.table, t.seq * a.pages.table_stride + __builtin_amdgcn_readfirstlane(p));
       if ((unsigned)id >= (unsigned)a.pages.num_pages) {
-        if (r0 >= 0 && r0 < keys) s_skip[(r0 / BN) & 3] = r0 / BN + 1;
+        if (!value && r0 < keys) s_skip[j & 3] = j + 1;
         id = 0;
       }
       const char* b = uniform_ptr(base + id * (value ? a.pages.v_ps : a.pages.k_ps) + (r - p * a.pages.page.d) * ts);
@@ -251,7 +256,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
           const int p = fdiv(r, a.pages.page);
           int id = a.pages.table[t.seq * a.pages.table_stride + p];
           if ((unsigned)id >= (unsigned)a.pages.num_pages) {
-            if (q >= 0 && q < keys) s_skip[(q / BN) & 3] = q / BN + 1;
+            if (!value && q < keys) s_skip[j & 3] = j + 1;
             id = 0;
           }
           b += id * (value ? a.pages.v_ps : a.pages.k_ps) + (r - p * a.pages.page.d) * ts;
