@@ -75,6 +75,15 @@ def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
     return t, ts if B * T > 1 else 0, t.stride(-2) if t.shape[-2] > 1 else 0
 
 
+def _places(t: torch.Tensor) -> tuple[int, int]:
+    """(token stride, head stride) of an output that _out has looked through: its own, at any
+    distance, for it is written in place and a copy may never stand for it."""
+    B = t.shape[0] if t.dim() == 4 else 1
+    T = t.shape[-3]
+    ts = t.stride(-3) if T > 1 else t.stride(0) if B > 1 else 0
+    return ts, t.stride(-2) if t.shape[-2] > 1 else 0
+
+
 def _out(out: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
     if out is None:
         return torch.empty(like.shape, dtype=like.dtype, device=like.device)
@@ -174,7 +183,7 @@ def attention_forward(q, k, v, scale, cu_seqlens, out, want_lse):
     q, qts, qhs = _rows(q)
     k, kts, khs = _rows(k)
     v, vts, vhs = _rows(v)
-    _, ots, ohs = _rows(o)
+    ots, ohs = _places(o)
     ws, ws_bytes = _workspace("hmx_causal_attention_workspace_bytes", q, N, B * T, H, k.shape[2], D,
                               int(cu is not None))
     _lib.call("hmx_causal_attention", q.data_ptr(), qts, qhs, k.data_ptr(), kts, khs,
@@ -263,7 +272,7 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     qts = qhs = ots = ohs = 0
     if q is not None:
         q, qts, qhs = _rows(q)
-        _, ots, ohs = _rows(ret)
+        ots, ohs = _places(ret)
     slot_mapping = slot_mapping.contiguous()
     cs = (None, 0, None, 0, 0, 0)
     if cos_sin is not None:
@@ -306,7 +315,7 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         with torch.cuda.device(q.device):
             return paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, scale, out=o)
     q, qts, qhs = _rows(q)
-    _, ots, ohs = _rows(o)
+    ots, ohs = _places(o)
     ws, ws_bytes = _workspace("hmx_paged_attention_decode_workspace_bytes", q, N, H, HKV, D,
                               block_table.shape[1] * k_cache.shape[1])
     _lib.call("hmx_paged_attention_decode", q.data_ptr(), qts, qhs, _lib.dtype_code(q),
@@ -350,7 +359,7 @@ def paged_causal_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     if T == 0:
         return o
     q, qts, qhs = _rows(q)
-    _, ots, ohs = _rows(o)
+    ots, ohs = _places(o)
     ws, ws_bytes = _workspace("hmx_paged_causal_attention_workspace_bytes", q, N, T, H, HKV, D,
                               block_table.shape[1] * k_cache.shape[1])
     _lib.call("hmx_paged_causal_attention", q.data_ptr(), qts, qhs, _lib.dtype_code(q),

@@ -36,3 +36,29 @@ def test_missing_pages_beside_every_cut_of_the_keys(dev, page, at, H, HKV, D):
         k, v = ks[n][keep[n]], vs[n][keep[n]]
         o, a = ref.rows(q[b:e], k, v, D ** -0.5, len(k) - (e - b))
         check_o(out[b:e], o, a, v, f"sequence {n}")
+
+
+def test_outputs_with_rows_far_apart(dev):
+    """Token strides of 2^25 elements and more, in every op that takes an output."""
+    gen = torch.Generator().manual_seed(6)
+    H, HKV, D, far = 4, 2, 64, 1 << 25
+    kc, vc = (randn(gen, 40, 16, HKV, D).to(dev) for _ in range(2))
+    table = torch.randperm(40, generator=gen).to(torch.int32).view(4, 10).to(dev)
+    lens = torch.tensor([100, 7, 33, 160], dtype=torch.int32, device=dev)
+    cu = torch.tensor([0, 1, 2, 3, 4], dtype=torch.int32, device=dev)
+    q, k, v = (randn(gen, 4, n, D).to(dev) for n in (H, HKV, HKV))
+    cs = torch.randn(9, 32, generator=gen).to(dev)
+    pos = torch.tensor([0, 8, 3, 1], device=dev)
+    slots = torch.full((4,), -1, device=dev)
+    room = torch.full((3 * far + H * D,), 7.0, dtype=BF, device=dev)
+    out = room.as_strided((4, H, D), (far, D, 1))
+    for run in (lambda **kw: hmx.paged_attention_decode(q, kc, vc, table, lens, **kw),
+                lambda **kw: hmx.paged_causal_attention(q, kc, vc, table, lens, cu, **kw),
+                lambda **kw: hmx.causal_attention(q[None], k[None], v[None], **{n: x[None] for n, x in kw.items()}),
+                lambda **kw: hmx.append_paged_kv(k, v, kc, vc, slots, q=q, positions=pos, cos_sin=cs,
+                                                 **{"q_" + n: x for n, x in kw.items()})):
+        room.fill_(7.0)
+        want = run()
+        got = run(out=out)
+        assert got.data_ptr() == room.data_ptr() and torch.equal(got.view(4, H, D), want.view(4, H, D))
+        assert (room[H * D:H * D + 4 * H * D] == 7).all() and int((room != 7).sum()) <= 4 * H * D

@@ -210,3 +210,17 @@ def test_short_workspaces_are_refused():
         with pytest.raises(ValueError, match="too small"):
             _lib.call("hmx_causal_attention", 256, 1024, 128, 256, 256, 128, 256, 256, 128, 1, 256, 1024, 128,
                       None, None, 1, 2048, 8, 2, 128, 1.0, 1, ws, size, None)
+
+
+def test_outputs_are_written_at_their_own_strides():
+    """Whatever out is accepted, its rows are addressed where they lie, far apart too; strides
+    of dimensions of one, which may be anything, go as 0."""
+    from hmx.ops.attention import _out, _places
+    far = 1 << 25
+    for shape, stride, want in (((1, 3, 2, 64), (1, far, 64, 1), (far, 64)), ((3, 2, 64), (far + 8, 64, 1), (far + 8, 64)),
+                                ((2, 3, 2, 64), (3 * far, far, 128, 1), (far, 128)), ((2, 1, 2, 64), (far, 5, 64, 1), (far, 64)),
+                                ((4, 2, 64), (64, 256, 1), (64, 256)), ((1, 1, 1, 64), (3, 5, 7, 1), (0, 0)),
+                                ((2, 3, 1, 64), (192, 64, 7, 1), (64, 0)), ((1, 4, 64), (9, 64, 1), (0, 64))):
+        out = torch.empty_strided(shape, stride, dtype=BF, device="meta")
+        assert _out(out, torch.empty(shape, dtype=BF, device="meta")) is out
+        assert _places(out) == want
