@@ -115,9 +115,10 @@ def _scale(scale: float | None, D: int) -> float:
     return scale
 
 
-def _offsets(cu_seqlens: torch.Tensor, T: int, device: torch.device) -> torch.Tensor:
-    """cu_seqlens as int32 on the device.  Host offsets are checked here; offsets on the
-    device are never read back (the kernels clamp them into the tokens)."""
+def _offsets(cu_seqlens: torch.Tensor, T: int, device: torch.device, any_first: bool = False) -> torch.Tensor:
+    """cu_seqlens as int32 on the device.  Host offsets are checked here, and start at 0 unless
+    ``any_first``; offsets on the device are never read back (the kernels clamp them into the
+    tokens)."""
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
         raise ValueError(f"cu_seqlens must be a vector of N + 1 offsets, got {tuple(cu_seqlens.shape)}")
     if cu_seqlens.dtype not in (torch.int32, torch.int64):
@@ -127,7 +128,12 @@ def _offsets(cu_seqlens: torch.Tensor, T: int, device: torch.device) -> torch.Te
             raise ValueError(f"tensors on {device} and {cu_seqlens.device}")
         return cu_seqlens if cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous() \
             else cu_seqlens.to(torch.int32).contiguous()
-    seq_bounds(cu_seqlens, 1, T)
+    if any_first:
+        cs = cu_seqlens.tolist()
+        if cs[0] < 0 or cs[-1] > T or any(b < a for a, b in zip(cs, cs[1:])):
+            raise ValueError(f"cu_seqlens must be non-decreasing from >= 0 to <= {T}: {cs}")
+    else:
+        seq_bounds(cu_seqlens, 1, T)
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("cu_seqlens must be on the device where a graph is captured")
     return cu_seqlens.to(torch.int32).pin_memory().to(device, non_blocking=True)
@@ -139,7 +145,8 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     """softmax(scale q k^T) v of every token over itself and the tokens before it.
 
     q [B, T, H, D], k and v [B, T, HKV, D]; with ``cu_seqlens`` (N + 1 offsets into the
-    tokens, B = 1) each of the N packed sequences by itself.  ``scale`` (default
+    tokens, B = 1; where they are on the host, the first is 0) each of the N packed sequences
+    by itself.  ``scale`` (default
     D ** -0.5) must be positive.  Returns [B, T, H, D] in q's type; rows of no sequence
     are 0, or left as they were in ``out`` (which may not overlap an input).  A value that
     is not finite reaches the rows that attend it and no others.
@@ -355,7 +362,7 @@ def paged_causal_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         with torch.cuda.device(q.device):
             return paged_causal_attention(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens,
                                           scale, out=out)
-    cu = _offsets(cu_seqlens, T, q.device)
+    cu = _offsets(cu_seqlens, T, q.device, any_first=True)
     if T == 0:
         return o
     q, qts, qhs = _rows(q)

@@ -62,3 +62,17 @@ def test_outputs_with_rows_far_apart(dev):
         got = run(out=out)
         assert got.data_ptr() == room.data_ptr() and torch.equal(got.view(4, H, D), want.view(4, H, D))
         assert (room[H * D:H * D + 4 * H * D] == 7).all() and int((room != 7).sum()) <= 4 * H * D
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_paged_host_offsets_of_later_sequences(dev, dtype):
+    """A slice of a batch's offsets, as the host holds them: the same as on the device."""
+    gen = torch.Generator().manual_seed(8)
+    kc, vc = (randn(gen, 40, 16, 2, 64).to(dev) for _ in range(2))
+    table = torch.randperm(40, generator=gen).to(torch.int32).view(4, 10).to(dev)
+    lens = torch.tensor([100, 7, 33, 160], dtype=torch.int32, device=dev)
+    cu = torch.tensor([0, 1, 2, 9, 20], dtype=dtype)
+    q = randn(gen, 23, 4, 64).to(dev)
+    for n in (0, 2, 4):
+        args = (q, kc, vc, table[n:], lens[n:])
+        assert torch.equal(hmx.paged_causal_attention(*args, cu[n:]), hmx.paged_causal_attention(*args, cu[n:].to(dev)))

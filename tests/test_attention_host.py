@@ -224,3 +224,19 @@ def test_outputs_are_written_at_their_own_strides():
         out = torch.empty_strided(shape, stride, dtype=BF, device="meta")
         assert _out(out, torch.empty(shape, dtype=BF, device="meta")) is out
         assert _places(out) == want
+
+
+def test_host_offsets_of_later_sequences(monkeypatch):
+    """The paged form takes a slice of a batch's host offsets, whose first need not be 0."""
+    from hmx.ops import attention
+    seen = []
+    monkeypatch.setattr(torch.Tensor, "pin_memory", lambda t: seen.append(t.tolist()) or t)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    dev = torch.device("cpu")
+    for cs in ([3, 5, 9], [0, 9], [9], [4, 4, 4], [0, 0, 2]):
+        for dt in (torch.int32, torch.int64):
+            got = attention._offsets(torch.tensor(cs, dtype=dt), 9, dev, any_first=True)
+            assert got.dtype == torch.int32 and got.tolist() == cs == seen[-1]
+    for cs in ([-1, 4], [3, 10], [3, 5, 4], [10]):
+        with pytest.raises(ValueError, match="cu_seqlens"):
+            attention._offsets(torch.tensor(cs), 9, dev, any_first=True)
