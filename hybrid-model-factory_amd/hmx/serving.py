@@ -479,7 +479,8 @@ def attention_forward_core(layer, qkv: torch.Tensor, positions: torch.Tensor | N
     n, tp, D = md.num_actual_tokens, layer.tp_size, layer.head_dim
     H, HKV = layer.num_heads // tp, layer.num_kv_heads // tp
     qkv = _cut(qkv, 0, n)
-    q, k, v = (x.view(n, -1, D) for x in qkv.split([H * D, HKV * D, HKV * D], dim=-1))
+    heads = (H, HKV, HKV)
+    q, k, v = (x.view(n, h, D) for h, x in zip(heads, qkv.split([h * D for h in heads], dim=-1)))
     rope = getattr(layer, "rotary_emb", None)
     if rope is not None:
         if positions is None:

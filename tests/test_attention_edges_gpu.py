@@ -1,10 +1,13 @@
 """Calls at the edges of what the attention ops accept, against the float64 definitions.
 
 Tolerances are elementwise and derived in attn_util.o_tolerance."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 
 import hmx
+import hmx.serving as serving
 from attn_util import bounds_of, check_o, paged, randn, ref
 
 pytestmark = pytest.mark.gpu
@@ -76,3 +79,17 @@ def test_paged_host_offsets_of_later_sequences(dev, dtype):
     for n in (0, 2, 4):
         args = (q, kc, vc, table[n:], lens[n:])
         assert torch.equal(hmx.paged_causal_attention(*args, cu[n:]), hmx.paged_causal_attention(*args, cu[n:].to(dev)))
+
+
+@pytest.mark.parametrize("rope", [True, False])
+def test_forward_core_of_no_tokens(dev, rope):
+    lay = SimpleNamespace(num_heads=4, num_kv_heads=2, head_dim=64, tp_size=1, rotary_emb=SimpleNamespace(
+        cos_sin_cache=torch.zeros(9, 64, device=dev), is_neox_style=True) if rope else None)
+    none = torch.zeros(0, dtype=torch.int32, device=dev)
+    md = SimpleNamespace(num_actual_tokens=0, num_decodes=0, num_decode_tokens=0, num_prefills=0, query_start_loc=none,
+                         seq_lens=none, block_table=none.view(0, 3), slot_mapping=none)
+    kc = torch.full((3, 16, 2, 64), 2.0, dtype=BF, device=dev)
+    for tokens in (0, 3):
+        out = torch.full((tokens, 4, 64), 5.0, dtype=BF, device=dev)
+        serving.attention_forward_core(lay, torch.zeros(tokens, 8 * 64, dtype=BF, device=dev), none, out, md, kc, kc.clone())
+        assert (out == 5).all() and (kc == 2).all()

@@ -1,6 +1,7 @@
 """Host-side checks of the attention ops (CPU): refusals before any launch, the C entry
 points' own checks, and the oracle's gradients against differences."""
 import ctypes
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -240,3 +241,22 @@ def test_host_offsets_of_later_sequences(monkeypatch):
     for cs in ([-1, 4], [3, 10], [3, 5, 4], [10]):
         with pytest.raises(ValueError, match="cu_seqlens"):
             attention._offsets(torch.tensor(cs), 9, dev, any_first=True)
+
+
+@pytest.mark.parametrize("rope", [True, False])
+def test_forward_core_of_no_tokens(monkeypatch, rope):
+    """A step of no tokens hands empty tensors to the append and runs no attention."""
+    import hmx.serving as serving
+    seen = []
+    monkeypatch.setattr(serving.ops, "append_paged_kv", lambda k, v, *a, q=None, **kw: seen.append((k, v, q)) or q)
+    lay = SimpleNamespace(num_heads=4, num_kv_heads=2, head_dim=64, tp_size=1,
+                          rotary_emb=SimpleNamespace(cos_sin_cache=torch.zeros(9, 64), is_neox_style=True) if rope else None)
+    none = torch.zeros(0, dtype=torch.int32)
+    md = SimpleNamespace(num_actual_tokens=0, num_decodes=0, num_decode_tokens=0, num_prefills=0, query_start_loc=none,
+                         seq_lens=none, block_table=none.view(0, 3), slot_mapping=none)
+    for tokens in (0, 3):
+        out = torch.full((tokens, 4, 64), 5.0, dtype=BF)
+        serving.attention_forward_core(lay, torch.zeros(tokens, 8 * 64, dtype=BF), none, out, md, *_cache())
+        assert (out == 5).all()
+    assert [tuple(x.shape) for x in seen[0][:2]] == [(0, 2, 64)] * 2 and len(seen) == 2
+    assert not rope or seen[0][2].shape == (0, 4, 64)
