@@ -462,8 +462,8 @@ def attention_forward_core(layer, qkv: torch.Tensor, positions: torch.Tensor | N
     run theirs: the position rotation and the append in one launch, then the batch's decodes
     (first, one token each) and its prefills, each written into ``core_attn_out`` in place.
 
-    ``layer``: num_heads, num_kv_heads, head_dim, tp_size, ``scaling`` (None: head_dim **
-    -0.5) and ``rotary_emb`` (None, or an object with cos_sin_cache [max position, rotary
+    ``layer``: num_heads and num_kv_heads of all ranks (a rank has one key/value head where
+    there are fewer than ranks), head_dim, tp_size, ``scaling`` (None: head_dim ** -0.5) and ``rotary_emb`` (None, or an object with cos_sin_cache [max position, rotary
     dim] and is_neox_style).  ``qkv`` [tokens, (H + 2 HKV) * head_dim] is the fused
     projection's output, with the layer's norms on q and k applied; ``positions`` [tokens];
     ``core_attn_out`` [tokens, H, head_dim]; caches [pages, page size, HKV, head_dim].
@@ -477,9 +477,12 @@ def attention_forward_core(layer, qkv: torch.Tensor, positions: torch.Tensor | N
     if md is None:
         return
     n, tp, D = md.num_actual_tokens, layer.tp_size, layer.head_dim
-    H, HKV = layer.num_heads // tp, layer.num_kv_heads // tp
-    qkv = _cut(qkv, 0, n)
+    H, HKV = layer.num_heads // tp, max(1, layer.num_kv_heads // tp)
     heads = (H, HKV, HKV)
+    if qkv.shape[-1] != sum(heads) * D:
+        raise ValueError(f"qkv rows of {qkv.shape[-1]} are not those of {H} heads and 2 x {HKV} key/value heads of {D} "
+                         f"({layer.num_heads} and {layer.num_kv_heads} over {tp} ranks)")
+    qkv = _cut(qkv, 0, n)
     q, k, v = (x.view(n, h, D) for h, x in zip(heads, qkv.split([h * D for h in heads], dim=-1)))
     rope = getattr(layer, "rotary_emb", None)
     if rope is not None:

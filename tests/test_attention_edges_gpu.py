@@ -93,3 +93,21 @@ def test_forward_core_of_no_tokens(dev, rope):
         out = torch.full((tokens, 4, 64), 5.0, dtype=BF, device=dev)
         serving.attention_forward_core(lay, torch.zeros(tokens, 8 * 64, dtype=BF, device=dev), none, out, md, kc, kc.clone())
         assert (out == 5).all() and (kc == 2).all()
+
+
+def test_forward_core_with_fewer_kv_heads_than_ranks(dev):
+    """Two key/value heads over four ranks: the rank's one head serves its four q heads."""
+    gen = torch.Generator().manual_seed(9)
+    H, D, n, page = 4, 64, 30, 16
+    qkv = randn(gen, n, (H + 2) * D)
+    kc, vc = (torch.zeros(4, page, 1, D, dtype=BF, device=dev) for _ in range(2))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
+    md = SimpleNamespace(num_actual_tokens=n, num_decodes=0, num_decode_tokens=0, num_prefills=1,
+                         query_start_loc=i32([0, n]), seq_lens=i32([n]), block_table=i32([[2, 0]]),
+                         slot_mapping=torch.cat([torch.arange(32, 48), torch.arange(14)]).to(dev))
+    lay = SimpleNamespace(num_heads=16, num_kv_heads=2, head_dim=D, tp_size=4)
+    out = torch.zeros(n, H, D, dtype=BF, device=dev)
+    serving.attention_forward_core(lay, qkv.to(dev), None, out, md, kc, vc)
+    q, k, v = (x.reshape(n, -1, D) for x in qkv.split([H * D, D, D], -1))
+    o, a = ref.rows(q, k, v, D ** -0.5, 0)
+    check_o(out, o, a, v, "one kv head")

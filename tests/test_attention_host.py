@@ -260,3 +260,22 @@ def test_forward_core_of_no_tokens(monkeypatch, rope):
         assert (out == 5).all()
     assert [tuple(x.shape) for x in seen[0][:2]] == [(0, 2, 64)] * 2 and len(seen) == 2
     assert not rope or seen[0][2].shape == (0, 4, 64)
+
+
+def test_forward_core_heads_of_a_rank(monkeypatch):
+    """A rank's heads; a key/value head of its own where there are fewer than ranks; a
+    projection of other sizes is refused by name."""
+    import hmx.serving as serving
+    seen = []
+    monkeypatch.setattr(serving.ops, "append_paged_kv", lambda k, v, *a, **kw: seen.append((k, v)))
+    none = torch.zeros(0, dtype=torch.int32)
+    md = SimpleNamespace(num_actual_tokens=0, num_decodes=0, num_decode_tokens=0, num_prefills=0, query_start_loc=none,
+                         seq_lens=none, block_table=none.view(0, 3), slot_mapping=none)
+    for heads, kv, tp, H, HKV in ((8, 4, 1, 8, 4), (8, 4, 2, 4, 2), (16, 2, 4, 4, 1), (8, 1, 8, 1, 1)):
+        lay = SimpleNamespace(num_heads=heads, num_kv_heads=kv, head_dim=64, tp_size=tp)
+        call = lambda width: serving.attention_forward_core(lay, torch.zeros(3, width, dtype=BF), None,
+                                                            torch.zeros(3, H, 64, dtype=BF), md, *_cache(HKV=HKV))
+        call((H + 2 * HKV) * 64)
+        assert [tuple(x.shape) for x in seen[-1]] == [(0, HKV, 64)] * 2
+        with pytest.raises(ValueError, match="key/value heads"):
+            call((H + 2 * HKV + 1) * 64)
