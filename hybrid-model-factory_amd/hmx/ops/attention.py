@@ -12,12 +12,17 @@ Head sizes 64 and 128, bf16 and fp16.  A cache is a pair of tensors
 both halves of one allocation pass as views); ``block_table`` [N, width] int32 lists the
 pages of every sequence.  Lengths, offsets, tables and slots are read on the device only,
 so a captured graph replays with other lengths.
+
+causal_attention alone has a backward; one through another op's result raises, and what is
+stored into a cache or written to ``out`` has no gradient.  There is no forward-mode
+derivative: inputs with tangents are refused.
 """
 from __future__ import annotations
 
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from .gdn import seq_bounds
@@ -38,6 +43,35 @@ def _same_device(ref: torch.Tensor, *tensors: torch.Tensor | None) -> None:
 def _elsewhere(t: torch.Tensor) -> bool:
     """Whether t's device is not the current one, to which launches go."""
     return t.get_device() != torch._C._cuda_getDevice()
+
+
+class _NoBackward(torch.autograd.Function):
+    """An op's result with its place in the graph, and a backward that says there is none."""
+
+    @staticmethod
+    def forward(ctx, result, what, *inputs):
+        ctx.what = what
+        return result[0]                # in a list: the result itself, not a view of an input
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise NotImplementedError(f"{ctx.what}: no backward is implemented")
+
+
+def _grad_of(*tensors: torch.Tensor | None) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _forward_only(what: str, result: torch.Tensor, out: torch.Tensor | None, *inputs) -> torch.Tensor:
+    """The result of an op without a backward, so that one through it raises; ``out``, where
+    the caller gave one, stands outside any graph."""
+    return _NoBackward.apply([result], what, *inputs) if out is None and _grad_of(*inputs) else result
+
+
+def _refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in tensors):
+        raise NotImplementedError(f"{what}: no forward-mode derivative is implemented")
 
 
 def _check_types(what: str, q: torch.Tensor, *others: torch.Tensor | None) -> None:
@@ -152,7 +186,8 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     is not finite reaches the rows that attend it and no others.
 
     Differentiable in q, k and v for bf16 (hmx.CausalAttention)."""
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    _refuse_tangents("causal_attention", q, k, v)
+    if _grad_of(q, k, v):
         if out is not None:
             raise ValueError("out is not supported where a gradient is needed")
         from .attention_train import CausalAttention
@@ -237,6 +272,7 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     outside the table gives NaN.  Without them k is stored and q returned as they are.
     ``q_out`` (may be q itself) receives the rotated q.  Returns it, or None without q."""
     what = "append_paged_kv"
+    _refuse_tangents(what, q, k, v)
     if k.dim() != 3 or k.shape != v.shape:
         raise ValueError(f"{what}: k and v [T, HKV, D], got {tuple(k.shape)} and {tuple(v.shape)}")
     T, HKV, D = k.shape
@@ -267,13 +303,14 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
             return append_paged_kv(k, v, k_cache, v_cache, slot_mapping, q=q, positions=positions,
                                    cos_sin=cos_sin, interleaved=interleaved, q_out=q_out)
     ret = None
+    ins = (q, k, v)
     if q is not None:
         if cos_sin is None and q_out is None:
             ret, q = q, None                    # nothing to do for q
         else:
             ret = _out(q_out, q)
     if T == 0:
-        return ret
+        return ret if q is None else _forward_only(what, ret, q_out, *ins)
     k, kts, khs = _rows(k)
     v, vts, vhs = _rows(v)
     qts = qhs = ots = ohs = 0
@@ -291,7 +328,7 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
               ots, ohs, _lib.paged_kv(k_cache, v_cache), slot_mapping.data_ptr(),
               int(slot_mapping.dtype == torch.int64), *cs, R, int(bool(interleaved)), T, H, HKV,
               D, _lib.stream_of(k))
-    return ret
+    return ret if q is None else _forward_only(what, ret, q_out, *ins)
 
 
 def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -305,6 +342,7 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     the cache holds no keys.  Returns [N, H, D] in q's type (``out``, which may not overlap
     an input)."""
     what = "paged_attention_decode"
+    _refuse_tangents(what, q, k_cache, v_cache)
     if q.dim() != 3:
         raise ValueError(f"{what}: q [N, H, D], got {tuple(q.shape)}")
     N, H, D = q.shape
@@ -316,11 +354,12 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     scale = _scale(scale, D)
     o = _out(out, q)
     _same_device(q, k_cache, v_cache, block_table, seq_lens, o)
+    ins = (q, k_cache, v_cache)
     if N == 0:
-        return o
+        return _forward_only(what, o, out, *ins)
     if _elsewhere(q):
         with torch.cuda.device(q.device):
-            return paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, scale, out=o)
+            return paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, scale, out=out)
     q, qts, qhs = _rows(q)
     ots, ohs = _places(o)
     ws, ws_bytes = _workspace("hmx_paged_attention_decode_workspace_bytes", q, N, H, HKV, D,
@@ -328,7 +367,7 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     _lib.call("hmx_paged_attention_decode", q.data_ptr(), qts, qhs, _lib.dtype_code(q),
               o.data_ptr(), ots, ohs, _lib.paged_kv(k_cache, v_cache, block_table, seq_lens),
               N, H, HKV, D, scale, _lib.ptr(ws), ws_bytes, _lib.stream_of(q))
-    return o
+    return _forward_only(what, o, out, *ins)
 
 
 def paged_causal_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -346,6 +385,7 @@ def paged_causal_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     [T, H, D] in q's type; rows of no sequence are 0, or left as they were in ``out`` (which
     may not overlap an input)."""
     what = "paged_causal_attention"
+    _refuse_tangents(what, q, k_cache, v_cache)
     if q.dim() != 3:
         raise ValueError(f"{what}: q [T, H, D], got {tuple(q.shape)}")
     T, H, D = q.shape
@@ -363,8 +403,9 @@ def paged_causal_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
             return paged_causal_attention(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens,
                                           scale, out=out)
     cu = _offsets(cu_seqlens, T, q.device, any_first=True)
+    ins = (q, k_cache, v_cache)
     if T == 0:
-        return o
+        return _forward_only(what, o, out, *ins)
     q, qts, qhs = _rows(q)
     ots, ohs = _places(o)
     ws, ws_bytes = _workspace("hmx_paged_causal_attention_workspace_bytes", q, N, T, H, HKV, D,
@@ -373,4 +414,4 @@ def paged_causal_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
               o.data_ptr(), ots, ohs, _lib.paged_kv(k_cache, v_cache, block_table, seq_lens),
               _lib.ptr(cu), N, T, H, HKV, D, scale, int(out is None), _lib.ptr(ws), ws_bytes,
               _lib.stream_of(q))
-    return o
+    return _forward_only(what, o, out, *ins)

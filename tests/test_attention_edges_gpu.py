@@ -111,3 +111,30 @@ def test_forward_core_with_fewer_kv_heads_than_ranks(dev):
     q, k, v = (x.reshape(n, -1, D) for x in qkv.split([H * D, D, D], -1))
     o, a = ref.rows(q, k, v, D ** -0.5, 0)
     check_o(out, o, a, v, "one kv head")
+
+
+def test_a_backward_through_the_cache_ops_raises(dev):
+    """A backward that would lose gradients in silence raises instead; the values are those
+    of a call that needs none."""
+    gen = torch.Generator().manual_seed(10)
+    kc, vc = (randn(gen, 20, 16, 2, 64).to(dev) for _ in range(2))
+    table = torch.arange(20, dtype=torch.int32, device=dev).view(2, 10)
+    lens = torch.tensor([100, 33], dtype=torch.int32, device=dev)
+    q, k, v = (randn(gen, 2, n, 64).to(dev) for n in (4, 2, 2))
+    kw = dict(positions=torch.tensor([3, 1], device=dev), cos_sin=torch.randn(9, 32, generator=gen).to(dev))
+    slots, cu = torch.full((2,), -1, device=dev), torch.tensor([0, 1, 2])
+    for run in (lambda q, k: hmx.paged_attention_decode(q, kc, vc, table, lens),
+                lambda q, k: hmx.paged_causal_attention(q, kc, vc, table, lens, cu),
+                lambda q, k: hmx.append_paged_kv(k, v, kc, vc, slots, q=q, **kw)):
+        want = run(q, k)
+        assert not want.requires_grad
+        got = run(q.clone().requires_grad_(), k.clone().requires_grad_())
+        assert torch.equal(got, want)
+        with pytest.raises(NotImplementedError, match="no backward"):
+            got.float().sum().backward()
+        with torch.no_grad():
+            assert not run(q.clone().requires_grad_(), k).requires_grad
+    x = q.clone().requires_grad_()               # without a rotation q passes through, gradient and all
+    assert hmx.append_paged_kv(k, v, kc, vc, slots, q=x) is x
+    out = torch.empty_like(q)
+    assert hmx.paged_attention_decode(x, kc, vc, table, lens, out=out) is out and not out.requires_grad

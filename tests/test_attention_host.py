@@ -279,3 +279,35 @@ def test_forward_core_heads_of_a_rank(monkeypatch):
         assert [tuple(x.shape) for x in seen[-1]] == [(0, HKV, 64)] * 2
         with pytest.raises(ValueError, match="key/value heads"):
             call((H + 2 * HKV + 1) * 64)
+
+
+def test_results_without_a_backward_say_so():
+    """A result that no backward reaches keeps its place in the graph, and raises there; it is
+    the op's own tensor otherwise, and may be changed in place."""
+    from hmx.ops.attention import _forward_only
+    x, y, o = torch.ones(3, requires_grad=True), torch.ones(3), torch.ones(3)
+    assert _forward_only("op", o, None, y, None) is o and _forward_only("op", o, o, x, y) is o
+    with torch.no_grad():
+        assert _forward_only("op", o, None, x) is o
+    got = _forward_only("op", o, None, y, None, x)
+    assert got.requires_grad and got.data_ptr() == o.data_ptr()
+    got.mul_(2)
+    with pytest.raises(NotImplementedError, match="op: no backward"):
+        got.sum().backward()
+
+
+def test_tangents_are_refused():
+    import torch.autograd.forward_ad as fwd
+    (q, k, v), (kc, vc) = _qkv(T=2), _cache()
+    table, lens = torch.zeros(2, 3, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))
+        for run in (lambda: hmx.causal_attention(dual(q), k, v), lambda: hmx.causal_attention(q, k, dual(v)),
+                    lambda: hmx.append_paged_kv(dual(k[0]), v[0], kc, vc, lens),
+                    lambda: hmx.append_paged_kv(k[0], v[0], kc, vc, lens, q=dual(q[0])),
+                    lambda: hmx.paged_attention_decode(dual(q[0]), kc, vc, table, lens),
+                    lambda: hmx.paged_causal_attention(q[0], kc, dual(vc), table, lens, torch.tensor([0, 1, 2]))):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                run()
+        with pytest.raises(RuntimeError, match="GPU"):
+            hmx.causal_attention(q, k, v)
