@@ -239,7 +239,12 @@ def load(path: str | os.PathLike | None = None):
             f"libhmx.so not found at {p}; build it with `python hybrid-model-factory_amd/hmx/build.py`")
     lib = ctypes.CDLL(str(p))
     for name, argtypes in SIGNATURES.items():
-        fn = getattr(lib, name)
+        try:
+            fn = getattr(lib, name)
+        except AttributeError:
+            raise HmxLibraryMissing(
+                f"{p} is older than this package (it has no {name}); build it again with "
+                f"`python hybrid-model-factory_amd/hmx/build.py`") from None
         fn.argtypes = argtypes
         fn.restype = _RESTYPES.get(name, ctypes.c_int)
     if path is None:

@@ -311,3 +311,15 @@ def test_tangents_are_refused():
                 run()
         with pytest.raises(RuntimeError, match="GPU"):
             hmx.causal_attention(q, k, v)
+
+
+def test_an_older_library_is_refused_by_name(tmp_path):
+    """A library without an entry point of the binding names it and how to build."""
+    import subprocess
+    src, lib = tmp_path / "old.c", tmp_path / "old.so"
+    kept = [n for n in _lib.SIGNATURES if "attention" not in n and "paged" not in n]
+    src.write_text("".join(f"int {n}(void) {{ return 13; }}\n" for n in kept))
+    subprocess.run(["gcc", "-shared", "-fPIC", "-o", str(lib), str(src)], check=True)
+    with pytest.raises(_lib.HmxLibraryMissing, match="no hmx_append_paged_kv.*build"):
+        _lib.load(lib)
+    assert _lib.load() is _lib.load()
