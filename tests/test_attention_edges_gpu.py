@@ -138,3 +138,82 @@ def test_a_backward_through_the_cache_ops_raises(dev):
     assert hmx.append_paged_kv(k, v, kc, vc, slots, q=x) is x
     out = torch.empty_like(q)
     assert hmx.paged_attention_decode(x, kc, vc, table, lens, out=out) is out and not out.requires_grad
+
+
+def _like(out, o, a, what):
+    """out finite where the definition o is, and within the rounding of its terms there; NaN
+    and the infinities where o has them."""
+    out = out.double().cpu()
+    fine = torch.isfinite(o)
+    assert torch.equal(torch.isfinite(out), fine), what
+    assert torch.equal(out.nan_to_num(0, 1, -1)[~fine], o.nan_to_num(0, 1, -1)[~fine]), what
+    # o_tolerance's terms at bf16's half step, |o| <= a, and 2^-25 of fewer than 2^9 values' sum in fp16
+    assert ((out - o).abs()[fine] <= (2.0 ** -7 + 2.0 ** -11) * a[fine] + 2.0 ** -16).all(), what
+
+
+@pytest.mark.parametrize("T,cu,H,HKV,D,dtype", [
+    (600, None, 4, 2, 128, BF), (600, None, 3, 3, 64, BF), (500, [0, 90, 90, 333, 480], 8, 1, 128, BF),
+    (2048, None, 2, 1, 128, BF), (2100, [3, 1000, 2100], 4, 4, 64, BF), (400, None, 5, 1, 128, FP),
+])
+def test_values_that_are_not_finite_at_every_distance(dev, T, cu, H, HKV, D, dtype):
+    """Infinities of both signs and NaN among the values, in different columns and in one: rows
+    that attend them have exactly them, the others none; keys split and whole, packed and not."""
+    gen = torch.Generator().manual_seed(T + D)
+    q, k, v = (randn(gen, 1, T, n, D, dtype=dtype) for n in (H, HKV, HKV))
+    for at, col, bad in ((7, 1, "nan"), (40, 2, "inf"), (61, 3, "-inf"), (130, 2, "-inf"), (131, 5, "inf"),
+                         (200, 6, "nan"), (T // 2, 9, "inf"), (T - 70, 11, "nan"), (T - 2, 12, "-inf"), (T - 1, 13, "inf")):
+        v[0, at, at % HKV, col] = float(bad)
+    out = hmx.causal_attention(q.to(dev), k.to(dev), v.to(dev),
+                               cu_seqlens=None if cu is None else torch.tensor(cu, device=dev, dtype=torch.int32))
+    o, a = ref.causal(q[0], k[0], v[0], D ** -0.5, [(0, T)] if cu is None else bounds_of(cu))
+    _like(out[0], o, a, f"T={T}")
+
+
+@pytest.mark.parametrize("news,lens,page", [([70, 1, 130], [300, 90, 130], 16), ([3, 2], [5000, 900], 16), ([40], [777], 7)])
+def test_cached_values_that_are_not_finite(dev, news, lens, page):
+    """The same over pages, where some lie outside the cache and all that is no key is NaN."""
+    gen = torch.Generator().manual_seed(sum(lens))
+    H, HKV, D = 4, 2, 64
+    kc, vc, table, ks, vs = paged(gen, lens, page, HKV, D, BF)
+    keep = []
+    for n, L in enumerate(lens):
+        for back, col, bad in ((0, 1, "inf"), (1, 2, "nan"), (20, 3, "-inf"), (64, 4, "inf"), (80, 4, "-inf")):
+            j = L - 1 - back
+            if j >= 0:
+                vc[table[n, j // page].long(), j % page, 1, col] = vs[n][j, 1, col] = float(bad)
+        key = torch.arange(L)
+        hole = key // page == (L - max(news[n], 30) - 1) // page if L > 200 else key < 0
+        table[n, key[hole] // page] = -1
+        keep.append(~hole)
+    cu = [0]
+    for m in news:
+        cu.append(cu[-1] + m)
+    q = randn(gen, cu[-1], H, D)
+    out = hmx.paged_causal_attention(q.to(dev), kc.to(dev), vc.to(dev), table.to(dev),
+                                     torch.tensor(lens, dtype=torch.int32, device=dev), torch.tensor(cu))
+    for n, (b, e) in enumerate(bounds_of(cu)):
+        # row i sees the keys up to its own that there are
+        for i in range(e - b):
+            seen = keep[n] & (torch.arange(lens[n]) <= lens[n] - (e - b) + i)
+            K, V = ks[n][seen], vs[n][seen]
+            o, a = ref.rows(q[b + i:b + i + 1], K, V, D ** -0.5, len(K) - 1)
+            _like(out[b + i:b + i + 1], o, a, f"sequence {n} row {i}")
+
+
+def test_values_that_are_not_finite_do_not_stall_a_call(dev):
+    """NaN in all values (a step that has diverged) costs a few times the call, not hundreds."""
+    q, k, v = (torch.randn(1, 2048, n, 128, device=dev).bfloat16() for n in (32, 8, 8))
+
+    def fastest(v):
+        best = float("inf")
+        for _ in range(6):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            hmx.causal_attention(q, k, v)
+            b.record()
+            b.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    fine = fastest(v)
+    assert fastest(torch.full_like(v, float("nan"))) < 30 * fine
