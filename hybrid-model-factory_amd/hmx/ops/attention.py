@@ -102,7 +102,7 @@ def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
     B = t.shape[0] if t.dim() == 4 else 1
     T = t.shape[-3]
     if not _aligned(t) or (B > 1 and T > 1 and t.stride(0) != T * t.stride(1)) \
-            or (T > 1 and t.stride(-3) >= 1 << 25):
+            or (B * T > 1 and t.stride(-3 if T > 1 else 0) >= 1 << 25):
         t = t.contiguous()
     ts = t.stride(-3) if T > 1 or B == 1 else t.stride(0)
     # strides of dimensions of one are never used, and may be anything

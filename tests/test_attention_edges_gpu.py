@@ -217,3 +217,15 @@ def test_values_that_are_not_finite_do_not_stall_a_call(dev):
 
     fine = fastest(v)
     assert fastest(torch.full_like(v, float("nan"))) < 30 * fine
+
+
+def test_a_batch_of_single_tokens_far_apart(dev):
+    B, H, HKV, D, far = 3, 4, 2, 64, 1 << 25
+    gen = torch.Generator().manual_seed(12)
+    q, k, v = (randn(gen, B, 1, n, D).to(dev) for n in (H, HKV, HKV))
+    room = torch.zeros(2 * far + H * D, dtype=BF, device=dev)
+    for x in (k, v):
+        y = room.as_strided(x.shape, (far, 8, D, 1))
+        y.copy_(x)
+        got = hmx.causal_attention(q, y if x is k else k, y if x is v else v)
+        assert torch.equal(got, hmx.causal_attention(q, k, v))

@@ -323,3 +323,16 @@ def test_an_older_library_is_refused_by_name(tmp_path):
     with pytest.raises(_lib.HmxLibraryMissing, match="no hmx_append_paged_kv.*build"):
         _lib.load(lib)
     assert _lib.load() is _lib.load()
+
+
+def test_inputs_far_apart_are_copied():
+    """Rows 2^25 elements or more apart, which the kernels' offsets do not span, are copied,
+    a batch's single tokens like a sequence's."""
+    from hmx.ops.attention import _rows
+    far = 1 << 25
+    for shape, stride in (((1, 3, 2, 64), (1, far, 64, 1)), ((2, 1, 2, 64), (far, 8, 64, 1)), ((3, 2, 64), (far, 64, 1))):
+        t = torch.empty_strided(shape, stride, dtype=BF, device="meta")
+        got, ts, hs = _rows(t)
+        assert got is not t and got.is_contiguous() and (ts, hs) == (128, 64)
+    near = torch.empty_strided((2, 1, 2, 64), (far - 8, 8, 64, 1), dtype=BF, device="meta")
+    assert _rows(near) == (near, far - 8, 64)
