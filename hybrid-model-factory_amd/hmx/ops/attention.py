@@ -270,6 +270,7 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     ``positions`` [T] the first R elements of every q and k head turn by their position's
     angles, in pairs (i, i + R / 2), or (2i, 2i + 1) with ``interleaved``; a position
     outside the table gives NaN.  Without them k is stored and q returned as they are.
+    Rows of the caches may not share memory with one another.
     ``q_out`` (may be q itself) receives the rotated q.  Returns it, or None without q."""
     what = "append_paged_kv"
     _refuse_tangents(what, q, k, v)
@@ -278,6 +279,9 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     T, HKV, D = k.shape
     _check_types(what, k, v, q)
     _cache(what, k, k_cache, v_cache, HKV)
+    if any(0 in c.stride() and any(s == 0 and m > 1 for s, m in zip(c.stride(), c.shape))
+           for c in (k_cache, v_cache)):
+        raise ValueError(f"{what}: caches must have a place of their own for every row")
     if (cos_sin is None) != (positions is None):
         raise ValueError(f"{what}: cos_sin and positions go together")
     for name, t in (("slot_mapping", slot_mapping), ("positions", positions)):

@@ -336,3 +336,20 @@ def test_inputs_far_apart_are_copied():
         assert got is not t and got.is_contiguous() and (ts, hs) == (128, 64)
     near = torch.empty_strided((2, 1, 2, 64), (far - 8, 8, 64, 1), dtype=BF, device="meta")
     assert _rows(near) == (near, far - 8, 64)
+
+
+def test_appending_to_rows_on_one_place_is_refused():
+    """Caches whose pages, tokens or heads share memory may be read, not written; strides of
+    dimensions of one do not matter."""
+    k, slots = torch.zeros(5, 2, 64, dtype=BF), torch.arange(5)
+    kc, vc = _cache()
+    one = lambda *shape: torch.zeros(*shape, dtype=BF).expand(3, 16, 2, 64)
+    for bad in (one(1, 16, 2, 64), one(3, 1, 2, 64), one(3, 16, 1, 64)):
+        for caches in ((bad, vc), (kc, bad)):
+            with pytest.raises(ValueError, match="place of their own"):
+                hmx.append_paged_kv(k, k, *caches, slots)
+        with pytest.raises(RuntimeError, match="GPU"):
+            hmx.paged_attention_decode(k, bad, bad, torch.zeros(5, 3, dtype=torch.int32), torch.ones(5, dtype=torch.int32))
+    page = torch.empty_strided((1, 16, 2, 64), (0, 128, 64, 1), dtype=BF)
+    with pytest.raises(RuntimeError, match="GPU"):
+        hmx.append_paged_kv(k, k, page, page.clone(), slots)
