@@ -35,7 +35,7 @@ struct BwdArgs {
   Seqs seqs;           // rows of tokens x G
   FastDiv G;
   int32_t H, HKV, slots;
-  int32_t fixed;       // a tile's rows lie at fixed 32-bit offsets from its first token
+  int32_t fixed;       // a tile's rows lie at fixed 32-bit offsets (unsigned) from its first token
   float c, scale;
 };
 
@@ -485,7 +485,7 @@ extern "C" int hmx_causal_attention_bwd(
   a.c = scale * attn::LOG2E;
   a.scale = scale;
   const int64_t G = H / HKV, span = attn::KR / G;
-  a.fixed = attn::KR % G == 0 && span * a.q_ts + G * a.q_hs < (1ll << 31) &&
+  a.fixed = attn::KR % G == 0 && a.q_ts >= 0 && a.q_hs >= 0 && a.do_ts >= 0 && a.do_hs >= 0 && span * a.q_ts + G * a.q_hs < (1ll << 31) &&
             span * a.do_ts + G * a.do_hs < (1ll << 31);
   const int64_t qs = attn::tile_slots<attn::QM>(cu_seqlens, N, T, H / HKV);
   const int64_t ks = attn::tile_slots<attn::KM>(cu_seqlens, N, T, 1);

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 import hmx
+from hmx import _lib
 import hmx.serving as serving
 from attn_util import bounds_of, check_o, paged, randn, ref
 
@@ -229,3 +230,25 @@ def test_a_batch_of_single_tokens_far_apart(dev):
         y.copy_(x)
         got = hmx.causal_attention(q, y if x is k else k, y if x is v else v)
         assert torch.equal(got, hmx.causal_attention(q, k, v))
+
+
+def test_c_calls_with_strides_that_go_back(dev):
+    """Heads in reverse order by a negative stride, in q and the output's gradient, through the
+    C entry points: what the reversed tensors give."""
+    gen = torch.Generator().manual_seed(13)
+    T, H, HKV, D = 150, 4, 2, 64
+    q, k, v, do = (randn(gen, 1, T, n, D).to(dev) for n in (H, HKV, HKV, H))
+    back = lambda x: (x.data_ptr() + (H - 1) * D * 2, H * D, -D)
+    fore = lambda x: (x.data_ptr(), x.shape[2] * D, D)
+    o, dq, dk, dv = (torch.empty_like(x) for x in (q, q, k, v))
+    lse, delta = (torch.empty(T, H, device=dev) for _ in range(2))
+    s = _lib.stream_of(q)
+    _lib.call("hmx_causal_attention", *back(q), *fore(k), *fore(v), _lib.HMX_BF16, *fore(o), lse.data_ptr(), None,
+              1, T, H, HKV, D, D ** -0.5, 1, None, 0, s)
+    _lib.call("hmx_causal_attention_bwd", *back(q), *fore(k), *fore(v), _lib.HMX_BF16, *fore(o), *back(do), lse.data_ptr(),
+              None, 1, T, H, HKV, D, D ** -0.5, *fore(dq), *fore(dk), *fore(dv), delta.data_ptr(), s)
+    ins = [x.clone().requires_grad_() for x in (q.flip(2), k, v)]
+    want = hmx.causal_attention(*ins)
+    assert torch.equal(o, want)
+    for x, y in zip((dq, dk, dv), torch.autograd.grad(want, ins, do.flip(2).contiguous())):
+        assert torch.equal(x, y)
