@@ -298,3 +298,39 @@ def test_shared_inputs_and_leaves(dev):
     one, = torch.autograd.grad(hmx.causal_attention(y, y, y).float().square().sum(), y)
     tol = 3 * 2.0 ** -8 * sum(s.abs().float() for s in sep) + 1e-30
     assert ((one.float() - sum(s.float() for s in sep)).abs() <= tol).all()
+
+
+def test_captured_prompts_whose_keys_are_split(dev):
+    """Packed prompts of few rows, whose keys are split and joined through a workspace: two
+    graphs replayed in turn with other offsets and inputs, eager work between them."""
+    gen = torch.Generator().manual_seed(14)
+    steps = []
+    for T, H, HKV, D in ((3000, 4, 1, 128), (2100, 2, 2, 64)):
+        q, k, v = (randn(gen, 1, T, n, D).to(dev) for n in (H, HKV, HKV))
+        cu = torch.tensor([0, 700, 700, T], dtype=torch.int32, device=dev)
+        st = SimpleNamespace(T=T, ins=(q, k, v), cu=cu)
+        st.step = lambda st=st: (hmx.causal_attention(*st.ins, cu_seqlens=st.cu), hmx.causal_attention(*st.ins))
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            st.step()
+        torch.cuda.current_stream().wait_stream(side)
+        st.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(st.graph):
+            st.out = st.step()
+        steps.append(st)
+    for cut in (1, 1000, 64, 2000):
+        for st in steps:
+            st.cu[1] = st.cu[2] = cut
+            st.cu[2] += 7
+            st.cu[3] = st.T - cut % 5
+            for x in st.ins:
+                x.copy_(randn(gen, *x.shape))
+            st.graph.replay()
+            got = [x.clone() for x in st.out]
+            torch.cuda.synchronize()
+            for x, y in zip(got, st.step()):
+                assert torch.equal(x, y)
+    for st in steps:                              # the case is one that splits
+        (_, T, H, D), HKV = st.ins[0].shape, st.ins[1].shape[2]
+        assert hmx._lib.load().hmx_causal_attention_workspace_bytes(3, T, H, HKV, D, 1) > 0

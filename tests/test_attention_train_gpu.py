@@ -136,3 +136,29 @@ def test_grads_where_the_forward_splits_its_keys(dev, cu):
     bounds = [(0, T)] if cu is None else bounds_of(cu)
     (_, *want), mags = ref.causal_grads(q[0], k[0], v[0], D ** -0.5, bounds, do[0])
     _check([g[0] for g in grads], want, mags, str(cu))
+
+
+@pytest.mark.parametrize("cu,H,HKV", [([0, 5, 5, 70, 400], 6, 2), ([3, 4, 5, 330], 4, 4), ([0, 128, 256, 400], 7, 1),
+                                      ([0, *range(1, 71), 400], 4, 2)])
+def test_grads_packed_at_the_larger_head_size(dev, cu, H, HKV):
+    T, D = 400, 128
+    q, k, v, do = _inputs(len(cu), 1, T, H, HKV, D)
+    ins = [x.to(dev).requires_grad_() for x in (q, k, v)]
+    o = hmx.causal_attention(*ins, cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=dev))
+    grads = torch.autograd.grad(o, ins, do.to(dev))
+    (_, *want), mags = ref.causal_grads(q[0], k[0], v[0], D ** -0.5, bounds_of(cu), do[0])
+    _check([g[0] for g in grads], want, mags, str(cu))
+    for g in grads:
+        assert (g[0, :cu[0]] == 0).all() and (g[0, cu[-1]:] == 0).all()
+
+
+@pytest.mark.parametrize("T,cu,H,HKV,D", [(2300, None, 4, 1, 128), (2300, [0, 1500, 2301], 2, 2, 128), (1801, None, 8, 2, 64)])
+def test_grads_of_long_sequences(dev, T, cu, H, HKV, D):
+    """Many tiles of rows and keys, the last ones ragged."""
+    T = cu[-1] if cu else T
+    q, k, v, do = _inputs(T, 1, T, H, HKV, D)
+    ins = [x.to(dev).requires_grad_() for x in (q, k, v)]
+    o = hmx.causal_attention(*ins, cu_seqlens=None if cu is None else torch.tensor(cu, device=dev))
+    grads = torch.autograd.grad(o, ins, do.to(dev))
+    (_, *want), mags = ref.causal_grads(q[0], k[0], v[0], D ** -0.5, [(0, T)] if cu is None else bounds_of(cu), do[0])
+    _check([g[0] for g in grads], want, mags, f"T={T}")
