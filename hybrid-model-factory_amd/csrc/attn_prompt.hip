@@ -157,6 +157,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
       char* orow = a.o + (int64_t)(t.bos + tok) * a.o_ts + (int64_t)head * a.o_hs;
 #pragma unroll
       for (int i = 0; i < NS; ++i) *reinterpret_cast<u32x4*>(orow + 32 * i + 16 * h) = u32x4{0, 0, 0, 0};
+      if (a.lse && h == 0) a.lse[(int64_t)(t.bos + tok) * a.H + head] = NEG_INF;
     }
     return;
   }

@@ -865,7 +865,7 @@ int hmx_paged_attention_decode(const void* q, int64_t q_token_stride, int64_t q_
  * the device offsets cu_seqlens [N + 1] (clamped into 0 .. T), or of T / N tokens each
  * where cu_seqlens is NULL.  lse: NULL, or fp32 [T, H], the base-2 logarithm of
  * sum_j 2^(log2(e) scale q . k_j), as hmx_causal_attention_bwd takes it.  fill_gaps: rows
- * of no sequence become 0 (else they are left as they were).  workspace: 16-byte aligned,
+ * of no sequence become 0, their lse minus infinity (else they are left as they were).  workspace: 16-byte aligned,
  * needed where *_workspace_bytes is not 0 (few rows with many keys); its contents before and
  * after do not matter.  packed: whether cu_seqlens is given.
  */

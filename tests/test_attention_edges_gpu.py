@@ -252,3 +252,28 @@ def test_c_calls_with_strides_that_go_back(dev):
     assert torch.equal(o, want)
     for x, y in zip((dq, dk, dv), torch.autograd.grad(want, ins, do.flip(2).contiguous())):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("T,cu", [(200, [5, 60, 60, 190]), (2500, [100, 2000, 2400])])
+def test_registered_row_statistics(dev, T, cu):
+    """The registered op's second output: the logarithm of every row's sum, minus infinity for
+    rows of no sequence, whose sum is empty.  fp32 scores leave 2^-12 of the sum, the hardware's
+    logarithm less."""
+    import hmx.library  # noqa: F401
+    gen = torch.Generator().manual_seed(T)
+    H, HKV, D = 4, 2, 64
+    q, k, v = (randn(gen, 1, T, n, D) for n in (H, HKV, HKV))
+    for _ in range(3):                            # memory that other results have left
+        torch.full((T, H), 3.0, device=dev)
+        o, lse = torch.ops.hmx.causal_attention(q.to(dev), k.to(dev), v.to(dev), None,
+                                                torch.tensor(cu, dtype=torch.int32, device=dev))
+    want = torch.full((T, H), -torch.inf, dtype=torch.float64)
+    for b, e in bounds_of(cu):
+        kk = k[0, b:e].double().repeat_interleave(H // HKV, 1)
+        s = torch.einsum("ihd,jhd->ijh", q[0, b:e].double(), kk) * D ** -0.5
+        s.masked_fill_(torch.ones(e - b, e - b, dtype=torch.bool).triu(1)[..., None], -torch.inf)
+        want[b:e] = torch.logsumexp(s, 1) / torch.log(torch.tensor(2.0, dtype=torch.float64))
+    there = torch.isfinite(want)
+    lse = lse.double().cpu()
+    assert torch.equal(torch.isfinite(lse), there) and (lse[~there] == -torch.inf).all()
+    assert ((lse - want).abs()[there] <= 2.0 ** -11 + 2.0 ** -20 * want[there].abs()).all()
