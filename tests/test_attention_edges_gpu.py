@@ -277,3 +277,42 @@ def test_registered_row_statistics(dev, T, cu):
     lse = lse.double().cpu()
     assert torch.equal(torch.isfinite(lse), there) and (lse[~there] == -torch.inf).all()
     assert ((lse - want).abs()[there] <= 2.0 ** -11 + 2.0 ** -20 * want[there].abs()).all()
+
+
+@pytest.mark.parametrize("H,HKV,D,page", [(8, 2, 128, 16), (14, 2, 64, 48)])
+def test_tables_wider_than_the_sequences(dev, H, HKV, D, page):
+    """An engine's table, as wide as its longest sequence may grow: short, empty and long
+    sequences beside one another, entries behind their pages outside the cache."""
+    gen = torch.Generator().manual_seed(page)
+    lens = [5, 0, 700, 64, 3333, 1]
+    kc, vc, table, ks, vs = paged(gen, lens, page, HKV, D, BF, width=20000 // page)
+    n32 = torch.tensor(lens, dtype=torch.int32, device=dev)
+    args = [x.to(dev) for x in (kc, vc, table)] + [n32]
+    q = randn(gen, 2 * len(lens), H, D)
+    out = hmx.paged_attention_decode(q[:len(lens)].to(dev), *args)
+    new = hmx.paged_causal_attention(q.to(dev), *args, torch.arange(0, 2 * len(lens) + 1, 2))
+    for n, L in enumerate(lens):
+        o, a = ref.rows(q[n:n + 1], ks[n], vs[n], D ** -0.5, L - 1)
+        check_o(out[n:n + 1], o, a, vs[n], f"decode {L}")
+        o, a = ref.rows(q[2 * n:2 * n + 2], ks[n], vs[n], D ** -0.5, L - 2)
+        check_o(new[2 * n:2 * n + 2], o, a, vs[n], f"new tokens of {L}")
+
+
+@pytest.mark.parametrize("width", [3, 200])
+def test_lengths_outside_the_table(dev, width):
+    """Lengths past the table's pages count as all of them, negative ones as none."""
+    gen = torch.Generator().manual_seed(width)
+    kc, vc = (randn(gen, 2 * width, 16, 2, 64).to(dev) for _ in range(2))
+    table = torch.randperm(2 * width, generator=gen).to(torch.int32).view(2, width).to(dev)
+    q = randn(gen, 5, 4, 64).to(dev)
+    cu = torch.tensor([0, 2, 5], dtype=torch.int32, device=dev)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)
+    for far, near in ((i32(10 ** 9, 2 ** 31 - 1), i32(16 * width, 16 * width)), (i32(16 * width + 1, -5), i32(16 * width, 0)),
+                      (i32(-(2 ** 31), 30), i32(0, 30))):
+        args = (kc, vc, table)
+        want = hmx.paged_attention_decode(q[:2], *args, near)
+        assert torch.equal(hmx.paged_attention_decode(q[:2], *args, far), want)
+        a, b = (hmx.paged_causal_attention(q, *args, n, cu).double() for n in (far, near))
+        # splits of other lengths: two roundings of terms whose magnitudes are below max |v| < 6
+        assert ((a - b).abs() <= 4 * 2.0 ** -8 * 6).all() and torch.equal(a == 0, b == 0)
+        assert (want[near == 0] == 0).all()
