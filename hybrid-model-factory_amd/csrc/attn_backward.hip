@@ -9,12 +9,14 @@
 // Products are transposed where that leaves P and dS as B operands in the C layout.
 // P and dS are rounded to bf16 (half a step, as the inputs themselves are); everything
 // else stays in fp32.  What that costs against float64, where rounding the results alone makes
-// an error of 1.7e-3: dK 2.3e-3; dQ 2.8e-3, for delta is formed from the rounded O.  Keeping
-// eight more bits of O beside it took dQ's to 2.6e-3, for 1.2 % of the step and half as much
-// memory again as O's (the rest of delta's error is O's own, from P's rounding); delta by a
-// pass of its own and dS in two parts for the rows of at most 512 keys, whose gradients are the
-// largest, took it to 2.5e-3 for 2 % of the step and 15 % of a packed step of 3001 tokens.
-// Neither is done.
+// an error of 1.7e-3: dV 2.3e-3, dK 2.4e-3, dQ 2.4 - 2.5e-3.  delta is formed from the rounded
+// O, and in rows that attend few keys its error, times P K, was more than all others together
+// (dQ 2.8 - 3.0e-3, up to 3.9e-3 in short sequences).  Since dS sums to 0, what it does sum to
+// is that error: dK's delta is put right by it, and dQ by it times the greatest P's keys.
+// Looking for those costs nothing measurable where no P passes 1/8, 1 - 2 % of the step in
+// peaked heads, 8 % at 512 tokens.  Eight more bits of O beside it took dQ's error to 2.6e-3
+// for 1.2 % of the step and half as much memory again as O's; dS in two parts would take its
+// rounding away too, for one more product.  Neither is done.
 //
 // Measured at 8 x 4096 tokens, 32 / 8 heads of 128 (forward 1.10 ms): dQ 1.53 ms, 1.08 PFLOP/s;
 // dK and dV 2.45 ms, 0.9; a large matrix product reaches 1.22 - 1.26.
@@ -83,6 +85,9 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_dq_kernel(BwdArgs a) {
   delta = pair_sum32(delta, delta);
   const float lse = a.lse[gt * a.H + head];
   float over = 0.f;                         // the sum of dS, own half's keys
+  // the own half's greatest P past 1/8, its place among the 16 of a unit in the low bits, and the unit
+  uint32_t top = __builtin_bit_cast(uint32_t, 0.125f) | 15;
+  int top_unit = -1;
 
   // staging as in the forward: the wave brings rows 16 wave .. 16 wave + 15 of a tile
   uint32_t koff[NL], voff[NL];
@@ -145,10 +150,25 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_dq_kernel(BwdArgs a) {
         for (int i = 0; i < 16; ++i)
           if (t0 + kt * 32 + 8 * (i >> 2) + 4 * h + (i & 3) > tok) st[i] = NEG_INF;
       }
+      uint32_t p[16];                       // P, as the bits of positive numbers
+#pragma unroll
+      for (int i = 0; i < 16; ++i) p[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_exp2f(st[i] * a.c - lse));
+      uint32_t mx = max(p[0], p[1]);
+#pragma unroll
+      for (int i = 2; i < 16; ++i) mx = max(mx, p[i]);
+      if (__any(mx > top)) {
+        mx = p[0] & ~15u;
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mx = max(mx, (p[i] & ~15u) | (uint32_t)i);
+        if (mx > top) {
+          top = mx;
+          top_unit = 2 * j + kt;
+        }
+      }
       float ds[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        ds[i] = __builtin_amdgcn_exp2f(st[i] * a.c - lse) * (dp[i] - delta);
+        ds[i] = __builtin_bit_cast(float, p[i]) * (dp[i] - delta);
         over += ds[i];
       }
       const v8 d0 = pack8<T>(ds[0], ds[1], ds[2], ds[3], ds[4], ds[5], ds[6], ds[7]);
@@ -171,6 +191,27 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_dq_kernel(BwdArgs a) {
   // sum to is delta's error, and dK gets a delta without it.
   over = pair_sum32(over, over);
   if (h == 0 && row < t.rows) a.delta[gt * a.H + head] = delta + over;
+  // dQ has -delta's error times P K.  P K would be another product, but where it is not small
+  // most of it is the greatest probabilities' keys, one of either half's: those are taken out.
+  const float w = top_unit < 0 ? 0.f : over * __builtin_bit_cast(float, top & ~15u);
+  // (clamped: where the row's own scores are NaN so is P behind its last key)
+  const int top_key = min(max(top_unit, 0) * 32 + 8 * (int)((top & 15) >> 2) + 4 * h + (int)(top & 3), tok);
+  const float w_other = shfl_xor(w, 32);
+  const int key_other = __shfl_xor(top_key, 32, 64);
+#pragma unroll 1
+  for (int x = 0; x < 2; ++x) {
+    const float wx = x ? w_other : w;
+    if (wx == 0.f) continue;
+    const T* kp = reinterpret_cast<const T*>(kbase + (x ? key_other : top_key) * a.k_ts) + 4 * h;
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const v4 kv = *reinterpret_cast<const v4*>(kp + 32 * d + 8 * i);
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) acc[d][4 * i + jj] -= wx * (float)kv[jj];
+      }
+  }
   if (row < t.rows) {
 #pragma unroll
     for (int d = 0; d < ND; ++d)

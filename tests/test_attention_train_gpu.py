@@ -162,3 +162,32 @@ def test_grads_of_long_sequences(dev, T, cu, H, HKV, D):
     grads = torch.autograd.grad(o, ins, do.to(dev))
     (_, *want), mags = ref.causal_grads(q[0], k[0], v[0], D ** -0.5, [(0, T)] if cu is None else bounds_of(cu), do[0])
     _check([g[0] for g in grads], want, mags, f"T={T}")
+
+
+@pytest.mark.parametrize("B,T,H,HKV,D", [(8, 16, 8, 2, 128), (4, 33, 4, 1, 64), (2, 64, 8, 8, 64), (1, 700, 4, 2, 128)])
+def test_query_gradients_of_peaked_rows(dev, B, T, H, HKV, D):
+    """Heads whose rows attend few keys.  The gradient's own rounding makes an error r, dS's
+    rounding another of its size, and what is left of the row term's error may be a third,
+    all independent: together sqrt(3) r.  (The row term is formed from a rounded output; its
+    error times P K alone would make 1.8 to 2.4 r here.)"""
+    q, k, v, do = _inputs(T, B, T, H, HKV, D)
+    q = (q.float() * 2.5).to(BF)
+    ins = [x.to(dev).requires_grad_() for x in (q, k, v)]
+    got = torch.autograd.grad(hmx.causal_attention(*ins), ins, do.to(dev))[0].double().cpu()
+    want = torch.stack([ref.causal_grads(q[b], k[b], v[b], D ** -0.5, [(0, T)], do[b])[0][1] for b in range(B)])
+    r = rel_err(want.to(BF), want)
+    assert rel_err(got, want) <= 3 ** 0.5 * r, (rel_err(got, want), r)
+
+
+def test_nan_rows_of_short_sequences(dev):
+    """Gradients are defined for finite inputs; NaN in one sequence stays in it, and reads
+    nothing behind it (its last row's scores are all NaN, those of no keys too)."""
+    H, HKV, D = 4, 2, 64
+    q, k, v, do = _inputs(2, 1, 12, H, HKV, D)
+    q[0, 11] = float("nan")
+    cu = torch.tensor([0, 1, 4, 10, 12], dtype=torch.int32, device=dev)
+    ins = [x.to(dev).requires_grad_() for x in (q, k, v)]
+    grads = torch.autograd.grad(hmx.causal_attention(*ins, cu_seqlens=cu), ins, do.to(dev))
+    (_, *want), mags = ref.causal_grads(q[0, :10], k[0, :10], v[0, :10], D ** -0.5, [(0, 1), (1, 4), (4, 10)], do[0, :10])
+    _check([g[0, :10] for g in grads], want, mags, "beside NaN")
+    assert grads[0][0, 11].isnan().all()
