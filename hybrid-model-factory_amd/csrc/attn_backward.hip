@@ -18,8 +18,8 @@
 // for 1.2 % of the step and half as much memory again as O's; dS in two parts would take its
 // rounding away too, for one more product.  Neither is done.
 //
-// Measured at 8 x 4096 tokens, 32 / 8 heads of 128 (forward 1.10 ms): dQ 1.53 ms, 1.08 PFLOP/s;
-// dK and dV 2.45 ms, 0.9; a large matrix product reaches 1.22 - 1.26.
+// Measured at 8 x 4096 tokens, 32 / 8 heads of 128 (forward 1.06 ms): dQ 1.55 ms, 1.07 PFLOP/s;
+// dK and dV 2.33 ms, 0.94; a large matrix product reaches 1.22 - 1.26.
 #include "attn.hpp"
 
 #include <type_traits>

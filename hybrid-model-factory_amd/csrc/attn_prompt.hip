@@ -16,12 +16,12 @@
 //
 // Bound by the matrix cores and the VALU together: they overlap little (the shares of the
 // time that each is at work add up to 100 - 115 %), and the clock falls to 1.6 - 1.8 GHz under
-// both, so what pays is fewer instructions.  Measured: one prompt of 32768, 16 / 4 heads of
-// 128, 3.75 - 4.0 ms, 1.1 PFLOP/s (a large matrix product reaches 1.22 - 1.26); packed prompts
-// of 64-wide heads, whose exponentials weigh twice as much against their products, 392 us at
-// 0.84; pieces of prompts over pages 850 us at 0.97; draft tokens of eight
-// sequences to 16384 keys 64 - 72 us and the joining 5 (76 us where every sequence's keys
-// were cut into as many splits).
+// both, so what pays is fewer instructions.  Measured (a range is that of the cards it was timed
+// on): one prompt of 32768, 16 / 4 heads of 128, 3.72 - 4.03 ms, 1.09 - 1.18 PFLOP/s (a large
+// matrix product reaches 1.22 - 1.26); packed prompts of 64-wide heads, whose exponentials weigh
+// twice as much against their products, 382 - 397 us, 0.83 - 0.86; pieces of prompts over pages
+// 842 - 902 us, 0.91 - 0.98; draft tokens of eight sequences to 16384 keys 63 - 75 us and the
+// joining 6 (76 us where every sequence's keys were cut into as many splits).
 #include "attn.hpp"
 
 namespace hmx {
@@ -131,7 +131,8 @@ __device__ __forceinline__ void add_nonfinite(const FwdArgs& a, const Tile& t, i
 // the loop multiplies K's keys 64 j .. 64 j + 63 and V's 64 j - 32 .. 64 j + 31, so both
 // tiles have two buffers, and arrive in LDS directly, a step ahead of their use.
 // Workgroups of a compute unit: two at head size 128, for the registers; at 64 three, which
-// spills some but hides more of the exponentials (404 -> 396 us on packed prompts).
+// hides more of the exponentials (404 -> 396 us on packed prompts).  Outside the loop registers
+// spill: 50 at 128 and 38 at 64 over contiguous keys, 4 and 6 over pages.
 template <typename T, int D, bool PAGED>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs a) {
   typedef typename El<T>::v8 v8;

@@ -180,10 +180,10 @@ def causal_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
 
     q [B, T, H, D], k and v [B, T, HKV, D]; with ``cu_seqlens`` (N + 1 offsets into the
     tokens, B = 1; where they are on the host, the first is 0) each of the N packed sequences
-    by itself.  ``scale`` (default
-    D ** -0.5) must be positive.  Returns [B, T, H, D] in q's type; rows of no sequence
-    are 0, or left as they were in ``out`` (which may not overlap an input).  A value that
-    is not finite reaches the rows that attend it and no others.
+    by itself.  ``scale`` (default D ** -0.5) must be positive.  Returns [B, T, H, D] in q's
+    type; rows of no sequence are 0, or left as they were in ``out`` (which may not overlap an
+    input).  A value that is not finite reaches the rows that attend it and no others; a row
+    whose scores are all minus infinity counts as one without keys, 0.
 
     Differentiable in q, k and v for bf16 (hmx.CausalAttention)."""
     _refuse_tangents("causal_attention", q, k, v)
@@ -270,8 +270,8 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     ``positions`` [T] the first R elements of every q and k head turn by their position's
     angles, in pairs (i, i + R / 2), or (2i, 2i + 1) with ``interleaved``; a position
     outside the table gives NaN.  Without them k is stored and q returned as they are.
-    Rows of the caches may not share memory with one another.
-    ``q_out`` (may be q itself) receives the rotated q.  Returns it, or None without q."""
+    Rows of the caches may not share memory.  ``q_out`` (may be q itself) receives the rotated
+    q.  Returns it, or None without q."""
     what = "append_paged_kv"
     _refuse_tangents(what, q, k, v)
     if k.dim() != 3 or k.shape != v.shape:
@@ -343,8 +343,9 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     q [N, H, D]; ``seq_lens`` [N] int32: keys of each sequence, the new token's among them
     (append_paged_kv stores it first); 0 gives a row of 0, and a length past the table
     row's pages counts as all of them.  ``block_table`` [N, width] int32; a page outside
-    the cache holds no keys.  Returns [N, H, D] in q's type (``out``, which may not overlap
-    an input)."""
+    the cache holds no keys.  A value that is not finite makes its column of its sequence's
+    rows infinite or NaN.  Returns [N, H, D] in q's type (``out``, which may not overlap an
+    input)."""
     what = "paged_attention_decode"
     _refuse_tangents(what, q, k_cache, v_cache)
     if q.dim() != 3:

@@ -49,7 +49,8 @@ extern "C" {
                                   arguments);
                               13: hmx_ssd_chunk_bwd (the SSD scan's backward); the
                                   attention entry points were added to 13, which
-                                  changed nothing before them */
+                                  changed nothing before them: a 13 built earlier
+                                  lacks their symbols */
 
 enum hmx_status {
   HMX_OK = 0,
