@@ -191,3 +191,39 @@ def test_nan_rows_of_short_sequences(dev):
     (_, *want), mags = ref.causal_grads(q[0, :10], k[0, :10], v[0, :10], D ** -0.5, [(0, 1), (1, 4), (4, 10)], do[0, :10])
     _check([g[0, :10] for g in grads], want, mags, "beside NaN")
     assert grads[0][0, 11].isnan().all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_the_end_of_a_long_prompt(dev, D):
+    """100003 tokens: the last rows' outputs and dQ, and dK and dV of the last keys, which no
+    other rows see, from the formulas over all keys."""
+    T, H, HKV, m = 100003, 4, 2, 5
+    gen = torch.Generator(device=dev).manual_seed(D)
+    q, k, v, do = (torch.randn(1, T, n, D, generator=gen, device=dev).to(BF).requires_grad_() for n in (H, HKV, HKV, H))
+    o = hmx.causal_attention(q, k, v)
+    grads = [g[0, -m:].double().cpu() for g in torch.autograd.grad(o, (q, k, v), do.detach())]
+    Q, K, V, dO = (x[0].detach().double() for x in (q, k, v, do))
+    scale, e = D ** -0.5, half_step(BF)
+    want = [torch.zeros(m, n, D, dtype=torch.float64) for n in (H, HKV, HKV)]
+    mags = [torch.zeros_like(x) for x in want]
+    for h in range(H):
+        kv = h // (H // HKV)
+        s = scale * (Q[-m:, h] @ K[:, kv].T)
+        s[:, -m:].masked_fill_(torch.ones(m, m, dtype=torch.bool, device=dev).triu(1), -torch.inf)
+        p = torch.softmax(s, -1)
+        O = p @ V[:, kv]
+        d = dO[-m:, h]
+        a = p @ V[:, kv].abs()
+        # P in bf16 and its scores' 2^-12, twice, and the result's rounding
+        t = (e + 2.0 ** -11) * a
+        assert ((o[0, -m:, h].detach().double() - O).abs() <= t + e * (O.abs() + t)).all()
+        ds = p * (d @ V[:, kv].T - (d * O).sum(-1, keepdim=True))
+        mag = p * (d.abs() @ V[:, kv].abs().T + (d.abs() * a).sum(-1, keepdim=True))
+        for x, ww in ((want, (scale * ds @ K[:, kv], scale * ds[:, -m:].T @ Q[-m:, h], p[:, -m:].T @ d)),
+                         (mags, (scale * mag @ K[:, kv].abs(), scale * mag[:, -m:].T @ Q[-m:, h].abs(), p[:, -m:].T @ d.abs()))):
+            x[0][:, h] = ww[0].cpu()
+            x[1][:, kv] += ww[1].cpu()
+            x[2][:, kv] += ww[2].cpu()
+    for name, g, w, mg, n in zip("qkv", grads, want, mags, (3, 3, 1)):
+        t = (n * e + 2.0 ** -11) * mg
+        assert ((g - w).abs() <= t + e * (w.abs() + t) + 1e-30).all(), name
