@@ -179,7 +179,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
   const int sp = t.sp, ns = t.ns;
   const int j_beg = (int)((int64_t)nt_all * sp / ns), j_end = (int)((int64_t)nt_all * (sp + 1) / ns);
   const int u_beg = 2 * j_beg, u_last = min(2 * j_end - 1, w_last < 0 ? -1 : w_last / 32);   // the wave's halves
-  if (tid < 4) s_skip[tid] = 0;
+  if (tid < 4) s_skip[tid] = -1;
   if (tid == 0) s_bad = 0;
 
   v8 qf[NS];
@@ -202,11 +202,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
   const char* kbase = (PAGED ? a.pages.k : a.k + (int64_t)t.bos * a.k_ts) + (int64_t)kvh * (PAGED ? a.pages.k_hs : a.k_hs);
   const char* vbase = (PAGED ? a.pages.v : a.v + (int64_t)t.bos * a.v_ts) + (int64_t)kvh * (PAGED ? a.pages.v_hs : a.v_hs);
   const bool whole = !PAGED || a.pages.page.d % 16 == 0;   // the wave's 16 rows lie in one page
-  // s_skip[j & 3] = j + 1: some page of key tile j lies outside the cache.  Only the staging of
-  // the tile's keys says so, in the step before the tile's own; while a step's waves read the
-  // flags of tiles j and j - 1 (mend has a barrier behind them), stage(j + 1) writes tile
-  // j + 1's alone.  Values need none: those that a product takes are of tiles whose keys were
-  // staged.
+  // s_skip[j & 3] = j + 1 (-1 at first): some page of key tile j lies outside the cache.  Only
+  // the staging of the tile's keys says so, in the step before the tile's own; while a step's
+  // waves read the flags of tiles j and j - 1 (mend has a barrier behind them), stage(j + 1)
+  // writes tile j + 1's alone.  Values need none: those that a product takes are of tiles whose
+  // keys were staged.
   auto stage_rows = [&](int j, int r0, bool value) __attribute__((always_inline)) {
     const uint32_t lds = lds_addr(smem) + (value ? 2 * TILE : 0) + ((j - j_beg) & 1) * TILE + wave * 16 * D * 2;
     const char* base = value ? vbase : kbase;
