@@ -54,6 +54,30 @@ __device__ __forceinline__ typename El<T>::v8 join(typename El<T>::v4 a, typenam
 }
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// Eight e4m3 values times a power of two, in a 16-bit type: exact, but for products outside
+// fp16's range (bf16's is fp32's).
+template <typename T> __device__ __forceinline__ typename El<T>::v8 from_e4m3(u32x2 x, float scale) {
+  typename El<T>::v8 y;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (__is_same(T, bf16)) {
+      const auto r = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[i >> 1], scale, true)
+                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[i >> 1], scale, false);
+      y[2 * i] = r[0];
+      y[2 * i + 1] = r[1];
+    } else {
+      const auto r = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[i >> 1], scale, true)
+                           : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x[i >> 1], scale, false);
+      y[2 * i] = r[0];
+      y[2 * i + 1] = r[1];
+    }
+  }
+  return y;
+}
+// The power of two 2^(code - 127) that a byte of scale stands for.
+__device__ __forceinline__ float scale_of(uint32_t code) { return __builtin_bit_cast(float, code << 23); }
 
 // The 16-byte chunk at which chunk c of row r of a tile sits in LDS.  Rows are read 16 at
 // a time at one chunk (row fragments) and four at a time over four chunks (the transposing
@@ -111,6 +135,10 @@ __device__ __forceinline__ void dma4(uint32_t lds, const char* at) {   // 4 byte
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
                :: "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(at) : "memory");
 }
+__device__ __forceinline__ void dma1(uint32_t lds, const uint8_t* at) {   // a byte a lane, widened to the 4 at lds + 4 l
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off"
+               :: "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(at) : "memory");
+}
 template <int N> __device__ __forceinline__ void dma_wait() {   // all but the last N
   asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory");
 }
@@ -154,6 +182,9 @@ struct Pages {
   const int32_t* lens;
   int32_t width, num_pages;
   FastDiv page;
+  // of a cache of 8 bits: bytes of scale [pages, HKV, page size], the places of a page together
+  const uint8_t *k_sc, *v_sc;
+  int64_t k_sc_ps, k_sc_hs, v_sc_ps, v_sc_hs;
 };
 
 // the kernels reach the 16 rows of a load group by 32-bit offsets
@@ -163,13 +194,27 @@ inline bool near_rows(int64_t token_stride) { return token_stride >= 0 && token_
 inline bool has_pages(const hmx_paged_kv& c) {
   return c.num_pages == 0 || c.table_width == 0 || (c.k && c.v && c.table);
 }
+inline bool has_scales(const hmx_paged_kv& c, const hmx_kv_scales* sc) {
+  return !sc || c.num_pages == 0 || c.table_width == 0 || (sc->k && sc->v);
+}
+// whether 16-byte loads reach every row of the cache in place
+inline bool aligned_pages(const hmx_paged_kv& c, bool bytes) {
+  const int64_t st = c.k_page_stride | c.k_token_stride | c.k_head_stride |
+                     c.v_page_stride | c.v_token_stride | c.v_head_stride;
+  return st % (bytes ? 16 : 8) == 0 && ((uintptr_t)c.k | (uintptr_t)c.v) % 16 == 0;
+}
 
-inline Pages make_pages(const hmx_paged_kv& c) {
-  Pages p;
+inline Pages make_pages(const hmx_paged_kv& c, const hmx_kv_scales* sc = nullptr) {
+  Pages p{};
+  const int64_t size = sc ? 1 : 2;   // bytes of an element
   p.k = static_cast<const char*>(c.k);
   p.v = static_cast<const char*>(c.v);
-  p.k_ps = 2 * c.k_page_stride; p.k_ts = 2 * c.k_token_stride; p.k_hs = 2 * c.k_head_stride;
-  p.v_ps = 2 * c.v_page_stride; p.v_ts = 2 * c.v_token_stride; p.v_hs = 2 * c.v_head_stride;
+  p.k_ps = size * c.k_page_stride; p.k_ts = size * c.k_token_stride; p.k_hs = size * c.k_head_stride;
+  p.v_ps = size * c.v_page_stride; p.v_ts = size * c.v_token_stride; p.v_hs = size * c.v_head_stride;
+  if (sc) {
+    p.k_sc = sc->k; p.k_sc_ps = sc->k_page_stride; p.k_sc_hs = sc->k_head_stride;
+    p.v_sc = sc->v; p.v_sc_ps = sc->v_page_stride; p.v_sc_hs = sc->v_head_stride;
+  }
   p.table = c.table; p.table_stride = c.table_stride; p.lens = c.seq_lens;
   p.width = c.num_pages > 0 ? c.table_width : 0;   // an empty cache holds no keys
   p.num_pages = c.num_pages; p.page = fast_div(c.page_size);
@@ -315,6 +360,29 @@ __device__ __forceinline__ Tile next_tile(const Seqs& s, const int32_t* lens, in
 __device__ __forceinline__ int place(int at, int blocks, int places) {
   return at >= places && blocks <= 2 * places ? blocks - 1 - (at - places) : at;
 }
+
+// The shares of rows over keys that several sequences have in common (attn_prompt.hip): for
+// split s < splits of row r = token * H + head D sums at part[(s rows + r) D], unnormalised,
+// and behind them all two numbers, the maximum of the scaled scores in base 2 and the sum.
+// Rows with fewer splits, or none, have NO_SHARE in the place of the first such maximum.
+constexpr uint32_t NO_SHARE = 0x7fc00000u;   // a NaN, in the place of a share's maximum: there is none
+struct PrefixShares {
+  float* part;
+  int64_t rows;
+  int32_t splits;
+};
+struct PrefixArgs {
+  const void* q;
+  int64_t q_ts, q_hs;        // elements
+  int32_t dtype;
+  Pages pages;               // the prefixes'
+  const int32_t* cu;         // offsets of the sequences behind each, or NULL: one prefix for all
+  int32_t M, N, H, HKV, D;
+  float scale;
+  bool eight;                // a cache of 8 bits
+};
+int prefix_splits(int64_t M, int64_t N, int H, int HKV, int64_t max_keys);
+void launch_prefix(const PrefixArgs& p, const PrefixShares& out, int64_t max_keys, hipStream_t s);
 
 template <int BM>
 inline int64_t tile_slots(const int32_t* cu, int64_t N, int64_t T, int64_t G) {

@@ -29,7 +29,6 @@ namespace attn {
 
 constexpr int BM = 128, BN = 64;
 constexpr float NO_MC = -1e30f;
-constexpr uint32_t NO_SHARE = 0x7fc00000u;   // a NaN, in the place of a share's maximum: there is none
 
 struct FwdArgs {
   const char *q, *k, *v;
@@ -57,6 +56,8 @@ __device__ __forceinline__ bool any_nonfinite(u32x4 x) {
   for (int i = 0; i < 4; ++i) b |= nonfinite<T>(x[i]) || nonfinite<T>(x[i] >> 16);
   return b;
 }
+// whether a byte of a cache of 8 bits is e4m3's NaN
+__device__ __forceinline__ bool nan8(uint32_t x) { return (x & 0x7f) == 0x7f; }
 // One key's row of k or v; NULL where its page lies outside the cache.
 template <typename T, bool PAGED>
 __device__ __forceinline__ const T* key_row(const FwdArgs& a, const Tile& t, int kvh, int j, bool value) {
@@ -90,7 +91,7 @@ __device__ __forceinline__ float* share_stats(const FwdArgs& a, int sp, int64_t 
 // Never reached with finite values.  A prompt of 4096 tokens, 32 / 8 heads of 128, takes 0.42 ms
 // with NaN in all values and 0.26 with one row of it, where finite ones take 0.17 (forming the
 // tile's rows again key by key took 83 and 40 ms).
-template <typename T, int D, bool PAGED>
+template <typename T, int D, bool PAGED, bool Q8, bool PREFIX>
 __device__ __forceinline__ void add_nonfinite(const FwdArgs& a, const Tile& t, int kvh, int k0, int k1, int h,
                                               char* orow, float* share) {
   typedef typename El<T>::v4 v4;
@@ -104,16 +105,22 @@ __device__ __forceinline__ void add_nonfinite(const FwdArgs& a, const Tile& t, i
     if (!v) continue;
 #pragma unroll
     for (int x = 0; x < NV; ++x) {
-      const u16x4 b = *reinterpret_cast<const u16x4*>(v + 8 * x + 4 * h);
-      const v4 f = __builtin_bit_cast(v4, b);
+      if constexpr (Q8) {
+        const uint32_t b = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const char*>(v) + 8 * x + 4 * h);
 #pragma unroll
-      for (int z = 0; z < 4; ++z) add[x][z] += nonfinite<T>(b[z]) ? (float)f[z] : 0.f;
+        for (int z = 0; z < 4; ++z) add[x][z] += nan8(b >> (8 * z)) ? __builtin_nanf("") : 0.f;
+      } else {
+        const u16x4 b = *reinterpret_cast<const u16x4*>(v + 8 * x + 4 * h);
+        const v4 f = __builtin_bit_cast(v4, b);
+#pragma unroll
+        for (int z = 0; z < 4; ++z) add[x][z] += nonfinite<T>(b[z]) ? (float)f[z] : 0.f;
+      }
     }
   }
 #pragma unroll
   for (int x = 0; x < NV; ++x) {
     if (add[x][0] == 0.f && add[x][1] == 0.f && add[x][2] == 0.f && add[x][3] == 0.f) continue;
-    if (a.nsplit > 1) {
+    if (PREFIX || a.nsplit > 1) {
       *reinterpret_cast<f32x4*>(share + 8 * x) += add[x];
     } else {
       v4* o = reinterpret_cast<v4*>(orow + 16 * x);
@@ -133,14 +140,24 @@ __device__ __forceinline__ void add_nonfinite(const FwdArgs& a, const Tile& t, i
 // Workgroups of a compute unit: two at head size 128, for the registers; at 64 three, which
 // hides more of the exponentials (404 -> 396 us on packed prompts).  Outside the loop registers
 // spill: 50 at 128 and 38 at 64 over contiguous keys, 4 and 6 over pages.
-template <typename T, int D, bool PAGED>
+//
+// Q8: a cache of 8 bits.  Its rows arrive in LDS as they are, with their bytes of scale, and
+// each wave turns the 16 rows of either tile that it brought into the inputs' type, so the
+// rest is the same; the tiles have one buffer each, the next step's bytes are on their way
+// meanwhile.  PREFIX: the rows of all sequences behind one prefix attend all its keys, and
+// leave their shares.
+template <typename T, int D, bool PAGED, bool Q8 = false, bool PREFIX = false>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs a) {
+  static_assert(PAGED || (!Q8 && !PREFIX), "");
   typedef typename El<T>::v8 v8;
   constexpr int NC = D / 8;                 // 16-byte chunks of a row
   constexpr int RI = 64 / NC, NL = 16 / RI; // rows of a wave's load, loads of its 16 rows of a tile
   constexpr int NS = D / 16, ND = D / 32;
   constexpr int TILE = BN * D * 2;          // bytes
-  __shared__ __align__(1024) char smem[4 * TILE];   // K, K, V, V
+  constexpr int VOFF = Q8 ? TILE : 2 * TILE;         // of the first tile of V
+  // K, K, V, V; or K, V, both in 8 bits and their scales, a wave's 16 rows of either in 32 words
+  constexpr int RAWK = 2 * TILE, RAWV = RAWK + TILE / 2, SCALES = RAWV + TILE / 2;
+  __shared__ __align__(1024) char smem[Q8 ? SCALES + 4 * 256 : 4 * TILE];
   __shared__ int s_bad, s_skip[4];
 
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
@@ -153,6 +170,11 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
   const int row = t.row0 + wave * 32 + l32;
   const int rowc = min(row, t.rows - 1);
   const int tok = fdiv(rowc, a.G), head = kvh * a.G.d + rowc - tok * a.G.d;
+  if (PREFIX && t.seq < 0) {                // rows behind no prefix
+    if (row < t.rows && h == 0)
+      share_stats<D>(a, 0, (int64_t)(t.bos + tok) * a.H + head)[0] = __builtin_bit_cast(float, NO_SHARE);
+    return;
+  }
   if (t.seq < 0) {                          // rows of no sequence
     if (a.fill && row < t.rows) {
       char* orow = a.o + (int64_t)(t.bos + tok) * a.o_ts + (int64_t)head * a.o_hs;
@@ -168,13 +190,15 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
     keys = (int)min((int64_t)max(uniform_load(a.pages.lens, t.seq), 0),
                     (int64_t)a.pages.width * a.pages.page.d);
   keys = __builtin_amdgcn_readfirstlane(keys);
-  const int off = keys - t.tokens;          // token i attends keys 0 .. off + i
-  const int klast = off + tok;
+  // token i attends keys 0 .. off + i; behind a prefix each attends all
+  const int off = PREFIX ? keys - 1 : keys - t.tokens;
+  auto token_of = [&](int r) __attribute__((always_inline)) { return PREFIX ? 0 : fdiv(r, a.G); };
+  const int klast = PREFIX ? off : off + tok;
   const int wrow = t.row0 + wave * 32;
-  const int w_first = off + fdiv(min(wrow, t.rows - 1), a.G);            // least last key of the wave's rows
-  const int w_last = off + fdiv(min(wrow + 31, t.rows - 1), a.G);        // and greatest
-  const int wg_first = off + fdiv(t.row0, a.G);
-  const int wg_last = off + fdiv(min(t.row0 + BM, t.rows) - 1, a.G);
+  const int w_first = off + token_of(min(wrow, t.rows - 1));             // least last key of the wave's rows
+  const int w_last = off + token_of(min(wrow + 31, t.rows - 1));         // and greatest
+  const int wg_first = off + token_of(t.row0);
+  const int wg_last = off + token_of(min(t.row0 + BM, t.rows) - 1);
   const int nt_all = wg_last < 0 ? 0 : wg_last / BN + 1;
   const int sp = t.sp, ns = t.ns;
   const int j_beg = (int)((int64_t)nt_all * sp / ns), j_end = (int)((int64_t)nt_all * (sp + 1) / ns);
@@ -246,9 +270,111 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
       }
     }
   };
+  // Of a cache of 8 bits: the wave's rows of step j's tiles as they are, RI8 to a load, and
+  // their bytes of scale, a word each (lanes 0 .. 15 keys, 16 .. 31 values); vlive, a bit for
+  // each of the values' rows that is a key.
+  constexpr int RI8 = 1024 / D, NL8 = 16 / RI8;
+  uint32_t vlive = 0;
+  auto stage_rows8 = [&](int j, bool value, const uint8_t*& sc) __attribute__((always_inline)) {
+    const int r0 = j * BN - (value ? 32 : 0) + wave * 16;
+    const uint32_t lds = lds_addr(smem) + (value ? RAWV : RAWK) + wave * 16 * D;
+    const char* base = value ? vbase : kbase;
+    const int64_t ps = value ? a.pages.v_ps : a.pages.k_ps, ts = value ? vts : kts;
+    const uint8_t* sbase = value ? a.pages.v_sc + kvh * a.pages.v_sc_hs : a.pages.k_sc + kvh * a.pages.k_sc_hs;
+    const int64_t sps = value ? a.pages.v_sc_ps : a.pages.k_sc_ps;
+    const bool mine = value == (bool)((lane >> 4) & 1);
+    uint32_t live = r0 < 0 ? 0 : (1u << min(max(keys - r0, 0), 16)) - 1;   // r0 is a multiple of 16
+    if (whole) {
+      const int r = max(min(r0, (keys - 1) & ~15), 0), p = fdiv(r, a.pages.page);
+      int id = uniform_load(a.pages.table, t.seq * a.pages.table_stride + __builtin_amdgcn_readfirstlane(p));
+      if ((unsigned)id >= (unsigned)a.pages.num_pages) {
+        if (!value && live) s_skip[j & 3] = j + 1;
+        id = 0;
+        live = 0;
+      }
+      const int in = r - p * a.pages.page.d;
+      const char* b = uniform_ptr(base + id * ps + in * ts);
+#pragma unroll
+      for (int i = 0; i < NL8; ++i)
+        dma16(lds + i * 1024, b, (uint32_t)((i * RI8 + lane / (D / 16)) * (int)ts + 16 * (lane % (D / 16))));
+      if (mine) sc = sbase + id * sps + in + (lane & 15);
+    } else {
+      int in;
+      auto page_of = [&](int x) __attribute__((always_inline)) {   // of row x, -1 outside the cache, and its place
+        const int r = max(min(r0 + x, keys - 1), 0), p = fdiv(r, a.pages.page);
+        const int id = a.pages.table[t.seq * a.pages.table_stride + p];
+        in = r - p * a.pages.page.d;
+        return (unsigned)id < (unsigned)a.pages.num_pages ? id : -1;
+      };
+      const int id = page_of(lane & 15);
+      const uint32_t there = (uint32_t)__ballot(id >= 0) & 0xffffu;
+      if (!value && (live & ~there)) s_skip[j & 3] = j + 1;
+      live &= there;
+      if (mine) sc = sbase + max(id, 0) * sps + in;
+#pragma unroll
+      for (int i = 0; i < NL8; ++i) {
+        const int64_t page = max(page_of(i * RI8 + lane / (D / 16)), 0);
+        dma16(lds + i * 1024, base + page * ps + in * ts + 16 * (lane % (D / 16)));
+      }
+    }
+    return live;
+  };
+  auto stage8 = [&](int j) __attribute__((always_inline)) {
+    const uint8_t* sc = a.pages.k_sc + kvh * a.pages.k_sc_hs;   // any byte, where the step brings no keys
+    if (j < j_end) stage_rows8(j, false, sc);
+    vlive = stage_rows8(j, true, sc);
+    dma1(lds_addr(smem) + SCALES + wave * 256, sc);
+  };
   auto stage = [&](int j) __attribute__((always_inline)) {                 // the keys and values of step j
-    if (j < j_end) stage_rows(j, j * BN + wave * 16, false);
-    stage_rows(j, j * BN - 32 + wave * 16, true);
+    if constexpr (Q8) {
+      stage8(j);
+    } else {
+      if (j < j_end) stage_rows(j, j * BN + wave * 16, false);
+      stage_rows(j, j * BN - 32 + wave * 16, true);
+    }
+  };
+  // The wave's rows of step j's tiles in the inputs' type.  Rows of V that are no keys become
+  // 0, and values that are not finite where some row's keys end among them, as in mend().
+  auto widen = [&](int j) __attribute__((always_inline)) {
+    constexpr int NP = D / 32;              // pieces of eight values a lane
+    const uint32_t* scales = reinterpret_cast<const uint32_t*>(smem + SCALES + wave * 256);
+    const bool edge = j * BN - 32 + BN > wg_first + 1;
+#pragma unroll
+    for (int value = 0; value < 2; ++value) {
+      if (!value && j >= j_end) continue;
+      const char* raw = smem + (value ? RAWV : RAWK) + wave * 16 * D;
+      bool bad = false;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int at = lane + 64 * i, r = at / NC, c = at % NC;
+        const u32x2 x = *reinterpret_cast<const u32x2*>(raw + 8 * at);
+        const uint32_t code = scales[16 * value + r];
+        v8 y = from_e4m3<T>(x, scale_of(code));
+        if constexpr (__is_same(T, f16)) {
+          if (code >= 127 + 8) {            // 448 times it passes fp16's range: the largest value there, NaN as it is
+#pragma unroll
+            for (int z = 0; z < 8; ++z) {
+              const float f = (float)y[z];
+              if (f > 65504.f) y[z] = (f16)65504.f;
+              if (f < -65504.f) y[z] = (f16)-65504.f;
+            }
+          }
+        }
+        u32x4 out = __builtin_bit_cast(u32x4, y);
+        if (value) {
+          if (!((vlive >> r) & 1)) {
+            out = u32x4{0, 0, 0, 0};
+          } else if (edge && any_nonfinite<T>(out)) {
+#pragma unroll
+            for (int z = 0; z < 8; ++z)
+              if (nonfinite<T>(out[z >> 1] >> (16 * (z & 1)))) out[z >> 1] &= z & 1 ? 0xffffu : 0xffff0000u;
+            bad = true;
+          }
+        }
+        *reinterpret_cast<u32x4*>(smem + (value ? VOFF : 0) + (wave * 16 + r) * D * 2 + swz<D>(wave * 16 + r, c) * 16) = out;
+      }
+      if (bad) s_bad = 1;
+    }
   };
   // Rows of step j's V that are no keys to 0 (their probability is 0, their memory anything).
   // Where some row's keys end among them, so do values that are not finite: 0 times one is not
@@ -300,6 +426,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
     vu[d] = tr_offset<D>(lane, d, true) * 2;
   }
   auto flip = [&]() __attribute__((always_inline)) {
+    if constexpr (Q8) return;
 #pragma unroll
     for (int s = 0; s < NS; ++s) ko[s] ^= TILE;
 #pragma unroll
@@ -374,7 +501,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
   // half's scores from K's half kt; the tiles are the buffers at `at`
   constexpr int AHEAD = 2;                  // LDS reads run so many products ahead
   auto half = [&](int u, const f32x16& cur, f32x16& nxt, int at, int kt, int r) __attribute__((always_inline)) {
-    const char *Kb = smem + at + kt * 32 * D * 2, *Vb = smem + at + 2 * TILE + r * D * 2;
+    const char *Kb = smem + at + kt * 32 * D * 2, *Vb = smem + at + VOFF + r * D * 2;
     constexpr int E = EAGER ? 8 : 16;       // elements of P formed beside the scores
     v8 kf[NS], vf[2 * ND], pf[2];
     float p[16], sum = 0.f, mx = NEG_INF;
@@ -440,7 +567,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
         for (int i = 0; i < 8; ++i) element(cur, 8 * b + i, p, l);
       }
       const v8 pf = pack(p + 8 * b);
-      const char* Vb = smem + 2 * TILE + (r + 16 * b) * D * 2;
+      const char* Vb = smem + VOFF + (r + 16 * b) * D * 2;
 #pragma unroll
       for (int d = 0; d < ND; ++d)
         acc[d] = El<T>::mma32(join<T>(tr4<T>(reinterpret_cast<const T*>(Vb + vo[d])),
@@ -450,8 +577,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
   auto arrive = [&](int j) __attribute__((always_inline)) {   // step j's tiles are there, step j + 1's on their way
     dma_wait<0>();
     __syncthreads();
+    if constexpr (Q8) widen(j);             // what the wave itself brought, over tiles that all have read
     if (j < j_end) stage(j + 1);
-    mend(j);
+    if constexpr (Q8) __syncthreads();
+    else mend(j);
   };
 
   if (j_beg < j_end) {
@@ -507,7 +636,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
   const int etok = fdiv(min(erow, t.rows - 1), a.G), ehead = kvh * a.G.d + min(erow, t.rows - 1) - etok * a.G.d;
   const int64_t r = (int64_t)(t.bos + etok) * a.H + ehead;
   char* eo = a.o + (int64_t)(t.bos + etok) * a.o_ts + (int64_t)ehead * a.o_hs + 8 * eh;
-  if (a.nsplit > 1) {
+  if (PREFIX || a.nsplit > 1) {
     if (erow < t.rows) {
       float* pp = share_row<D>(a, sp, r) + 4 * eh;
 #pragma unroll
@@ -539,8 +668,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
   __syncthreads();
   // the first tile with an edge begins behind wg_first - 63
   if (s_bad && erow < t.rows)
-    add_nonfinite<T, D, PAGED>(a, t, kvh, max(j_beg * BN, off + fdiv(t.row0, a.G) - 62), min(j_end * BN, off + etok + 1),
-                               eh, eo, share_row<D>(a, sp, r) + 4 * eh);
+    add_nonfinite<T, D, PAGED, Q8, PREFIX>(a, t, kvh, max(j_beg * BN, off + token_of(t.row0) - 62),
+                                           min(j_end * BN, off + (PREFIX ? 0 : etok) + 1), eh, eo,
+                                           share_row<D>(a, sp, r) + 4 * eh);
 }
 
 // The splits' shares of a row joined: sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.  The
@@ -589,19 +719,52 @@ static Splits splits(int64_t tiles, int HKV, int64_t max_keys, int least) {
   return Splits{(int32_t)even, (int32_t)(2 * even < most ? 2 * even : most), (int32_t)(want / HKV), least};
 }
 
-template <typename T, bool PAGED>
+template <typename T, bool PAGED, bool Q8 = false, bool PREFIX = false>
 static void launch_fwd(FwdArgs a, int D, hipStream_t s) {
   a.places = (int32_t)(cu_count() / a.HKV);
   int64_t blocks = a.slots;                 // of a kv head
-  if (a.nsplit > 1) blocks = !a.seqs.cu || a.seqs.N > LANE_SEQS ? blocks * a.split.even : blocks + a.split.blocks;
+  if (a.split.even > 1) blocks = !a.seqs.cu || a.seqs.N > LANE_SEQS ? blocks * a.split.even : blocks + a.split.blocks;
   const dim3 grid((unsigned)(blocks * a.HKV));
-  if (D == 64) hipLaunchKernelGGL((attn_fwd_kernel<T, 64, PAGED>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((attn_fwd_kernel<T, 128, PAGED>), grid, dim3(256), 0, s, a);
-  if (a.nsplit > 1) {
+  if (D == 64) hipLaunchKernelGGL((attn_fwd_kernel<T, 64, PAGED, Q8, PREFIX>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((attn_fwd_kernel<T, 128, PAGED, Q8, PREFIX>), grid, dim3(256), 0, s, a);
+  if (!PREFIX && a.nsplit > 1) {
     const int64_t rows = (int64_t)a.seqs.T * a.H, rpb = 1024 / D;
     const dim3 jg((unsigned)((rows + rpb - 1) / rpb));
     if (D == 64) hipLaunchKernelGGL((attn_join_kernel<T, 64>), jg, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((attn_join_kernel<T, 128>), jg, dim3(256), 0, s, a);
+  }
+}
+
+// The rows of N sequences, one token each, over the M prefixes that they share.
+static Splits shared_splits(int64_t M, int64_t N, int H, int HKV, int64_t max_keys, bool packed) {
+  const int32_t some = 0;
+  const int64_t slots = tile_slots<BM>(packed ? &some : nullptr, M, N, H / HKV);
+  return splits(packed ? slots - 2 : slots, HKV, max_keys, 4);
+}
+int prefix_splits(int64_t M, int64_t N, int H, int HKV, int64_t max_keys) {
+  const int one = shared_splits(M, N, H, HKV, max_keys, true).most;
+  return M == 1 && one < shared_splits(M, N, H, HKV, max_keys, false).most
+             ? shared_splits(M, N, H, HKV, max_keys, false).most : one;
+}
+void launch_prefix(const PrefixArgs& p, const PrefixShares& out, int64_t max_keys, hipStream_t s) {
+  FwdArgs a{};
+  a.q = (const char*)p.q;
+  a.q_ts = 2 * p.q_ts; a.q_hs = 2 * p.q_hs;
+  a.pages = p.pages;
+  a.seqs = Seqs{p.cu, p.M, p.N, p.H / p.HKV};
+  a.G = fast_div(p.H / p.HKV);
+  a.H = p.H; a.HKV = p.HKV;
+  a.slots = (int32_t)tile_slots<BM>(p.cu, p.M, p.N, p.H / p.HKV);
+  a.split = shared_splits(p.M, p.N, p.H, p.HKV, max_keys, p.cu != nullptr);
+  a.nsplit = out.splits;
+  a.part = out.part;
+  a.c = p.scale * LOG2E;
+  if (p.dtype == HMX_BF16) {
+    if (p.eight) launch_fwd<bf16, true, true, true>(a, p.D, s);
+    else launch_fwd<bf16, true, false, true>(a, p.D, s);
+  } else {
+    if (p.eight) launch_fwd<f16, true, true, true>(a, p.D, s);
+    else launch_fwd<f16, true, false, true>(a, p.D, s);
   }
 }
 
@@ -687,28 +850,29 @@ extern "C" size_t hmx_paged_causal_attention_workspace_bytes(int32_t N, int64_t 
   return ns == 1 ? 0 : (size_t)ns * T * H * (D + 2) * sizeof(float);
 }
 
-extern "C" int hmx_paged_causal_attention(const void* q, int64_t q_token_stride,
-                                          int64_t q_head_stride, int32_t dtype, void* o,
-                                          int64_t o_token_stride, int64_t o_head_stride,
-                                          const hmx_paged_kv* cache, const int32_t* cu_seqlens,
-                                          int32_t N, int64_t T, int32_t H, int32_t HKV, int32_t D,
-                                          float scale, int32_t fill_gaps, void* workspace,
-                                          size_t workspace_bytes, void* stream) {
+static int paged_causal_attention(const void* q, int64_t q_token_stride,
+                                  int64_t q_head_stride, int32_t dtype, void* o,
+                                  int64_t o_token_stride, int64_t o_head_stride,
+                                  const hmx_paged_kv* cache, const hmx_kv_scales* scales,
+                                  const int32_t* cu_seqlens,
+                                  int32_t N, int64_t T, int32_t H, int32_t HKV, int32_t D,
+                                  float scale, int32_t fill_gaps, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
   ATTN_COMMON_CHECKS("hmx_paged_causal_attention")
   HMX_REQUIRE(cache && cache->num_pages >= 0 && cache->page_size > 0 && cache->table_width >= 0, HMX_EINVAL,
               "hmx_paged_causal_attention: cache");
   if (T == 0) return HMX_OK;
-  HMX_REQUIRE(q && o && cu_seqlens && (N == 0 || (cache->seq_lens && attn::has_pages(*cache))),
+  HMX_REQUIRE(q && o && cu_seqlens && (N == 0 || (cache->seq_lens && attn::has_pages(*cache) &&
+                                                     attn::has_scales(*cache, scales))),
               HMX_EINVAL, "hmx_paged_causal_attention: null pointer");
   const int64_t max_keys = (int64_t)cache->table_width * cache->page_size;
   HMX_REQUIRE(max_keys < (1ll << 31) - 256, HMX_EUNSUPPORTED,
               "hmx_paged_causal_attention: a table row holds %lld keys", (long long)max_keys);
-  const int64_t st = q_token_stride | q_head_stride | o_token_stride | o_head_stride |
-                     cache->k_page_stride | cache->k_token_stride | cache->k_head_stride |
-                     cache->v_page_stride | cache->v_token_stride | cache->v_head_stride;
-  const uintptr_t al = (uintptr_t)q | (uintptr_t)o | (uintptr_t)cache->k | (uintptr_t)cache->v;
-  HMX_REQUIRE(st % 8 == 0 && al % 16 == 0, HMX_EINVAL,
-              "hmx_paged_causal_attention: strides must be multiples of 8 elements and pointers 16-byte aligned");
+  const int64_t st = q_token_stride | q_head_stride | o_token_stride | o_head_stride;
+  const uintptr_t al = (uintptr_t)q | (uintptr_t)o;
+  HMX_REQUIRE(st % 8 == 0 && al % 16 == 0 && attn::aligned_pages(*cache, scales != nullptr), HMX_EINVAL,
+              "hmx_paged_causal_attention: strides must be multiples of 8 elements (a cache's of 16 bytes) and "
+              "pointers 16-byte aligned");
   HMX_REQUIRE(attn::near_rows(cache->k_token_stride) && attn::near_rows(cache->v_token_stride), HMX_EUNSUPPORTED,
               "hmx_paged_causal_attention: token strides of the cache past 2^25 elements");
   attn::FwdArgs a{};
@@ -717,7 +881,7 @@ extern "C" int hmx_paged_causal_attention(const void* q, int64_t q_token_stride,
   a.o_ts = 2 * o_token_stride; a.o_hs = 2 * o_head_stride;
   a.seqs = attn::Seqs{cu_seqlens, N, (int32_t)T, H / HKV};
   a.G = attn::fast_div(H / HKV);
-  a.pages = attn::make_pages(*cache);
+  a.pages = attn::make_pages(*cache, scales);
   const int64_t slots = attn::tile_slots<attn::BM>(cu_seqlens, N, T, H / HKV);
   HMX_REQUIRE(slots * HKV < (1ll << 31), HMX_EUNSUPPORTED, "hmx_paged_causal_attention: %lld tiles",
               (long long)slots);
@@ -730,7 +894,39 @@ extern "C" int hmx_paged_causal_attention(const void* q, int64_t q_token_stride,
                    workspace_bytes >= hmx_paged_causal_attention_workspace_bytes(N, T, H, HKV, D, max_keys)),
               HMX_EINVAL, "hmx_paged_causal_attention: workspace of %zu bytes is too small", workspace_bytes);
   a.c = scale * attn::LOG2E;
-  if (dtype == HMX_BF16) attn::launch_fwd<bf16, true>(a, D, (hipStream_t)stream);
-  else attn::launch_fwd<f16, true>(a, D, (hipStream_t)stream);
+  hipStream_t st_ = (hipStream_t)stream;
+  if (dtype == HMX_BF16) {
+    if (scales) attn::launch_fwd<bf16, true, true>(a, D, st_);
+    else attn::launch_fwd<bf16, true>(a, D, st_);
+  } else {
+    if (scales) attn::launch_fwd<f16, true, true>(a, D, st_);
+    else attn::launch_fwd<f16, true>(a, D, st_);
+  }
   return check_launch("hmx_paged_causal_attention");
+}
+
+extern "C" int hmx_paged_causal_attention(const void* q, int64_t q_token_stride,
+                                          int64_t q_head_stride, int32_t dtype, void* o,
+                                          int64_t o_token_stride, int64_t o_head_stride,
+                                          const hmx_paged_kv* cache, const int32_t* cu_seqlens,
+                                          int32_t N, int64_t T, int32_t H, int32_t HKV, int32_t D,
+                                          float scale, int32_t fill_gaps, void* workspace,
+                                          size_t workspace_bytes, void* stream) {
+  return paged_causal_attention(q, q_token_stride, q_head_stride, dtype, o, o_token_stride, o_head_stride, cache,
+                                nullptr, cu_seqlens, N, T, H, HKV, D, scale, fill_gaps, workspace, workspace_bytes,
+                                stream);
+}
+
+extern "C" int hmx_paged_causal_attention8(const void* q, int64_t q_token_stride,
+                                           int64_t q_head_stride, int32_t dtype, void* o,
+                                           int64_t o_token_stride, int64_t o_head_stride,
+                                           const hmx_paged_kv* cache, const hmx_kv_scales* scales,
+                                           const int32_t* cu_seqlens,
+                                           int32_t N, int64_t T, int32_t H, int32_t HKV, int32_t D,
+                                           float scale, int32_t fill_gaps, void* workspace,
+                                           size_t workspace_bytes, void* stream) {
+  HMX_REQUIRE(scales, HMX_EINVAL, "hmx_paged_causal_attention8: no scales");
+  return paged_causal_attention(q, q_token_stride, q_head_stride, dtype, o, o_token_stride, o_head_stride, cache,
+                                scales, cu_seqlens, N, T, H, HKV, D, scale, fill_gaps, workspace, workspace_bytes,
+                                stream);
 }

@@ -128,6 +128,19 @@ SIGNATURES: dict[str, list] = {
     "hmx_paged_causal_attention": [_P, _I64, _I64, _I32, _P, _I64, _I64, _P, _P, _I32, _I64, _I32,
                                    _I32, _I32, _F32, _I32, _P, ctypes.c_size_t, _P],
     "hmx_paged_causal_attention_workspace_bytes": [_I32, _I64, _I32, _I32, _I32, _I64],
+    "hmx_append_paged_kv8": [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _P, _I64, _I64,
+                             _P, _P, _P, _I32, _P, _I32, _P, _I32, _I64, _I64, _I32, _I32, _I64,
+                             _I32, _I32, _I32, _P],
+    "hmx_paged_attention_decode8": [_P, _I64, _I64, _I32, _P, _I64, _I64, _P, _P, _I32, _I32, _I32,
+                                    _I32, _F32, _P, ctypes.c_size_t, _P],
+    "hmx_paged_causal_attention8": [_P, _I64, _I64, _I32, _P, _I64, _I64, _P, _P, _P, _I32, _I64,
+                                    _I32, _I32, _I32, _F32, _I32, _P, ctypes.c_size_t, _P],
+    "hmx_shared_prefix_decode": [_P, _I64, _I64, _I32, _P, _I64, _I64, _P, _P, _P, _I64, _I32, _P,
+                                 _P, _I32, _I32, _I32, _I32, _I32, _F32, _P, ctypes.c_size_t, _P],
+    "hmx_shared_prefix_decode_workspace_bytes": [_I32, _I32, _I32, _I32, _I32, _I64, _I64],
+    "hmx_rotary_embedding": [*([_P, _I64, _I64, _I64] * 4), _I32, _P, _I32, _I64, _P, _I32, _F32,
+                             _I32, _I32, _I32, _I32, _I64, _I32, _I32, _I32, _P],
+    "hmx_rotary_table": [_P, _I32, _F32, _I64, _I32, _P, _P],
 }
 _RESTYPES = {"hmx_last_error": ctypes.c_char_p, "hmx_gdn_chunk_workspace_bytes": ctypes.c_size_t,
              "hmx_gka_chunk_workspace_bytes": ctypes.c_size_t,
@@ -138,7 +151,8 @@ _RESTYPES = {"hmx_last_error": ctypes.c_char_p, "hmx_gdn_chunk_workspace_bytes":
              "hmx_ssd_chunk_bwd_workspace_bytes": ctypes.c_size_t,
              "hmx_paged_attention_decode_workspace_bytes": ctypes.c_size_t,
              "hmx_causal_attention_workspace_bytes": ctypes.c_size_t,
-             "hmx_paged_causal_attention_workspace_bytes": ctypes.c_size_t}
+             "hmx_paged_causal_attention_workspace_bytes": ctypes.c_size_t,
+             "hmx_shared_prefix_decode_workspace_bytes": ctypes.c_size_t}
 
 
 
@@ -219,6 +233,19 @@ def paged_kv(k_cache: torch.Tensor, v_cache: torch.Tensor, table: torch.Tensor |
         k_cache.data_ptr(), *ks, v_cache.data_ptr(), *vs, ptr(table),
         0 if table is None else table.stride(0), ptr(seq_lens),
         0 if table is None else table.shape[1], n[0], n[1]))
+
+
+class KVScales(ctypes.Structure):
+    """hmx_kv_scales (include/hmx.h): the bytes of scale of a cache of 8 bits."""
+    _fields_ = [("k", _P), ("k_page_stride", _I64), ("k_head_stride", _I64),
+                ("v", _P), ("v_page_stride", _I64), ("v_head_stride", _I64)]
+
+
+def kv_scales(k_scales: torch.Tensor, v_scales: torch.Tensor):
+    """ctypes pointer to an hmx_kv_scales of bytes [pages, HKV, page size]; strides of
+    dimensions of one go as 0."""
+    ks, vs = ([x if m > 1 else 0 for x, m in zip(t.stride()[:2], t.shape)] for t in (k_scales, v_scales))
+    return ctypes.pointer(KVScales(k_scales.data_ptr(), *ks, v_scales.data_ptr(), *vs))
 
 
 _lib = None

@@ -4,7 +4,7 @@ from .gdn import (chunk_gated_delta_rule, chunk_gated_delta_rule_gqa, fused_gdn_
 from .gka import (chebyshev_iteration_gqa, fused_gka_gating, gka_chebyshev_gla,
                   gka_chebyshev_gla_decode, gka_chebyshev_gla_prefill, torch_decoding_one_step)
 from .attention import (append_paged_kv, causal_attention, paged_attention_decode,
-                        paged_causal_attention)
+                        paged_causal_attention, shared_prefix_attention_decode)
 from .attention_train import CausalAttention
 from .conv import causal_conv1d_fn, causal_conv1d_update
 from .gates import ProjGates
@@ -12,6 +12,7 @@ from .gdn_train import ChunkGatedDeltaRule
 from .gka_train import ChebyshevIteration, GkaChebyshevGla, latent_chebyshev
 from .ssd_train import MambaChunkScanCombined
 from .norm import rms_norm_gated
+from .rotary import RotaryEmbedding, rotary_embedding, rotary_frequencies, rotary_table
 from .ssd import (mamba_chunk_scan_combined, mamba_chunk_scan_combined_varlen,
                   selective_state_update)
 
@@ -44,4 +45,9 @@ __all__ = [
     "append_paged_kv",
     "paged_attention_decode",
     "paged_causal_attention",
+    "shared_prefix_attention_decode",
+    "rotary_embedding",
+    "RotaryEmbedding",
+    "rotary_frequencies",
+    "rotary_table",
 ]

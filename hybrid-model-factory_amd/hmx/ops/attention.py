@@ -5,6 +5,7 @@ prompts, and over a paged key/value cache that ``append_paged_kv`` fills.
 - ``append_paged_kv``         position rotation of q and k, k and v stored into the cache
 - ``paged_causal_attention``  several new tokens a sequence behind a cached context
 - ``paged_attention_decode``  one new token a sequence
+- ``shared_prefix_attention_decode``  the same where groups of sequences share a prefix
 
 q carries H heads, k and v HKV heads that groups of H / HKV consecutive q heads share.
 Head sizes 64 and 128, bf16 and fp16.  A cache is a pair of tensors
@@ -12,6 +13,13 @@ Head sizes 64 and 128, bf16 and fp16.  A cache is a pair of tensors
 both halves of one allocation pass as views); ``block_table`` [N, width] int32 lists the
 pages of every sequence.  Lengths, offsets, tables and slots are read on the device only,
 so a captured graph replays with other lengths.
+
+A cache may be of 8 bits: k_cache and v_cache torch.float8_e4m3fn, beside them ``k_scales``
+and ``v_scales`` [pages, HKV, page size] (uint8, the places of a page contiguous), a byte c
+for every row, which stands for 2^(c - 127) times its values (c from 1 to 254).
+append_paged_kv fills it, with the least power of two, from 2^-126 on, of which the row's
+largest finite magnitude is at most 448; every op over a cache reads it.  q and the outputs
+are bf16 or fp16 as ever.
 
 causal_attention alone has a backward; one through another op's result raises, and what is
 stored into a cache or written to ``out`` has no gradient.  There is no forward-mode
@@ -84,13 +92,14 @@ def _check_types(what: str, q: torch.Tensor, *others: torch.Tensor | None) -> No
             raise ValueError(f"{what}: types {q.dtype} and {t.dtype} differ")
 
 
-def _aligned(t: torch.Tensor) -> bool:
-    """Whether 16-byte loads reach every row of [..., heads, D] in place."""
+def _aligned(t: torch.Tensor, unit: int = 8) -> bool:
+    """Whether 16-byte loads reach every row of [..., heads, D] in place; ``unit``: elements
+    of 16 bytes."""
     if t.is_contiguous():
         return t.data_ptr() % 16 == 0
     st, n = t.stride(), t.shape
     return (st[-1] == 1 and t.data_ptr() % 16 == 0
-            and all(s % 8 == 0 or m == 1 for s, m in zip(st[:-1], n[:-1])))
+            and all(s % unit == 0 or m == 1 for s, m in zip(st[:-1], n[:-1])))
 
 
 def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
@@ -149,14 +158,15 @@ def _scale(scale: float | None, D: int) -> float:
     return scale
 
 
-def _offsets(cu_seqlens: torch.Tensor, T: int, device: torch.device, any_first: bool = False) -> torch.Tensor:
+def _offsets(cu_seqlens: torch.Tensor, T: int, device: torch.device, any_first: bool = False,
+             name: str = "cu_seqlens") -> torch.Tensor:
     """cu_seqlens as int32 on the device.  Host offsets are checked here, and start at 0 unless
     ``any_first``; offsets on the device are never read back (the kernels clamp them into the
     tokens)."""
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1:
-        raise ValueError(f"cu_seqlens must be a vector of N + 1 offsets, got {tuple(cu_seqlens.shape)}")
+        raise ValueError(f"{name} must be a vector of N + 1 offsets, got {tuple(cu_seqlens.shape)}")
     if cu_seqlens.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"cu_seqlens must be int32 or int64, got {cu_seqlens.dtype}")
+        raise ValueError(f"{name} must be int32 or int64, got {cu_seqlens.dtype}")
     if cu_seqlens.is_cuda:
         if cu_seqlens.device != device:
             raise ValueError(f"tensors on {device} and {cu_seqlens.device}")
@@ -165,11 +175,11 @@ def _offsets(cu_seqlens: torch.Tensor, T: int, device: torch.device, any_first: 
     if any_first:
         cs = cu_seqlens.tolist()
         if cs[0] < 0 or cs[-1] > T or any(b < a for a, b in zip(cs, cs[1:])):
-            raise ValueError(f"cu_seqlens must be non-decreasing from >= 0 to <= {T}: {cs}")
+            raise ValueError(f"{name} must be non-decreasing from >= 0 to <= {T}: {cs}")
     else:
         seq_bounds(cu_seqlens, 1, T)
     if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError("cu_seqlens must be on the device where a graph is captured")
+        raise RuntimeError(f"{name} must be on the device where a graph is captured")
     return cu_seqlens.to(torch.int32).pin_memory().to(device, non_blocking=True)
 
 
@@ -235,32 +245,57 @@ def attention_forward(q, k, v, scale, cu_seqlens, out, want_lse):
     return o, lse, cu
 
 
-def _cache(what: str, q: torch.Tensor, k_cache, v_cache, HKV: int | None = None) -> None:
+def _cache(what: str, q: torch.Tensor, k_cache, v_cache, HKV: int | None = None,
+           k_scales: torch.Tensor | None = None, v_scales: torch.Tensor | None = None) -> None:
     if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[-1] != q.shape[-1] \
             or k_cache.shape[1] == 0 or k_cache.shape[2] == 0 \
             or (HKV is not None and k_cache.shape[2] != HKV):
         raise ValueError(f"{what}: caches [pages, page size, HKV, D], got {tuple(k_cache.shape)} and "
                          f"{tuple(v_cache.shape)} for heads of {q.shape[-1]}")
-    _check_types(what, q, k_cache, v_cache)
+    eight = k_cache.dtype == torch.float8_e4m3fn or v_cache.dtype == torch.float8_e4m3fn
+    if eight or k_scales is not None or v_scales is not None:
+        _check_types(what, q)
+        if not eight or k_cache.dtype != v_cache.dtype or k_scales is None or v_scales is None:
+            raise ValueError(f"{what}: a cache of 8 bits is two of torch.float8_e4m3fn with k_scales and v_scales, "
+                             f"got {k_cache.dtype} and {v_cache.dtype}")
+        n = k_cache.shape
+        for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
+            if t.dtype != torch.uint8 or tuple(t.shape) != (n[0], n[2], n[1]) or (n[1] > 1 and t.stride(2) != 1):
+                raise ValueError(f"{what}: {name} [{n[0]}, {n[2]}, {n[1]}] uint8 with the places of a page "
+                                 f"contiguous, got {tuple(t.shape)} {t.dtype}")
+    else:
+        _check_types(what, q, k_cache, v_cache)
     # never copied: a cache is written in place and as large as memory
-    if not (_aligned(k_cache) and _aligned(v_cache)):
+    if not (_aligned(k_cache, 16 if eight else 8) and _aligned(v_cache, 16 if eight else 8)):
         raise ValueError(f"{what}: caches need D contiguous and strides and bases of whole 16-byte units")
 
 
-def _table(what: str, block_table: torch.Tensor, seq_lens: torch.Tensor, N: int) -> None:
-    for name, t in (("block_table", block_table), ("seq_lens", seq_lens)):
+def _paged_call(name: str, head: tuple, kv, k_scales, v_scales, tail: tuple) -> None:
+    """The entry point of a cache in 16 bits, or the one in 8, which takes the scales behind
+    the cache."""
+    if k_scales is None:
+        _lib.call(name, *head, kv, *tail)
+    else:
+        _lib.call(name + "8", *head, kv, _lib.kv_scales(k_scales, v_scales), *tail)
+
+
+def _table(what: str, block_table: torch.Tensor, seq_lens: torch.Tensor, N: int,
+           table_name: str = "block_table", lens_name: str = "seq_lens") -> None:
+    for name, t in ((table_name, block_table), (lens_name, seq_lens)):
         if t.dtype != torch.int32:
             raise ValueError(f"{what}: {name} must be int32, got {t.dtype}")
     if block_table.dim() != 2 or block_table.shape[0] != N or tuple(seq_lens.shape) != (N,) \
             or not seq_lens.is_contiguous() or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError(f"{what}: block_table [{N}, width] with contiguous rows and seq_lens [{N}], got "
+        raise ValueError(f"{what}: {table_name} [{N}, width] with contiguous rows and {lens_name} [{N}], got "
                          f"{tuple(block_table.shape)} and {tuple(seq_lens.shape)}")
 
 
 def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                     slot_mapping: torch.Tensor, *, q: torch.Tensor | None = None,
                     positions: torch.Tensor | None = None, cos_sin: torch.Tensor | None = None,
-                    interleaved: bool = False, q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+                    interleaved: bool = False, q_out: torch.Tensor | None = None,
+                    k_scales: torch.Tensor | None = None,
+                    v_scales: torch.Tensor | None = None) -> torch.Tensor | None:
     """Stores k and v [T, HKV, D] into the cache, k rotated, and returns q [T, H, D] rotated.
 
     ``slot_mapping`` [T] (int32 or int64): page * page size + place in the page; a token
@@ -271,16 +306,20 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     angles, in pairs (i, i + R / 2), or (2i, 2i + 1) with ``interleaved``; a position
     outside the table gives NaN.  Without them k is stored and q returned as they are.
     Rows of the caches may not share memory.  ``q_out`` (may be q itself) receives the rotated
-    q.  Returns it, or None without q."""
+    q.  Returns it, or None without q.
+
+    Into a cache of 8 bits (``k_scales``, ``v_scales``) a row goes as its scale and e4m3
+    values to the nearest, ties to even, k straight from its rotation in fp32; what is not
+    finite is stored as NaN, and the scale is that of the others."""
     what = "append_paged_kv"
     _refuse_tangents(what, q, k, v)
     if k.dim() != 3 or k.shape != v.shape:
         raise ValueError(f"{what}: k and v [T, HKV, D], got {tuple(k.shape)} and {tuple(v.shape)}")
     T, HKV, D = k.shape
     _check_types(what, k, v, q)
-    _cache(what, k, k_cache, v_cache, HKV)
-    if any(0 in c.stride() and any(s == 0 and m > 1 for s, m in zip(c.stride(), c.shape))
-           for c in (k_cache, v_cache)):
+    _cache(what, k, k_cache, v_cache, HKV, k_scales, v_scales)
+    if any(c is not None and 0 in c.stride() and any(s == 0 and m > 1 for s, m in zip(c.stride(), c.shape))
+           for c in (k_cache, v_cache, k_scales, v_scales)):
         raise ValueError(f"{what}: caches must have a place of their own for every row")
     if (cos_sin is None) != (positions is None):
         raise ValueError(f"{what}: cos_sin and positions go together")
@@ -301,11 +340,12 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
         if cos_sin.stride(1) != 1 or cos_sin.stride(0) % 8 or cos_sin.data_ptr() % 16:
             cos_sin = cos_sin.contiguous()
     H = 0 if q is None else q.shape[1]
-    _same_device(k, v, k_cache, v_cache, slot_mapping, q, positions, cos_sin, q_out)
+    _same_device(k, v, k_cache, v_cache, slot_mapping, q, positions, cos_sin, q_out, k_scales, v_scales)
     if _elsewhere(k):
         with torch.cuda.device(k.device):
             return append_paged_kv(k, v, k_cache, v_cache, slot_mapping, q=q, positions=positions,
-                                   cos_sin=cos_sin, interleaved=interleaved, q_out=q_out)
+                                   cos_sin=cos_sin, interleaved=interleaved, q_out=q_out, k_scales=k_scales,
+                                   v_scales=v_scales)
     ret = None
     ins = (q, k, v)
     if q is not None:
@@ -327,17 +367,20 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
         positions = positions.contiguous()
         cs = (positions.data_ptr(), int(positions.dtype == torch.int64), cos_sin.data_ptr(),
               _lib.dtype_code(cos_sin), cos_sin.stride(0), cos_sin.shape[0])
-    _lib.call("hmx_append_paged_kv", _lib.ptr(q), qts, qhs, k.data_ptr(), kts, khs,
-              v.data_ptr(), vts, vhs, _lib.dtype_code(k), None if q is None else ret.data_ptr(),
-              ots, ohs, _lib.paged_kv(k_cache, v_cache), slot_mapping.data_ptr(),
-              int(slot_mapping.dtype == torch.int64), *cs, R, int(bool(interleaved)), T, H, HKV,
-              D, _lib.stream_of(k))
+    _paged_call("hmx_append_paged_kv",
+                (_lib.ptr(q), qts, qhs, k.data_ptr(), kts, khs, v.data_ptr(), vts, vhs, _lib.dtype_code(k),
+                 None if q is None else ret.data_ptr(), ots, ohs),
+                _lib.paged_kv(k_cache, v_cache), k_scales, v_scales,
+                (slot_mapping.data_ptr(), int(slot_mapping.dtype == torch.int64), *cs, R, int(bool(interleaved)),
+                 T, H, HKV, D, _lib.stream_of(k)))
     return ret if q is None else _forward_only(what, ret, q_out, *ins)
 
 
 def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                            block_table: torch.Tensor, seq_lens: torch.Tensor,
-                           scale: float | None = None, *, out: torch.Tensor | None = None) -> torch.Tensor:
+                           scale: float | None = None, *, out: torch.Tensor | None = None,
+                           k_scales: torch.Tensor | None = None,
+                           v_scales: torch.Tensor | None = None) -> torch.Tensor:
     """softmax(scale q k^T) v of one token a sequence over its keys in the cache.
 
     q [N, H, D]; ``seq_lens`` [N] int32: keys of each sequence, the new token's among them
@@ -345,40 +388,99 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     row's pages counts as all of them.  ``block_table`` [N, width] int32; a page outside
     the cache holds no keys.  A value that is not finite makes its column of its sequence's
     rows infinite or NaN.  Returns [N, H, D] in q's type (``out``, which may not overlap an
-    input)."""
+    input).  ``k_scales``, ``v_scales``: of a cache of 8 bits."""
     what = "paged_attention_decode"
     _refuse_tangents(what, q, k_cache, v_cache)
     if q.dim() != 3:
         raise ValueError(f"{what}: q [N, H, D], got {tuple(q.shape)}")
     N, H, D = q.shape
-    _cache(what, q, k_cache, v_cache)
+    _cache(what, q, k_cache, v_cache, None, k_scales, v_scales)
     HKV = k_cache.shape[2]
     if H == 0 or H % HKV != 0:
         raise ValueError(f"{what}: {H} heads cannot share {HKV}")
     _table(what, block_table, seq_lens, N)
     scale = _scale(scale, D)
     o = _out(out, q)
-    _same_device(q, k_cache, v_cache, block_table, seq_lens, o)
+    _same_device(q, k_cache, v_cache, block_table, seq_lens, o, k_scales, v_scales)
     ins = (q, k_cache, v_cache)
     if N == 0:
         return _forward_only(what, o, out, *ins)
     if _elsewhere(q):
         with torch.cuda.device(q.device):
-            return paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, scale, out=out)
+            return paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, scale, out=out,
+                                          k_scales=k_scales, v_scales=v_scales)
     q, qts, qhs = _rows(q)
     ots, ohs = _places(o)
     ws, ws_bytes = _workspace("hmx_paged_attention_decode_workspace_bytes", q, N, H, HKV, D,
                               block_table.shape[1] * k_cache.shape[1])
-    _lib.call("hmx_paged_attention_decode", q.data_ptr(), qts, qhs, _lib.dtype_code(q),
-              o.data_ptr(), ots, ohs, _lib.paged_kv(k_cache, v_cache, block_table, seq_lens),
-              N, H, HKV, D, scale, _lib.ptr(ws), ws_bytes, _lib.stream_of(q))
+    _paged_call("hmx_paged_attention_decode",
+                (q.data_ptr(), qts, qhs, _lib.dtype_code(q), o.data_ptr(), ots, ohs),
+                _lib.paged_kv(k_cache, v_cache, block_table, seq_lens), k_scales, v_scales,
+                (N, H, HKV, D, scale, _lib.ptr(ws), ws_bytes, _lib.stream_of(q)))
+    return _forward_only(what, o, out, *ins)
+
+
+def shared_prefix_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                                   block_table: torch.Tensor, seq_lens: torch.Tensor,
+                                   prefix_table: torch.Tensor, prefix_lens: torch.Tensor,
+                                   cu_prefix: torch.Tensor | None = None, scale: float | None = None, *,
+                                   out: torch.Tensor | None = None, k_scales: torch.Tensor | None = None,
+                                   v_scales: torch.Tensor | None = None) -> torch.Tensor:
+    """paged_attention_decode of sequences that share prefixes, each prefix read once for all
+    sequences behind it.
+
+    ``prefix_table`` [M, width] and ``prefix_lens`` [M] int32: the pages and keys of M
+    prefixes; sequences cu_prefix[m] .. cu_prefix[m + 1] - 1 are behind prefix m
+    (``cu_prefix`` [M + 1], on the host or the device, the first need not be 0; without it M
+    is 1 and all are).  ``block_table`` [N, width] and ``seq_lens`` [N] list each sequence's
+    own keys only, behind the prefix's; where a serving engine's tables begin with the
+    prefix's whole pages, ``block_table[:, pages:]`` and ``seq_lens - pages * page_size`` are
+    they.  A sequence behind no prefix attends its own keys, one without own keys its
+    prefix's, and one without either gives 0.  The rest as in paged_attention_decode."""
+    what = "shared_prefix_attention_decode"
+    _refuse_tangents(what, q, k_cache, v_cache)
+    if q.dim() != 3:
+        raise ValueError(f"{what}: q [N, H, D], got {tuple(q.shape)}")
+    N, H, D = q.shape
+    _cache(what, q, k_cache, v_cache, None, k_scales, v_scales)
+    HKV = k_cache.shape[2]
+    if H == 0 or H % HKV != 0:
+        raise ValueError(f"{what}: {H} heads cannot share {HKV}")
+    _table(what, block_table, seq_lens, N)
+    M = prefix_table.shape[0] if prefix_table.dim() == 2 else 0
+    _table(what, prefix_table, prefix_lens, M, "prefix_table", "prefix_lens")
+    if (M != 1) if cu_prefix is None else (cu_prefix.dim() != 1 or cu_prefix.shape[0] != M + 1):
+        raise ValueError(f"{what}: cu_prefix [{M + 1}] for {M} prefixes, got "
+                         f"{None if cu_prefix is None else tuple(cu_prefix.shape)}")
+    scale = _scale(scale, D)
+    o = _out(out, q)
+    _same_device(q, k_cache, v_cache, block_table, seq_lens, prefix_table, prefix_lens, o, k_scales, v_scales)
+    if _elsewhere(q):
+        with torch.cuda.device(q.device):
+            return shared_prefix_attention_decode(q, k_cache, v_cache, block_table, seq_lens, prefix_table, prefix_lens,
+                                                  cu_prefix, scale, out=out, k_scales=k_scales, v_scales=v_scales)
+    cu = None if cu_prefix is None else _offsets(cu_prefix, N, q.device, any_first=True, name="cu_prefix")
+    ins = (q, k_cache, v_cache)
+    if N == 0:
+        return _forward_only(what, o, out, *ins)
+    q, qts, qhs = _rows(q)
+    ots, ohs = _places(o)
+    page = k_cache.shape[1]
+    ws, ws_bytes = _workspace("hmx_shared_prefix_decode_workspace_bytes", q, N, M, H, HKV, D,
+                              block_table.shape[1] * page, prefix_table.shape[1] * page)
+    _lib.call("hmx_shared_prefix_decode", q.data_ptr(), qts, qhs, _lib.dtype_code(q), o.data_ptr(), ots, ohs,
+              _lib.paged_kv(k_cache, v_cache, block_table, seq_lens),
+              None if k_scales is None else _lib.kv_scales(k_scales, v_scales), prefix_table.data_ptr(),
+              prefix_table.stride(0), prefix_table.shape[1], prefix_lens.data_ptr(), _lib.ptr(cu), N, M, H, HKV, D,
+              scale, _lib.ptr(ws), ws_bytes, _lib.stream_of(q))
     return _forward_only(what, o, out, *ins)
 
 
 def paged_causal_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                            block_table: torch.Tensor, seq_lens: torch.Tensor,
                            cu_seqlens: torch.Tensor, scale: float | None = None, *,
-                           out: torch.Tensor | None = None) -> torch.Tensor:
+                           out: torch.Tensor | None = None, k_scales: torch.Tensor | None = None,
+                           v_scales: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of new tokens that are the last of their sequences in the cache:
     prompts in pieces, prompts behind a cached prefix, draft tokens.
 
@@ -388,13 +490,14 @@ def paged_causal_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     keys, the new tokens' among them: token i of n attends keys 0 .. seq_len - n + i, and
     gives 0 where that is none.  Cache and table as in paged_attention_decode.  Returns
     [T, H, D] in q's type; rows of no sequence are 0, or left as they were in ``out`` (which
-    may not overlap an input)."""
+    may not overlap an input).  ``k_scales``, ``v_scales``: of a cache of 8 bits; with fp16 what
+    it holds past that type's range counts as its largest value."""
     what = "paged_causal_attention"
     _refuse_tangents(what, q, k_cache, v_cache)
     if q.dim() != 3:
         raise ValueError(f"{what}: q [T, H, D], got {tuple(q.shape)}")
     T, H, D = q.shape
-    _cache(what, q, k_cache, v_cache)
+    _cache(what, q, k_cache, v_cache, None, k_scales, v_scales)
     HKV = k_cache.shape[2]
     if H == 0 or H % HKV != 0:
         raise ValueError(f"{what}: {H} heads cannot share {HKV}")
@@ -402,11 +505,11 @@ def paged_causal_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     _table(what, block_table, seq_lens, N)
     scale = _scale(scale, D)
     o = _out(out, q)
-    _same_device(q, k_cache, v_cache, block_table, seq_lens, o)
+    _same_device(q, k_cache, v_cache, block_table, seq_lens, o, k_scales, v_scales)
     if _elsewhere(q):
         with torch.cuda.device(q.device):
             return paged_causal_attention(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens,
-                                          scale, out=out)
+                                          scale, out=out, k_scales=k_scales, v_scales=v_scales)
     cu = _offsets(cu_seqlens, T, q.device, any_first=True)
     ins = (q, k_cache, v_cache)
     if T == 0:
@@ -415,8 +518,8 @@ def paged_causal_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     ots, ohs = _places(o)
     ws, ws_bytes = _workspace("hmx_paged_causal_attention_workspace_bytes", q, N, T, H, HKV, D,
                               block_table.shape[1] * k_cache.shape[1])
-    _lib.call("hmx_paged_causal_attention", q.data_ptr(), qts, qhs, _lib.dtype_code(q),
-              o.data_ptr(), ots, ohs, _lib.paged_kv(k_cache, v_cache, block_table, seq_lens),
-              _lib.ptr(cu), N, T, H, HKV, D, scale, int(out is None), _lib.ptr(ws), ws_bytes,
-              _lib.stream_of(q))
+    _paged_call("hmx_paged_causal_attention",
+                (q.data_ptr(), qts, qhs, _lib.dtype_code(q), o.data_ptr(), ots, ohs),
+                _lib.paged_kv(k_cache, v_cache, block_table, seq_lens), k_scales, v_scales,
+                (_lib.ptr(cu), N, T, H, HKV, D, scale, int(out is None), _lib.ptr(ws), ws_bytes, _lib.stream_of(q)))
     return _forward_only(what, o, out, *ins)

@@ -825,6 +825,19 @@ typedef struct hmx_paged_kv {
 } hmx_paged_kv;
 
 /*
+ * The bytes of scale of a cache of 8 bits, whose k and v hold e4m3 values (strides in
+ * elements of one byte, multiples of 16): k and v [num_pages, HKV, page_size] with page and
+ * head strides, the places of a page contiguous.  A row stands for 2^(byte - 127) times its
+ * D values; bytes 1 .. 254.  A host pointer, read during the call.
+ */
+typedef struct hmx_kv_scales {
+  uint8_t* k;
+  int64_t k_page_stride, k_head_stride;
+  uint8_t* v;
+  int64_t v_page_stride, v_head_stride;
+} hmx_kv_scales;
+
+/*
  * Keys and values of new tokens into a paged cache, k (and q) rotated by their positions.
  *  k, v [tokens, HKV, D], q [tokens, H, D] or NULL, q_out as q (may be q); bf16 or fp16,
  *  D 64 or 128; token and head strides multiples of 8, pointers 16-byte aligned.
@@ -845,6 +858,22 @@ int hmx_append_paged_kv(const void* q, int64_t q_token_stride, int64_t q_head_st
                         const void* cos_sin, int32_t cos_sin_dtype, int64_t cos_sin_stride,
                         int64_t max_position, int32_t rotary_dim, int32_t interleaved,
                         int64_t tokens, int32_t H, int32_t HKV, int32_t D, void* stream);
+/*
+ * The same into a cache of 8 bits.  Of every row, k rotated in fp32 and not rounded before:
+ * byte - 127 is the least exponent >= -126 with max |x| <= 448 * 2^(byte - 127) over its
+ * finite elements, the values are x / 2^(byte - 127) to the nearest e4m3, ties to even.
+ * What is not finite is stored as NaN.
+ */
+int hmx_append_paged_kv8(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                         const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                         const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                         int32_t dtype, void* q_out, int64_t q_out_token_stride,
+                         int64_t q_out_head_stride, const hmx_paged_kv* cache,
+                         const hmx_kv_scales* scales, const void* slots,
+                         int32_t slots_int64, const void* positions, int32_t positions_int64,
+                         const void* cos_sin, int32_t cos_sin_dtype, int64_t cos_sin_stride,
+                         int64_t max_position, int32_t rotary_dim, int32_t interleaved,
+                         int64_t tokens, int32_t H, int32_t HKV, int32_t D, void* stream);
 
 /*
  * Attention of one new token a sequence: o[n] = softmax(scale q[n] . k_j) v_j over the
@@ -860,6 +889,33 @@ int hmx_paged_attention_decode(const void* q, int64_t q_token_stride, int64_t q_
                                int64_t o_head_stride, const hmx_paged_kv* cache, int32_t N,
                                int32_t H, int32_t HKV, int32_t D, float scale, void* workspace,
                                size_t workspace_bytes, void* stream);
+/* The same over a cache of 8 bits (q and o in 16); the same workspace. */
+int hmx_paged_attention_decode8(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                int32_t dtype, void* o, int64_t o_token_stride,
+                                int64_t o_head_stride, const hmx_paged_kv* cache,
+                                const hmx_kv_scales* scales, int32_t N,
+                                int32_t H, int32_t HKV, int32_t D, float scale, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
+/*
+ * Attention of one new token a sequence behind prefixes that groups of sequences share:
+ * sequences cu_prefix[m] .. cu_prefix[m + 1] - 1 (device offsets, clamped into 0 .. N;
+ * NULL: M = 1, all) attend the prefix_lens[m] keys that prefix_table's row m lists and, with
+ * them in one softmax, their own seq_lens[n] keys (cache->table), where a sequence of no
+ * group has its own alone and one without any key gives 0.  Both tables' pages lie in one
+ * cache, of 8 bits where scales is not NULL.  workspace as for the decode, max_keys and
+ * max_prefix the table widths times page_size.
+ */
+size_t hmx_shared_prefix_decode_workspace_bytes(int32_t N, int32_t M, int32_t H, int32_t HKV,
+                                                int32_t D, int64_t max_keys, int64_t max_prefix);
+int hmx_shared_prefix_decode(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                             int32_t dtype, void* o, int64_t o_token_stride,
+                             int64_t o_head_stride, const hmx_paged_kv* cache,
+                             const hmx_kv_scales* scales, const int32_t* prefix_table,
+                             int64_t prefix_table_stride, int32_t prefix_table_width,
+                             const int32_t* prefix_lens, const int32_t* cu_prefix, int32_t N,
+                             int32_t M, int32_t H, int32_t HKV, int32_t D, float scale,
+                             void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Causal attention over whole sequences: q, o [T, H, D], k, v [T, HKV, D]; N sequences at
@@ -912,6 +968,46 @@ int hmx_paged_causal_attention(const void* q, int64_t q_token_stride, int64_t q_
                                const int32_t* cu_seqlens, int32_t N, int64_t T, int32_t H,
                                int32_t HKV, int32_t D, float scale, int32_t fill_gaps,
                                void* workspace, size_t workspace_bytes, void* stream);
+
+/* The same over a cache of 8 bits (q and o in 16; with fp16, what the cache holds past that
+ * type's range counts as its largest value); the same workspace. */
+int hmx_paged_causal_attention8(const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                                int32_t dtype, void* o, int64_t o_token_stride,
+                                int64_t o_head_stride, const hmx_paged_kv* cache,
+                                const hmx_kv_scales* scales,
+                                const int32_t* cu_seqlens, int32_t N, int64_t T, int32_t H,
+                                int32_t HKV, int32_t D, float scale, int32_t fill_gaps,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The position rotation by frequencies: of the first rotary_dim elements of every head of
+ * x [B, T, heads, D] the pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) with interleaved, by
+ * positions[b, t] * inv_freq[i], times factor; the others are copied.  The angle is formed
+ * in 64 bits.  backward: by minus the angle, which is the gradient's rotation.  q and k are
+ * rotated alike into q_out and k_out (which may be q and k); k may be NULL.
+ *  bf16 or fp16, D 64 or 128, rotary_dim a multiple of 16; token t of sequence b lies at
+ *  b * batch stride + t * token stride; strides multiples of 8, pointers 16-byte aligned.
+ *  positions int64, or int32 where positions_int64 is 0, positions_stride apart for a
+ *  sequence (0: the same for all); inv_freq [rotary_dim / 2] fp64, or fp32 where
+ *  inv_freq_f64 is 0.
+ * No counterpart in the reference, whose attention layers are vLLM's own.
+ */
+int hmx_rotary_embedding(const void* q, int64_t q_batch_stride, int64_t q_token_stride,
+                         int64_t q_head_stride, void* q_out, int64_t q_out_batch_stride,
+                         int64_t q_out_token_stride, int64_t q_out_head_stride, const void* k,
+                         int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
+                         void* k_out, int64_t k_out_batch_stride, int64_t k_out_token_stride,
+                         int64_t k_out_head_stride, int32_t dtype, const void* positions,
+                         int32_t positions_int64, int64_t positions_stride, const void* inv_freq,
+                         int32_t inv_freq_f64, float factor, int32_t rotary_dim,
+                         int32_t interleaved, int32_t backward, int32_t B, int64_t T, int32_t H,
+                         int32_t HKV, int32_t D, void* stream);
+/*
+ * The table [positions, rotary_dim] fp32 that hmx_append_paged_kv reads, of positions 0 ..
+ * positions - 1: factor times cosines, then sines, from the same angles.
+ */
+int hmx_rotary_table(const void* inv_freq, int32_t inv_freq_f64, float factor,
+                     int64_t positions, int32_t rotary_dim, float* table, void* stream);
 
 #ifdef __cplusplus
 }

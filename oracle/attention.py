@@ -91,3 +91,42 @@ def rotate(x, cos_sin, positions, interleaved):
             u, w = x[t, :, a].clone(), x[t, :, b].clone()
             x[t, :, a], x[t, :, b] = u * c - w * s, w * c + u * s
     return x
+
+
+def to_e4m3(x):
+    """float64 values to the nearest of e4m3's (1 sign, 4 exponent and 3 mantissa bits, bias 7,
+    largest 448), ties to the even one; |x| <= 448."""
+    x = x.to(F64)
+    _, e = torch.frexp(x)                          # x = m 2^e, 1/2 <= |m| < 1
+    step = torch.ldexp(torch.ones_like(x), e.clamp(min=-5) - 4)
+    return torch.round(x / step) * step
+
+
+def quantise(x):
+    """(e4m3 values in float64, exponents) of rows x [..., D]: the least exponent e >= -126 with
+    max |x| <= 448 * 2^e over the finite elements; what is not finite becomes NaN."""
+    x = x.to(F64)
+    top = torch.where(torch.isfinite(x), x.abs(), torch.zeros_like(x)).amax(-1)
+    m, e = torch.frexp(top)
+    e = torch.where(top == 0, torch.full_like(e, -126), e - 9 + (m > 0.875)).clamp(min=-126)
+    y = torch.where(torch.isfinite(x), x, torch.full_like(x, torch.nan))
+    return to_e4m3(torch.ldexp(y, -e[..., None])), e
+
+
+def behind_prefix(q, pk, pv, k, v, scale):
+    """One token's q [H, D] over a prefix pk, pv [P, HKV, D] and keys k, v of its own: (o, a) of
+    rows() over both."""
+    k, v = torch.cat([pk, k]), torch.cat([pv, v])
+    o, a = rows(q[None], k, v, scale, k.shape[0] - 1)
+    return o[0], a[0]
+
+
+def rotate_by(x, angles, factor, interleaved):
+    """x [..., heads, D] with its first pairs turned by angles [..., R / 2] and multiplied by factor."""
+    x = x.to(F64).clone()
+    h = angles.shape[-1]
+    c, s = factor * torch.cos(angles)[..., None, :], factor * torch.sin(angles)[..., None, :]
+    a, b = (slice(0, 2 * h, 2), slice(1, 2 * h, 2)) if interleaved else (slice(0, h), slice(h, 2 * h))
+    u, w = x[..., a].clone(), x[..., b].clone()
+    x[..., a], x[..., b] = u * c - w * s, w * c + u * s
+    return x

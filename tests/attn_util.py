@@ -58,8 +58,25 @@ def paged(gen, lens, page, HKV, D, dtype, spare=3, width=None, fill=float("nan")
     return kc, vc, table, ks, vs
 
 
+def paged8(gen, lens, page, HKV, D, grow=1.0, **kw):
+    """(k_cache, v_cache, k_scales, v_scales, table, k list, v list) in 8 bits, the lists what
+    the cache stands for in float64: rows of magnitudes up to 2^grow apart; what is no key of
+    a sequence is NaN in both values and scales (255)."""
+    kc, vc, table, ks, vs = paged(gen, lens, page, HKV, D, torch.bfloat16, **kw)
+    caches, scales, lists = [], [], []
+    for c in (kc, vc):
+        c = c.double() * torch.exp2((torch.rand(*c.shape[:3], 1, generator=gen) * grow).round())
+        values, e = ref.quantise(c)
+        none = torch.isnan(values).all(-1)
+        caches.append(values.to(torch.float8_e4m3fn))
+        scales.append(torch.where(none, torch.full_like(e, 255), e + 127).to(torch.uint8).transpose(1, 2).contiguous())
+        whole = torch.ldexp(values, e[..., None])
+        lists.append([ref.gather(whole, t, n) for t, n in zip(table, lens)])
+    return *caches, *scales, table, *lists
+
+
 def bounds_of(cu):
     return list(zip(cu, cu[1:]))
 
 
-__all__ = ["ref", "randn", "half_step", "o_tolerance", "check_o", "paged", "bounds_of"]
+__all__ = ["ref", "randn", "half_step", "o_tolerance", "check_o", "paged", "paged8", "bounds_of"]
