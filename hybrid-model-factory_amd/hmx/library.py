@@ -10,8 +10,9 @@ kernels are forward-only, so a backward through them raises NotImplementedError
 instead of silently returning no gradient.  The in-place decode ops declare their
 mutations; torch refuses autograd through them by itself.  The training GKA op
 with its backward is the autograd function behind ``hmx.gka_chebyshev_gla`` and
-``hmx.ChebyshevIteration`` (hmx.ops.gka_train).  ``causal_attention`` is differentiable
-here too: its backward is a registered op of its own.
+``hmx.ChebyshevIteration`` (hmx.ops.gka_train).  ``causal_attention`` and ``rotary_embedding``
+are differentiable here too: the first's backward is a registered op of its own, the second's
+is the op itself.  The ops over a cache of 8 bits are registered beside those in 16.
 
 ``torch.ops.hmx.<name>`` is the registered op; the functions of the same name
 in this module wrap it with the reference's Python signature (optional
@@ -393,6 +394,101 @@ def _(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale):
 _forward_only(_paged_prompt, "paged_causal_attention")
 
 
+@torch.library.custom_op("hmx::append_paged_kv8", mutates_args=("k_cache", "v_cache", "k_scales", "v_scales"))
+def _append8(k: Tensor, v: Tensor, k_cache: Tensor, v_cache: Tensor, k_scales: Tensor, v_scales: Tensor,
+             slot_mapping: Tensor, q: Optional[Tensor], positions: Optional[Tensor],
+             cos_sin: Optional[Tensor], interleaved: bool) -> Tensor:
+    out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ops.append_paged_kv(k, v, k_cache, v_cache, slot_mapping, q=q, positions=positions,
+                        cos_sin=cos_sin, interleaved=interleaved, q_out=out, k_scales=k_scales,
+                        v_scales=v_scales)
+    return k.new_empty(0) if q is None else out
+
+
+@_append8.register_fake
+def _(k, v, k_cache, v_cache, k_scales, v_scales, slot_mapping, q, positions, cos_sin, interleaved):
+    return k.new_empty(0) if q is None else q.new_empty(q.shape)
+
+
+@torch.library.custom_op("hmx::paged_attention_decode8", mutates_args=())
+def _paged_decode8(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_scales: Tensor, v_scales: Tensor,
+                   block_table: Tensor, seq_lens: Tensor, scale: Optional[float]) -> Tensor:
+    return ops.paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, scale,
+                                      k_scales=k_scales, v_scales=v_scales)
+
+
+@_paged_decode8.register_fake
+def _(q, k_cache, v_cache, k_scales, v_scales, block_table, seq_lens, scale):
+    return q.new_empty(q.shape)
+
+
+_forward_only(_paged_decode8, "paged_attention_decode")
+
+
+@torch.library.custom_op("hmx::paged_causal_attention8", mutates_args=())
+def _paged_prompt8(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_scales: Tensor, v_scales: Tensor,
+                   block_table: Tensor, seq_lens: Tensor, cu_seqlens: Tensor,
+                   scale: Optional[float]) -> Tensor:
+    return ops.paged_causal_attention(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale,
+                                      k_scales=k_scales, v_scales=v_scales)
+
+
+@_paged_prompt8.register_fake
+def _(q, k_cache, v_cache, k_scales, v_scales, block_table, seq_lens, cu_seqlens, scale):
+    return q.new_empty(q.shape)
+
+
+_forward_only(_paged_prompt8, "paged_causal_attention")
+
+
+@torch.library.custom_op("hmx::shared_prefix_attention_decode", mutates_args=())
+def _shared(q: Tensor, k_cache: Tensor, v_cache: Tensor, k_scales: Optional[Tensor], v_scales: Optional[Tensor],
+            block_table: Tensor, seq_lens: Tensor, prefix_table: Tensor, prefix_lens: Tensor,
+            cu_prefix: Optional[Tensor], scale: Optional[float]) -> Tensor:
+    return ops.shared_prefix_attention_decode(q, k_cache, v_cache, block_table, seq_lens, prefix_table,
+                                              prefix_lens, cu_prefix, scale, k_scales=k_scales,
+                                              v_scales=v_scales)
+
+
+@_shared.register_fake
+def _(q, k_cache, v_cache, k_scales, v_scales, block_table, seq_lens, prefix_table, prefix_lens, cu_prefix, scale):
+    return q.new_empty(q.shape)
+
+
+_forward_only(_shared, "shared_prefix_attention_decode")
+
+
+@torch.library.custom_op("hmx::rotary_embedding", mutates_args=())
+def _rotary(q: Tensor, k: Optional[Tensor], positions: Tensor, inv_freq: Tensor, factor: float,
+            interleaved: bool, backward: bool) -> tuple[Tensor, Tensor]:
+    # backward: by minus the angle, which minus the positions are
+    with torch.no_grad():
+        a, b = ops.rotary_embedding(q, k, -positions if backward else positions, inv_freq, factor=factor,
+                                    interleaved=interleaved)
+    return a, q.new_empty(0) if b is None else b
+
+
+@_rotary.register_fake
+def _(q, k, positions, inv_freq, factor, interleaved, backward):
+    return q.new_empty(q.shape), q.new_empty(0) if k is None else k.new_empty(k.shape)
+
+
+def _rotary_setup(ctx, inputs, output):
+    _, k, positions, inv_freq, *ctx.args, ctx.back = inputs
+    ctx.has_k = k is not None
+    ctx.save_for_backward(positions, inv_freq)
+
+
+def _rotary_grad(ctx, dq, dk):
+    positions, inv_freq = ctx.saved_tensors
+    dq, dk = torch.ops.hmx.rotary_embedding(dq, dk if ctx.has_k else None, positions, inv_freq, *ctx.args,
+                                            not ctx.back)
+    return dq, dk if ctx.has_k else None, None, None, None, None, None
+
+
+_rotary.register_autograd(_rotary_grad, setup_context=_rotary_setup)
+
+
 # ------------------------------------------------------- reference-signature wrappers
 def chunk_gated_delta_rule_gqa(q, k, v, g, beta, scale=None, initial_state=None,
                                output_final_state=False, cu_seqlens=None,
@@ -525,27 +621,53 @@ def causal_attention(q, k, v, scale=None, cu_seqlens=None):
 
 
 def append_paged_kv(k, v, k_cache, v_cache, slot_mapping, *, q=None, positions=None, cos_sin=None,
-                    interleaved=False):
-    """``torch.ops.hmx.append_paged_kv``; the caches are written in place, q (None without
-    one) is returned rotated."""
-    out = torch.ops.hmx.append_paged_kv(k, v, k_cache, v_cache, slot_mapping, q, positions, cos_sin,
-                                        bool(interleaved))
+                    interleaved=False, k_scales=None, v_scales=None):
+    """``torch.ops.hmx.append_paged_kv``, or ``append_paged_kv8`` where the cache is of 8 bits; the
+    caches are written in place, q (None without one) is returned rotated."""
+    if k_scales is not None:
+        out = torch.ops.hmx.append_paged_kv8(k, v, k_cache, v_cache, k_scales, v_scales, slot_mapping, q,
+                                             positions, cos_sin, bool(interleaved))
+    else:
+        out = torch.ops.hmx.append_paged_kv(k, v, k_cache, v_cache, slot_mapping, q, positions, cos_sin,
+                                            bool(interleaved))
     return None if q is None else out
 
 
-def paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, scale=None):
-    """``torch.ops.hmx.paged_attention_decode``."""
+def paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, scale=None, *, k_scales=None,
+                           v_scales=None):
+    """``torch.ops.hmx.paged_attention_decode``, or ``paged_attention_decode8``."""
+    if k_scales is not None:
+        return torch.ops.hmx.paged_attention_decode8(q, k_cache, v_cache, k_scales, v_scales, block_table,
+                                                     seq_lens, scale)
     return torch.ops.hmx.paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, scale)
 
 
-def paged_causal_attention(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale=None):
-    """``torch.ops.hmx.paged_causal_attention``."""
+def paged_causal_attention(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale=None, *,
+                           k_scales=None, v_scales=None):
+    """``torch.ops.hmx.paged_causal_attention``, or ``paged_causal_attention8``."""
+    if k_scales is not None:
+        return torch.ops.hmx.paged_causal_attention8(q, k_cache, v_cache, k_scales, v_scales, block_table,
+                                                     seq_lens, cu_seqlens, scale)
     return torch.ops.hmx.paged_causal_attention(q, k_cache, v_cache, block_table, seq_lens,
                                                 cu_seqlens, scale)
+
+
+def shared_prefix_attention_decode(q, k_cache, v_cache, block_table, seq_lens, prefix_table, prefix_lens,
+                                   cu_prefix=None, scale=None, *, k_scales=None, v_scales=None):
+    """``torch.ops.hmx.shared_prefix_attention_decode``."""
+    return torch.ops.hmx.shared_prefix_attention_decode(q, k_cache, v_cache, k_scales, v_scales, block_table,
+                                                        seq_lens, prefix_table, prefix_lens, cu_prefix, scale)
+
+
+def rotary_embedding(q, k, positions, inv_freq, *, factor=1.0, interleaved=False):
+    """``torch.ops.hmx.rotary_embedding``: both rotated (None without k), differentiable."""
+    a, b = torch.ops.hmx.rotary_embedding(q, k, positions, inv_freq, float(factor), bool(interleaved), False)
+    return a, None if k is None else b
 
 
 __all__ = ["chunk_gated_delta_rule_gqa", "fused_recurrent_gated_delta_rule_gqa",
            "gka_chebyshev_gla_prefill", "gka_chebyshev_gla_decode",
            "mamba_chunk_scan_combined_varlen", "selective_state_update", "causal_conv1d_fn",
            "causal_conv1d_update", "rms_norm_gated", "causal_attention", "append_paged_kv",
-           "paged_attention_decode", "paged_causal_attention"]
+           "paged_attention_decode", "paged_causal_attention", "shared_prefix_attention_decode",
+           "rotary_embedding"]

@@ -457,7 +457,8 @@ def mamba2_conv_ssm_forward(layer, projected_states: torch.Tensor, output: torch
 
 def attention_forward_core(layer, qkv: torch.Tensor, positions: torch.Tensor | None,
                            core_attn_out: torch.Tensor, attn_metadata, k_cache: torch.Tensor,
-                           v_cache: torch.Tensor) -> None:
+                           v_cache: torch.Tensor, k_scales: torch.Tensor | None = None,
+                           v_scales: torch.Tensor | None = None) -> None:
     """The attention layer of a hybrid model over a paged cache, as the mixer cores above
     run theirs: the position rotation and the append in one launch, then the batch's decodes
     (first, one token each) and its prefills, each written into ``core_attn_out`` in place.
@@ -472,7 +473,13 @@ def attention_forward_core(layer, qkv: torch.Tensor, positions: torch.Tensor | N
     step's tokens among them), block_table [N, width], slot_mapping [tokens]; int32 on the
     device (slot_mapping int64 too), and nothing is read back.  Where decodes carry draft
     tokens (num_decode_tokens > num_decodes) all requests go through the prefill form.  Rows
-    past num_actual_tokens are left as they were."""
+    past num_actual_tokens are left as they were.
+
+    ``k_scales``, ``v_scales`` [pages, HKV, page size]: of a cache of 8 bits.  Where the metadata
+    has a prefix_table (not None), with prefix_lens and cu_prefix (None: one prefix for all),
+    the decodes share prefixes: their rows of block_table and seq_lens are then of their own
+    keys, behind the prefix's (hmx.shared_prefix_attention_decode), the prefills' whole as
+    ever.  Not together with draft tokens."""
     md = attn_metadata
     if md is None:
         return
@@ -482,6 +489,10 @@ def attention_forward_core(layer, qkv: torch.Tensor, positions: torch.Tensor | N
     if qkv.shape[-1] != sum(heads) * D:
         raise ValueError(f"qkv rows of {qkv.shape[-1]} are not those of {H} heads and 2 x {HKV} key/value heads of {D} "
                          f"({layer.num_heads} and {layer.num_kv_heads} over {tp} ranks)")
+    prefix = getattr(md, "prefix_table", None)
+    if prefix is not None and md.num_decode_tokens != md.num_decodes:
+        raise NotImplementedError("shared prefixes together with draft tokens are not implemented")
+    eight = {} if k_scales is None and v_scales is None else {"k_scales": k_scales, "v_scales": v_scales}
     qkv = _cut(qkv, 0, n)
     q, k, v = (x.view(n, h, D) for h, x in zip(heads, qkv.split([h * D for h in heads], dim=-1)))
     rope = getattr(layer, "rotary_emb", None)
@@ -490,20 +501,24 @@ def attention_forward_core(layer, qkv: torch.Tensor, positions: torch.Tensor | N
             raise ValueError("rotary_emb needs the tokens' positions")
         q = ops.append_paged_kv(k, v, k_cache, v_cache, md.slot_mapping[:n], q=q,
                                 positions=positions[:n], cos_sin=rope.cos_sin_cache,
-                                interleaved=not rope.is_neox_style)
+                                interleaved=not rope.is_neox_style, **eight)
     else:
-        ops.append_paged_kv(k, v, k_cache, v_cache, md.slot_mapping[:n])
+        ops.append_paged_kv(k, v, k_cache, v_cache, md.slot_mapping[:n], **eight)
     scale = getattr(layer, "scaling", None)
     nd, npf = md.num_decodes, md.num_prefills
-    if md.num_decode_tokens != nd:
+    if nd > 0 and prefix is not None:
+        ops.shared_prefix_attention_decode(q[:nd], k_cache, v_cache, md.block_table[:nd], md.seq_lens[:nd],
+                                           prefix, md.prefix_lens, getattr(md, "cu_prefix", None), scale,
+                                           out=core_attn_out[:nd], **eight)
+    elif md.num_decode_tokens != nd:
         nd, npf = 0, nd + npf
-    if nd > 0:
+    elif nd > 0:
         ops.paged_attention_decode(q[:nd], k_cache, v_cache, md.block_table[:nd], md.seq_lens[:nd],
-                                   scale, out=core_attn_out[:nd])
+                                   scale, out=core_attn_out[:nd], **eight)
     if npf > 0:
         ops.paged_causal_attention(q, k_cache, v_cache, md.block_table[nd:nd + npf],
                                    md.seq_lens[nd:nd + npf], md.query_start_loc[nd:nd + npf + 1],
-                                   scale, out=core_attn_out[:n])
+                                   scale, out=core_attn_out[:n], **eight)
 
 
 def _mamba2_prefill_blocks(layer, md, hbc, dt, x, out, idx_p, lc_p, ls_p, conv_state, ssm_state,
