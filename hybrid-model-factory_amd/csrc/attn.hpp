@@ -381,6 +381,26 @@ struct PrefixArgs {
   float scale;
   bool eight;                // a cache of 8 bits
 };
+// Few new tokens a sequence over a cache of 8 bits (attn_rows.hip).  few_rows: they are where
+// each sequence's rows fill a block of 16 on average; the blocks are then at most twice the
+// sequences however unequal they are, so no order of long sequences is read often.
+struct FewRows {
+  const void* q;
+  void* o;
+  int64_t q_ts, q_hs, o_ts, o_hs;   // elements
+  int32_t dtype;
+  Pages pages;
+  const int32_t* cu;
+  int32_t N, T, H, HKV, D;
+  int64_t max_keys;
+  float scale;
+  int32_t fill;
+  float* workspace;
+};
+bool few_rows(int64_t N, int64_t T, int64_t G);
+size_t few_rows_workspace_bytes(int64_t N, int64_t T, int32_t H, int32_t HKV, int32_t D, int64_t max_keys);
+void launch_few_rows(const FewRows& f, hipStream_t s);
+
 int prefix_splits(int64_t M, int64_t N, int H, int HKV, int64_t max_keys);
 void launch_prefix(const PrefixArgs& p, const PrefixShares& out, int64_t max_keys, hipStream_t s);
 

@@ -38,8 +38,7 @@ struct DecArgs {
   Pages pages;
   int32_t N, HKV, G, hblocks, W;    // hblocks: blocks of 16 heads of a group; W = 0: worker w takes sequence w
   float c;
-  float* part;   // [slots][HKV * hblocks][16][D], then [slots][HKV * hblocks][16][2]
-  int64_t slots; // two a worker; where all shares are kept, N more for the sequences that are not cut
+  float* part;   // [W][2][HKV * hblocks][16][D], then [W][2][HKV * hblocks][16][2]
 };
 
 __device__ __forceinline__ int seq_keys(const DecArgs& a, int n) {
@@ -86,8 +85,7 @@ __device__ __forceinline__ int64_t units_per(const DecArgs& a, int64_t total) {
   return per < MIN_UNITS ? MIN_UNITS : per;
 }
 
-// SHARES: every sequence leaves its share, to be joined with those of the keys before its own.
-template <typename T, int D, bool SHARES = false>
+template <typename T, int D>
 __global__ __launch_bounds__(64 * NW) void attn_decode_kernel(DecArgs a) {
   typedef typename El<T>::v8 v8;
   typedef typename El<T>::v4 v4;
@@ -106,7 +104,6 @@ __global__ __launch_bounds__(64 * NW) void attn_decode_kernel(DecArgs a) {
   const int ng = min(16, a.G - g0);
 
   auto zero_row = [&](int n) {
-    if constexpr (SHARES) return;
     for (int i = tid; i < ng * (D / 8); i += 64 * NW)
       *reinterpret_cast<u32x4*>(a.o + (int64_t)n * a.o_ts + (int64_t)(kvh * a.G + g0 + i / (D / 8)) * a.o_hs +
                                 16 * (i % (D / 8))) = u32x4{0, 0, 0, 0};
@@ -278,10 +275,9 @@ __global__ __launch_bounds__(64 * NW) void attn_decode_kernel(DecArgs a) {
     __syncthreads();
     const bool whole = k_beg == 0 && k_end == keys;
     const int piece = u_beg < first ? 1 : 0;
-    const int64_t at = SHARES && whole ? (int64_t)a.W * 2 + seq : (int64_t)w * 2 + piece;
-    const int64_t slot = at * a.HKV * a.hblocks + hb;
+    const int64_t slot = ((int64_t)w * 2 + piece) * a.HKV * a.hblocks + hb;
     float* pp = a.part + slot * 16 * D;
-    float* pm = a.part + a.slots * a.HKV * a.hblocks * 16 * D + slot * 32;
+    float* pm = a.part + (int64_t)a.W * 2 * a.HKV * a.hblocks * 16 * D + slot * 32;
     for (int i = tid; i < ng * (D / 4); i += 64 * NW) {
       const int g = i / (D / 4), d = 4 * (i % (D / 4));
       float mm = NEG_INF, ll = 0.f;
@@ -293,289 +289,7 @@ __global__ __launch_bounds__(64 * NW) void attn_decode_kernel(DecArgs a) {
         ll += f * s_ml[x][g][1];
         o += f * *reinterpret_cast<const f32x4*>(ob + (x * 16 + g) * D + d);
       }
-      if (whole && !SHARES) {
-        const float inv = ll == 0.f ? 0.f : 1.f / ll;
-        typename El<T>::v4 y;
-#pragma unroll
-        for (int z = 0; z < 4; ++z) y[z] = (T)(o[z] * inv);
-        *reinterpret_cast<typename El<T>::v4*>(a.o + (int64_t)seq * a.o_ts +
-                                               (int64_t)(kvh * a.G + g0 + g) * a.o_hs + 2 * d) = y;
-      } else {
-        *reinterpret_cast<f32x4*>(pp + g * D + d) = o;
-        if (d == 0) {
-          pm[2 * g] = mm;
-          pm[2 * g + 1] = ll;
-        }
-      }
-    }
-    __syncthreads();
-    u = stop;
-    first += units;
-    ++seq;
-  }
-}
-
-// The same over a cache of 8 bits.  A wave's turn is 32 keys, the bytes of 16 in 16 bits, and
-// their bytes of scale.  A lane widens its fragments of K and V (every e4m3 value is a bf16
-// and an fp16 value) where they are read; a key's scale multiplies its scores, and the
-// probabilities before their product with V, both in fp32, so neither type's range matters.
-// V's fragments come from the transposing read of bytes: eight keys of one column, the first
-// four of the lane group's from the first sixteen keys and four from the second, the order in
-// which the two tiles of scores hold them.
-template <int D> __device__ __forceinline__ int swz8k(int r, int c) {   // rows read eight at a time at one chunk
-  return D == 128 ? c ^ (r & 7) : c ^ ((r >> 1) & 3);
-}
-template <int D> __device__ __forceinline__ int swz8v(int r, int c) {   // rows 4 i .. 4 i + 3 and 16 on at one chunk
-  return D == 128 ? c ^ ((r & 3) | (r >> 2 & 4)) : c ^ ((r >> 1 & 1) | (r >> 3 & 2));
-}
-__device__ __forceinline__ u32x2 tr8(const char* p) {
-  typedef int i32x2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(p)));
-}
-
-template <typename T, int D, bool SHARES = false>
-__global__ __launch_bounds__(64 * NW) void attn_decode8_kernel(DecArgs a) {
-  typedef typename El<T>::v8 v8;
-  constexpr int KT8 = 32;                    // keys of a wave's turn
-  constexpr int NP = D / 64, ND = D / 16, NC = D / 16;   // pairs of score steps, column tiles, 16-byte chunks of a row
-  constexpr int RI = 64 / NC, NL = KT8 / RI; // rows of a load, loads of K (and V) of a turn
-  constexpr int RING = D == 128 ? 4 : 8;     // turns
-  constexpr int KV = KT8 * D;                // bytes of a turn's K, and of its V behind it, then the scales
-  constexpr int TURN = 2 * KV + 256;
-  __shared__ __align__(1024) char smem[NW * RING * TURN];   // the rings, then the shares [16][D] in fp32
-  __shared__ float s_ml[NW][16][2];
-  __shared__ int64_t s_scan[8];
-
-  const int tid = threadIdx.x, lane = tid & 63, q4 = lane >> 4, l16 = lane & 15;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int hb = blockIdx.x % (a.HKV * a.hblocks), w = blockIdx.x / (a.HKV * a.hblocks);
-  const int kvh = hb % a.HKV, g0 = (hb / a.HKV) * 16;
-  const int ng = min(16, a.G - g0);
-
-  auto zero_row = [&](int n) {
-    if constexpr (SHARES) return;
-    for (int i = tid; i < ng * (D / 8); i += 64 * NW)
-      *reinterpret_cast<u32x4*>(a.o + (int64_t)n * a.o_ts + (int64_t)(kvh * a.G + g0 + i / (D / 8)) * a.o_hs +
-                                16 * (i % (D / 8))) = u32x4{0, 0, 0, 0};
-  };
-  int seq = __builtin_amdgcn_readfirstlane(w);
-  int64_t first = 0, u_beg = 0, u_end;
-  if (a.W == 0) {
-    u_end = (seq_keys(a, w) + UNIT - 1) / UNIT;
-    if (u_end == 0) zero_row(w);
-  } else {
-    // rows without keys, a worker every W-th sequence
-    for (int n = w; n < a.N; n += a.W)
-      if (seq_keys(a, n) == 0) zero_row(n);
-    const Place pl = find_share(a, w, s_scan);
-    u_beg = w * pl.per;
-    u_end = min(pl.total, u_beg + pl.per);
-    seq = __builtin_amdgcn_readfirstlane(pl.seq);
-    first = pl.first;
-  }
-  if (u_beg >= u_end) return;
-  int64_t u = u_beg;
-
-  char* ring = smem + wave * RING * TURN;
-  const uint32_t ring_at = lds_addr(ring);
-  int ko[NP], vo[ND];                       // the lane's byte offsets into a turn's K and V
-#pragma unroll
-  for (int p = 0; p < NP; ++p) ko[p] = l16 * D + swz8k<D>(l16, 4 * p + q4) * 16;   // (row 16 + l16: the same chunk)
-#pragma unroll
-  for (int d = 0; d < ND; ++d) {
-    const int i = l16 >> 1, r = 4 * q4 + (i & 3) + (i & 4) * 4;
-    vo[d] = KV + r * D + swz8v<D>(r, d) * 16 + 8 * (l16 & 1);
-  }
-  const char *kbase = a.pages.k + (int64_t)kvh * a.pages.k_hs, *vbase = a.pages.v + (int64_t)kvh * a.pages.v_hs;
-  // lanes 0 .. 31 bring the scales of the keys, 32 .. 63 of the values
-  const uint8_t* sbase = lane < 32 ? a.pages.k_sc + kvh * a.pages.k_sc_hs : a.pages.v_sc + kvh * a.pages.v_sc_hs;
-  const int64_t sps = lane < 32 ? a.pages.k_sc_ps : a.pages.v_sc_ps;
-  const bool whole_pages = a.pages.page.d % 16 == 0;   // sixteen rows of a turn lie in one page
-
-  while (u < u_end) {
-    // this worker's share of sequence seq: keys k_beg .. k_end - 1
-    int keys = __builtin_amdgcn_readfirstlane(seq_keys(a, seq));
-    while (keys == 0) keys = __builtin_amdgcn_readfirstlane(seq_keys(a, ++seq));     // u < total: a sequence with keys follows
-    const int64_t units = (keys + UNIT - 1) / UNIT;
-    const int k_beg = __builtin_amdgcn_readfirstlane((int)(u - first) * UNIT);
-    const int64_t stop = min(u_end, first + units);
-    const int k_end = __builtin_amdgcn_readfirstlane(min(keys, (int)(stop - first) * UNIT));
-    const int32_t* table = a.pages.table + (int64_t)seq * a.pages.table_stride;
-
-    v8 qf[2 * NP];                          // step 2 p takes the first eight of the lane's sixteen, 2 p + 1 the others
-    {
-      const int hq = kvh * a.G + g0 + min(l16, ng - 1);
-      const char* qp = a.q + (int64_t)seq * a.q_ts + (int64_t)hq * a.q_hs + 32 * q4;
-#pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        qf[2 * p] = *reinterpret_cast<const v8*>(qp + 128 * p);
-        qf[2 * p + 1] = *reinterpret_cast<const v8*>(qp + 128 * p + 16);
-      }
-    }
-    f32x4 acc[ND];
-#pragma unroll
-    for (int d = 0; d < ND; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = NEG_INF, l = 0.f;
-
-    // turn x of the wave's: keys k_beg + (x NW + wave) KT8 ..; live: which of its rows are keys
-    const int turns = k_end - k_beg > wave * KT8 ? (k_end - k_beg - wave * KT8 + NW * KT8 - 1) / (NW * KT8) : 0;
-    uint32_t live[RING];
-    auto fetch = [&](int x) __attribute__((always_inline)) {
-      const int k0 = k_beg + (x * NW + wave) * KT8;
-      const uint32_t lds = ring_at + (x % RING) * TURN;
-      const int n = k_end - k0;
-      uint32_t mask = n >= KT8 ? ~0u : (1u << n) - 1;
-      if (whole_pages) {
-        // rows behind the last key are the page's own: what they hold is masked
-        const char *kb[2], *vb[2];
-        const uint8_t* sc[2];
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const int r = min(k0 + 16 * s, (k_end - 1) & ~15), p = __builtin_amdgcn_readfirstlane(fdiv(r, a.pages.page));
-          int64_t id = uniform_load(table, p);
-          if ((uint64_t)id >= (uint64_t)(int64_t)a.pages.num_pages) id = 0, mask &= ~(0xffffu << 16 * s);
-          const int64_t in = r - p * a.pages.page.d;
-          kb[s] = uniform_ptr(kbase + id * a.pages.k_ps + in * a.pages.k_ts);
-          vb[s] = uniform_ptr(vbase + id * a.pages.v_ps + in * a.pages.v_ts);
-          sc[s] = sbase + id * sps + in + l16;
-        }
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-          const int r = i * RI + lane / NC, c = lane % NC;
-          dma16(lds + i * 1024, kb[i * RI / 16], (uint32_t)((r & 15) * (int)a.pages.k_ts + 16 * swz8k<D>(r, c)));
-        }
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-          const int r = i * RI + lane / NC, c = lane % NC;
-          dma16(lds + KV + i * 1024, vb[i * RI / 16], (uint32_t)((r & 15) * (int)a.pages.v_ts + 16 * swz8v<D>(r, c)));
-        }
-        dma1(lds + 2 * KV, lane & 16 ? sc[1] : sc[0]);
-      } else {
-        int64_t in;
-        auto page_of = [&](int r) __attribute__((always_inline)) {   // of row r, -1 outside the cache, and its place
-          const int key = min(k0 + r, k_end - 1), p = fdiv(key, a.pages.page), id = table[p];
-          in = key - p * a.pages.page.d;
-          return (unsigned)id < (unsigned)a.pages.num_pages ? id : -1;
-        };
-        const int64_t mine = page_of(lane & 31);
-        mask &= (uint32_t)__ballot(mine >= 0);
-        const uint8_t* sc = sbase + max(mine, (int64_t)0) * sps + in;
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-          const int r = i * RI + lane / NC, c = lane % NC;
-          const int64_t id = max(page_of(r), 0);
-          dma16(lds + i * 1024, kbase + id * a.pages.k_ps + in * a.pages.k_ts + 16 * swz8k<D>(r, c));
-          dma16(lds + KV + i * 1024, vbase + id * a.pages.v_ps + in * a.pages.v_ts + 16 * swz8v<D>(r, c));
-        }
-        dma1(lds + 2 * KV, sc);
-      }
-      return mask;
-    };
-    // x is a multiple of RING plus the constant i: live[] stays in registers
-    auto turn = [&](int x, int i) __attribute__((always_inline)) {
-      if (x + RING - 2 < turns) dma_wait<(RING - 2) * (2 * NL + 1)>();
-      else dma_wait<0>();
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the turn before has been read
-      char* tile = ring + i * TURN;
-      const uint32_t mask = live[i];
-      if (x + RING - 1 < turns) live[(i + RING - 1) % RING] = fetch(x + RING - 1);
-      if (mask != ~0u) {
-        // V rows that are no keys, and their scales, to 0: their probability is 0, their memory anything
-#pragma unroll
-        for (int z = 0; z < NL; ++z)
-          if (!((mask >> (z * RI + lane / NC)) & 1))
-            *reinterpret_cast<u32x4*>(tile + KV + (z * 64 + lane) * 16) = u32x4{0, 0, 0, 0};
-        if (lane >= 32 && !((mask >> (lane - 32)) & 1)) *reinterpret_cast<uint32_t*>(tile + 2 * KV + 4 * lane) = 0;
-      }
-      f32x4 st[2];
-      u32x4 ks[2], vs[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        ks[t] = *reinterpret_cast<const u32x4*>(tile + 2 * KV + 64 * t + 16 * q4);
-        vs[t] = *reinterpret_cast<const u32x4*>(tile + 2 * KV + 128 + 64 * t + 16 * q4);
-        st[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int p = 0; p < NP; ++p) {
-          const u32x4 x = *reinterpret_cast<const u32x4*>(tile + 16 * t * D + ko[p]);
-          st[t] = El<T>::mma16(from_e4m3<T>(u32x2{x[0], x[1]}, 1.f), qf[2 * p], st[t]);
-          st[t] = El<T>::mma16(from_e4m3<T>(u32x2{x[2], x[3]}, 1.f), qf[2 * p + 1], st[t]);
-        }
-#pragma unroll
-        for (int z = 0; z < 4; ++z) st[t][z] *= scale_of(ks[t][z]);
-      }
-      if (mask != ~0u) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int z = 0; z < 4; ++z)
-            if (!((mask >> (16 * t + 4 * q4 + z)) & 1)) st[t][z] = NEG_INF;
-      }
-      float mx = fmaxf(fmaxf(fmaxf(st[0][0], st[0][1]), fmaxf(st[0][2], st[0][3])),
-                       fmaxf(fmaxf(st[1][0], st[1][1]), fmaxf(st[1][2], st[1][3])));
-      mx = q4_max(mx);
-      if (__any((mx - m) * a.c > 8.f)) {
-        const float mn = fmaxf(m, mx);
-        const float f = m == NEG_INF ? 0.f : __builtin_amdgcn_exp2f((m - mn) * a.c);
-        m = mn;
-        l *= f;
-#pragma unroll
-        for (int d = 0; d < ND; ++d) acc[d] *= f;
-      }
-      const float mc = m == NEG_INF ? 0.f : m * a.c;
-      bf16x8 pf, pr;                        // P times V's scales, and what its rounding leaves
-#pragma unroll
-      for (int z = 0; z < 8; ++z) {
-        const float p = __builtin_amdgcn_exp2f(st[z >> 2][z & 3] * a.c - mc);
-        l += p;
-        const float y = p * scale_of(vs[z >> 2][z & 3]);
-        pf[z] = (bf16)y;
-        pr[z] = (bf16)(y - (float)pf[z]);
-      }
-#pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        const bf16x8 v = from_e4m3<bf16>(tr8(tile + vo[d]), 1.f);
-        acc[d] = mfma16(v, pr, mfma16(v, pf, acc[d]));
-      }
-    };
-#pragma unroll
-    for (int i = 0; i < RING - 1; ++i)
-      if (i < turns) live[i] = fetch(i);
-    for (int x = 0; x < turns; x += RING) {
-#pragma unroll
-      for (int i = 0; i < RING; ++i)
-        if (x + i < turns) turn(x + i, i);
-    }
-    l = q4_sum(l);
-
-    // the waves' shares joined through LDS: O^T rows 16 d + 4 q4 + i, column l16
-    __syncthreads();
-    float* ob = reinterpret_cast<float*>(smem);       // [wave][16][D]
-#pragma unroll
-    for (int d = 0; d < ND; ++d)
-      *reinterpret_cast<f32x4*>(ob + (wave * 16 + l16) * D + 16 * d + 4 * q4) = acc[d];
-    if (q4 == 0) {
-      s_ml[wave][l16][0] = m * a.c;
-      s_ml[wave][l16][1] = l;
-    }
-    __syncthreads();
-    const bool whole = k_beg == 0 && k_end == keys;
-    const int piece = u_beg < first ? 1 : 0;
-    const int64_t at = SHARES && whole ? (int64_t)a.W * 2 + seq : (int64_t)w * 2 + piece;
-    const int64_t slot = at * a.HKV * a.hblocks + hb;
-    float* pp = a.part + slot * 16 * D;
-    float* pm = a.part + a.slots * a.HKV * a.hblocks * 16 * D + slot * 32;
-    for (int i = tid; i < ng * (D / 4); i += 64 * NW) {
-      const int g = i / (D / 4), d = 4 * (i % (D / 4));
-      float mm = NEG_INF, ll = 0.f;
-      for (int x = 0; x < NW; ++x) mm = fmaxf(mm, s_ml[x][g][0]);
-      const float ref = mm == NEG_INF ? 0.f : mm;
-      f32x4 o = {0.f, 0.f, 0.f, 0.f};
-      for (int x = 0; x < NW; ++x) {
-        const float f = __builtin_amdgcn_exp2f(s_ml[x][g][0] - ref);
-        ll += f * s_ml[x][g][1];
-        o += f * *reinterpret_cast<const f32x4*>(ob + (x * 16 + g) * D + d);
-      }
-      if (whole && !SHARES) {
+      if (whole) {
         const float inv = ll == 0.f ? 0.f : 1.f / ll;
         typename El<T>::v4 y;
 #pragma unroll
@@ -630,7 +344,7 @@ __global__ __launch_bounds__(256) void attn_decode_join_kernel(DecArgs a) {
   const int64_t per = units_per(a, total), last = before + (keys + UNIT - 1) / UNIT - 1;
   const int w0 = (int)(before / per), w1 = (int)(last / per);
   if (w0 == w1) return;
-  const int64_t hbs = (int64_t)a.HKV * a.hblocks, stats = a.slots * hbs * 16 * D;
+  const int64_t hbs = (int64_t)a.HKV * a.hblocks, stats = (int64_t)a.W * 2 * hbs * 16 * D;
   const int d = tid % TPS, sh = tid / TPS;
   float m = NEG_INF, l = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -667,87 +381,6 @@ __global__ __launch_bounds__(256) void attn_decode_join_kernel(DecArgs a) {
   }
 }
 
-// The shares of a sequence's own keys and of the prefix before them joined, as above; a
-// sequence without any keys gives 0.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void attn_shared_join_kernel(DecArgs a, PrefixShares pre) {
-  constexpr int TPS = D / 4, SH = 256 / TPS;
-  __shared__ int64_t s_scan[8];
-  __shared__ __align__(16) f32x4 s_o[SH][TPS];
-  __shared__ float s_ml[SH][2];
-  const int H = a.HKV * a.G, head = blockIdx.x % H, n = blockIdx.x / H;
-  const int kvh = head / a.G, g = head - kvh * a.G, hb = (g >> 4) * a.HKV + kvh;
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int keys = seq_keys(a, n);
-  int64_t before = 0, per = 1, w0 = 0, w1 = keys > 0 ? 0 : -1;   // workers w0 .. w1 have a share
-  if (a.W > 0 && keys > UNIT) {             // may be cut
-    int64_t total = 0;
-    for (int x = tid; x < a.N; x += 256) {
-      const int64_t u = (seq_keys(a, x) + UNIT - 1) / UNIT;
-      total += u;
-      if (x < n) before += u;
-    }
-    for (int d = 32; d >= 1; d >>= 1) {
-      before += __shfl_xor(before, d, 64);
-      total += __shfl_xor(total, d, 64);
-    }
-    if (lane == 0) {
-      s_scan[tid >> 6] = before;
-      s_scan[4 + (tid >> 6)] = total;
-    }
-    __syncthreads();
-    before = s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
-    total = s_scan[4] + s_scan[5] + s_scan[6] + s_scan[7];
-    per = units_per(a, total);
-    w0 = before / per;
-    w1 = (before + (keys + UNIT - 1) / UNIT - 1) / per;
-  }
-  const int64_t hbs = (int64_t)a.HKV * a.hblocks, stats = a.slots * hbs * 16 * D;
-  const int d = tid % TPS, sh = tid / TPS;
-  float m = NEG_INF, l = 0.f;
-  f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  auto add = [&](const float* row, const float* ml) __attribute__((always_inline)) {
-    const f32x4 x = *reinterpret_cast<const f32x4*>(row + 4 * d);
-    const float mn = fmaxf(m, ml[0]), ref = mn == NEG_INF ? 0.f : mn;
-    const float f = __builtin_amdgcn_exp2f(m - ref), e = __builtin_amdgcn_exp2f(ml[0] - ref);
-    l = l * f + ml[1] * e;
-    o = o * f + x * e;
-    m = mn;
-  };
-  for (int64_t w = w0 + sh; w <= w1; w += SH) {
-    const int64_t at = w0 == w1 ? (int64_t)a.W * 2 + n : w * 2 + (w * per < before ? 1 : 0);
-    const int64_t slot = at * hbs + hb;
-    add(a.part + (slot * 16 + (g & 15)) * D, a.part + stats + slot * 32 + 2 * (g & 15));
-  }
-  const int64_t r = (int64_t)n * H + head;
-  const float* pstats = pre.part + (int64_t)pre.splits * pre.rows * D;
-  for (int s = sh; s < pre.splits; s += SH) {
-    const float* ml = pstats + ((int64_t)s * pre.rows + r) * 2;
-    if (__builtin_bit_cast(uint32_t, pstats[2 * r]) == NO_SHARE || __builtin_bit_cast(uint32_t, ml[0]) == NO_SHARE) break;
-    add(pre.part + ((int64_t)s * pre.rows + r) * D, ml);
-  }
-  s_o[sh][d] = o;
-  if (d == 0) {
-    s_ml[sh][0] = m;
-    s_ml[sh][1] = l;
-  }
-  __syncthreads();
-  if (sh == 0) {
-    for (int i = 1; i < SH; ++i) {
-      const float mi = s_ml[i][0], mn = fmaxf(m, mi), ref = mn == NEG_INF ? 0.f : mn;
-      const float f = __builtin_amdgcn_exp2f(m - ref), e = __builtin_amdgcn_exp2f(mi - ref);
-      l = l * f + s_ml[i][1] * e;
-      o = o * f + s_o[i][d] * e;
-      m = mn;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    typename El<T>::v4 y;
-#pragma unroll
-    for (int z = 0; z < 4; ++z) y[z] = (T)(o[z] * inv);
-    *reinterpret_cast<typename El<T>::v4*>(a.o + (int64_t)n * a.o_ts + (int64_t)head * a.o_hs + 8 * d) = y;
-  }
-}
-
 // Workers: as many as there are compute units (a workgroup fills one's LDS), and no more than
 // the keys a table can hold give MIN_UNITS to.
 static int64_t workers(int64_t N, int64_t HKV, int64_t hblocks, int64_t max_keys) {
@@ -760,63 +393,12 @@ static int64_t workers(int64_t N, int64_t HKV, int64_t hblocks, int64_t max_keys
 }
 
 template <typename T, int D>
-static void launch(const DecArgs& a, bool eight, bool join, hipStream_t s) {
+static void launch(const DecArgs& a, bool join, hipStream_t s) {
   const unsigned hbs = (unsigned)(a.HKV * a.hblocks);
-  const dim3 grid(hbs * (unsigned)(a.W ? a.W : a.N));
-  if (eight) hipLaunchKernelGGL((attn_decode8_kernel<T, D>), grid, dim3(64 * NW), 0, s, a);
-  else hipLaunchKernelGGL((attn_decode_kernel<T, D>), grid, dim3(64 * NW), 0, s, a);
+  hipLaunchKernelGGL((attn_decode_kernel<T, D>), dim3(hbs * (unsigned)(a.W ? a.W : a.N)), dim3(64 * NW), 0, s, a);
   if (join)
     hipLaunchKernelGGL((attn_decode_join_kernel<T, D>), dim3((unsigned)(a.HKV * a.G * a.N)), dim3(256), 0, s, a);
 }
-
-template <typename T, int D>
-static void launch_shared(const DecArgs& a, bool eight, const PrefixShares& pre, hipStream_t s) {
-  const dim3 grid((unsigned)(a.HKV * a.hblocks) * (unsigned)(a.W ? a.W : a.N));
-  if (a.pages.width > 0) {                  // some sequence may have keys of its own
-    if (eight) hipLaunchKernelGGL((attn_decode8_kernel<T, D, true>), grid, dim3(64 * NW), 0, s, a);
-    else hipLaunchKernelGGL((attn_decode_kernel<T, D, true>), grid, dim3(64 * NW), 0, s, a);
-  }
-  hipLaunchKernelGGL((attn_shared_join_kernel<T, D>), dim3((unsigned)(a.HKV * a.G * a.N)), dim3(256), 0, s, a, pre);
-}
-
-// What both decodes check and hand on; the workspace and the launches are theirs.
-static int decode_args(const char* what, const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t dtype,
-                       void* o, int64_t o_token_stride, int64_t o_head_stride, const hmx_paged_kv* cache,
-                       const hmx_kv_scales* scales, int32_t N, int32_t H, int32_t HKV, int32_t D, float scale,
-                       DecArgs* out) {
-  HMX_REQUIRE(D == 64 || D == 128, HMX_EUNSUPPORTED, "%s: head size %d not in {64, 128}", what, D);
-  HMX_REQUIRE(dtype == HMX_BF16 || dtype == HMX_F16, HMX_EUNSUPPORTED, "%s: dtype code %d (bf16 or fp16)", what, dtype);
-  HMX_REQUIRE(N >= 0 && HKV > 0 && H > 0 && H % HKV == 0, HMX_EINVAL, "%s: N=%d H=%d HKV=%d", what, N, H, HKV);
-  HMX_REQUIRE(scale > 0.f && scale < __builtin_inff(), HMX_EINVAL, "%s: scale %g must be positive", what, (double)scale);
-  HMX_REQUIRE(cache && cache->num_pages >= 0 && cache->page_size > 0 && cache->table_width >= 0, HMX_EINVAL,
-              "%s: cache", what);
-  if (N == 0) return HMX_OK;
-  HMX_REQUIRE(q && o && cache->seq_lens && has_pages(*cache) && has_scales(*cache, scales), HMX_EINVAL,
-              "%s: null pointer", what);
-  const int64_t max_keys = (int64_t)cache->table_width * cache->page_size;
-  HMX_REQUIRE(max_keys < (1ll << 31) - 256, HMX_EUNSUPPORTED, "%s: a table row holds %lld keys", what,
-              (long long)max_keys);
-  const int64_t st = q_token_stride | q_head_stride | o_token_stride | o_head_stride;
-  const uintptr_t al = (uintptr_t)q | (uintptr_t)o;
-  HMX_REQUIRE(st % 8 == 0 && al % 16 == 0 && aligned_pages(*cache, scales != nullptr), HMX_EINVAL,
-              "%s: strides must be multiples of 8 elements (a cache's of 16 bytes) and pointers 16-byte aligned", what);
-  HMX_REQUIRE(near_rows(cache->k_token_stride) && near_rows(cache->v_token_stride), HMX_EUNSUPPORTED,
-              "%s: token strides of the cache past 2^25 elements", what);
-  HMX_REQUIRE((int64_t)N * H < (1ll << 31), HMX_EUNSUPPORTED, "%s: %d sequences of %d heads", what, N, H);
-  DecArgs& a = *out;
-  a.q = (const char*)q; a.o = (char*)o;
-  a.q_ts = 2 * q_token_stride; a.q_hs = 2 * q_head_stride;
-  a.o_ts = 2 * o_token_stride; a.o_hs = 2 * o_head_stride;
-  a.pages = make_pages(*cache, scales);
-  a.N = N; a.HKV = HKV; a.G = H / HKV; a.hblocks = (a.G + 15) / 16;
-  a.W = (int32_t)workers(N, HKV, a.hblocks, max_keys);
-  a.slots = 2ll * a.W;
-  a.c = scale * LOG2E;
-  return HMX_OK;
-}
-
-static size_t share_bytes(int64_t slots, int64_t hbs, int32_t D) { return (size_t)(slots * hbs * 16 * (D + 2)) * sizeof(float); }
-static size_t prefix_bytes(int64_t splits, int64_t rows, int32_t D) { return (size_t)(splits * rows * (D + 2)) * sizeof(float); }
 
 }  // namespace attn
 }  // namespace hmx
@@ -831,111 +413,58 @@ extern "C" size_t hmx_paged_attention_decode_workspace_bytes(int32_t N, int32_t 
   return (size_t)w * 2 * HKV * hb * 16 * (D + 2) * sizeof(float);
 }
 
-static int paged_attention_decode(const char* what, const void* q, int64_t q_token_stride, int64_t q_head_stride,
-                                  int32_t dtype, void* o, int64_t o_token_stride, int64_t o_head_stride,
-                                  const hmx_paged_kv* cache, const hmx_kv_scales* scales, int32_t N, int32_t H,
-                                  int32_t HKV, int32_t D, float scale, void* workspace, size_t workspace_bytes,
-                                  void* stream) {
-  attn::DecArgs a{};
-  const int rc = attn::decode_args(what, q, q_token_stride, q_head_stride, dtype, o, o_token_stride, o_head_stride,
-                                   cache, scales, N, H, HKV, D, scale, &a);
-  if (rc != HMX_OK || N == 0) return rc;
-  a.part = static_cast<float*>(workspace);
-  const bool join = a.W > 1;
-  HMX_REQUIRE(!join || (workspace && (uintptr_t)workspace % 16 == 0 &&
-                        workspace_bytes >= hmx_paged_attention_decode_workspace_bytes(
-                                               N, H, HKV, D, (int64_t)cache->table_width * cache->page_size)),
-              HMX_EINVAL, "%s: workspace of %zu bytes is too small", what, workspace_bytes);
-  hipStream_t s = (hipStream_t)stream;
-  if (dtype == HMX_BF16) {
-    if (D == 64) attn::launch<bf16, 64>(a, scales, join, s);
-    else attn::launch<bf16, 128>(a, scales, join, s);
-  } else {
-    if (D == 64) attn::launch<f16, 64>(a, scales, join, s);
-    else attn::launch<f16, 128>(a, scales, join, s);
-  }
-  return check_launch(what);
-}
-
 extern "C" int hmx_paged_attention_decode(const void* q, int64_t q_token_stride,
                                           int64_t q_head_stride, int32_t dtype, void* o,
                                           int64_t o_token_stride, int64_t o_head_stride,
                                           const hmx_paged_kv* cache, int32_t N, int32_t H,
                                           int32_t HKV, int32_t D, float scale, void* workspace,
                                           size_t workspace_bytes, void* stream) {
-  return paged_attention_decode("hmx_paged_attention_decode", q, q_token_stride, q_head_stride, dtype, o,
-                                o_token_stride, o_head_stride, cache, nullptr, N, H, HKV, D, scale, workspace,
-                                workspace_bytes, stream);
-}
-
-extern "C" int hmx_paged_attention_decode8(const void* q, int64_t q_token_stride,
-                                           int64_t q_head_stride, int32_t dtype, void* o,
-                                           int64_t o_token_stride, int64_t o_head_stride,
-                                           const hmx_paged_kv* cache, const hmx_kv_scales* scales,
-                                           int32_t N, int32_t H, int32_t HKV, int32_t D, float scale,
-                                           void* workspace, size_t workspace_bytes, void* stream) {
-  HMX_REQUIRE(scales, HMX_EINVAL, "hmx_paged_attention_decode8: no scales");
-  return paged_attention_decode("hmx_paged_attention_decode8", q, q_token_stride, q_head_stride, dtype, o,
-                                o_token_stride, o_head_stride, cache, scales, N, H, HKV, D, scale, workspace,
-                                workspace_bytes, stream);
-}
-
-extern "C" size_t hmx_shared_prefix_decode_workspace_bytes(int32_t N, int32_t M, int32_t H, int32_t HKV,
-                                                           int32_t D, int64_t max_keys,
-                                                           int64_t max_prefix) {
-  if (N <= 0 || M < 0 || HKV <= 0 || H <= 0 || H % HKV != 0) return 0;
-  const int64_t hb = (H / HKV + 15) / 16, w = attn::workers(N, HKV, hb, max_keys);
-  return attn::share_bytes(2 * w + N, HKV * hb, D) +
-         attn::prefix_bytes(M == 0 ? 1 : attn::prefix_splits(M, N, H, HKV, max_prefix), (int64_t)N * H, D);
-}
-
-extern "C" int hmx_shared_prefix_decode(const void* q, int64_t q_token_stride, int64_t q_head_stride,
-                                        int32_t dtype, void* o, int64_t o_token_stride,
-                                        int64_t o_head_stride, const hmx_paged_kv* cache,
-                                        const hmx_kv_scales* scales, const int32_t* prefix_table,
-                                        int64_t prefix_table_stride, int32_t prefix_table_width,
-                                        const int32_t* prefix_lens, const int32_t* cu_prefix, int32_t N,
-                                        int32_t M, int32_t H, int32_t HKV, int32_t D, float scale,
-                                        void* workspace, size_t workspace_bytes, void* stream) {
-  const char* what = "hmx_shared_prefix_decode";
-  attn::DecArgs a{};
-  const int rc = attn::decode_args(what, q, q_token_stride, q_head_stride, dtype, o, o_token_stride, o_head_stride,
-                                   cache, scales, N, H, HKV, D, scale, &a);
-  if (rc != HMX_OK) return rc;
-  HMX_REQUIRE(M >= 0 && prefix_table_width >= 0 && (cu_prefix || M == 1), HMX_EINVAL,
-              "%s: %d prefixes %s offsets, tables of %d pages", what, M, cu_prefix ? "with" : "without",
-              prefix_table_width);
+  HMX_REQUIRE(D == 64 || D == 128, HMX_EUNSUPPORTED,
+              "hmx_paged_attention_decode: head size %d not in {64, 128}", D);
+  HMX_REQUIRE(dtype == HMX_BF16 || dtype == HMX_F16, HMX_EUNSUPPORTED,
+              "hmx_paged_attention_decode: dtype code %d (bf16 or fp16)", dtype);
+  HMX_REQUIRE(N >= 0 && HKV > 0 && H > 0 && H % HKV == 0, HMX_EINVAL,
+              "hmx_paged_attention_decode: N=%d H=%d HKV=%d", N, H, HKV);
+  HMX_REQUIRE(scale > 0.f && scale < __builtin_inff(), HMX_EINVAL,
+              "hmx_paged_attention_decode: scale %g must be positive", (double)scale);
+  HMX_REQUIRE(cache && cache->num_pages >= 0 && cache->page_size > 0 && cache->table_width >= 0, HMX_EINVAL,
+              "hmx_paged_attention_decode: cache");
   if (N == 0) return HMX_OK;
-  hmx_paged_kv far = *cache;
-  far.table = prefix_table; far.table_stride = prefix_table_stride; far.table_width = prefix_table_width;
-  far.seq_lens = prefix_lens;
-  HMX_REQUIRE(M == 0 || (prefix_lens && attn::has_pages(far) && attn::has_scales(far, scales)), HMX_EINVAL,
-              "%s: null pointer", what);
+  HMX_REQUIRE(q && o && cache->seq_lens && attn::has_pages(*cache), HMX_EINVAL,
+              "hmx_paged_attention_decode: null pointer");
   const int64_t max_keys = (int64_t)cache->table_width * cache->page_size;
-  const int64_t max_prefix = (int64_t)prefix_table_width * cache->page_size;
-  HMX_REQUIRE(max_prefix < (1ll << 31) - 256, HMX_EUNSUPPORTED, "%s: a table row holds %lld keys", what,
-              (long long)max_prefix);
-  HMX_REQUIRE((int64_t)N * a.G < (1ll << 30) && ((int64_t)N * a.G / 128 + M + 2) * HKV < (1ll << 24), HMX_EUNSUPPORTED,
-              "%s: %d sequences of %d heads behind %d prefixes", what, N, H, M);
-  HMX_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0 &&
-                  workspace_bytes >= hmx_shared_prefix_decode_workspace_bytes(N, M, H, HKV, D, max_keys, max_prefix),
-              HMX_EINVAL, "%s: workspace of %zu bytes is too small", what, workspace_bytes);
-  a.slots += N;
+  HMX_REQUIRE(max_keys < (1ll << 31) - 256, HMX_EUNSUPPORTED,
+              "hmx_paged_attention_decode: a table row holds %lld keys", (long long)max_keys);
+  const int64_t st = q_token_stride | q_head_stride | o_token_stride | o_head_stride |
+                     cache->k_page_stride | cache->k_token_stride | cache->k_head_stride |
+                     cache->v_page_stride | cache->v_token_stride | cache->v_head_stride;
+  const uintptr_t al = (uintptr_t)q | (uintptr_t)o | (uintptr_t)cache->k | (uintptr_t)cache->v;
+  HMX_REQUIRE(st % 8 == 0 && al % 16 == 0, HMX_EINVAL,
+              "hmx_paged_attention_decode: strides must be multiples of 8 elements and pointers 16-byte aligned");
+  HMX_REQUIRE(attn::near_rows(cache->k_token_stride) && attn::near_rows(cache->v_token_stride), HMX_EUNSUPPORTED,
+              "hmx_paged_attention_decode: token strides of the cache past 2^25 elements");
+  attn::DecArgs a{};
+  a.q = (const char*)q; a.o = (char*)o;
+  a.q_ts = 2 * q_token_stride; a.q_hs = 2 * q_head_stride;
+  a.o_ts = 2 * o_token_stride; a.o_hs = 2 * o_head_stride;
+  a.pages = attn::make_pages(*cache);
+  a.N = N; a.HKV = HKV; a.G = H / HKV; a.hblocks = (a.G + 15) / 16;
+  a.W = (int32_t)attn::workers(N, HKV, a.hblocks, max_keys);
+  a.c = scale * attn::LOG2E;
   a.part = static_cast<float*>(workspace);
-  attn::PrefixShares pre{a.part + attn::share_bytes(a.slots, (int64_t)HKV * a.hblocks, D) / sizeof(float),
-                         (int64_t)N * H, M == 0 ? 0 : attn::prefix_splits(M, N, H, HKV, max_prefix)};
+  HMX_REQUIRE((int64_t)N * H < (1ll << 31), HMX_EUNSUPPORTED,
+              "hmx_paged_attention_decode: %d sequences of %d heads", N, H);
+  const bool join = a.W > 1;
+  HMX_REQUIRE(!join || (workspace && (uintptr_t)workspace % 16 == 0 &&
+                        workspace_bytes >= hmx_paged_attention_decode_workspace_bytes(N, H, HKV, D, max_keys)),
+              HMX_EINVAL, "hmx_paged_attention_decode: workspace of %zu bytes is too small", workspace_bytes);
   hipStream_t s = (hipStream_t)stream;
-  if (M > 0) {
-    const attn::PrefixArgs p{q, q_token_stride, q_head_stride, dtype, attn::make_pages(far, scales), cu_prefix,
-                             M, N, H, HKV, D, scale, scales != nullptr};
-    attn::launch_prefix(p, pre, max_prefix, s);
-  }
   if (dtype == HMX_BF16) {
-    if (D == 64) attn::launch_shared<bf16, 64>(a, scales, pre, s);
-    else attn::launch_shared<bf16, 128>(a, scales, pre, s);
+    if (D == 64) attn::launch<bf16, 64>(a, join, s);
+    else attn::launch<bf16, 128>(a, join, s);
   } else {
-    if (D == 64) attn::launch_shared<f16, 64>(a, scales, pre, s);
-    else attn::launch_shared<f16, 128>(a, scales, pre, s);
+    if (D == 64) attn::launch<f16, 64>(a, join, s);
+    else attn::launch<f16, 128>(a, join, s);
   }
-  return check_launch(what);
+  return check_launch("hmx_paged_attention_decode");
 }

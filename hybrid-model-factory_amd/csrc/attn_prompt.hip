@@ -850,6 +850,14 @@ extern "C" size_t hmx_paged_causal_attention_workspace_bytes(int32_t N, int64_t 
   return ns == 1 ? 0 : (size_t)ns * T * H * (D + 2) * sizeof(float);
 }
 
+extern "C" size_t hmx_paged_causal_attention8_workspace_bytes(int32_t N, int64_t T, int32_t H,
+                                                              int32_t HKV, int32_t D,
+                                                              int64_t max_keys) {
+  if (N <= 0 || T <= 0 || HKV <= 0 || H <= 0 || H % HKV != 0 || max_keys < 0) return 0;
+  return attn::few_rows(N, T, H / HKV) ? attn::few_rows_workspace_bytes(N, T, H, HKV, D, max_keys)
+                                       : hmx_paged_causal_attention_workspace_bytes(N, T, H, HKV, D, max_keys);
+}
+
 static int paged_causal_attention(const void* q, int64_t q_token_stride,
                                   int64_t q_head_stride, int32_t dtype, void* o,
                                   int64_t o_token_stride, int64_t o_head_stride,
@@ -875,6 +883,18 @@ static int paged_causal_attention(const void* q, int64_t q_token_stride,
               "pointers 16-byte aligned");
   HMX_REQUIRE(attn::near_rows(cache->k_token_stride) && attn::near_rows(cache->v_token_stride), HMX_EUNSUPPORTED,
               "hmx_paged_causal_attention: token strides of the cache past 2^25 elements");
+  const size_t need = scales ? hmx_paged_causal_attention8_workspace_bytes(N, T, H, HKV, D, max_keys)
+                             : hmx_paged_causal_attention_workspace_bytes(N, T, H, HKV, D, max_keys);
+  HMX_REQUIRE(need == 0 || (workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need), HMX_EINVAL,
+              "hmx_paged_causal_attention: workspace of %zu bytes is too small", workspace_bytes);
+  if (scales && attn::few_rows(N, T, H / HKV)) {
+    HMX_REQUIRE(T * H < (1ll << 31), HMX_EUNSUPPORTED, "hmx_paged_causal_attention8: %lld tokens", (long long)T);
+    attn::launch_few_rows(attn::FewRows{q, o, q_token_stride, q_head_stride, o_token_stride, o_head_stride, dtype,
+                                        attn::make_pages(*cache, scales), cu_seqlens, N, (int32_t)T, H, HKV, D, max_keys,
+                                        scale, fill_gaps, static_cast<float*>(workspace)},
+                          (hipStream_t)stream);
+    return check_launch("hmx_paged_causal_attention8");
+  }
   attn::FwdArgs a{};
   a.q = (const char*)q; a.o = (char*)o;
   a.q_ts = 2 * q_token_stride; a.q_hs = 2 * q_head_stride;
@@ -889,10 +909,6 @@ static int paged_causal_attention(const void* q, int64_t q_token_stride,
   a.split = N == 0 ? attn::NO_SPLITS : paged_splits(N, T, H, HKV, max_keys);
   a.nsplit = a.split.most;
   a.part = static_cast<float*>(workspace);
-  HMX_REQUIRE(a.nsplit == 1 ||
-                  (workspace && (uintptr_t)workspace % 16 == 0 &&
-                   workspace_bytes >= hmx_paged_causal_attention_workspace_bytes(N, T, H, HKV, D, max_keys)),
-              HMX_EINVAL, "hmx_paged_causal_attention: workspace of %zu bytes is too small", workspace_bytes);
   a.c = scale * attn::LOG2E;
   hipStream_t st_ = (hipStream_t)stream;
   if (dtype == HMX_BF16) {

@@ -133,6 +133,8 @@ SIGNATURES: dict[str, list] = {
                              _I32, _I32, _I32, _P],
     "hmx_paged_attention_decode8": [_P, _I64, _I64, _I32, _P, _I64, _I64, _P, _P, _I32, _I32, _I32,
                                     _I32, _F32, _P, ctypes.c_size_t, _P],
+    "hmx_paged_attention_decode8_workspace_bytes": [_I32, _I32, _I32, _I32, _I64],
+    "hmx_paged_causal_attention8_workspace_bytes": [_I32, _I64, _I32, _I32, _I32, _I64],
     "hmx_paged_causal_attention8": [_P, _I64, _I64, _I32, _P, _I64, _I64, _P, _P, _P, _I32, _I64,
                                     _I32, _I32, _I32, _F32, _I32, _P, ctypes.c_size_t, _P],
     "hmx_shared_prefix_decode": [_P, _I64, _I64, _I32, _P, _I64, _I64, _P, _P, _P, _I64, _I32, _P,
@@ -152,6 +154,8 @@ _RESTYPES = {"hmx_last_error": ctypes.c_char_p, "hmx_gdn_chunk_workspace_bytes":
              "hmx_paged_attention_decode_workspace_bytes": ctypes.c_size_t,
              "hmx_causal_attention_workspace_bytes": ctypes.c_size_t,
              "hmx_paged_causal_attention_workspace_bytes": ctypes.c_size_t,
+             "hmx_paged_attention_decode8_workspace_bytes": ctypes.c_size_t,
+             "hmx_paged_causal_attention8_workspace_bytes": ctypes.c_size_t,
              "hmx_shared_prefix_decode_workspace_bytes": ctypes.c_size_t}
 
 

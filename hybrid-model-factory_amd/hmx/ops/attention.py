@@ -411,7 +411,8 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
                                           k_scales=k_scales, v_scales=v_scales)
     q, qts, qhs = _rows(q)
     ots, ohs = _places(o)
-    ws, ws_bytes = _workspace("hmx_paged_attention_decode_workspace_bytes", q, N, H, HKV, D,
+    eight = "" if k_scales is None else "8"
+    ws, ws_bytes = _workspace(f"hmx_paged_attention_decode{eight}_workspace_bytes", q, N, H, HKV, D,
                               block_table.shape[1] * k_cache.shape[1])
     _paged_call("hmx_paged_attention_decode",
                 (q.data_ptr(), qts, qhs, _lib.dtype_code(q), o.data_ptr(), ots, ohs),
@@ -491,7 +492,7 @@ def paged_causal_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     gives 0 where that is none.  Cache and table as in paged_attention_decode.  Returns
     [T, H, D] in q's type; rows of no sequence are 0, or left as they were in ``out`` (which
     may not overlap an input).  ``k_scales``, ``v_scales``: of a cache of 8 bits; with fp16 what
-    it holds past that type's range counts as its largest value."""
+    it holds past that type's range may count as its largest value."""
     what = "paged_causal_attention"
     _refuse_tangents(what, q, k_cache, v_cache)
     if q.dim() != 3:
@@ -516,7 +517,8 @@ def paged_causal_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         return _forward_only(what, o, out, *ins)
     q, qts, qhs = _rows(q)
     ots, ohs = _places(o)
-    ws, ws_bytes = _workspace("hmx_paged_causal_attention_workspace_bytes", q, N, T, H, HKV, D,
+    eight = "" if k_scales is None else "8"
+    ws, ws_bytes = _workspace(f"hmx_paged_causal_attention{eight}_workspace_bytes", q, N, T, H, HKV, D,
                               block_table.shape[1] * k_cache.shape[1])
     _paged_call("hmx_paged_causal_attention",
                 (q.data_ptr(), qts, qhs, _lib.dtype_code(q), o.data_ptr(), ots, ohs),

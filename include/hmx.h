@@ -889,7 +889,9 @@ int hmx_paged_attention_decode(const void* q, int64_t q_token_stride, int64_t q_
                                int64_t o_head_stride, const hmx_paged_kv* cache, int32_t N,
                                int32_t H, int32_t HKV, int32_t D, float scale, void* workspace,
                                size_t workspace_bytes, void* stream);
-/* The same over a cache of 8 bits (q and o in 16); the same workspace. */
+/* The same over a cache of 8 bits (q and o in 16), with a workspace size of its own. */
+size_t hmx_paged_attention_decode8_workspace_bytes(int32_t N, int32_t H, int32_t HKV, int32_t D,
+                                                   int64_t max_keys);
 int hmx_paged_attention_decode8(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                                 int32_t dtype, void* o, int64_t o_token_stride,
                                 int64_t o_head_stride, const hmx_paged_kv* cache,
@@ -970,7 +972,9 @@ int hmx_paged_causal_attention(const void* q, int64_t q_token_stride, int64_t q_
                                void* workspace, size_t workspace_bytes, void* stream);
 
 /* The same over a cache of 8 bits (q and o in 16; with fp16, what the cache holds past that
- * type's range counts as its largest value); the same workspace. */
+ * type's range may count as its largest value), with a workspace size of its own. */
+size_t hmx_paged_causal_attention8_workspace_bytes(int32_t N, int64_t T, int32_t H, int32_t HKV,
+                                                   int32_t D, int64_t max_keys);
 int hmx_paged_causal_attention8(const void* q, int64_t q_token_stride, int64_t q_head_stride,
                                 int32_t dtype, void* o, int64_t o_token_stride,
                                 int64_t o_head_stride, const hmx_paged_kv* cache,

@@ -245,21 +245,21 @@ def test_new_tokens_values_that_are_nan(dev, tokens, far):
 
 
 def test_half_precision_past_its_range(dev):
-    """Values past fp16's range, which a cache written in bf16 may hold: its largest value counts
-    for new tokens; a decode forms them in fp32 and rounds its result."""
+    """Values past fp16's range, which a cache written in bf16 may hold, count as its largest
+    where prompts form them in fp16."""
     page = torch.ones(1, 16, 1, 64)
     kc, vc = page.to(F8).to(dev), (page * 448).to(F8).to(dev)
     ks = torch.full((1, 1, 16), 127, dtype=torch.uint8, device=dev)
     vs = torch.full((1, 1, 16), 127 + 8, dtype=torch.uint8, device=dev)   # 448 * 2^8 = 114688
-    q = torch.zeros(1, 2, 64, dtype=F16, device=dev)
+    q = torch.zeros(20, 2, 64, dtype=F16, device=dev)
     table, lens = (torch.tensor(x, dtype=torch.int32, device=dev) for x in ([[0]], [3]))
-    cu = torch.tensor([0, 1], dtype=torch.int32, device=dev)
+    cu = torch.tensor([0, 20], dtype=torch.int32, device=dev)            # tokens 17 .. 19 have keys
     o = hmx.paged_causal_attention(q, kc, vc, table, lens, cu, k_scales=ks, v_scales=vs)
-    # three probabilities of 1, exact in fp16, times 65504, over 3 by its fp32 reciprocal
-    assert ((o.float() - 65504).abs() <= 32).all()
+    # up to three probabilities of 1, exact in fp16, times 65504, over their sum by its fp32 reciprocal
+    assert (o[:17] == 0).all() and ((o[17:].float() - 65504).abs() <= 32).all()
     vs -= 1                                                              # 57344
-    for o in (hmx.paged_causal_attention(q, kc, vc, table, lens, cu, k_scales=ks, v_scales=vs),
-              hmx.paged_attention_decode(q, kc, vc, table, lens, k_scales=ks, v_scales=vs)):
+    for o in (hmx.paged_causal_attention(q, kc, vc, table, lens, cu, k_scales=ks, v_scales=vs)[17:],
+              hmx.paged_attention_decode(q[:1], kc, vc, table, lens, k_scales=ks, v_scales=vs)):
         assert ((o.float() - 57344).abs() <= 32).all()
 
 
