@@ -129,7 +129,8 @@ def _places(t: torch.Tensor) -> tuple[int, int]:
 
 def _out(out: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        return torch.empty_like(like) if like.is_contiguous() \
+            else torch.empty(like.shape, dtype=like.dtype, device=like.device)
     if out.shape != like.shape or out.dtype != like.dtype:
         raise ValueError(f"out {tuple(out.shape)} {out.dtype} must be {tuple(like.shape)} {like.dtype}")
     if not _aligned(out) or (out.dim() == 4 and out.shape[0] > 1 and out.shape[1] > 1
@@ -259,8 +260,9 @@ def _cache(what: str, q: torch.Tensor, k_cache, v_cache, HKV: int | None = None,
             raise ValueError(f"{what}: a cache of 8 bits is two of torch.float8_e4m3fn with k_scales and v_scales, "
                              f"got {k_cache.dtype} and {v_cache.dtype}")
         n = k_cache.shape
+        want = (n[0], n[2], n[1])
         for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
-            if t.dtype != torch.uint8 or tuple(t.shape) != (n[0], n[2], n[1]) or (n[1] > 1 and t.stride(2) != 1):
+            if t.dtype != torch.uint8 or t.shape != want or (n[1] > 1 and t.stride(2) != 1):
                 raise ValueError(f"{what}: {name} [{n[0]}, {n[2]}, {n[1]}] uint8 with the places of a page "
                                  f"contiguous, got {tuple(t.shape)} {t.dtype}")
     else:

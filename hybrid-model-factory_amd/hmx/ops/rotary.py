@@ -100,7 +100,16 @@ def _strided(t: torch.Tensor | None) -> tuple[int, int, int, int]:
     one, which may be anything, as 0."""
     if t is None:
         return 0, 0, 0, 0
+    if t.is_contiguous():
+        _, T, H, D = t.shape
+        return t.data_ptr(), T * H * D, H * D, D
     return (t.data_ptr(), *(s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape)))
+
+
+def _new(t: torch.Tensor | None) -> torch.Tensor | None:
+    if t is None or t.is_contiguous():
+        return None if t is None else torch.empty_like(t)
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, factor: float,
@@ -111,21 +120,23 @@ def rotate(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv
     if _elsewhere(q):
         with torch.cuda.device(q.device):
             return rotate(q, k, positions, inv_freq, factor, interleaved, backward, q_out, k_out)
-    outs = [o if o is not None else None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
-            for t, o in ((q, q_out), (k, k_out))]
+    q_out, k_out = q_out if q_out is not None else _new(q), k_out if k_out is not None else _new(k)
     B, T, H, D = q.shape
     if q.numel() == 0:
-        return outs[0], outs[1]
-    q, k = (t if t is None or _aligned(t) else t.clone(memory_format=torch.contiguous_format) for t in (q, k))
+        return q_out, k_out
+    if not _aligned(q):
+        q = q.clone(memory_format=torch.contiguous_format)
+    if k is not None and not _aligned(k):
+        k = k.clone(memory_format=torch.contiguous_format)
     inv_freq = inv_freq.contiguous()
     if T > 1 and positions.stride(-1) != 1:
         positions = positions.contiguous()
     pos_stride = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
-    _lib.call("hmx_rotary_embedding", *_strided(q), *_strided(outs[0]), *_strided(k), *_strided(outs[1]),
+    _lib.call("hmx_rotary_embedding", *_strided(q), *_strided(q_out), *_strided(k), *_strided(k_out),
               _lib.dtype_code(q), positions.data_ptr(), int(positions.dtype == torch.int64), pos_stride,
               inv_freq.data_ptr(), int(inv_freq.dtype == torch.float64), float(factor), 2 * inv_freq.shape[0],
               int(interleaved), int(backward), B, T, H, 0 if k is None else k.shape[2], D, _lib.stream_of(q))
-    return outs[0], outs[1]
+    return q_out, k_out
 
 
 class RotaryEmbedding(torch.autograd.Function):
@@ -143,12 +154,15 @@ class RotaryEmbedding(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dq, dk):
         positions, inv_freq = ctx.saved_tensors
-        turn = lambda a, b: RotaryEmbedding.apply(a, b, positions, inv_freq, *ctx.args, not ctx.back)
-        need = [d if n else None for d, n in zip((dq, dk), ctx.needs_input_grad)]
-        if need[0] is not None:
-            dq, dk = turn(*need)
+        # as a function of its own only where a graph of the gradients is asked for
+        turn = RotaryEmbedding.apply if torch.is_grad_enabled() else rotate
+        needs_q, needs_k = ctx.needs_input_grad[:2]
+        if dq is not None and needs_q:
+            dq, dk = turn(dq, dk if needs_k else None, positions, inv_freq, *ctx.args, not ctx.back)
         else:
-            dq, dk = None, None if need[1] is None else turn(need[1], None)[0]
+            dq = None
+            if dk is not None:
+                dk = turn(dk, None, positions, inv_freq, *ctx.args, not ctx.back)[0] if needs_k else None
         return dq, dk, None, None, None, None, None
 
 
@@ -193,18 +207,19 @@ def rotary_embedding(q: torch.Tensor, k: torch.Tensor | None, positions: torch.T
     R = 2 * inv_freq.shape[0]
     if R == 0 or R > D or R % 16:
         raise ValueError(f"{what}: {inv_freq.shape[0]} frequencies: a multiple of 8 up to {D // 2}")
-    lead = q.shape[:-2]
-    fits = [tuple(lead)] if q.dim() == 3 else [tuple(lead), (1, lead[1]), (lead[1],)]
-    if tuple(positions.shape) not in fits or positions.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{what}: positions {' or '.join(map(str, fits))} int32 or int64, got "
-                         f"{tuple(positions.shape)} {positions.dtype}")
+    lead, at = q.shape[:-2], positions.shape
+    if not (at == lead or (q.dim() == 4 and (at == lead[1:] or at == (1, lead[1])))) \
+            or positions.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"{what}: positions {tuple(lead)}{', or without B,' if q.dim() == 4 else ''} int32 or int64, "
+                         f"got {tuple(at)} {positions.dtype}")
     if inv_freq.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError(f"{what}: no gradient of the frequencies is implemented")
-    for name, out, like in (("q_out", q_out, q), ("k_out", k_out, k)):
-        if out is not None:
-            if like is None:
-                raise ValueError(f"{what}: {name} without k")
-            _check_out(what, name, out, like)
+    if q_out is not None:
+        _check_out(what, "q_out", q_out, q)
+    if k_out is not None:
+        if k is None:
+            raise ValueError(f"{what}: k_out without k")
+        _check_out(what, "k_out", k_out, k)
     _same_device(q, k, positions, inv_freq, q_out, k_out)
     interleaved = bool(interleaved)
     flat = q.dim() == 3
