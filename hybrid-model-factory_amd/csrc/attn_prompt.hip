@@ -141,11 +141,11 @@ __device__ __forceinline__ void add_nonfinite(const FwdArgs& a, const Tile& t, i
 // hides more of the exponentials (404 -> 396 us on packed prompts).  Outside the loop registers
 // spill: 50 at 128 and 38 at 64 over contiguous keys, 4 and 6 over pages.
 //
-// Q8: a cache of 8 bits.  Its rows arrive in LDS as they are, with their bytes of scale, and
-// each wave turns the 16 rows of either tile that it brought into the inputs' type, so the
-// rest is the same; the tiles have one buffer each, the next step's bytes are on their way
-// meanwhile.  PREFIX: the rows of all sequences behind one prefix attend all its keys, and
-// leave their shares.
+// Q8: a cache of 8 bits.  Its rows arrive in LDS as they are, in the upper halves of the places
+// that a wave's 16 rows of either tile will take, and the wave turns them into the inputs' type
+// there before the step that reads them, so the rest is the same.
+// PREFIX: the rows of all sequences behind one prefix attend all its keys, and leave their
+// shares.
 template <typename T, int D, bool PAGED, bool Q8 = false, bool PREFIX = false>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs a) {
   static_assert(PAGED || (!Q8 && !PREFIX), "");
@@ -154,10 +154,9 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
   constexpr int RI = 64 / NC, NL = 16 / RI; // rows of a wave's load, loads of its 16 rows of a tile
   constexpr int NS = D / 16, ND = D / 32;
   constexpr int TILE = BN * D * 2;          // bytes
-  constexpr int VOFF = Q8 ? TILE : 2 * TILE;         // of the first tile of V
-  // K, K, V, V; or K, V, both in 8 bits and their scales, a wave's 16 rows of either in 32 words
-  constexpr int RAWK = 2 * TILE, RAWV = RAWK + TILE / 2, SCALES = RAWV + TILE / 2;
-  __shared__ __align__(1024) char smem[Q8 ? SCALES + 4 * 256 : 4 * TILE];
+  // K, K, V, V; of 8 bits two steps' scales too, a wave's 16 rows of either tile in 32 words
+  constexpr int SCALES = 4 * TILE;
+  __shared__ __align__(1024) char smem[SCALES + (Q8 ? 2 * 1024 : 0)];
   __shared__ int s_bad, s_skip[4];
 
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5, l32 = lane & 31;
@@ -277,7 +276,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
   uint32_t vlive = 0;
   auto stage_rows8 = [&](int j, bool value, const uint8_t*& sc) __attribute__((always_inline)) {
     const int r0 = j * BN - (value ? 32 : 0) + wave * 16;
-    const uint32_t lds = lds_addr(smem) + (value ? RAWV : RAWK) + wave * 16 * D;
+    const uint32_t lds = lds_addr(smem) + (value ? 2 * TILE : 0) + ((j - j_beg) & 1) * TILE + wave * 16 * D * 2 + 16 * D;
     const char* base = value ? vbase : kbase;
     const int64_t ps = value ? a.pages.v_ps : a.pages.k_ps, ts = value ? vts : kts;
     const uint8_t* sbase = value ? a.pages.v_sc + kvh * a.pages.v_sc_hs : a.pages.k_sc + kvh * a.pages.k_sc_hs;
@@ -323,7 +322,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
     const uint8_t* sc = a.pages.k_sc + kvh * a.pages.k_sc_hs;   // any byte, where the step brings no keys
     if (j < j_end) stage_rows8(j, false, sc);
     vlive = stage_rows8(j, true, sc);
-    dma1(lds_addr(smem) + SCALES + wave * 256, sc);
+    dma1(lds_addr(smem) + SCALES + ((j - j_beg) & 1) * 1024 + wave * 256, sc);
   };
   auto stage = [&](int j) __attribute__((always_inline)) {                 // the keys and values of step j
     if constexpr (Q8) {
@@ -333,25 +332,32 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
       stage_rows(j, j * BN - 32 + wave * 16, true);
     }
   };
-  // The wave's rows of step j's tiles in the inputs' type.  Rows of V that are no keys become
-  // 0, and values that are not finite where some row's keys end among them, as in mend().
+  // The wave's rows of step j's tiles in the inputs' type, where they lie: all are read before
+  // the first is written.  Rows of V that are no keys become 0, and values that are not finite
+  // where some row's keys end among them, as in mend().
   auto widen = [&](int j) __attribute__((always_inline)) {
     constexpr int NP = D / 32;              // pieces of eight values a lane
-    const uint32_t* scales = reinterpret_cast<const uint32_t*>(smem + SCALES + wave * 256);
+    const uint32_t* scales = reinterpret_cast<const uint32_t*>(smem + SCALES + ((j - j_beg) & 1) * 1024 + wave * 256);
     const bool edge = j * BN - 32 + BN > wg_first + 1;
 #pragma unroll
     for (int value = 0; value < 2; ++value) {
       if (!value && j >= j_end) continue;
-      const char* raw = smem + (value ? RAWV : RAWK) + wave * 16 * D;
+      char* rows = smem + (value ? 2 * TILE : 0) + ((j - j_beg) & 1) * TILE + wave * 16 * D * 2;
+      u32x2 x[NP];
+      uint32_t code[NP];
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        x[i] = *reinterpret_cast<const u32x2*>(rows + 16 * D + 8 * (lane + 64 * i));
+        code[i] = scales[16 * value + (lane + 64 * i) / NC];
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       bool bad = false;
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         const int at = lane + 64 * i, r = at / NC, c = at % NC;
-        const u32x2 x = *reinterpret_cast<const u32x2*>(raw + 8 * at);
-        const uint32_t code = scales[16 * value + r];
-        v8 y = from_e4m3<T>(x, scale_of(code));
+        v8 y = from_e4m3<T>(x[i], scale_of(code[i]));
         if constexpr (__is_same(T, f16)) {
-          if (code >= 127 + 8) {            // 448 times it passes fp16's range: the largest value there, NaN as it is
+          if (code[i] >= 127 + 8) {         // 448 times it passes fp16's range: the largest value there, NaN as it is
 #pragma unroll
             for (int z = 0; z < 8; ++z) {
               const float f = (float)y[z];
@@ -371,7 +377,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
             bad = true;
           }
         }
-        *reinterpret_cast<u32x4*>(smem + (value ? VOFF : 0) + (wave * 16 + r) * D * 2 + swz<D>(wave * 16 + r, c) * 16) = out;
+        *reinterpret_cast<u32x4*>(rows + r * D * 2 + swz<D>(wave * 16 + r, c) * 16) = out;
       }
       if (bad) s_bad = 1;
     }
@@ -426,7 +432,6 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
     vu[d] = tr_offset<D>(lane, d, true) * 2;
   }
   auto flip = [&]() __attribute__((always_inline)) {
-    if constexpr (Q8) return;
 #pragma unroll
     for (int s = 0; s < NS; ++s) ko[s] ^= TILE;
 #pragma unroll
@@ -501,7 +506,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
   // half's scores from K's half kt; the tiles are the buffers at `at`
   constexpr int AHEAD = 2;                  // LDS reads run so many products ahead
   auto half = [&](int u, const f32x16& cur, f32x16& nxt, int at, int kt, int r) __attribute__((always_inline)) {
-    const char *Kb = smem + at + kt * 32 * D * 2, *Vb = smem + at + VOFF + r * D * 2;
+    const char *Kb = smem + at + kt * 32 * D * 2, *Vb = smem + at + 2 * TILE + r * D * 2;
     constexpr int E = EAGER ? 8 : 16;       // elements of P formed beside the scores
     v8 kf[NS], vf[2 * ND], pf[2];
     float p[16], sum = 0.f, mx = NEG_INF;
@@ -567,7 +572,7 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
         for (int i = 0; i < 8; ++i) element(cur, 8 * b + i, p, l);
       }
       const v8 pf = pack(p + 8 * b);
-      const char* Vb = smem + VOFF + (r + 16 * b) * D * 2;
+      const char* Vb = smem + 2 * TILE + (r + 16 * b) * D * 2;
 #pragma unroll
       for (int d = 0; d < ND; ++d)
         acc[d] = El<T>::mma32(join<T>(tr4<T>(reinterpret_cast<const T*>(Vb + vo[d])),
@@ -576,11 +581,10 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
   };
   auto arrive = [&](int j) __attribute__((always_inline)) {   // step j's tiles are there, step j + 1's on their way
     dma_wait<0>();
+    if constexpr (Q8) widen(j);             // what the wave itself brought
     __syncthreads();
-    if constexpr (Q8) widen(j);             // what the wave itself brought, over tiles that all have read
     if (j < j_end) stage(j + 1);
-    if constexpr (Q8) __syncthreads();
-    else mend(j);
+    if constexpr (!Q8) mend(j);
   };
 
   if (j_beg < j_end) {
