@@ -351,10 +351,25 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
         code[i] = scales[16 * value + (lane + 64 * i) / NC];
       }
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      bool bad = false;
+      if (value && (edge || vlive != 0xffffu)) {
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            uint32_t n = 0;
+#pragma unroll
+            for (int b = 0; b < 32; b += 8) n |= nan8(x[i][z] >> b) ? 0xffu << b : 0u;
+            const bool key = (vlive >> ((lane + 64 * i) / NC)) & 1;
+            bad |= key && edge && n;
+            x[i][z] = key ? (edge ? x[i][z] & ~n : x[i][z]) : 0;
+            if (!key) code[i] = 1;          // the power may be anything too
+          }
+        if (bad) s_bad = 1;
+      }
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
-        const int at = lane + 64 * i, r = at / NC, c = at % NC;
+        const int r = (lane + 64 * i) / NC, c = lane % NC;
         v8 y = from_e4m3<T>(x[i], scale_of(code[i]));
         if constexpr (__is_same(T, f16)) {
           if (code[i] >= 127 + 8) {         // 448 times it passes fp16's range: the largest value there, NaN as it is
@@ -366,20 +381,8 @@ __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs 
             }
           }
         }
-        u32x4 out = __builtin_bit_cast(u32x4, y);
-        if (value) {
-          if (!((vlive >> r) & 1)) {
-            out = u32x4{0, 0, 0, 0};
-          } else if (edge && any_nonfinite<T>(out)) {
-#pragma unroll
-            for (int z = 0; z < 8; ++z)
-              if (nonfinite<T>(out[z >> 1] >> (16 * (z & 1)))) out[z >> 1] &= z & 1 ? 0xffffu : 0xffff0000u;
-            bad = true;
-          }
-        }
-        *reinterpret_cast<u32x4*>(rows + r * D * 2 + swz<D>(wave * 16 + r, c) * 16) = out;
+        *reinterpret_cast<v8*>(rows + r * D * 2 + swz<D>(wave * 16 + r, c) * 16) = y;
       }
-      if (bad) s_bad = 1;
     }
   };
   // Rows of step j's V that are no keys to 0 (their probability is 0, their memory anything).
