@@ -361,7 +361,7 @@ __device__ __forceinline__ int place(int at, int blocks, int places) {
   return at >= places && blocks <= 2 * places ? blocks - 1 - (at - places) : at;
 }
 
-// The shares of rows over keys that several sequences have in common (attn_prompt.hip): for
+// The shares of rows over keys that several sequences have in common (attn_tile.hpp): for
 // split s < splits of row r = token * H + head D sums at part[(s rows + r) D], unnormalised,
 // and behind them all two numbers, the maximum of the scaled scores in base 2 and the sum.
 // Rows with fewer splits, or none, have NO_SHARE in the place of the first such maximum.
@@ -370,16 +370,6 @@ struct PrefixShares {
   float* part;
   int64_t rows;
   int32_t splits;
-};
-struct PrefixArgs {
-  const void* q;
-  int64_t q_ts, q_hs;        // elements
-  int32_t dtype;
-  Pages pages;               // the prefixes'
-  const int32_t* cu;         // offsets of the sequences behind each, or NULL: one prefix for all
-  int32_t M, N, H, HKV, D;
-  float scale;
-  bool eight;                // a cache of 8 bits
 };
 // Few new tokens a sequence over a cache of 8 bits (attn_rows.hip).  few_rows: they are where
 // each sequence's rows fill a block of 16 on average; the blocks are then at most twice the
@@ -400,9 +390,6 @@ struct FewRows {
 bool few_rows(int64_t N, int64_t T, int64_t G);
 size_t few_rows_workspace_bytes(int64_t N, int64_t T, int32_t H, int32_t HKV, int32_t D, int64_t max_keys);
 void launch_few_rows(const FewRows& f, hipStream_t s);
-
-int prefix_splits(int64_t M, int64_t N, int H, int HKV, int64_t max_keys);
-void launch_prefix(const PrefixArgs& p, const PrefixShares& out, int64_t max_keys, hipStream_t s);
 
 template <int BM>
 inline int64_t tile_slots(const int32_t* cu, int64_t N, int64_t T, int64_t G) {

@@ -24,7 +24,7 @@
 // and four of the second, the order in which the two tiles of scores hold them.
 // P enters its product rounded and, beside it, what that rounding leaves: the matrix cores wait
 // for memory anyway.  Scores, statistics and O stay in fp32.
-#include "attn.hpp"
+#include "attn_tile.hpp"
 
 namespace hmx {
 namespace attn {
@@ -143,29 +143,33 @@ __device__ __forceinline__ u32x2 tr8(const char* p) {
   typedef int i32x2 __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(p)));
 }
-// whether a byte of a cache of 8 bits is e4m3's NaN
-__device__ __forceinline__ bool nan8(uint32_t x) { return (x & 0x7f) == 0x7f; }
+// The ring of a wave: turns of KT keys, K's bytes, V's behind them, then the scales.
+template <int D, bool Q8, int RING> struct Shared {
+  static constexpr int KT = Q8 ? 32 : 16;
+  static constexpr int KV = KT * D * (Q8 ? 1 : 2), TURN = 2 * KV + (Q8 ? 256 : 0);
+  static constexpr int BYTES = NW * RING * TURN;     // the rings, then the shares [16][D] in fp32
+  static_assert(NW == 4 && RING * TURN >= 16 * D * 4, "find_share, and the shares in LDS");
+  float ml[NW][16][2];
+  int64_t scan[8];
+  int bad;                                  // the last share of whose keys some were spoiled
+};
 
 // Q8: a cache of 8 bits.  SHARES: every block leaves its share.
-template <typename T, int D, bool Q8, bool SHARES>
-__global__ __launch_bounds__(64 * NW, OCC) void attn_rows_kernel(Args a) {
+template <typename T, int D, bool Q8, bool SHARES, int RING>
+__device__ __forceinline__ void attn_rows(const Args& a, char* smem, Shared<D, Q8, RING>& shared, int blk) {
   typedef typename El<T>::v8 v8;
   typedef typename El<T>::v4 v4;
-  constexpr int KT = Q8 ? 32 : 16;           // keys of a wave's turn
+  constexpr int KT = Shared<D, Q8, RING>::KT;  // keys of a wave's turn
   constexpr int ES = Q8 ? 1 : 2;             // bytes of an element of the cache
   constexpr int ROW = D * ES;                // bytes of a row
   constexpr int NH = KT / 16;                // halves of a turn: sixteen keys, one page where pages are of sixteens
   constexpr int NS = D / 32, ND = D / 16, NC = ROW / 16;
   constexpr int RI = 64 / NC, NL = KT / RI;  // rows of a load, loads of K (and V) of a turn
-  constexpr int RING = D == 128 ? 2 : 4;     // turns: 64 KB of LDS for the four waves
-  constexpr int KV = KT * ROW;               // bytes of a turn's K, and of its V behind it, then the scales
-  constexpr int TURN = 2 * KV + (Q8 ? 256 : 0);
+  constexpr int KV = Shared<D, Q8, RING>::KV, TURN = Shared<D, Q8, RING>::TURN;
   constexpr uint32_t ALL = Q8 ? ~0u : 0xffffu;
-  static_assert(NW == 4 && RING * TURN >= 16 * D * 4, "find_share and the shares in LDS");
-  __shared__ __align__(1024) char smem[NW * RING * TURN];   // the rings, then the shares [16][D] in fp32
-  __shared__ float s_ml[NW][16][2];
-  __shared__ int64_t s_scan[8];
-  __shared__ int s_bad;                      // the last share of whose keys some were spoiled
+  auto& s_ml = shared.ml;
+  auto& s_scan = shared.scan;
+  int& s_bad = shared.bad;
 
   const int tid = threadIdx.x, lane = tid & 63, q4 = lane >> 4, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -175,7 +179,7 @@ __global__ __launch_bounds__(64 * NW, OCC) void attn_rows_kernel(Args a) {
   // line once (two sequences to 131072 keys, 14 / 2 heads of 64: 38.5 -> 29.7 us); rows of whole
   // lines are better spread (256 sequences to 8192 keys: 483 us, by worker 500).
   constexpr bool BY_WORKER = ROW < 128;
-  const int blk = blockIdx.x, eights = BY_WORKER ? (a.W ? a.W : a.N) & ~7 : 0;
+  const int eights = BY_WORKER ? (a.W ? a.W : a.N) & ~7 : 0;
   const bool in8 = blk < eights * a.HKV;
   const int rem = in8 ? blk % (8 * a.HKV) : blk - eights * a.HKV;
   const int kvh = in8 ? rem >> 3 : rem % a.HKV;
@@ -543,6 +547,37 @@ __global__ __launch_bounds__(64 * NW, OCC) void attn_rows_kernel(Args a) {
   }
 }
 
+// Turns of a wave's ring: 64 KB of LDS for the four waves, so that two workgroups fit; three
+// beside the tiles of head size 64, of which three workgroups fit.
+template <int D> constexpr int ring() { return D == 128 ? 2 : 4; }
+
+template <typename T, int D, bool Q8, bool SHARES>
+__global__ __launch_bounds__(64 * NW, OCC) void attn_rows_kernel(Args a) {
+  __shared__ __align__(1024) char smem[Shared<D, Q8, ring<D>()>::BYTES];
+  __shared__ Shared<D, Q8, ring<D>()> shared;
+  attn_rows<T, D, Q8, SHARES, ring<D>()>(a, smem, shared, blockIdx.x);
+}
+
+// Many rows behind prefixes in tiles, and the sequences' own keys, in one launch: the first are
+// bound by the matrix cores, the second by memory, and workgroups of both kinds, eight of one
+// and eight of the other in turn, run at once.
+template <typename T, int D, bool Q8>
+__global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void attn_shared_kernel(Args a, FwdArgs f, int tiles, int blocks) {
+  constexpr int RING = D == 128 ? 2 : 3;
+  constexpr int BYTES = FwdShared<D, Q8>::BYTES > Shared<D, Q8, RING>::BYTES ? FwdShared<D, Q8>::BYTES : Shared<D, Q8, RING>::BYTES;
+  __shared__ __align__(1024) char smem[BYTES];
+  __shared__ Shared<D, Q8, RING> shared;
+  __shared__ FwdShared<D, Q8> flags;
+  const int both = 2 * min((tiles + 7) >> 3, (blocks + 7) >> 3), at = blockIdx.x >> 3;
+  const bool tile = at < both ? !(at & 1) : tiles > blocks;
+  const int i = (at < both ? at >> 1 : at - (both >> 1)) * 8 + (blockIdx.x & 7);
+  if (tile) {
+    if (i < tiles) attn_fwd<T, D, true, Q8, true>(f, smem, flags, i, tiles);
+  } else {
+    if (i < blocks) attn_rows<T, D, Q8, true, RING>(a, smem, shared, i);
+  }
+}
+
 // Shares joined: sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s, of the workers that a row's block
 // is cut over and (SHARES) of its prefix, whose shares lie here too or, of many rows, in `pre`.
 // A workgroup takes RP heads of one token; its threads take a row's shares in turn, D / 4 to a
@@ -660,8 +695,16 @@ static int64_t workers_of(int64_t N, int64_t T, int64_t G, int64_t HKV, int64_t 
 }
 
 template <typename T, int D, bool Q8, bool SHARES>
-static void launch(const Args& a, const PrefixShares& pre, hipStream_t s) {
-  hipLaunchKernelGGL((attn_rows_kernel<T, D, Q8, SHARES>), dim3((unsigned)(a.HKV * (a.W ? a.W : a.N))), dim3(64 * NW), 0, s, a);
+static void launch(const Args& a, const FwdArgs* f, const PrefixShares& pre, hipStream_t s) {
+  const int blocks = a.HKV * (a.W ? a.W : a.N);
+  if constexpr (SHARES) {
+    if (f) {
+      const int tiles = (int)(fwd_blocks(*f) * a.HKV);
+      const dim3 grid((unsigned)(8 * ((tiles + 7) / 8 + (blocks + 7) / 8)));
+      hipLaunchKernelGGL((attn_shared_kernel<T, D, Q8>), grid, dim3(64 * NW), 0, s, a, *f, tiles, blocks);
+    }
+  }
+  if (!f) hipLaunchKernelGGL((attn_rows_kernel<T, D, Q8, SHARES>), dim3((unsigned)blocks), dim3(64 * NW), 0, s, a);
   if (!SHARES && a.W <= 1) return;
   const int64_t H = a.HKV * a.G.d, rows = H * a.T;
   // eight rows a workgroup, which finds their entries once, where that leaves enough workgroups
@@ -671,14 +714,28 @@ static void launch(const Args& a, const PrefixShares& pre, hipStream_t s) {
     hipLaunchKernelGGL((attn_rows_join_kernel<T, D, SHARES, 1>), dim3((unsigned)rows), dim3(256), 0, s, a, pre);
 }
 template <bool Q8, bool SHARES>
-static void launch_types(const Args& a, int32_t dtype, int32_t D, const PrefixShares& pre, hipStream_t s) {
+static void launch_types(const Args& a, int32_t dtype, int32_t D, hipStream_t s, const FwdArgs* f = nullptr,
+                         const PrefixShares& pre = PrefixShares{}) {
   if (dtype == HMX_BF16) {
-    if (D == 64) launch<bf16, 64, Q8, SHARES>(a, pre, s);
-    else launch<bf16, 128, Q8, SHARES>(a, pre, s);
+    if (D == 64) launch<bf16, 64, Q8, SHARES>(a, f, pre, s);
+    else launch<bf16, 128, Q8, SHARES>(a, f, pre, s);
   } else {
-    if (D == 64) launch<f16, 64, Q8, SHARES>(a, pre, s);
-    else launch<f16, 128, Q8, SHARES>(a, pre, s);
+    if (D == 64) launch<f16, 64, Q8, SHARES>(a, f, pre, s);
+    else launch<f16, 128, Q8, SHARES>(a, f, pre, s);
   }
+}
+
+// The rows of N sequences, one token each, over the M prefixes that they share, in tiles.
+static Splits tile_splits(int64_t M, int64_t N, int64_t G, int HKV, int64_t max_prefix, bool packed) {
+  const int32_t some = 0;
+  const int64_t slots = tile_slots<BM>(packed ? &some : nullptr, M, N, G);
+  return splits(packed ? slots - 2 : slots, HKV, max_prefix, 4);
+}
+// splits whose shares there is room for, with offsets or without
+static int64_t tile_splits_most(int64_t M, int64_t N, int64_t G, int HKV, int64_t max_prefix) {
+  const int64_t a = tile_splits(M, N, G, HKV, max_prefix, true).most;
+  const int64_t b = M == 1 ? tile_splits(M, N, G, HKV, max_prefix, false).most : 1;
+  return a > b ? a : b;
 }
 
 // What the entry points check alike.
@@ -732,7 +789,7 @@ void launch_few_rows(const FewRows& f, hipStream_t s) {
   a.W = (int32_t)rows::workers_of(f.N, f.T, a.G.d, f.HKV, f.max_keys);
   a.c = f.scale * LOG2E; a.fill = f.fill;
   a.part = f.workspace; a.slots = 2ll * a.W;
-  rows::launch_types<true, false>(a, f.dtype, f.D, PrefixShares{}, s);
+  rows::launch_types<true, false>(a, f.dtype, f.D, s);
 }
 
 }  // namespace attn
@@ -759,7 +816,7 @@ extern "C" int hmx_paged_attention_decode8(const void* q, int64_t q_token_stride
   a.W = (int32_t)attn::rows::workers_of(N, N, a.G.d, HKV, max_keys);
   a.slots = 2ll * a.W;
   a.part = static_cast<float*>(workspace);
-  attn::rows::launch_types<true, false>(a, dtype, D, attn::PrefixShares{}, (hipStream_t)stream);
+  attn::rows::launch_types<true, false>(a, dtype, D, (hipStream_t)stream);
   return check_launch(what);
 }
 
@@ -785,7 +842,7 @@ SharedPlan shared_plan(int64_t N, int64_t M, int32_t H, int32_t HKV, int64_t max
   const int64_t pblocks = p.few && M > 0 ? N * G / 16 + M + 2 : 0;
   p.W = attn::rows::workers(HKV, attn::rows::units_at_most(N * hb, max_keys) + attn::rows::units_at_most(pblocks, max_prefix));
   p.slots = 2 * p.W + N * hb + pblocks;
-  p.splits = p.few || M == 0 ? 0 : attn::prefix_splits(M, N, H, HKV, max_prefix);
+  p.splits = p.few || M == 0 ? 0 : attn::rows::tile_splits_most(M, N, G, HKV, max_prefix);
   return p;
 }
 }  // namespace
@@ -836,15 +893,24 @@ extern "C" int hmx_shared_prefix_decode(const void* q, int64_t q_token_stride, i
   const attn::PrefixShares pre{a.part + attn::rows::share_bytes(a.slots, HKV, D) / sizeof(float), (int64_t)N * H,
                                (int32_t)plan.splits};
   hipStream_t s = (hipStream_t)stream;
+  attn::FwdArgs f{};
   if (M > 0 && plan.few) {
     a.M = M; a.p_table = prefix_table; a.p_stride = prefix_table_stride; a.p_lens = prefix_lens; a.p_cu = cu_prefix;
     a.p_width = cache->num_pages > 0 ? prefix_table_width : 0;
   } else if (M > 0) {
-    const attn::PrefixArgs p{q, q_token_stride, q_head_stride, dtype, attn::make_pages(far, scales), cu_prefix,
-                             M, N, H, HKV, D, scale, scales != nullptr};
-    attn::launch_prefix(p, pre, max_prefix, s);
+    f.q = a.q; f.q_ts = a.q_ts; f.q_hs = a.q_hs;
+    f.pages = attn::make_pages(far, scales);
+    f.seqs = attn::Seqs{cu_prefix, M, N, a.G.d};
+    f.G = a.G; f.H = H; f.HKV = HKV;
+    f.slots = (int32_t)attn::tile_slots<attn::BM>(cu_prefix, M, N, a.G.d);
+    f.split = attn::rows::tile_splits(M, N, a.G.d, HKV, max_prefix, cu_prefix != nullptr);
+    f.nsplit = pre.splits;
+    f.places = (int32_t)(cu_count() / HKV);
+    f.part = pre.part;
+    f.c = a.c;
   }
-  if (scales) attn::rows::launch_types<true, true>(a, dtype, D, pre, s);
-  else attn::rows::launch_types<false, true>(a, dtype, D, pre, s);
+  const attn::FwdArgs* tiles = pre.splits > 0 ? &f : nullptr;
+  if (scales) attn::rows::launch_types<true, true>(a, dtype, D, s, tiles, pre);
+  else attn::rows::launch_types<false, true>(a, dtype, D, s, tiles, pre);
   return check_launch(what);
 }
