@@ -639,6 +639,7 @@ __global__ __launch_bounds__(256) void attn_rows_join_kernel(Args a, PrefixShare
     const int64_t w0 = (bfirst + SETUP) / per, w1 = (bfirst + SETUP + units - 1) / per;
     if (!SHARES && w0 == w1) continue;      // stored
     store = true;
+#pragma unroll 4
     for (int64_t w = w0 + sh; w <= w1; w += SH) {
       const int64_t at = SHARES && w0 == w1 ? own_slot(a, e, x, b) : w * 2 + (w * per < bfirst ? 1 : 0);
       const int64_t slot = at * a.HKV + kvh;
@@ -679,8 +680,8 @@ __global__ __launch_bounds__(256) void attn_rows_join_kernel(Args a, PrefixShare
 }
 
 // Workers of a kv head: as many as run at once, and no more than `most` units give MIN_UNITS to.
-static int64_t workers(int64_t HKV, int64_t most) {
-  int64_t w = (int64_t)OCC * cu_count() / HKV;
+static int64_t workers(int64_t HKV, int64_t most, int per_cu = OCC) {
+  int64_t w = (int64_t)per_cu * cu_count() / HKV;
   const int64_t need = (most + MIN_UNITS - 1) / MIN_UNITS;
   if (w > need) w = need;
   return w < 1 ? 1 : w;
@@ -725,11 +726,14 @@ static void launch_types(const Args& a, int32_t dtype, int32_t D, hipStream_t s,
   }
 }
 
-// The rows of N sequences, one token each, over the M prefixes that they share, in tiles.
+// The rows of N sequences, one token each, over the M prefixes that they share, in tiles.  Of
+// the two workgroups of a compute unit one takes tiles and one the sequences' own keys, so that
+// all run at once (256 sequences to 1031 keys behind two prefixes to 16384: 202 us; with twice
+// as many tiles 256, workers 242, both 221).
 static Splits tile_splits(int64_t M, int64_t N, int64_t G, int HKV, int64_t max_prefix, bool packed) {
   const int32_t some = 0;
   const int64_t slots = tile_slots<BM>(packed ? &some : nullptr, M, N, G);
-  return splits(packed ? slots - 2 : slots, HKV, max_prefix, 4);
+  return splits(packed ? slots - 2 : slots, HKV, max_prefix, 4, 1);
 }
 // splits whose shares there is room for, with offsets or without
 static int64_t tile_splits_most(int64_t M, int64_t N, int64_t G, int HKV, int64_t max_prefix) {
@@ -826,8 +830,10 @@ extern "C" size_t hmx_paged_attention_decode8_workspace_bytes(int32_t N, int32_t
   return attn::few_rows_workspace_bytes(N, N, H, HKV, D, max_keys);
 }
 
-// The rows behind the prefixes are few where they do not fill a tile of the prompt kernel
-// twice over, so that the blocks' rereading of a prefix costs less than the tile's idle rows.
+// Rows behind a prefix are few up to half a tile of 128: four blocks then read the prefix, and
+// the tile's idle rows cost about as much (32 / 8 heads of 128 in 8 bits: 64 rows behind 16384
+// keys 40.5 us, by tiles 42.8, behind 4096 26.9 and 24.4; 96 rows 29.4 and 26.5; 32 rows 21.7
+// either way).
 static bool few_behind(int64_t N, int64_t M, int64_t G) { return N * G <= 64 * M; }
 
 namespace {
@@ -840,7 +846,8 @@ SharedPlan shared_plan(int64_t N, int64_t M, int32_t H, int32_t HKV, int64_t max
   SharedPlan p;
   p.few = few_behind(N, M, G);
   const int64_t pblocks = p.few && M > 0 ? N * G / 16 + M + 2 : 0;
-  p.W = attn::rows::workers(HKV, attn::rows::units_at_most(N * hb, max_keys) + attn::rows::units_at_most(pblocks, max_prefix));
+  p.W = attn::rows::workers(HKV, attn::rows::units_at_most(N * hb, max_keys) + attn::rows::units_at_most(pblocks, max_prefix),
+                            p.few || M == 0 ? attn::rows::OCC : 1);
   p.slots = 2 * p.W + N * hb + pblocks;
   p.splits = p.few || M == 0 ? 0 : attn::rows::tile_splits_most(M, N, G, HKV, max_prefix);
   return p;

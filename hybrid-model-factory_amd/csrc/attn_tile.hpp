@@ -670,8 +670,8 @@ __device__ __forceinline__ void attn_fwd(const FwdArgs& a, char* smem, FwdShared
 // are few rows, eight over contiguous keys.  A tile of a longer sequence may take twice as many.
 // Prompts, without splits and with: 2048 tokens, 8 / 2 heads of 128, 42.5 -> 31.6 us; 4096,
 // 4 / 4 of 64, 58 -> 28; 16384, 2 / 1 of 128, 276 -> 175.
-inline Splits splits(int64_t tiles, int HKV, int64_t max_keys, int least) {
-  const int64_t live = tiles * HKV, want = 2ll * cu_count(), most = max_keys / (least * BN);
+inline Splits splits(int64_t tiles, int HKV, int64_t max_keys, int least, int per_cu = 2) {
+  const int64_t live = tiles * HKV, want = (int64_t)per_cu * cu_count(), most = max_keys / (least * BN);
   int64_t even = live > 0 ? want / live : 1;
   if (even > most) even = most;
   if (even > 64) even = 64;
