@@ -67,7 +67,10 @@ class _NoBackward(torch.autograd.Function):
 
 
 def _grad_of(*tensors: torch.Tensor | None) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return torch.is_grad_enabled()
+    return False
 
 
 def _forward_only(what: str, result: torch.Tensor, out: torch.Tensor | None, *inputs) -> torch.Tensor:
@@ -106,7 +109,7 @@ def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
     """(t, token stride, head stride) of [tokens, heads, D], or of [B, T, heads, D] whose
     tokens lie at one stride; a contiguous copy where there is no such view."""
     if t.is_contiguous() and t.data_ptr() % 16 == 0:
-        H, D = t.shape[-2:]
+        *_, H, D = t.shape
         return t, H * D, D
     B = t.shape[0] if t.dim() == 4 else 1
     T = t.shape[-3]
@@ -248,10 +251,10 @@ def attention_forward(q, k, v, scale, cu_seqlens, out, want_lse):
 
 def _cache(what: str, q: torch.Tensor, k_cache, v_cache, HKV: int | None = None,
            k_scales: torch.Tensor | None = None, v_scales: torch.Tensor | None = None) -> None:
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[-1] != q.shape[-1] \
-            or k_cache.shape[1] == 0 or k_cache.shape[2] == 0 \
-            or (HKV is not None and k_cache.shape[2] != HKV):
-        raise ValueError(f"{what}: caches [pages, page size, HKV, D], got {tuple(k_cache.shape)} and "
+    n = k_cache.shape
+    if len(n) != 4 or n != v_cache.shape or n[3] != q.shape[-1] or n[1] == 0 or n[2] == 0 \
+            or (HKV is not None and n[2] != HKV):
+        raise ValueError(f"{what}: caches [pages, page size, HKV, D], got {tuple(n)} and "
                          f"{tuple(v_cache.shape)} for heads of {q.shape[-1]}")
     eight = k_cache.dtype == torch.float8_e4m3fn or v_cache.dtype == torch.float8_e4m3fn
     if eight or k_scales is not None or v_scales is not None:
@@ -259,10 +262,9 @@ def _cache(what: str, q: torch.Tensor, k_cache, v_cache, HKV: int | None = None,
         if not eight or k_cache.dtype != v_cache.dtype or k_scales is None or v_scales is None:
             raise ValueError(f"{what}: a cache of 8 bits is two of torch.float8_e4m3fn with k_scales and v_scales, "
                              f"got {k_cache.dtype} and {v_cache.dtype}")
-        n = k_cache.shape
         want = (n[0], n[2], n[1])
         for name, t in (("k_scales", k_scales), ("v_scales", v_scales)):
-            if t.dtype != torch.uint8 or t.shape != want or (n[1] > 1 and t.stride(2) != 1):
+            if t.dtype != torch.uint8 or t.shape != want or not (t.is_contiguous() or n[1] == 1 or t.stride(2) == 1):
                 raise ValueError(f"{what}: {name} [{n[0]}, {n[2]}, {n[1]}] uint8 with the places of a page "
                                  f"contiguous, got {tuple(t.shape)} {t.dtype}")
     else:
@@ -283,11 +285,11 @@ def _paged_call(name: str, head: tuple, kv, k_scales, v_scales, tail: tuple) -> 
 
 def _table(what: str, block_table: torch.Tensor, seq_lens: torch.Tensor, N: int,
            table_name: str = "block_table", lens_name: str = "seq_lens") -> None:
-    for name, t in ((table_name, block_table), (lens_name, seq_lens)):
-        if t.dtype != torch.int32:
-            raise ValueError(f"{what}: {name} must be int32, got {t.dtype}")
-    if block_table.dim() != 2 or block_table.shape[0] != N or tuple(seq_lens.shape) != (N,) \
-            or not seq_lens.is_contiguous() or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+    if block_table.dtype != torch.int32 or seq_lens.dtype != torch.int32:
+        raise ValueError(f"{what}: {table_name} and {lens_name} must be int32, got {block_table.dtype} and {seq_lens.dtype}")
+    n = block_table.shape
+    if len(n) != 2 or n[0] != N or seq_lens.shape != (N,) \
+            or not seq_lens.is_contiguous() or (n[1] > 1 and block_table.stride(1) != 1):
         raise ValueError(f"{what}: {table_name} [{N}, width] with contiguous rows and {lens_name} [{N}], got "
                          f"{tuple(block_table.shape)} and {tuple(seq_lens.shape)}")
 
@@ -320,13 +322,13 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     T, HKV, D = k.shape
     _check_types(what, k, v, q)
     _cache(what, k, k_cache, v_cache, HKV, k_scales, v_scales)
-    if any(c is not None and 0 in c.stride() and any(s == 0 and m > 1 for s, m in zip(c.stride(), c.shape))
+    if any(c is not None and not c.is_contiguous() and any(s == 0 and m > 1 for s, m in zip(c.stride(), c.shape))
            for c in (k_cache, v_cache, k_scales, v_scales)):
         raise ValueError(f"{what}: caches must have a place of their own for every row")
     if (cos_sin is None) != (positions is None):
         raise ValueError(f"{what}: cos_sin and positions go together")
     for name, t in (("slot_mapping", slot_mapping), ("positions", positions)):
-        if t is not None and (tuple(t.shape) != (T,) or t.dtype not in (torch.int32, torch.int64)):
+        if t is not None and (t.shape != (T,) or t.dtype not in (torch.int64, torch.int32)):
             raise ValueError(f"{what}: {name} must be [{T}] int32 or int64, got {tuple(t.shape)} {t.dtype}")
     if q is None and q_out is not None:
         raise ValueError(f"{what}: q_out without q")
@@ -335,7 +337,7 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     R = 0
     if cos_sin is not None:
         R = cos_sin.shape[-1] if cos_sin.dim() == 2 else 0
-        if cos_sin.dim() != 2 or cos_sin.shape[0] == 0 or R == 0 or R > D or R % 16 != 0:
+        if R == 0 or cos_sin.shape[0] == 0 or R > D or R % 16 != 0:
             raise ValueError(f"{what}: cos_sin [positions, R] with R a multiple of 16 up to {D}, got "
                              f"{tuple(cos_sin.shape)}")
         _lib.dtype_code(cos_sin)
@@ -362,7 +364,7 @@ def append_paged_kv(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_c
     qts = qhs = ots = ohs = 0
     if q is not None:
         q, qts, qhs = _rows(q)
-        ots, ohs = _places(ret)
+        ots, ohs = (H * D, D) if q_out is None else _places(ret)
     slot_mapping = slot_mapping.contiguous()
     cs = (None, 0, None, 0, 0, 0)
     if cos_sin is not None:
@@ -412,7 +414,7 @@ def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
             return paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, scale, out=out,
                                           k_scales=k_scales, v_scales=v_scales)
     q, qts, qhs = _rows(q)
-    ots, ohs = _places(o)
+    ots, ohs = (H * D, D) if out is None else _places(o)
     eight = "" if k_scales is None else "8"
     ws, ws_bytes = _workspace(f"hmx_paged_attention_decode{eight}_workspace_bytes", q, N, H, HKV, D,
                               block_table.shape[1] * k_cache.shape[1])
@@ -467,7 +469,7 @@ def shared_prefix_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cac
     if N == 0:
         return _forward_only(what, o, out, *ins)
     q, qts, qhs = _rows(q)
-    ots, ohs = _places(o)
+    ots, ohs = (H * D, D) if out is None else _places(o)
     page = k_cache.shape[1]
     ws, ws_bytes = _workspace("hmx_shared_prefix_decode_workspace_bytes", q, N, M, H, HKV, D,
                               block_table.shape[1] * page, prefix_table.shape[1] * page)
@@ -518,7 +520,7 @@ def paged_causal_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
     if T == 0:
         return _forward_only(what, o, out, *ins)
     q, qts, qhs = _rows(q)
-    ots, ohs = _places(o)
+    ots, ohs = (H * D, D) if out is None else _places(o)
     eight = "" if k_scales is None else "8"
     ws, ws_bytes = _workspace(f"hmx_paged_causal_attention{eight}_workspace_bytes", q, N, T, H, HKV, D,
                               block_table.shape[1] * k_cache.shape[1])
