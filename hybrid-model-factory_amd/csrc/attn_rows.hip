@@ -14,9 +14,9 @@
 // launch from fp32 shares.
 //
 // A worker's four waves take KT keys in turn; nothing is shared between them until a block's
-// share ends.  K and V rows go straight into the wave's own ring in LDS, RING - 1 turns ahead
-// (the pages' numbers one turn before that), and are read there as the A operands of
-// S^T = K Q^T and (transposed) of O^T = V^T P^T.
+// share ends.  K and V rows go straight into the wave's own ring in LDS, RING - 1 turns ahead,
+// and are read there as the A operands of S^T = K Q^T and (transposed) of O^T = V^T P^T.  Where
+// they lie is formed for 64 times 16 keys at once, a lane each.
 // A cache of 8 bits is widened where its fragments are read (every e4m3 value is a bf16 and an
 // fp16 value); a key's scale multiplies its scores, and its probabilities before their product
 // with V, both in fp32, so neither type's range matters.  V's fragments come from the
@@ -294,34 +294,47 @@ __device__ __forceinline__ void attn_rows(const Args& a, char* smem, Shared<D, Q
     // turn x of the wave's: keys k_beg + (x NW + wave) KT ..; live: which of its rows are keys
     const int turns = k_end - k_beg > wave * KT ? (k_end - k_beg - wave * KT + NW * KT - 1) / (NW * KT) : 0;
     uint32_t live[RING];
-    struct Ids { int p[NH], id[NH]; };
-    // the pages of turn x's halves, of the last key's where it lies behind the last
-    auto ids_of = [&](int x) __attribute__((always_inline)) {
-      Ids r;
-#pragma unroll
-      for (int s = 0; s < NH; ++s) {
-        r.p[s] = __builtin_amdgcn_readfirstlane(fdiv(min(k_beg + (x * NW + wave) * KT + 16 * s, (k_end - 1) & ~15), a.pages.page));
-        r.id[s] = uniform_load(table, r.p[s]);
-      }
-      return r;
+    // The places of 64 halves on: lane i holds half i's first row of K and of V, its page and the
+    // row's place there; good: the halves whose pages lie in the cache.  The pages' numbers are
+    // asked for 64 halves ahead, and arrive with rows that are waited for anyway.
+    constexpr int TURNS = 64 / NH;
+    const char *kat = nullptr, *vat = nullptr;
+    int at_id = 0, at_in = 0, ahead = 0;
+    uint64_t good = 0;
+    auto row_at = [&](int x) __attribute__((always_inline)) {   // of the lane's half; the last key's where it lies behind it
+      return min(k_beg + ((x + lane / NH) * NW + wave) * KT + 16 * (lane % NH), (k_end - 1) & ~15);
     };
-    auto fetch = [&](int x, const Ids& ids) __attribute__((always_inline)) {
+    auto places = [&](int x) __attribute__((always_inline)) {
+      const int r = row_at(x), p = fdiv(r, a.pages.page);
+      const bool in_cache = (unsigned)ahead < (unsigned)a.pages.num_pages;
+      at_id = in_cache ? ahead : 0;
+      at_in = r - p * a.pages.page.d;
+      good = __ballot(in_cache);
+      kat = kbase + at_id * a.pages.k_ps + at_in * a.pages.k_ts;
+      vat = vbase + at_id * a.pages.v_ps + at_in * a.pages.v_ts;
+      ahead = table[fdiv(row_at(x + TURNS), a.pages.page)];
+    };
+    auto lane_ptr = [&](const char* p, int i) __attribute__((always_inline)) {
+      const uint64_t x = (uint64_t)p;
+      return (const char*)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)x, i) |
+                           (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), i) << 32);
+    };
+    if (whole_pages) ahead = table[fdiv(row_at(0), a.pages.page)];
+    auto fetch = [&](int x) __attribute__((always_inline)) {
       const int k0 = k_beg + (x * NW + wave) * KT;
       const uint32_t lds = ring_at + (x % RING) * TURN;
       const int n = k_end - k0;
       uint32_t mask = n >= KT ? ALL : (1u << n) - 1;
       if (whole_pages) {
         // rows behind the last key are the page's own: what they hold is masked
+        const int h = x % TURNS * NH;
+        if (h == 0) places(x);
         const char *kb[NH], *vb[NH];
-        const uint8_t* sc[2];
 #pragma unroll
         for (int s = 0; s < NH; ++s) {
-          int64_t id = ids.id[s];
-          if ((uint32_t)ids.id[s] >= (uint32_t)a.pages.num_pages) id = 0, mask &= ~(0xffffu << 16 * s);
-          const int64_t in = min(k0 + 16 * s, (k_end - 1) & ~15) - ids.p[s] * a.pages.page.d;
-          kb[s] = uniform_ptr(kbase + id * a.pages.k_ps + in * a.pages.k_ts);
-          vb[s] = uniform_ptr(vbase + id * a.pages.v_ps + in * a.pages.v_ts);
-          if constexpr (Q8) sc[s] = sbase + id * sps + in + l16;
+          kb[s] = lane_ptr(kat, h + s);
+          vb[s] = lane_ptr(vat, h + s);
+          if (!((good >> (h + s)) & 1)) mask &= ~(0xffffu << 16 * s);
         }
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
@@ -333,7 +346,11 @@ __device__ __forceinline__ void attn_rows(const Args& a, char* smem, Shared<D, Q
           const int r = i * RI + lane / NC, c = lane % NC;
           dma16(lds + KV + i * 1024, vb[i * RI / 16], (uint32_t)((r & 15) * (int)a.pages.v_ts + vchunk(r, c)));
         }
-        if constexpr (Q8) dma1(lds + 2 * KV, lane & 16 ? sc[1] : sc[0]);
+        if constexpr (Q8) {
+          const int i0 = __builtin_amdgcn_readlane(at_id, h), i1 = __builtin_amdgcn_readlane(at_id, h + 1);
+          const int n0 = __builtin_amdgcn_readlane(at_in, h), n1 = __builtin_amdgcn_readlane(at_in, h + 1);
+          dma1(lds + 2 * KV, sbase + (lane & 16 ? i1 : i0) * sps + ((lane & 16 ? n1 : n0) + l16));
+        }
       } else {
         int64_t in;
         auto page_of = [&](int r) __attribute__((always_inline)) {   // of row r, -1 outside the cache, and its place
@@ -355,7 +372,6 @@ __device__ __forceinline__ void attn_rows(const Args& a, char* smem, Shared<D, Q
       }
       return mask;
     };
-    Ids next = ids_of(RING - 1);
     // x is a multiple of RING plus the constant i: live[] stays in registers
     auto turn = [&](int x, int i) __attribute__((always_inline)) {
       if (x + RING - 2 < turns) dma_wait<(RING - 2) * (2 * NL + (Q8 ? 1 : 0))>();
@@ -364,8 +380,7 @@ __device__ __forceinline__ void attn_rows(const Args& a, char* smem, Shared<D, Q
       char* tile = ring + i * TURN;
       const uint32_t mask = live[i];
       if (x + RING - 1 < turns) {
-        live[(i + RING - 1) % RING] = fetch(x + RING - 1, next);
-        next = ids_of(x + RING);
+        live[(i + RING - 1) % RING] = fetch(x + RING - 1);
       }
       const int k0 = k_beg + (x * NW + wave) * KT;
       const bool edge = k0 + KT - 1 > kfirst;   // some row's keys end before the turn's last
@@ -378,16 +393,14 @@ __device__ __forceinline__ void attn_rows(const Args& a, char* smem, Shared<D, Q
         if (Q8 && lane >= 32 && !((mask >> (lane - 32)) & 1)) *reinterpret_cast<uint32_t*>(tile + 2 * KV + 4 * lane) = 0;
       }
       if constexpr (Q8) {
-        if (edge && !prefix) {
+        if (edge && kfirst < keys - 1) {
           // nor may a NaN spoil the rows that do not attend it: they are brought to those that do below
 #pragma unroll
           for (int z = 0; z < NL; ++z) {
             uint32_t* p = reinterpret_cast<uint32_t*>(tile + KV + (z * 64 + lane) * 16);
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
-              uint32_t v = p[y], n = 0;
-#pragma unroll
-              for (int b8 = 0; b8 < 32; b8 += 8) n |= nan8(v >> b8) ? 0xffu << b8 : 0u;
+              const uint32_t v = p[y], n = nan_bytes(v);
               if (n) {
                 p[y] = v & ~n;
                 bad = true;
@@ -474,14 +487,9 @@ __device__ __forceinline__ void attn_rows(const Args& a, char* smem, Shared<D, Q
         }
       }
     };
-    {
-      Ids ids[RING - 1];                    // all asked for before the first is used
 #pragma unroll
-      for (int i = 0; i < RING - 1; ++i) ids[i] = ids_of(i);
-#pragma unroll
-      for (int i = 0; i < RING - 1; ++i)
-        if (i < turns) live[i] = fetch(i, ids[i]);
-    }
+    for (int i = 0; i < RING - 1; ++i)
+      if (i < turns) live[i] = fetch(i);
     for (int x = 0; x < turns; x += RING) {
 #pragma unroll
       for (int i = 0; i < RING; ++i)

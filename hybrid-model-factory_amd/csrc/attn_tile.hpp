@@ -38,6 +38,11 @@ __device__ __forceinline__ bool any_nonfinite(u32x4 x) {
 }
 // whether a byte of a cache of 8 bits is e4m3's NaN
 __device__ __forceinline__ bool nan8(uint32_t x) { return (x & 0x7f) == 0x7f; }
+// and of four bytes, 0xff for each that is
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t x) {
+  const uint32_t n = ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+  return n | (n - (n >> 7));
+}
 // One key's row of k or v; NULL where its page lies outside the cache.
 template <typename T, bool PAGED>
 __device__ __forceinline__ const T* key_row(const FwdArgs& a, const Tile& t, int kvh, int j, bool value) {
@@ -341,9 +346,7 @@ __device__ __forceinline__ void attn_fwd(const FwdArgs& a, char* smem, FwdShared
         for (int i = 0; i < NP; ++i)
 #pragma unroll
           for (int z = 0; z < 2; ++z) {
-            uint32_t n = 0;
-#pragma unroll
-            for (int b = 0; b < 32; b += 8) n |= nan8(x[i][z] >> b) ? 0xffu << b : 0u;
+            const uint32_t n = nan_bytes(x[i][z]);
             const bool key = (vlive >> ((lane + 64 * i) / NC)) & 1;
             bad |= key && edge && n;
             x[i][z] = key ? (edge ? x[i][z] & ~n : x[i][z]) : 0;
