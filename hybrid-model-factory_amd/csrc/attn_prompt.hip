@@ -29,9 +29,11 @@ namespace attn {
 
 template <typename T, int D, bool PAGED, bool Q8 = false>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_fwd_kernel(FwdArgs a) {
-  __shared__ __align__(1024) char smem[FwdShared<D, Q8>::BYTES];
-  __shared__ FwdShared<D, Q8> flags;
-  attn_fwd<T, D, PAGED, Q8, false>(a, smem, flags, blockIdx.x, gridDim.x);
+  constexpr bool PREFIX = false;
+  __shared__ __align__(1024) char smem[tile_bytes<D, Q8>()];
+  __shared__ int s_bad, s_skip[4];
+  const unsigned block = blockIdx.x, blocks = gridDim.x;
+#include "attn_tile_body.hpp"
 }
 
 // The splits' shares of a row joined: sum_s 2^(m_s - m) O_s / sum_s 2^(m_s - m) l_s.  The

@@ -572,17 +572,23 @@ __global__ __launch_bounds__(64 * NW, OCC) void attn_rows_kernel(Args a) {
 template <typename T, int D, bool Q8>
 __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void attn_shared_kernel(Args a, FwdArgs f, int tiles, int blocks) {
   constexpr int RING = D == 128 ? 2 : 3;
-  constexpr int BYTES = FwdShared<D, Q8>::BYTES > Shared<D, Q8, RING>::BYTES ? FwdShared<D, Q8>::BYTES : Shared<D, Q8, RING>::BYTES;
+  constexpr int BYTES = tile_bytes<D, Q8>() > Shared<D, Q8, RING>::BYTES ? tile_bytes<D, Q8>() : Shared<D, Q8, RING>::BYTES;
   __shared__ __align__(1024) char smem[BYTES];
   __shared__ Shared<D, Q8, RING> shared;
-  __shared__ FwdShared<D, Q8> flags;
+  __shared__ int s_bad, s_skip[4];
   const int both = 2 * min((tiles + 7) >> 3, (blocks + 7) >> 3), at = blockIdx.x >> 3;
   const bool tile = at < both ? !(at & 1) : tiles > blocks;
   const int i = (at < both ? at >> 1 : at - (both >> 1)) * 8 + (blockIdx.x & 7);
-  if (tile) {
-    if (i < tiles) attn_fwd<T, D, true, Q8, true>(f, smem, flags, i, tiles);
-  } else {
+  if (!tile) {
     if (i < blocks) attn_rows<T, D, Q8, true, RING>(a, smem, shared, i);
+    return;
+  }
+  if (i >= tiles) return;
+  {
+    constexpr bool PAGED = true, PREFIX = true;
+    const FwdArgs& a = f;
+    const unsigned block = i, blocks = tiles;
+#include "attn_tile_body.hpp"
   }
 }
 
