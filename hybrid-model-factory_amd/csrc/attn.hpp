@@ -123,12 +123,25 @@ __device__ __forceinline__ float q4_max(float a) {
 __device__ __forceinline__ uint32_t lds_addr(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)(p);
 }
+// ONCE: rows that nobody reads again, past the caches' allocation (256 sequences to 8192 keys in
+// 8 bits, other caches' rows read in between: 512 -> 477 us; 64 to 2100: 48 -> 44; rows of half a
+// line, whose other half another workgroup reads, 28 -> 30, so not those).
+template <bool ONCE = false>
 __device__ __forceinline__ void dma16(uint32_t lds, const char* base, uint32_t off) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+                 :: "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(base) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                :: "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(off), "s"(base) : "memory");
 }
+template <bool ONCE = false>
 __device__ __forceinline__ void dma16(uint32_t lds, const char* at) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+  if constexpr (ONCE)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt"
+                 :: "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(at) : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                :: "s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(at) : "memory");
 }
 __device__ __forceinline__ void dma4(uint32_t lds, const char* at) {   // 4 bytes a lane, to lds + 4 l

@@ -179,6 +179,7 @@ __device__ __forceinline__ void attn_rows(const Args& a, char* smem, Shared<D, Q
   // line once (two sequences to 131072 keys, 14 / 2 heads of 64: 38.5 -> 29.7 us); rows of whole
   // lines are better spread (256 sequences to 8192 keys: 483 us, by worker 500).
   constexpr bool BY_WORKER = ROW < 128;
+  constexpr bool ONCE = !SHARES && ROW >= 128;   // (a prefix is read by several blocks)
   const int eights = BY_WORKER ? (a.W ? a.W : a.N) & ~7 : 0;
   const bool in8 = blk < eights * a.HKV;
   const int rem = in8 ? blk % (8 * a.HKV) : blk - eights * a.HKV;
@@ -339,12 +340,12 @@ __device__ __forceinline__ void attn_rows(const Args& a, char* smem, Shared<D, Q
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
           const int r = i * RI + lane / NC, c = lane % NC;
-          dma16(lds + i * 1024, kb[i * RI / 16], (uint32_t)((r & 15) * (int)a.pages.k_ts + kchunk(r, c)));
+          dma16<ONCE>(lds + i * 1024, kb[i * RI / 16], (uint32_t)((r & 15) * (int)a.pages.k_ts + kchunk(r, c)));
         }
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
           const int r = i * RI + lane / NC, c = lane % NC;
-          dma16(lds + KV + i * 1024, vb[i * RI / 16], (uint32_t)((r & 15) * (int)a.pages.v_ts + vchunk(r, c)));
+          dma16<ONCE>(lds + KV + i * 1024, vb[i * RI / 16], (uint32_t)((r & 15) * (int)a.pages.v_ts + vchunk(r, c)));
         }
         if constexpr (Q8) {
           const int i0 = __builtin_amdgcn_readlane(at_id, h), i1 = __builtin_amdgcn_readlane(at_id, h + 1);
@@ -365,8 +366,8 @@ __device__ __forceinline__ void attn_rows(const Args& a, char* smem, Shared<D, Q
         for (int i = 0; i < NL; ++i) {
           const int r = i * RI + lane / NC, c = lane % NC;
           const int64_t id = max(page_of(r), 0);
-          dma16(lds + i * 1024, kbase + id * a.pages.k_ps + in * a.pages.k_ts + kchunk(r, c));
-          dma16(lds + KV + i * 1024, vbase + id * a.pages.v_ps + in * a.pages.v_ts + vchunk(r, c));
+          dma16<ONCE>(lds + i * 1024, kbase + id * a.pages.k_ps + in * a.pages.k_ts + kchunk(r, c));
+          dma16<ONCE>(lds + KV + i * 1024, vbase + id * a.pages.v_ps + in * a.pages.v_ts + vchunk(r, c));
         }
         if constexpr (Q8) dma1(lds + 2 * KV, sc);
       }
