@@ -7,7 +7,9 @@
 // Layout: as where the cache is filled (paged_kv.hip) a thread owns two 8-element chunks of a
 // head that hold whole pairs, forms its eight angles once and walks `per` heads of its token
 // with their cosines and sines in registers, BATCH heads' loads ahead of their stores.
-// Bound by memory: q and k in and out.
+// Bound by memory: q and k in and out.  Measured: 8 x 4096 tokens, 32 / 8 heads of 128, 140 us,
+// 4.8 TB/s, what a large copy reaches; 100003 tokens of 16 / 4 heads, half of each turned,
+// 189 us, 5.4 TB/s; 197 tokens 5 us, a launch.
 #include "attn.hpp"
 
 namespace hmx {
@@ -39,7 +41,20 @@ __device__ __forceinline__ double freq_at(const void* p, int i, int is64) {
   return is64 ? static_cast<const double*>(p)[i] : (double)static_cast<const float*>(p)[i];
 }
 
-template <typename T, int D>
+template <typename V, bool FAR> __device__ __forceinline__ V load16(const char* p) {
+  typedef attn::u32x4 u;
+  if constexpr (FAR) return __builtin_bit_cast(V, __builtin_nontemporal_load(reinterpret_cast<const u*>(p)));
+  else return *reinterpret_cast<const V*>(p);
+}
+template <bool FAR, typename V> __device__ __forceinline__ void store16(char* p, V x) {
+  typedef attn::u32x4 u;
+  if constexpr (FAR) __builtin_nontemporal_store(__builtin_bit_cast(u, x), reinterpret_cast<u*>(p));
+  else *reinterpret_cast<V*>(p) = x;
+}
+
+// FAR: past the caches' allocation, where q and k in and out are more than they hold (100003
+// tokens, 16 / 4 heads of 128: 202 -> 189 us; 8192 such tokens, which they hold, 18.2 -> 20.9).
+template <typename T, int D, bool FAR>
 __global__ __launch_bounds__(256) void rotary_kernel(Args a) {
   typedef typename attn::El<T>::v8 v8;
   constexpr int TPR = D / 16;             // threads of a row
@@ -50,19 +65,21 @@ __global__ __launch_bounds__(256) void rotary_kernel(Args a) {
   if (n >= a.tokens) return;
   const int b = attn::fdiv(n, a.T);
   const int64_t t = n - (int64_t)b * a.T.d;
-  const int rc = a.R >> 4;                // chunk pairs that rotate
-  const bool rot = j < rc;
-  // halves pair chunk j with j + rc; what does not rotate, and pairs inside a chunk, take neighbours
-  const int c0 = rot ? (a.inter ? 2 * j : j) : 2 * j;
-  const int c1 = rot && !a.inter ? j + rc : c0 + 1;
+  // Halves pair chunk j with j + rc; chunks that hold whole pairs, and those that do not
+  // rotate, are paired so that a row's lanes read and write neighbouring chunks.
+  const int rc = a.R >> 4;
+  const int c0 = a.inter || j < rc ? j : 2 * rc + j - rc, c1 = a.inter ? j + TPR : j < rc ? j + rc : c0 + TPR - rc;
+  const bool rot0 = a.inter ? c0 < 2 * rc : j < rc, rot1 = a.inter ? c1 < 2 * rc : j < rc;
   float cs[8], sn[8];
-  if (rot) {
+  if (rot0) {
     const int64_t at = b * a.pos_stride + t;
     const double pos = a.pos64 ? (double)static_cast<const int64_t*>(a.pos)[at] : (double)static_cast<const int32_t*>(a.pos)[at];
-    // pair i of the chunks is pair 8 j + i of the head either way
+    // halves: pair 8 j + i of the head; neighbours: pairs 4 c .. 4 c + 3 of either chunk
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      turn_of(pos, freq_at(a.inv, 8 * j + i, a.inv64), a.factor, cs[i], sn[i]);
+      if (a.inter && i >= 4 && !rot1) break;
+      const int pair = a.inter ? 4 * (i < 4 ? c0 : c1) + (i & 3) : 8 * j + i;
+      turn_of(pos, freq_at(a.inv, pair, a.inv64), a.factor, cs[i], sn[i]);
       if (a.back) sn[i] = -sn[i];
     }
   }
@@ -74,14 +91,14 @@ __global__ __launch_bounds__(256) void rotary_kernel(Args a) {
       const int h = min(h0 + i, h1 - 1);
       const char* p = h < a.H ? a.q.in + b * a.q.bs + t * a.q.ts + h * a.q.hs
                               : a.k.in + b * a.k.bs + t * a.k.ts + (h - a.H) * a.k.hs;
-      x[i] = *reinterpret_cast<const v8*>(p + 16 * c0);
-      y[i] = *reinterpret_cast<const v8*>(p + 16 * c1);
+      x[i] = load16<v8, FAR>(p + 16 * c0);
+      y[i] = load16<v8, FAR>(p + 16 * c1);
     }
 #pragma unroll
     for (int i = 0; i < BATCH; ++i) {
       const int h = h0 + i;
       if (h >= h1) break;
-      if (rot) {
+      if (rot0) {
         float u[8], w[8];
 #pragma unroll
         for (int z = 0; z < 8; ++z) {
@@ -93,6 +110,7 @@ __global__ __launch_bounds__(256) void rotary_kernel(Args a) {
           for (int z = 0; z < 4; ++z) {
             x[i][2 * z] = (T)(u[2 * z] * cs[z] - u[2 * z + 1] * sn[z]);
             x[i][2 * z + 1] = (T)(u[2 * z + 1] * cs[z] + u[2 * z] * sn[z]);
+            if (!rot1) continue;
             y[i][2 * z] = (T)(w[2 * z] * cs[4 + z] - w[2 * z + 1] * sn[4 + z]);
             y[i][2 * z + 1] = (T)(w[2 * z + 1] * cs[4 + z] + w[2 * z] * sn[4 + z]);
           }
@@ -106,10 +124,16 @@ __global__ __launch_bounds__(256) void rotary_kernel(Args a) {
       }
       char* p = h < a.H ? a.q.out + b * a.q.obs + t * a.q.ots + h * a.q.ohs
                         : a.k.out + b * a.k.obs + t * a.k.ots + (h - a.H) * a.k.ohs;
-      *reinterpret_cast<v8*>(p + 16 * c0) = x[i];
-      *reinterpret_cast<v8*>(p + 16 * c1) = y[i];
+      store16<FAR>(p + 16 * c0, x[i]);
+      store16<FAR>(p + 16 * c1, y[i]);
     }
   }
+}
+
+template <typename T, int D>
+static void launch(const Args& a, bool far, dim3 grid, hipStream_t s) {
+  if (far) hipLaunchKernelGGL((rotary_kernel<T, D, true>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((rotary_kernel<T, D, false>), grid, dim3(256), 0, s, a);
 }
 
 __global__ __launch_bounds__(256) void table_kernel(const void* inv, int inv64, float factor, int64_t positions, int R,
@@ -173,12 +197,13 @@ extern "C" int hmx_rotary_embedding(const void* q, int64_t q_batch_stride, int64
   a.per = (a.per + 3) / 4 * 4;
   const dim3 grid((unsigned)bx, (unsigned)((heads + a.per - 1) / a.per));
   hipStream_t s = (hipStream_t)stream;
+  const bool far = 4ll * a.tokens * heads * D > 256ll << 20;   // of the last cache's 256 MB
   if (dtype == HMX_BF16) {
-    if (D == 64) hipLaunchKernelGGL((rotary::rotary_kernel<bf16, 64>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((rotary::rotary_kernel<bf16, 128>), grid, dim3(256), 0, s, a);
+    if (D == 64) rotary::launch<bf16, 64>(a, far, grid, s);
+    else rotary::launch<bf16, 128>(a, far, grid, s);
   } else {
-    if (D == 64) hipLaunchKernelGGL((rotary::rotary_kernel<f16, 64>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((rotary::rotary_kernel<f16, 128>), grid, dim3(256), 0, s, a);
+    if (D == 64) rotary::launch<f16, 64>(a, far, grid, s);
+    else rotary::launch<f16, 128>(a, far, grid, s);
   }
   return check_launch("hmx_rotary_embedding");
 }
