@@ -202,7 +202,8 @@ static int paged_causal_attention(const void* q, int64_t q_token_stride,
   HMX_REQUIRE(need == 0 || (workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need), HMX_EINVAL,
               "hmx_paged_causal_attention: workspace of %zu bytes is too small", workspace_bytes);
   if (scales && attn::few_rows(N, T, H / HKV)) {
-    HMX_REQUIRE(T * H < (1ll << 31), HMX_EUNSUPPORTED, "hmx_paged_causal_attention8: %lld tokens", (long long)T);
+    HMX_REQUIRE(T * H < (1ll << 31) && (int64_t)N * H < (1ll << 30), HMX_EUNSUPPORTED,
+                "hmx_paged_causal_attention8: %lld tokens of %d sequences", (long long)T, N);
     attn::launch_few_rows(attn::FewRows{q, o, q_token_stride, q_head_stride, o_token_stride, o_head_stride, dtype,
                                         attn::make_pages(*cache, scales), cu_seqlens, N, (int32_t)T, H, HKV, D, max_keys,
                                         scale, fill_gaps, static_cast<float*>(workspace)},

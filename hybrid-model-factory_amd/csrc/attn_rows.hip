@@ -41,8 +41,10 @@ constexpr int OCC = 2;
 // 8; eight sequences to 129 keys behind one prefix of 4096 35 -> 21 either way).
 constexpr int SETUP = 4;
 constexpr int MIN_UNITS = 4; // of a worker: below that the joining costs more than it gains
-// Where a table holds no more keys than this, a worker takes whole sequences: one launch and
-// no scan of the lengths.
+// Where a table holds no more keys than this, a worker takes one sequence, or of several tokens
+// one block: one launch, and no scan of the lengths (64 sequences to 1024 keys, 32 / 8 heads of
+// 128, 4 tokens each 28 us, cut evenly and joined 36; one of 190 tokens among 63 of one 40, 43,
+// by whole sequences 585).
 constexpr int SHORT_KEYS = 1024;
 
 struct Args {
@@ -53,7 +55,8 @@ struct Args {
   const int32_t* cu;                // their tokens; NULL: sequence n has token n alone
   const int32_t *p_table, *p_lens, *p_cu;   // M prefixes (p_cu NULL: one for all tokens)
   int64_t p_stride;
-  int32_t p_width, M, N, T, HKV, W; // W = 0: worker w takes sequence w
+  int32_t p_width, M, N, T, HKV, W; // W = 0: worker w takes sequence w, or with cu the w-th block
+  int32_t blocks;                   // workgroups of a key/value head
   FastDiv G;
   float c;                          // scale log2(e)
   int32_t fill;                     // rows of no sequence become 0
@@ -97,15 +100,16 @@ __device__ __forceinline__ int64_t own_slot(const Args& a, int e, const Entry& x
                                : (int64_t)a.N * per + (((int64_t)x.bos * a.G.d) >> 4) + e + b);
 }
 
-// The list of units, seen by one workgroup: `total` units, and where unit w * per lies, per
-// being the workers' share: its entry and that entry's first unit.  Every thread adds up the
-// entries of its own run.  All threads call it; sh holds 8 int64.
-struct Place { int64_t total, per; int entry; int64_t first; };
-__device__ __forceinline__ Place find_share(const Args& a, int w, int64_t* sh) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, E = a.M + a.N;
+// A list of the entries' work, seen by one workgroup: the total, and where unit at(total) lies:
+// its entry and that entry's first unit (none past the total: nothing to rely on).  Every thread
+// adds up the entries of its own run.  All threads call it; sh holds 8 int64.
+struct Place { int64_t total, at; int entry; int64_t first; };
+template <typename Work, typename At>
+__device__ __forceinline__ Place find_place(int E, Work work, At at_of, int64_t* sh) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int run = (E + 255) >> 8, n0 = min(tid * run, E), n1 = min(n0 + run, E);
   int64_t mine = 0;
-  for (int n = n0; n < n1; ++n) mine += work_of(a, entry_of(a, n));
+  for (int n = n0; n < n1; ++n) mine += work(n);
   int64_t x = mine;
   for (int d = 1; d < 64; d <<= 1) {
     const int64_t y = __shfl_up(x, d, 64);
@@ -117,11 +121,10 @@ __device__ __forceinline__ Place find_share(const Args& a, int w, int64_t* sh) {
   for (int i = 0; i < wave; ++i) before += sh[i];
   Place p;
   p.total = sh[0] + sh[1] + sh[2] + sh[3];
-  p.per = units_per(a, p.total);
-  const int64_t at = w * p.per;
-  if (at >= before && at < before + mine) {   // one thread, where there is such a unit
+  p.at = at_of(p.total);
+  if (p.at >= before && p.at < before + mine) {   // one thread, where there is such a unit
     int n = n0;
-    for (int64_t u; (u = work_of(a, entry_of(a, n))) <= at - before; ++n) before += u;
+    for (int64_t u; (u = work(n)) <= p.at - before; ++n) before += u;
     sh[4] = n;
     sh[5] = before;
   }
@@ -148,7 +151,7 @@ template <int D, bool Q8, int RING> struct Shared {
   static constexpr int KT = Q8 ? 32 : 16;
   static constexpr int KV = KT * D * (Q8 ? 1 : 2), TURN = 2 * KV + (Q8 ? 256 : 0);
   static constexpr int BYTES = NW * RING * TURN;     // the rings, then the shares [16][D] in fp32
-  static_assert(NW == 4 && RING * TURN >= 16 * D * 4, "find_share, and the shares in LDS");
+  static_assert(NW == 4 && RING * TURN >= 16 * D * 4, "find_place, and the shares in LDS");
   float ml[NW][16][2];
   int64_t scan[8];
   int bad;                                  // the last share of whose keys some were spoiled
@@ -180,7 +183,7 @@ __device__ __forceinline__ void attn_rows(const Args& a, char* smem, Shared<D, Q
   // lines are better spread (256 sequences to 8192 keys: 483 us, by worker 500).
   constexpr bool BY_WORKER = ROW < 128;
   constexpr bool ONCE = !SHARES && ROW >= 128;   // (a prefix is read by several blocks)
-  const int eights = BY_WORKER ? (a.W ? a.W : a.N) & ~7 : 0;
+  const int eights = BY_WORKER ? a.blocks & ~7 : 0;
   const bool in8 = blk < eights * a.HKV;
   const int rem = in8 ? blk % (8 * a.HKV) : blk - eights * a.HKV;
   const int kvh = in8 ? rem >> 3 : rem % a.HKV;
@@ -196,16 +199,26 @@ __device__ __forceinline__ void attn_rows(const Args& a, char* smem, Shared<D, Q
   int e = __builtin_amdgcn_readfirstlane(w);
   int64_t first = 0, u_beg = 0, u_end;
   if (tid == 0) s_bad = 0;
-  if (!SHARES && a.cu && a.fill) {           // rows of no sequence, a workgroup every W-th (N-th) token
-    const int step = a.W ? a.W : a.N, beg = bound(a.cu, 0, a.T), end = bound(a.cu, a.N, a.T);
-    for (int t = w; t < beg; t += step) zero_rows(t, t + 1);
-    for (int t = end + w; t < a.T; t += step) zero_rows(t, t + 1);
+  if (!SHARES && a.cu && a.fill) {           // rows of no sequence, a workgroup every so many tokens
+    const int beg = bound(a.cu, 0, a.T), end = bound(a.cu, a.N, a.T);
+    for (int t = w; t < beg; t += a.blocks) zero_rows(t, t + 1);
+    for (int t = end + w; t < a.T; t += a.blocks) zero_rows(t, t + 1);
   }
-  if (!SHARES && a.W == 0) {
+  if (!SHARES && a.W == 0 && !a.cu) {
     const Entry x = entry_of(a, w);
     u_end = work_of(a, x);
     if (x.keys == 0) zero_rows(x.bos, x.bos + x.tokens);
     __syncthreads();                        // s_bad is clear
+  } else if (!SHARES && a.W == 0) {         // of all sequences' blocks the w-th
+    const Place pl = find_place(a.N, [&](int n) { return (int64_t)blocks_of(a, entry_of(a, n)); },
+                                [&](int64_t) { return (int64_t)w; }, s_scan);
+    if (pl.at >= pl.total) return;
+    e = __builtin_amdgcn_readfirstlane(pl.entry);
+    const Entry x = entry_of(a, e);
+    const int b = (int)(pl.at - pl.first);
+    if (x.keys == 0 && b == 0) zero_rows(x.bos, x.bos + x.tokens);
+    u_beg = (int64_t)b * (units_of(x) + SETUP);
+    u_end = x.keys == 0 ? u_beg : u_beg + units_of(x) + SETUP;
   } else {
     // rows without keys, a worker every W-th sequence
     if (!SHARES)
@@ -213,9 +226,11 @@ __device__ __forceinline__ void attn_rows(const Args& a, char* smem, Shared<D, Q
         const Entry x = entry_of(a, n);
         if (x.keys == 0) zero_rows(x.bos, x.bos + x.tokens);
       }
-    const Place pl = find_share(a, w, s_scan);
-    u_beg = w * pl.per;
-    u_end = min(pl.total, u_beg + pl.per);
+    int64_t per = 0;
+    const Place pl = find_place(a.M + a.N, [&](int n) { return work_of(a, entry_of(a, n)); },
+                                [&](int64_t total) { return w * (per = units_per(a, total)); }, s_scan);
+    u_beg = pl.at;
+    u_end = min(pl.total, u_beg + per);
     e = __builtin_amdgcn_readfirstlane(pl.entry);
     first = pl.first;
   }
@@ -712,7 +727,7 @@ static int64_t workers_of(int64_t N, int64_t T, int64_t G, int64_t HKV, int64_t 
 
 template <typename T, int D, bool Q8, bool SHARES>
 static void launch(const Args& a, const FwdArgs* f, const PrefixShares& pre, hipStream_t s) {
-  const int blocks = a.HKV * (a.W ? a.W : a.N);
+  const int blocks = a.HKV * a.blocks;
   if constexpr (SHARES) {
     if (f) {
       const int tiles = (int)(fwd_blocks(*f) * a.HKV);
@@ -806,6 +821,7 @@ void launch_few_rows(const FewRows& f, hipStream_t s) {
   a.pages = f.pages; a.cu = f.cu;
   a.N = f.N; a.T = f.T; a.HKV = f.HKV; a.G = fast_div(f.H / f.HKV);
   a.W = (int32_t)rows::workers_of(f.N, f.T, a.G.d, f.HKV, f.max_keys);
+  a.blocks = a.W ? a.W : (int32_t)((int64_t)f.T * a.G.d / 16 + f.N);   // (at most)
   a.c = f.scale * LOG2E; a.fill = f.fill;
   a.part = f.workspace; a.slots = 2ll * a.W;
   rows::launch_types<true, false>(a, f.dtype, f.D, s);
@@ -833,6 +849,7 @@ extern "C" int hmx_paged_attention_decode8(const void* q, int64_t q_token_stride
   HMX_REQUIRE(need == 0 || (workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need), HMX_EINVAL,
               "%s: workspace of %zu bytes is too small", what, workspace_bytes);
   a.W = (int32_t)attn::rows::workers_of(N, N, a.G.d, HKV, max_keys);
+  a.blocks = a.W ? a.W : N;
   a.slots = 2ll * a.W;
   a.part = static_cast<float*>(workspace);
   attn::rows::launch_types<true, false>(a, dtype, D, (hipStream_t)stream);
@@ -909,7 +926,7 @@ extern "C" int hmx_shared_prefix_decode(const void* q, int64_t q_token_stride, i
                   workspace_bytes >= hmx_shared_prefix_decode_workspace_bytes(N, M, H, HKV, D, max_keys, max_prefix),
               HMX_EINVAL, "%s: workspace of %zu bytes is too small", what, workspace_bytes);
   const SharedPlan plan = shared_plan(N, M, H, HKV, max_keys, max_prefix);
-  a.W = (int32_t)plan.W;
+  a.W = a.blocks = (int32_t)plan.W;
   a.slots = plan.slots;
   a.part = static_cast<float*>(workspace);
   const attn::PrefixShares pre{a.part + attn::rows::share_bytes(a.slots, HKV, D) / sizeof(float), (int64_t)N * H,
