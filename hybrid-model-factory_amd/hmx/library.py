@@ -27,6 +27,7 @@ import torch
 from torch import Tensor
 
 from . import ops
+from .ops.rotary import turn as _turn
 
 _FORWARD_ONLY = ("hmx kernels are forward-only: no backward is implemented for {}")
 
@@ -461,10 +462,8 @@ _forward_only(_shared, "shared_prefix_attention_decode")
 @torch.library.custom_op("hmx::rotary_embedding", mutates_args=())
 def _rotary(q: Tensor, k: Optional[Tensor], positions: Tensor, inv_freq: Tensor, factor: float,
             interleaved: bool, backward: bool) -> tuple[Tensor, Tensor]:
-    # backward: by minus the angle, which minus the positions are
     with torch.no_grad():
-        a, b = ops.rotary_embedding(q, k, -positions if backward else positions, inv_freq, factor=factor,
-                                    interleaved=interleaved)
+        a, b = _turn(q, k, positions, inv_freq, factor, interleaved, backward)
     return a, q.new_empty(0) if b is None else b
 
 

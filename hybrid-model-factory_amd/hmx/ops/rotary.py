@@ -155,14 +155,14 @@ class RotaryEmbedding(torch.autograd.Function):
     def backward(ctx, dq, dk):
         positions, inv_freq = ctx.saved_tensors
         # as a function of its own only where a graph of the gradients is asked for
-        turn = RotaryEmbedding.apply if torch.is_grad_enabled() else rotate
+        again = RotaryEmbedding.apply if torch.is_grad_enabled() else rotate
         needs_q, needs_k = ctx.needs_input_grad[:2]
         if dq is not None and needs_q:
-            dq, dk = turn(dq, dk if needs_k else None, positions, inv_freq, *ctx.args, not ctx.back)
+            dq, dk = again(dq, dk if needs_k else None, positions, inv_freq, *ctx.args, not ctx.back)
         else:
             dq = None
             if dk is not None:
-                dk = turn(dk, None, positions, inv_freq, *ctx.args, not ctx.back)[0] if needs_k else None
+                dk = again(dk, None, positions, inv_freq, *ctx.args, not ctx.back)[0] if needs_k else None
         return dq, dk, None, None, None, None, None
 
 
@@ -189,6 +189,13 @@ def rotary_embedding(q: torch.Tensor, k: torch.Tensor | None, positions: torch.T
     gradient is needed.  Returns both.
 
     Differentiable in q and k (hmx.RotaryEmbedding), not in the frequencies."""
+    return turn(q, k, positions, inv_freq, factor, interleaved, False, q_out, k_out)
+
+
+def turn(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor, factor: float,
+         interleaved: bool, backward: bool, q_out: torch.Tensor | None = None,
+         k_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """rotary_embedding; backward: by minus the angle."""
     what = "rotary_embedding"
     _refuse_tangents(what, q, k, inv_freq)
     if q.dim() not in (3, 4) or (k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2]
@@ -228,7 +235,7 @@ def rotary_embedding(q: torch.Tensor, k: torch.Tensor | None, positions: torch.T
     if _grad_of(q, k):
         if q_out is not None or k_out is not None:
             raise ValueError(f"{what}: q_out and k_out are not supported where a gradient is needed")
-        q, k = RotaryEmbedding.apply(q, k, positions, inv_freq, factor, interleaved, False)
+        q, k = RotaryEmbedding.apply(q, k, positions, inv_freq, factor, interleaved, backward)
     else:
-        q, k = rotate(q, k, positions, inv_freq, factor, interleaved, False, q_out, k_out)
+        q, k = rotate(q, k, positions, inv_freq, factor, interleaved, backward, q_out, k_out)
     return (q.squeeze(0), k if k is None else k.squeeze(0)) if flat else (q, k)

@@ -175,3 +175,18 @@ def test_captured_steps(dev):
         torch.cuda.synchronize()
         got = [x.clone() for x in out]
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+def test_registered_gradient_at_the_ends_of_int32(dev):
+    """The registered op's gradient turns by minus the angle at every position, the least int32
+    (which minus itself is itself) among them."""
+    from hmx import library
+    gen = torch.Generator().manual_seed(7)
+    q, do = randn(gen, 1, 3, 2, 64).to(dev).requires_grad_(), randn(gen, 1, 3, 2, 64).to(dev)
+    pos = torch.tensor([-2 ** 31, 2 ** 31 - 1, -5], dtype=torch.int32, device=dev)
+    inv, _ = hmx.rotary_frequencies(64, device=dev)
+    a, = torch.autograd.grad(library.rotary_embedding(q, None, pos, inv)[0], q, do)
+    b, = torch.autograd.grad(hmx.rotary_embedding(q, None, pos, inv)[0], q, do)
+    assert torch.equal(a, b)
+    ang = torch.remainder(pos.cpu().double()[:, None] * inv.cpu(), 2 * math.pi)   # off by 2^-21 of a radian
+    _check(a, do.cpu(), -ang, 1.0, False, "the ends")
