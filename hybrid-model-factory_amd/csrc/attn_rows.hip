@@ -583,8 +583,11 @@ __global__ __launch_bounds__(64 * NW, OCC) void attn_rows_kernel(Args a) {
 }
 
 // Many rows behind prefixes in tiles, and the sequences' own keys, in one launch: the first are
-// bound by the matrix cores, the second by memory, and workgroups of both kinds, eight of one
-// and eight of the other in turn, run at once.
+// bound by the matrix cores, the second by memory, and workgroups of both kinds, as many of one
+// and of the other in turn as there are compute units, run at once (256 sequences to 1031 keys
+// behind two prefixes to 16384, 32 / 8 heads of 128: 195 -> 190 us, in 8 bits 181 -> 162, with
+// eight of each in turn the first; 138 to 19 keys behind two of 666 28.4 -> 30.6).
+constexpr int IN_TURN = 256;
 template <typename T, int D, bool Q8>
 __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void attn_shared_kernel(Args a, FwdArgs f, int tiles, int blocks) {
   constexpr int RING = D == 128 ? 2 : 3;
@@ -592,9 +595,9 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 3 : 2) void attn_shared_kernel(A
   __shared__ __align__(1024) char smem[BYTES];
   __shared__ Shared<D, Q8, RING> shared;
   __shared__ int s_bad, s_skip[4];
-  const int both = 2 * min((tiles + 7) >> 3, (blocks + 7) >> 3), at = blockIdx.x >> 3;
+  const int both = 2 * min((tiles + IN_TURN - 1) / IN_TURN, (blocks + IN_TURN - 1) / IN_TURN), at = blockIdx.x / IN_TURN;
   const bool tile = at < both ? !(at & 1) : tiles > blocks;
-  const int i = (at < both ? at >> 1 : at - (both >> 1)) * 8 + (blockIdx.x & 7);
+  const int i = (at < both ? at >> 1 : at - (both >> 1)) * IN_TURN + blockIdx.x % IN_TURN;
   if (!tile) {
     if (i < blocks) attn_rows<T, D, Q8, true, RING>(a, smem, shared, i);
     return;
@@ -731,7 +734,7 @@ static void launch(const Args& a, const FwdArgs* f, const PrefixShares& pre, hip
   if constexpr (SHARES) {
     if (f) {
       const int tiles = (int)(fwd_blocks(*f) * a.HKV);
-      const dim3 grid((unsigned)(8 * ((tiles + 7) / 8 + (blocks + 7) / 8)));
+      const dim3 grid((unsigned)(IN_TURN * ((tiles + IN_TURN - 1) / IN_TURN + (blocks + IN_TURN - 1) / IN_TURN)));
       hipLaunchKernelGGL((attn_shared_kernel<T, D, Q8>), grid, dim3(64 * NW), 0, s, a, *f, tiles, blocks);
     }
   }
