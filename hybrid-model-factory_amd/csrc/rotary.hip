@@ -7,8 +7,8 @@
 // Layout: as where the cache is filled (paged_kv.hip) a thread owns two 8-element chunks of a
 // head that hold whole pairs, forms its eight angles once and walks `per` heads of its token
 // with their cosines and sines in registers, BATCH heads' loads ahead of their stores.
-// Bound by memory: q and k in and out.  Measured: 8 x 4096 tokens, 32 / 8 heads of 128, 140 us,
-// 4.8 TB/s, what a large copy reaches; 100003 tokens of 16 / 4 heads, half of each turned,
+// Bound by memory: q and k in and out.  Measured: 8 x 4096 tokens, 32 / 8 heads of 128, 136 us,
+// 4.9 TB/s, what a large copy reaches; 100003 tokens of 16 / 4 heads, half of each turned,
 // 189 us, 5.4 TB/s; 197 tokens 5 us, a launch.
 #include "attn.hpp"
 

@@ -39,6 +39,18 @@ def test_oracle_quantise_by_hand():
     assert torch.isnan(v[4, 0]) and v[4, 1] == 448.0 and v[5, 0] == 0.0
 
 
+@pytest.mark.parametrize("inter", [False, True])
+def test_oracle_rotation_as_complex_products(inter):
+    gen = torch.Generator().manual_seed(1)
+    x, ang = torch.randn(5, 3, 64, generator=gen).double(), torch.rand(5, 8, generator=gen).double() * 9
+    pairs = x[..., :16].unflatten(-1, (8, 2) if inter else (2, 8))
+    re, im = pairs.unbind(-1 if inter else -2)
+    z = torch.complex(re, im) * torch.polar(torch.full_like(ang, 1.5), ang)[:, None]
+    want = torch.stack([z.real, z.imag], -1 if inter else -2).flatten(-2)
+    got = ref.rotate_by(x, ang, 1.5, inter)
+    assert (got[..., :16] - want).abs().max() <= 2.0 ** -48 and torch.equal(got[..., 16:], x[..., 16:])
+
+
 def test_append_refusals():
     k = torch.zeros(5, 2, 64, dtype=BF)
     kc, vc, ks, vs = _cache8()
