@@ -20,8 +20,9 @@
 // on): one prompt of 32768, 16 / 4 heads of 128, 3.72 - 4.03 ms, 1.09 - 1.18 PFLOP/s (a large
 // matrix product reaches 1.22 - 1.26); packed prompts of 64-wide heads, whose exponentials weigh
 // twice as much against their products, 382 - 397 us, 0.83 - 0.86; pieces of prompts over pages
-// 842 - 902 us, 0.91 - 0.98, over a cache of 8 bits 949 - 987, 0.83 - 0.87; draft tokens of eight sequences to 16384 keys 63 - 75 us and the
-// joining 6 (76 us where every sequence's keys were cut into as many splits).
+// 842 - 902 us, 0.91 - 0.98, over a cache of 8 bits 949 - 987, 0.83 - 0.87; draft tokens of eight
+// sequences to 16384 keys 63 - 75 us and the joining 6 (76 us where every sequence's keys were cut
+// into as many splits).
 #include "attn_tile.hpp"
 
 namespace hmx {
