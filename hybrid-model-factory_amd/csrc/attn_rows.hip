@@ -769,7 +769,7 @@ static void launch_types(const Args& a, int32_t dtype, int32_t D, hipStream_t s,
 // The rows of N sequences, one token each, over the M prefixes that they share, in tiles.  Of
 // the two workgroups of a compute unit one takes tiles and one the sequences' own keys, so that
 // all run at once (256 sequences to 1031 keys behind two prefixes to 16384: 190 us, with twice as
-// many tiles 205).
+// many tiles 205, with twice as many workers 200).
 static Splits tile_splits(int64_t M, int64_t N, int64_t G, int HKV, int64_t max_prefix, bool packed) {
   const int32_t some = 0;
   const int64_t slots = tile_slots<BM>(packed ? &some : nullptr, M, N, G);
