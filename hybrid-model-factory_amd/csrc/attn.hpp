@@ -384,9 +384,11 @@ struct PrefixShares {
   int64_t rows;
   int32_t splits;
 };
-// Few new tokens a sequence over a cache of 8 bits (attn_rows.hip).  few_rows: they are where
-// each sequence's rows fill a block of 16 on average; the blocks are then at most twice the
-// sequences however unequal they are, so no order of long sequences is read often.
+// Few new tokens a sequence over a cache of 8 bits (attn_rows.hip).  few_rows: they are where each
+// sequence's rows fill a block of 16 on average; the blocks are then at most twice the sequences.
+// Against tiles of 128 rows, 32 / 8 heads of 128: 64 sequences of 4 tokens to 4096 keys 70 us, by tiles
+// 144; 255 of one and one of 512 tokens 380 and 472; at worst, all keys behind the one sequence
+// that has most of the tokens, 255 of 100 keys and 700 tokens behind 32768, 1755 and 954.
 struct FewRows {
   const void* q;
   void* o;
