@@ -31,6 +31,7 @@
 // heads of 64, 20; the joining launch 6 - 11.  Behind prefixes: eight to 129 keys behind 4096 13,
 // 256 to 1031 keys in 16 bits behind two to 16384 178, where one read of all and the products
 // alone would take 139.
+#include "attn_rows_plan.hpp"
 #include "attn_tile.hpp"
 
 namespace hmx {
@@ -325,7 +326,7 @@ __device__ __forceinline__ void attn_rows(const Args& a, char* smem, Shared<D, Q
     int at_id = 0, at_in = 0, ahead = 0;
     uint64_t good = 0;
     auto row_at = [&](int x) __attribute__((always_inline)) {   // of the lane's half; the last key's where it lies behind it
-      return min(k_beg + ((x + lane / NH) * NW + wave) * KT + 16 * (lane % NH), (k_end - 1) & ~15);
+      return half_row<NW, KT>(k_beg, k_end, x + lane / NH, wave, lane % NH);
     };
     auto places = [&](int x) __attribute__((always_inline)) {
       const int r = row_at(x), p = fdiv(r, a.pages.page);

@@ -1,0 +1,31 @@
+"""Ends of what the ops over caches of 8 bits and shared prefixes take: the longest table rows."""
+import pytest
+import torch
+
+import hmx
+
+pytestmark = pytest.mark.gpu
+BF, F16, F8 = torch.bfloat16, torch.float16, torch.float8_e4m3fn
+
+
+@pytest.mark.parametrize("eight", [True, False])
+def test_the_longest_table_rows(dev, eight):
+    """2^31 - 320 keys of one page of 64, listed over and over: rows asked for ahead of a share's end
+    pass 2^31.  Scores of 0 and whole values up to 8, so a wave's sums (2^20 keys) are exact, and
+    the mean is off by the joining of at most 512 workers' shares in fp32 and one rounding."""
+    page, D = 64, 64
+    keys = (1 << 31) - 320
+    gen = torch.Generator().manual_seed(0)
+    k, v = (torch.randint(0, 9, (1, page, 1, D), generator=gen).float() for _ in range(2))
+    kc, vc = (x.to(F8 if eight else BF).to(dev) for x in (k, v))
+    sc = {n: torch.full((1, 1, page), 127, dtype=torch.uint8, device=dev) for n in ("k_scales", "v_scales")} if eight else {}
+    table = torch.zeros(1, keys // page, dtype=torch.int32, device=dev)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)
+    n, q = i32(keys), torch.zeros(2, 4, D, dtype=BF, device=dev)
+    outs = [hmx.shared_prefix_attention_decode(q, kc, vc, table[:, :1].expand(2, 1), i32(0, 0), table, n, **sc)]
+    if eight:
+        outs += [hmx.paged_attention_decode(q[:1], kc, vc, table, n, **sc),
+                 hmx.paged_causal_attention(q, kc, vc, table, n, i32(0, 2), **sc)]
+    want = v[0, :, 0].double().mean(0)
+    for o in outs:
+        assert ((o.double().cpu() - want).abs() <= (2.0 ** -8 + 520 * 2.0 ** -24) * want).all()
