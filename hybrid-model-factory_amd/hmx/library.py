@@ -473,6 +473,8 @@ def _(q, k, positions, inv_freq, factor, interleaved, backward):
 
 
 def _rotary_setup(ctx, inputs, output):
+    if ctx.needs_input_grad[3]:
+        raise NotImplementedError("rotary_embedding: no gradient of the frequencies is implemented")
     _, k, positions, inv_freq, *ctx.args, ctx.back = inputs
     ctx.has_k = k is not None
     ctx.save_for_backward(positions, inv_freq)
