@@ -621,11 +621,18 @@ def causal_attention(q, k, v, scale=None, cu_seqlens=None):
     return torch.ops.hmx.causal_attention(q, k, v, scale, cu_seqlens)[0]
 
 
+def _eight(k_scales, v_scales) -> bool:
+    """Whether the scales of a cache of 8 bits are given; one of the two alone is refused."""
+    if (k_scales is None) != (v_scales is None):
+        raise ValueError("k_scales and v_scales go together")
+    return k_scales is not None
+
+
 def append_paged_kv(k, v, k_cache, v_cache, slot_mapping, *, q=None, positions=None, cos_sin=None,
                     interleaved=False, k_scales=None, v_scales=None):
     """``torch.ops.hmx.append_paged_kv``, or ``append_paged_kv8`` where the cache is of 8 bits; the
     caches are written in place, q (None without one) is returned rotated."""
-    if k_scales is not None:
+    if _eight(k_scales, v_scales):
         out = torch.ops.hmx.append_paged_kv8(k, v, k_cache, v_cache, k_scales, v_scales, slot_mapping, q,
                                              positions, cos_sin, bool(interleaved))
     else:
@@ -637,7 +644,7 @@ def append_paged_kv(k, v, k_cache, v_cache, slot_mapping, *, q=None, positions=N
 def paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, scale=None, *, k_scales=None,
                            v_scales=None):
     """``torch.ops.hmx.paged_attention_decode``, or ``paged_attention_decode8``."""
-    if k_scales is not None:
+    if _eight(k_scales, v_scales):
         return torch.ops.hmx.paged_attention_decode8(q, k_cache, v_cache, k_scales, v_scales, block_table,
                                                      seq_lens, scale)
     return torch.ops.hmx.paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, scale)
@@ -646,7 +653,7 @@ def paged_attention_decode(q, k_cache, v_cache, block_table, seq_lens, scale=Non
 def paged_causal_attention(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens, scale=None, *,
                            k_scales=None, v_scales=None):
     """``torch.ops.hmx.paged_causal_attention``, or ``paged_causal_attention8``."""
-    if k_scales is not None:
+    if _eight(k_scales, v_scales):
         return torch.ops.hmx.paged_causal_attention8(q, k_cache, v_cache, k_scales, v_scales, block_table,
                                                      seq_lens, cu_seqlens, scale)
     return torch.ops.hmx.paged_causal_attention(q, k_cache, v_cache, block_table, seq_lens,
@@ -656,6 +663,7 @@ def paged_causal_attention(q, k_cache, v_cache, block_table, seq_lens, cu_seqlen
 def shared_prefix_attention_decode(q, k_cache, v_cache, block_table, seq_lens, prefix_table, prefix_lens,
                                    cu_prefix=None, scale=None, *, k_scales=None, v_scales=None):
     """``torch.ops.hmx.shared_prefix_attention_decode``."""
+    _eight(k_scales, v_scales)
     return torch.ops.hmx.shared_prefix_attention_decode(q, k_cache, v_cache, k_scales, v_scales, block_table,
                                                         seq_lens, prefix_table, prefix_lens, cu_prefix, scale)
 

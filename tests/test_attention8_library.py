@@ -20,3 +20,19 @@ def test_frequencies_that_need_a_gradient_are_refused():
             with torch.no_grad():
                 assert not call()[0].requires_grad
         assert lib.rotary_embedding(q, None, pos, inv.detach())[0].requires_grad == grad
+
+
+def test_one_of_two_scales_is_refused():
+    """Never taken for a cache of 16 bits, nor dropped beside one."""
+    m = torch.device("meta")
+    q, k = torch.empty(5, 4, 64, dtype=BF, device=m), torch.empty(5, 2, 64, dtype=BF, device=m)
+    sc = torch.empty(3, 2, 16, dtype=torch.uint8, device=m)
+    tab, n = torch.empty(5, 2, dtype=torch.int32, device=m), torch.empty(5, dtype=torch.int32, device=m)
+    for kv in (torch.empty(3, 16, 2, 64, dtype=t, device=m) for t in (BF, F8)):
+        for one in (dict(k_scales=sc), dict(v_scales=sc)):
+            for call in (lambda: lib.append_paged_kv(k, k, kv, kv.clone(), n, **one),
+                         lambda: lib.paged_attention_decode(q, kv, kv, tab, n, **one),
+                         lambda: lib.paged_causal_attention(q, kv, kv, tab, n, n, **one),
+                         lambda: lib.shared_prefix_attention_decode(q, kv, kv, tab, n, tab[:1], n[:1], **one)):
+                with pytest.raises(ValueError, match="k_scales and v_scales"):
+                    call()
