@@ -65,7 +65,8 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
         at = lambda n: rotary_dim * math.log(start / (n * 2 * math.pi)) / (2 * math.log(base))
         low, high = max(math.floor(at(fast)), 0), min(math.ceil(at(slow)), rotary_dim - 1)
         for i, f in enumerate(inv):
-            mix = min(max((i - low) / max(high - low, 1e-3), 0.0), 1.0)
+            # (a ramp that ends before pair 0 has no pair in it)
+            mix = 1.0 if at(slow) < 0 else min(max((i - low) / max(high - low, 1e-3), 0.0), 1.0)
             inv[i] = f / s * mix + f * (1 - mix)
         factor = float(cfg.get("attention_factor", 0.1 * math.log(s) + 1))
     return torch.tensor(inv, dtype=torch.float64, device=device), factor
