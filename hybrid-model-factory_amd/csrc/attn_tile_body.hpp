@@ -365,6 +365,10 @@
     }
     l += sum;
   };
+  // P in the inputs' type: each is off by half a step of itself, so O by at most half a step of
+  // sum p |v|, what its own rounding costs it too.  What that leaves as a product of its own, as
+  // in the kernels of few rows, which wait for memory, would be half as many matrix products
+  // again here, where they are the bound.
   auto pack = [&](const float* p) __attribute__((always_inline)) {
     return pack8<T>(p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]);
   };

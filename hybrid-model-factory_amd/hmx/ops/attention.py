@@ -441,7 +441,11 @@ def shared_prefix_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cac
     own keys only, behind the prefix's; where a serving engine's tables begin with the
     prefix's whole pages, ``block_table[:, pages:]`` and ``seq_lens - pages * page_size`` are
     they.  A sequence behind no prefix attends its own keys, one without own keys its
-    prefix's, and one without either gives 0.  The rest as in paged_attention_decode."""
+    prefix's, and one without either gives 0.  Where more than 64 rows (sequences times H / HKV)
+    a prefix share it on average, their part over the prefixes is formed as in
+    paged_causal_attention: the probabilities are rounded to q's type, and with fp16 what a
+    cache of 8 bits holds past that type's range may count as its largest value.  The rest as
+    in paged_attention_decode."""
     what = "shared_prefix_attention_decode"
     _refuse_tangents(what, q, k_cache, v_cache)
     if q.dim() != 3:

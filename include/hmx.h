@@ -905,8 +905,10 @@ int hmx_paged_attention_decode8(const void* q, int64_t q_token_stride, int64_t q
  * NULL: M = 1, all) attend the prefix_lens[m] keys that prefix_table's row m lists and, with
  * them in one softmax, their own seq_lens[n] keys (cache->table), where a sequence of no
  * group has its own alone and one without any key gives 0.  Both tables' pages lie in one
- * cache, of 8 bits where scales is not NULL.  workspace as for the decode, max_keys and
- * max_prefix the table widths times page_size.
+ * cache, of 8 bits where scales is not NULL.  Where N H / HKV > 64 M the prefixes' part has its
+ * probabilities rounded to q's type, as in hmx_paged_causal_attention, and with fp16 what a
+ * cache of 8 bits holds past that type's range counts as its largest value there.  workspace
+ * as for the decode, max_keys and max_prefix the table widths times page_size.
  */
 size_t hmx_shared_prefix_decode_workspace_bytes(int32_t N, int32_t M, int32_t H, int32_t HKV,
                                                 int32_t D, int64_t max_keys, int64_t max_prefix);
