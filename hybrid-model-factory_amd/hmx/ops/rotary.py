@@ -233,9 +233,12 @@ def turn(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_f
     flat = q.dim() == 3
     if flat:
         q, k, q_out, k_out = (t if t is None else t.unsqueeze(0) for t in (q, k, q_out, k_out))
+    outs = [t for t in (q_out, k_out) if t is not None]
+    if outs and _grad_of(q, k, *outs):
+        raise ValueError(f"{what}: q_out and k_out are not supported where a gradient is needed")
+    if outs:                            # a graph that has saved what is written over says so
+        torch.autograd.graph.increment_version(outs)
     if _grad_of(q, k):
-        if q_out is not None or k_out is not None:
-            raise ValueError(f"{what}: q_out and k_out are not supported where a gradient is needed")
         q, k = RotaryEmbedding.apply(q, k, positions, inv_freq, factor, interleaved, backward)
     else:
         q, k = rotate(q, k, positions, inv_freq, factor, interleaved, backward, q_out, k_out)

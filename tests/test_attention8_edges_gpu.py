@@ -29,3 +29,25 @@ def test_the_longest_table_rows(dev, eight):
     want = v[0, :, 0].double().mean(0)
     for o in outs:
         assert ((o.double().cpu() - want).abs() <= (2.0 ** -8 + 520 * 2.0 ** -24) * want).all()
+
+
+def test_rotating_in_place_beside_graphs(dev):
+    """A graph that has saved what q_out or k_out writes over refuses its backward, as torch's own
+    operations in place make it; tensors that need a gradient themselves are no outputs."""
+    pos, (inv, _) = torch.arange(5, device=dev), hmx.rotary_frequencies(64, device=dev)
+    x = torch.randn(1, 5, 2, 64, device=dev, dtype=BF).requires_grad_()
+    for name in ("q_out", "k_out"):
+        y = x * 2
+        z = (y * y).sum()                                                # saves y
+        other, mine = torch.zeros_like(x), y.detach()
+        q, k = (mine, other) if name == "q_out" else (other, mine)
+        hmx.rotary_embedding(q, k, pos, inv, **{name: mine})
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.backward()
+        with pytest.raises(ValueError, match="gradient"):
+            hmx.rotary_embedding(other, other, pos, inv, **{name: x})
+        with torch.no_grad():
+            assert hmx.rotary_embedding(other, other, pos, inv, **{name: x})[name == "k_out"] is x
+    with torch.inference_mode():
+        t = torch.ones(5, 2, 64, device=dev, dtype=BF)
+        assert hmx.rotary_embedding(t, None, pos, inv, q_out=t)[0].shape == t.shape
