@@ -388,7 +388,9 @@ struct PrefixShares {
 // sequence's rows fill a block of 16 on average; the blocks are then at most twice the sequences.
 // Against tiles of 128 rows, 32 / 8 heads of 128: 64 sequences of 4 tokens to 4096 keys 70 us, by tiles
 // 144; 255 of one and one of 512 tokens 380 and 472; at worst, all keys behind the one sequence
-// that has most of the tokens, 255 of 100 keys and 700 tokens behind 32768, 1755 and 954.
+// that has most of the tokens, 255 of 100 keys and 700 tokens behind 32768, 1755 and 954.  The
+// other way round, 255 of four tokens and one of 512 to 4096 keys go in tiles: 482, where the two
+// kinds alone take 246 and 74.  The lengths are known on the device only, so one rule decides for all.
 struct FewRows {
   const void* q;
   void* o;
