@@ -76,7 +76,15 @@ def _grad_of(*tensors: torch.Tensor | None) -> bool:
 def _forward_only(what: str, result: torch.Tensor, out: torch.Tensor | None, *inputs) -> torch.Tensor:
     """The result of an op without a backward, so that one through it raises; ``out``, where
     the caller gave one, stands outside any graph."""
-    return _NoBackward.apply([result], what, *inputs) if out is None and _grad_of(*inputs) else result
+    if out is not None:
+        written(out)
+        return result
+    return _NoBackward.apply([result], what, *inputs) if _grad_of(*inputs) else result
+
+
+def written(*outs: torch.Tensor) -> None:
+    """The caller's tensors count as written: a graph that has saved one refuses its backward."""
+    torch._C._increment_version(outs)
 
 
 def _refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
@@ -246,6 +254,8 @@ def attention_forward(q, k, v, scale, cu_seqlens, out, want_lse):
               v.data_ptr(), vts, vhs, _lib.dtype_code(q), o.data_ptr(), ots, ohs,
               _lib.ptr(lse), _lib.ptr(cu), N, B * T, H, k.shape[2], D, scale,
               int(out is None), _lib.ptr(ws), ws_bytes, _lib.stream_of(q))
+    if out is not None:
+        written(out)
     return o, lse, cu
 
 

@@ -12,7 +12,7 @@ import math
 import torch
 
 from .. import _lib
-from .attention import _HEAD_SIZES, _aligned, _elsewhere, _grad_of, _refuse_tangents, _same_device
+from .attention import _HEAD_SIZES, _aligned, _elsewhere, _grad_of, _refuse_tangents, _same_device, written
 
 _SCALINGS = {"default": set(), "linear": {"factor"}, "ntk": {"factor"},
              "yarn": {"factor", "original_max_position_embeddings", "beta_fast", "beta_slow", "attention_factor"}}
@@ -236,8 +236,8 @@ def turn(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, inv_f
     outs = [t for t in (q_out, k_out) if t is not None]
     if outs and _grad_of(q, k, *outs):
         raise ValueError(f"{what}: q_out and k_out are not supported where a gradient is needed")
-    if outs:                            # a graph that has saved what is written over says so
-        torch.autograd.graph.increment_version(outs)
+    if outs:
+        written(*outs)
     if _grad_of(q, k):
         q, k = RotaryEmbedding.apply(q, k, positions, inv_freq, factor, interleaved, backward)
     else:

@@ -1,4 +1,5 @@
-"""Ends of what the ops over caches of 8 bits and shared prefixes take: the longest table rows."""
+"""Ends of what the ops over caches of 8 bits, shared prefixes and the rotation take: the longest
+table rows, and outputs that graphs have saved."""
 import pytest
 import torch
 
@@ -51,3 +52,41 @@ def test_rotating_in_place_beside_graphs(dev):
     with torch.inference_mode():
         t = torch.ones(5, 2, 64, device=dev, dtype=BF)
         assert hmx.rotary_embedding(t, None, pos, inv, q_out=t)[0].shape == t.shape
+
+
+@pytest.mark.parametrize("eight", [True, False])
+def test_an_append_that_rotates_in_place_beside_graphs(dev, eight):
+    """q_out that a graph has saved counts as written."""
+    kc, vc = (torch.zeros(1, 16, 2, 64, dtype=torch.uint8 if eight else BF, device=dev) for _ in range(2))
+    sc = {n: torch.ones(1, 2, 16, dtype=torch.uint8, device=dev) for n in ("k_scales", "v_scales")} if eight else {}
+    kc, vc = (x.view(F8) if eight else x for x in (kc, vc))
+    x = torch.randn(5, 2, 64, device=dev, dtype=BF).requires_grad_()
+    at, table = torch.arange(5, device=dev), torch.rand(9, 64, device=dev)
+    y = x * 2
+    z = (y * y).sum()
+    mine = y.detach()
+    got = hmx.append_paged_kv(torch.ones_like(mine), torch.ones_like(mine), kc, vc, at, q=mine, positions=at, cos_sin=table, q_out=mine, **sc)
+    assert got is mine
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+
+
+def test_outputs_of_attention_beside_graphs(dev):
+    """``out`` that a graph has saved counts as written, whichever op writes it."""
+    kc, vc = (torch.zeros(2, 16, 2, 64, dtype=BF, device=dev) for _ in range(2))
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)
+    q, table, lens = torch.ones(2, 4, 64, dtype=BF, device=dev), i32(0, 1)[:, None], i32(9, 3)
+    kv = torch.ones(1, 2, 2, 64, dtype=BF, device=dev)
+    calls = [lambda out: hmx.paged_attention_decode(q, kc, vc, table, lens, out=out),
+             lambda out: hmx.paged_causal_attention(q, kc, vc, table, lens, i32(0, 1, 2), out=out),
+             lambda out: hmx.shared_prefix_attention_decode(q, kc, vc, table, lens, table[:1], lens[:1], out=out),
+             lambda out: hmx.causal_attention(q[None], kv, kv, out=out[None])]
+    x = torch.randn(2, 4, 64, device=dev, dtype=BF).requires_grad_()
+    for call in calls:
+        y = x * 2
+        z = (y * y).sum()
+        call(y.detach())
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            z.backward()
+        with torch.inference_mode():
+            call(torch.empty_like(q))
